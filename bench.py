@@ -730,6 +730,7 @@ class ProgressiveC5:
     traffic_file = "c5_progressive_b_hbm_traffic.json"
     cpu_batch = 2
     eager_only = True
+    max_norm = None  # --max-norm: the step clips its gradients
 
     def edges(self) -> int:  # tokens per step
         c = self.config
@@ -744,7 +745,7 @@ class ProgressiveC5:
     def make_step(self, torch, dev, impl: str = "native", batch: int | None = None, graph: bool = False):
         """graph: the step will be captured into a HIP graph -- AdamW keeps its
         step counts on the device (capturable) and autocast keeps no cast cache."""
-        from jakal_net.progressive import ProgressiveBConfig, ProgressiveBStep
+        from jakal_net.progressive import ProgressiveBConfig, ProgressiveBStep, train_step
 
         c = self.config
         B = batch or c["batch"]
@@ -761,13 +762,10 @@ class ProgressiveC5:
         target = torch.randint(0, c["vocab"] - 1, (B, c["query"]), generator=g).to(dev)
         use_autocast = dev.type == "cuda"  # the CPU baseline runs fp32
 
+        autocast = dict(device_type=dev.type, dtype=torch.bfloat16, enabled=use_autocast, cache_enabled=not graph)
+
         def step() -> None:
-            opt.zero_grad(set_to_none=True)
-            with torch.autocast(device_type=dev.type, dtype=torch.bfloat16, enabled=use_autocast,
-                                cache_enabled=not graph):
-                loss = model(prefix, target)
-            loss.backward()
-            opt.step()
+            train_step(model, opt, prefix, target, max_norm=self.max_norm, autocast=autocast)
         return step
 
 
@@ -827,6 +825,9 @@ def main() -> int:
                     help="score arithmetic of the top-k select (library default: split-f16)")
     ap.add_argument("--gemm-tile", type=int, choices=[0, 64, 128], default=0,
                     help="force the GEMM workgroup tile (0: chosen per call)")
+    ap.add_argument("--max-norm", type=float, default=None,
+                    help="c5-progressive-b: clip the gradients to this global norm in the timed step (default: the "
+                         "step does not clip)")
     ap.add_argument("--eager", action="store_true",
                     help="time eager steps only (default for the operator workloads: time replays of the step "
                          "captured into one HIP graph, torch.cuda.CUDAGraph, after timing the same number of "
@@ -852,6 +853,11 @@ def main() -> int:
     jn.set_gemm_tile(args.gemm_tile)
     jn.set_select_mode(jn.SELECT_SPLIT_F16 if args.select_mode == "split-f16" else jn.SELECT_F32)
     wl = WORKLOADS[args.workload]
+    if args.max_norm is not None:
+        if not isinstance(wl, ProgressiveC5):
+            ap.error("--max-norm is of the c5-progressive-b workload")
+        wl.max_norm = args.max_norm
+        wl.workload += f", gradients clipped to a global norm of {args.max_norm:g}"
     dev = torch.device("cuda:0")
     # C5's full-size step is timed eagerly: capturing it into a HIP graph after
     # eager steps has ended in a host segmentation fault inside torch's

@@ -39,7 +39,7 @@ typedef void* jn_stream_t;
 /* Message of the last failing call on this host thread ("" if none). */
 const char* jn_last_error(void);
 
-/* ABI revision of this header (bumped on any signature or accepted-range change); this is 17. */
+/* ABI revision of this header (bumped on any signature or accepted-range change); this is 18. */
 int jn_abi_version(void);
 
 /*
@@ -887,6 +887,87 @@ int jn_lowrank_pair_backward(const float* query_val, const float* source_val, co
                              jn_stream_t stream);
 size_t jn_lowrank_pair_backward_workspace_bytes(int64_t batch, int64_t query_nodes, int64_t source_nodes,
                                                 int64_t query_dim, int64_t source_dim, int64_t rank, int64_t edges);
+
+/*
+ * Operators of a training step beside the propagation ops.  Their tensors are
+ * void pointers with an element type code each; all compute in fp32 (the
+ * gradient norm's sum in 64 bits) and round once on the way out.
+ */
+#define JN_F32 0
+#define JN_BF16 1
+#define JN_F16 2
+
+/*
+ * Layer norm of `rows` rows of `dim` elements, with the scale of the path that
+ * a layer update comes through and, beside it, the states of the same nodes:
+ *   v = scale * x;  m = mean(v);  r = 1 / sqrt(mean((v - m)^2) + eps)
+ *   y = (v - m) r weight + bias;  state_out = tanh(scale * state)
+ * weight and bias [dim] may be null (1 and 0), and state with state_out null
+ * (a layer norm alone).  x, y are of `type`, state and state_out [rows] of
+ * `state_type`, weight and bias of `param_type` (JN_F32 or `type`).  stats
+ * [rows, 2] receives m and r for the backward, or is null.  x and y are
+ * contiguous and need no alignment beyond their elements'.
+ * Replaces _stabilize_layer and the scaled merge before it
+ * (scripts/progressive_b_example.py:282-292, 1011-1024) and the scan's value
+ * norm (native/jakal_net_native_cuda.cu:473-674).
+ */
+int jn_layer_norm_forward(const void* state, const void* x, const void* weight, const void* bias, int64_t rows,
+                          int64_t dim, float scale, float eps, int32_t type, int32_t state_type, int32_t param_type,
+                          void* state_out, void* y, float* stats, jn_stream_t stream);
+
+/*
+ * Its gradients: state, x, weight, stats as in the forward; grad_y of `type`,
+ * grad_state_out of `state_type`; each of grad_state, grad_x, grad_weight and
+ * grad_bias may be null (not wanted).  grad_state needs state and
+ * grad_state_out, the other three x, stats and grad_y.  The parameter
+ * gradients are sums over the rows in a fixed order (no atomics).
+ */
+size_t jn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t dim);
+int jn_layer_norm_backward(const void* state, const void* x, const void* weight, const float* stats,
+                           const void* grad_state_out, const void* grad_y, int64_t rows, int64_t dim, float scale,
+                           int32_t type, int32_t state_type, int32_t param_type, void* grad_state, void* grad_x,
+                           void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                           jn_stream_t stream);
+
+/*
+ * Cross entropy of logits [rows, classes] against target [rows]:
+ *   loss[row] = log(sum_j exp z_j) - z_target, 0 where target == ignore_index
+ * reduction 0 (none): loss only; 1 (sum) and 2 (mean over the rows that count):
+ * reduced[0] receives it and reduced[1] the rows that count (a mean over no
+ * row is NaN).  stats [rows, 2] receives each row's maximum and the logarithm
+ * of its sum of exponentials above it for the backward, or is null.  A target
+ * outside [0, classes) that is not ignore_index reads no logit: its row's loss
+ * and gradient are NaN.  Rows that are ignored read no logits at all.
+ * Replaces the vocabulary loss of the query block
+ * (scripts/progressive_b_example.py:2997-3006).
+ */
+int jn_cross_entropy_forward(const void* logits, const int64_t* target, int64_t rows, int64_t classes,
+                             int64_t ignore_index, int32_t reduction, int32_t type, float* loss, float* stats,
+                             float* reduced, jn_stream_t stream);
+
+/*
+ * grad_logits = (softmax(z) - onehot(target)) * c, 0 in ignored rows; c is
+ * grad_loss[row] (none), grad_loss[0] (sum) or grad_loss[0] / reduced[1] (mean).
+ */
+int jn_cross_entropy_backward(const void* logits, const int64_t* target, const float* stats, const float* reduced,
+                              const float* grad_loss, int64_t rows, int64_t classes, int64_t ignore_index,
+                              int32_t reduction, int32_t type, void* grad_logits, jn_stream_t stream);
+
+/*
+ * Norm over all elements of a list of tensors (no counterpart in the
+ * reference): norm_kind 0 the Euclidean norm, 1 the largest absolute value;
+ * 0 for an empty list.  The lists are host arrays, read before the call
+ * returns: device pointers, element counts and element types of dense tensors.
+ * jn_grads_clip writes out[i] = grads[i] * min(1, max_norm / (norm + 1e-6))
+ * (NaN where that factor is), out[i] being grads[i] itself or apart from every
+ * tensor of the list, and the unclipped norm.
+ */
+size_t jn_grads_workspace_bytes(int64_t tensors);
+int jn_grads_norm(const void* const* grads, const int64_t* counts, const int32_t* types, int64_t tensors,
+                  int32_t norm_kind, float* norm, void* workspace, size_t workspace_bytes, jn_stream_t stream);
+int jn_grads_clip(const void* const* grads, void* const* out, const int64_t* counts, const int32_t* types,
+                  const int32_t* out_types, int64_t tensors, double max_norm, int32_t norm_kind, float* norm,
+                  void* workspace, size_t workspace_bytes, jn_stream_t stream);
 
 #ifdef __cplusplus
 }

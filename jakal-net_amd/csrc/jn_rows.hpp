@@ -1,0 +1,52 @@
+// Element types and row reductions of the training-step operators (jn_norm.hip,
+// jn_loss.hip, jn_clip.hip), which take fp32, bf16 and fp16 tensors and compute
+// in fp32.
+#pragma once
+
+#include "jn_common.hpp"
+
+namespace jakal {
+
+// Element type codes of the C ABI (JN_F32, JN_BF16, JN_F16 in jakal_net_hip.h).
+constexpr int kTypeF32 = 0, kTypeBf16 = 1, kTypeF16 = 2;
+typedef _Float16 f16_t;
+
+inline bool known_type(int32_t t) { return t >= kTypeF32 && t <= kTypeF16; }
+inline int type_bytes(int32_t t) { return t == kTypeF32 ? 4 : 2; }
+
+// Calls f with a null pointer of the element type that a code names.
+template <typename F>
+int with_type(int32_t code, F f) {
+  if (code == kTypeBf16) return f(static_cast<bf16_t*>(nullptr));
+  if (code == kTypeF16) return f(static_cast<f16_t*>(nullptr));
+  return f(static_cast<float*>(nullptr));
+}
+
+// One element of a tensor whose type is known at run time only (the branch is uniform).
+__device__ __forceinline__ float load_any(const void* p, int64_t i, int code) {
+  if (code == kTypeF32) return static_cast<const float*>(p)[i];
+  if (code == kTypeBf16) return (float)static_cast<const bf16_t*>(p)[i];
+  return (float)static_cast<const f16_t*>(p)[i];
+}
+__device__ __forceinline__ void store_any(void* p, int64_t i, int code, float v) {
+  if (code == kTypeF32) static_cast<float*>(p)[i] = v;
+  else if (code == kTypeBf16) static_cast<bf16_t*>(p)[i] = (bf16_t)v;
+  else static_cast<f16_t*>(p)[i] = (f16_t)v;
+}
+
+// Sum over a workgroup of WAVES waves, the same in every thread (fixed order).
+// `lds` holds WAVES floats and may be reused after the next barrier.
+template <int WAVES>
+__device__ __forceinline__ float group_sum(float v, float* lds) {
+  v = wave_sum(v);
+  if constexpr (WAVES == 1) return v;
+  __syncthreads();  // earlier readers of lds are done
+  if (lane_id() == 0) lds[wave_id()] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) s += lds[i];
+  return s;
+}
+
+}  // namespace jakal

@@ -44,11 +44,12 @@ from dataclasses import dataclass
 
 import torch
 from torch import Tensor, nn
-from torch.nn import functional as F
 
-from jakal_net.core import Layer, LayerDelta
+from jakal_net.core import ImplementationMode, Layer, LayerDelta
 from jakal_net.modules import LowRankBilinearPairwise, LowRankBilinearRoute
+from jakal_net.norm import LayerNorm, stabilize_layer
 from jakal_net.propagation import SparsePropagation
+from jakal_net.training import clip_grad_norm_, cross_entropy
 from jakal_net.transition import SparseTransition
 
 # (alpha_b, beta_s_to_b, beta_b_to_s) of the reference's lite and mid stages
@@ -92,8 +93,9 @@ def _replace_scaled(layer: Layer, delta: LayerDelta, scale: float) -> Layer:
     return layer.with_tensors(state=delta.delta_state * scale, val=delta.delta_val * scale)
 
 
-def _stabilize(layer: Layer, norm: nn.Module) -> Layer:
-    return layer.with_tensors(state=torch.tanh(layer.state), val=norm(layer.val))
+def _update(layer: Layer, delta: LayerDelta, scale: float, norm: LayerNorm) -> Layer:
+    """The stabilised layer after an update by the scaled delta; a zero scale keeps the layer."""
+    return stabilize_layer(layer, norm) if scale == 0.0 else stabilize_layer(layer, norm, delta, scale)
 
 
 class PositionEncoding(nn.Module):
@@ -133,7 +135,7 @@ class _JointBlock(nn.Module):
         d, r, k = cfg.dim, cfg.rank, cfg.topk
         self.cfg = cfg
         self.alpha_b, self.beta_s_to_b, self.beta_b_to_s = stage
-        self.s_norm, self.exp_norm, self.cmp_norm = nn.LayerNorm(d), nn.LayerNorm(d), nn.LayerNorm(d)
+        self.s_norm, self.exp_norm, self.cmp_norm = (LayerNorm(d, implementation=implementation) for _ in range(3))
         self.exp_slot_state = nn.Parameter(0.02 * torch.randn(cfg.expanded))
         self.exp_slot_val = nn.Parameter(0.02 * torch.randn(cfg.expanded, d))
         self.cmp_slot_state = nn.Parameter(0.02 * torch.randn(cfg.compressed))
@@ -156,25 +158,22 @@ class _JointBlock(nn.Module):
     def forward(self, s: Layer, cmp: Layer | None) -> tuple[Layer, Layer]:
         c = self.cfg
         a = self.alpha_b
-        s = _stabilize(_replace_scaled(s, self.s_prop.compute_delta(s), c.s_scale), self.s_norm)
+        s = _update(s, self.s_prop.compute_delta(s), c.s_scale, self.s_norm)
         if cmp is None:
             cmp = _slot_layer(self.cmp_slot_state, self.cmp_slot_val, s)
         elif cmp.num_nodes != c.compressed:
             raise NotImplementedError("B_cmp changes size between blocks: the compressed adapter is not built")
-        cmp = _stabilize(cmp, self.cmp_norm)
+        cmp = stabilize_layer(cmp, self.cmp_norm)
 
         exp = _slot_layer(self.exp_slot_state, self.exp_slot_val, s)
         exp = _replace_scaled(exp, self.expand.compute_delta(cmp, exp), a * c.b_scale)
-        exp = _replace_scaled(exp, self.exp_prop.compute_delta(exp), a * c.b_scale)
-        exp = _stabilize(exp, self.exp_norm)
+        exp = _update(exp, self.exp_prop.compute_delta(exp), a * c.b_scale, self.exp_norm)
 
-        s = _replace_scaled(s, self.b_to_s.compute_delta(exp, s), a * self.beta_b_to_s * c.cross_scale)
-        s = _stabilize(s, self.s_norm)
+        s = _update(s, self.b_to_s.compute_delta(exp, s), a * self.beta_b_to_s * c.cross_scale, self.s_norm)
 
         nxt = _replace_scaled(cmp, self.compress.compute_delta(exp, cmp), a * c.b_scale)
         nxt = _replace_scaled(nxt, self.s_to_b.compute_delta(s, nxt), a * self.beta_s_to_b * c.cross_scale)
-        nxt = _replace_scaled(nxt, self.cmp_prop.compute_delta(nxt), a * c.b_scale)
-        return s, _stabilize(nxt, self.cmp_norm)
+        return s, _update(nxt, self.cmp_prop.compute_delta(nxt), a * c.b_scale, self.cmp_norm)
 
 
 class ProgressiveBStep(nn.Module):
@@ -184,20 +183,21 @@ class ProgressiveBStep(nn.Module):
     the shifted targets (a start token, then targets[:-1]) as their inputs and
     predict the targets; the loss is the mean cross entropy over all slots."""
 
-    def __init__(self, cfg: ProgressiveBConfig = ProgressiveBConfig(), *, implementation: str = "native") -> None:
+    def __init__(self, cfg: ProgressiveBConfig = ProgressiveBConfig(), *, implementation: ImplementationMode = "native") -> None:
         super().__init__()
         d, r, k = cfg.dim, cfg.rank, cfg.topk
         self.cfg = cfg
+        self.implementation = implementation
         self.embed = nn.Embedding(cfg.vocab, d)
         self.positions = PositionEncoding(d)
         self.state_init = nn.Linear(d, 1)
         nn.init.zeros_(self.state_init.weight)
         nn.init.zeros_(self.state_init.bias)
-        self.s_norm = nn.LayerNorm(d)
+        self.s_norm = LayerNorm(d, implementation=implementation)
         # one pairwise module per layer family, shared by every operator of the family
         s_pairwise, exp_pairwise = LowRankBilinearPairwise(d, r), LowRankBilinearPairwise(d, r)
         cmp_pairwise, q_pairwise = LowRankBilinearPairwise(d, r), LowRankBilinearPairwise(d, r)
-        self.q_norm = nn.LayerNorm(d)
+        self.q_norm = LayerNorm(d, implementation=implementation)
         self.q_transition = SparseTransition(LowRankBilinearRoute(d, d, rank=r), topk=k, implementation=implementation)
         # the query propagation runs as a causal window of query - 1 over the slots
         self.q_prop = SparsePropagation(q_pairwise, sparse_type="window", window=cfg.query - 1,
@@ -211,8 +211,8 @@ class ProgressiveBStep(nn.Module):
         self.refine = nn.ModuleList(
             SparsePropagation(s_pairwise, sparse_type="window", window=cfg.s_window, implementation=implementation)
             for _ in range(cfg.refine))
-        self.head_norm = nn.LayerNorm(d)
-        self.feedback_norm = nn.LayerNorm(d)
+        self.head_norm = LayerNorm(d, implementation=implementation)
+        self.feedback_norm = LayerNorm(d, implementation=implementation)
         self.feedback_proj = nn.Linear(d, d)
         self.head = nn.Sequential(nn.Linear(d, 4 * d), nn.GELU(), nn.Linear(4 * d, cfg.vocab))
         self.start_token = cfg.vocab - 1
@@ -222,14 +222,14 @@ class ProgressiveBStep(nn.Module):
         val = self.embed(prefix_ids)
         val = val + self.positions(prefix_ids.shape[-1], device=val.device, dtype=val.dtype).unsqueeze(0)
         s = Layer(dim=c.dim, num_nodes=val.shape[-2], state=self.state_init(val).squeeze(-1), val=val)
-        s = _stabilize(s, self.s_norm)
+        s = stabilize_layer(s, self.s_norm)
         for op in self.warmup:
-            s = _stabilize(_replace_scaled(s, op.compute_delta(s), c.warmup_scale), self.s_norm)
+            s = _update(s, op.compute_delta(s), c.warmup_scale, self.s_norm)
         cmp = None
         for block in self.blocks:
             s, cmp = block(s, cmp)
         for op in self.refine:
-            s = _stabilize(_replace_scaled(s, op.compute_delta(s), c.refine_scale), self.s_norm)
+            s = _update(s, op.compute_delta(s), c.refine_scale, self.s_norm)
         return s
 
     def query_logits(self, s: Layer, target_ids: Tensor) -> Tensor:
@@ -237,14 +237,35 @@ class ProgressiveBStep(nn.Module):
         shifted = torch.cat([torch.full_like(target_ids[:, :1], self.start_token), target_ids[:, :-1]], dim=1)
         feedback = self.feedback_proj(self.feedback_norm(self.embed(shifted)))
         q = Layer(dim=c.dim, num_nodes=shifted.shape[-1], state=self.state_init(feedback).squeeze(-1), val=feedback)
-        q = _stabilize(q, self.q_norm)
+        q = stabilize_layer(q, self.q_norm)
         for _ in range(c.query_refine):
-            q = _stabilize(_replace_scaled(q, self.q_transition.compute_delta(s, q), c.cross_scale), self.q_norm)
-            q = _stabilize(_replace_scaled(q, self.q_prop.compute_delta(q), c.s_scale), self.q_norm)
+            q = _update(q, self.q_transition.compute_delta(s, q), c.cross_scale, self.q_norm)
+            q = _update(q, self.q_prop.compute_delta(q), c.s_scale, self.q_norm)
         return self.head(self.head_norm(q.val))
 
     def forward(self, prefix_ids: Tensor, target_ids: Tensor) -> Tensor:
         logits = self.query_logits(self.encode_prefix(prefix_ids), target_ids)
-        if logits.dtype in (torch.float16, torch.bfloat16):
-            logits = logits.float()  # the loss of half-precision logits is taken in fp32
-        return F.cross_entropy(logits.reshape(-1, logits.shape[-1]), target_ids.reshape(-1))
+        # the loss of half-precision logits is taken in fp32
+        return cross_entropy(logits, target_ids, implementation=self.implementation)
+
+
+def train_step(model: ProgressiveBStep, optimizer: torch.optim.Optimizer, prefix_ids: Tensor, target_ids: Tensor, *,
+               max_norm: float | None = None, autocast: dict | None = None) -> tuple[Tensor, Tensor | None]:
+    """One training step: forward, backward, the gradients clipped to the global
+    norm ``max_norm`` (None: left as they are), the optimizer's update.
+
+    ``autocast`` holds torch.autocast's arguments for the forward (None: none).
+    Returns the loss and the norm before clipping (None without a limit); neither
+    has been waited for."""
+    optimizer.zero_grad(set_to_none=True)
+    if autocast is None:
+        loss = model(prefix_ids, target_ids)
+    else:
+        with torch.autocast(**autocast):
+            loss = model(prefix_ids, target_ids)
+    loss.backward()
+    norm = None
+    if max_norm is not None:
+        norm = clip_grad_norm_(model.parameters(), max_norm, implementation=model.implementation)
+    optimizer.step()
+    return loss.detach(), norm

@@ -933,8 +933,8 @@ int jn_layer_norm_backward(const void* state, const void* x, const void* weight,
  * Cross entropy of logits [rows, classes] against target [rows]:
  *   loss[row] = log(sum_j exp z_j) - z_target, 0 where target == ignore_index
  * reduction 0 (none): loss only; 1 (sum) and 2 (mean over the rows that count):
- * reduced[0] receives it and reduced[1] the rows that count (a mean over no
- * row is NaN).  stats [rows, 2] receives each row's maximum and the logarithm
+ * *reduced receives it and *count the rows that count (a mean over no row is
+ * NaN).  stats [rows, 2] receives each row's maximum and the logarithm
  * of its sum of exponentials above it for the backward, or is null.  A target
  * outside [0, classes) that is not ignore_index reads no logit: its row's loss
  * and gradient are NaN.  Rows that are ignored read no logits at all.
@@ -943,13 +943,13 @@ int jn_layer_norm_backward(const void* state, const void* x, const void* weight,
  */
 int jn_cross_entropy_forward(const void* logits, const int64_t* target, int64_t rows, int64_t classes,
                              int64_t ignore_index, int32_t reduction, int32_t type, float* loss, float* stats,
-                             float* reduced, jn_stream_t stream);
+                             float* reduced, float* count, jn_stream_t stream);
 
 /*
  * grad_logits = (softmax(z) - onehot(target)) * c, 0 in ignored rows; c is
- * grad_loss[row] (none), grad_loss[0] (sum) or grad_loss[0] / reduced[1] (mean).
+ * grad_loss[row] (none), grad_loss[0] (sum) or grad_loss[0] / *count (mean).
  */
-int jn_cross_entropy_backward(const void* logits, const int64_t* target, const float* stats, const float* reduced,
+int jn_cross_entropy_backward(const void* logits, const int64_t* target, const float* stats, const float* count,
                               const float* grad_loss, int64_t rows, int64_t classes, int64_t ignore_index,
                               int32_t reduction, int32_t type, void* grad_logits, jn_stream_t stream);
 

@@ -27,7 +27,8 @@ struct LossArgs {
   float* loss;       // [rows]
   float* stats;      // [rows][2]: M, L
   int reduction;
-  float* reduced;    // [2]: the reduced loss and the rows that count
+  float* reduced;    // the reduced loss
+  float* count;      // the rows that count
   const float* grad;  // one, or [rows] with reduction none
   void* dz;
 };
@@ -95,8 +96,8 @@ __global__ __launch_bounds__(kReduceThreads) void loss_reduce_kernel(LossArgs a)
   }
   if (threadIdx.x == 0) {
     // no counted row: 0 / 0 = NaN for the mean, as its definition has it
-    a.reduced[0] = (float)(a.reduction == kMean ? sums[0] / counts[0] : sums[0]);
-    a.reduced[1] = (float)counts[0];
+    *a.reduced = (float)(a.reduction == kMean ? sums[0] / counts[0] : sums[0]);
+    *a.count = (float)counts[0];
   }
 }
 
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_backward_any_kernel(LossArg
     }
     const float m = a.stats[2 * row], l = a.stats[2 * row + 1];
     float c = a.grad[a.reduction == kNone ? row : 0];
-    if (a.reduction == kMean) c /= a.reduced[1];
+    if (a.reduction == kMean) c /= *a.count;
     for (int64_t i = threadIdx.x; i < a.classes; i += kLossThreads) {
       const float p = expf(((float)z[i] - m) - l);
       dz[i] = (T)((p - (i == t ? 1.0f : 0.0f)) * c);
@@ -143,12 +144,13 @@ extern "C" {
 
 int jn_cross_entropy_forward(const void* logits, const int64_t* target, int64_t rows, int64_t classes,
                              int64_t ignore_index, int32_t reduction, int32_t type, float* loss, float* stats,
-                             float* reduced, jn_stream_t stream) {
+                             float* reduced, float* count, jn_stream_t stream) {
   LossArgs a{};
   a.z = logits, a.target = target, a.rows = rows, a.classes = classes, a.ignore = ignore_index;
   a.reduction = reduction, a.loss = loss, a.stats = stats, a.reduced = reduced;
+  a.count = count;
   if (const int rc = check_loss(a, type)) return rc;
-  JN_REQUIRE(logits && target && loss && (reduced || reduction == kNone), kInvalidArgument, "null tensor pointer");
+  JN_REQUIRE(logits && target && loss && ((reduced && count) || reduction == kNone), kInvalidArgument, "null tensor pointer");
   const auto s = static_cast<hipStream_t>(stream);
   const int rc = with_type(type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -164,15 +166,15 @@ int jn_cross_entropy_forward(const void* logits, const int64_t* target, int64_t 
   return kOk;
 }
 
-int jn_cross_entropy_backward(const void* logits, const int64_t* target, const float* stats, const float* reduced,
+int jn_cross_entropy_backward(const void* logits, const int64_t* target, const float* stats, const float* count,
                               const float* grad_loss, int64_t rows, int64_t classes, int64_t ignore_index,
                               int32_t reduction, int32_t type, void* grad_logits, jn_stream_t stream) {
   LossArgs a{};
   a.z = logits, a.target = target, a.rows = rows, a.classes = classes, a.ignore = ignore_index;
-  a.reduction = reduction, a.stats = const_cast<float*>(stats), a.reduced = const_cast<float*>(reduced);
+  a.reduction = reduction, a.stats = const_cast<float*>(stats), a.count = const_cast<float*>(count);
   a.grad = grad_loss, a.dz = grad_logits;
   if (const int rc = check_loss(a, type)) return rc;
-  JN_REQUIRE(logits && target && stats && grad_loss && grad_logits && (reduced || reduction != kMean),
+  JN_REQUIRE(logits && target && stats && grad_loss && grad_logits && (count || reduction != kMean),
              kInvalidArgument, "null tensor pointer");
   const auto s = static_cast<hipStream_t>(stream);
   return with_type(type, [&](auto* t) -> int {

@@ -158,27 +158,18 @@ def require_native_for_device(op_name: str, device_type: str) -> None:
     raise RuntimeError(f"native backend {status.backend_name} does not implement {op_name!r}")
 
 
-def takes_native(op_name: str, device_type: str, implementation: str) -> bool:
-    """Whether a call of a functional operator goes to the native module.  With
-    implementation="native" a GPU tensor that it cannot take raises here."""
-    if implementation not in ("native", "kernel") or native_disabled_by_env():
-        return False
-    if native_runs(op_name, device_type):
-        return True
-    if implementation == "native":
-        require_native_for_device(op_name, device_type)
-    return False
-
-
-def call_native(op_name: str, implementation: str, *args: Any, **kwargs: Any) -> Any:
-    """The native module's op, or None where it declines the call (limits, types)
-    and the implementation allows another path."""
-    try:
-        return getattr(_native_module(), op_name)(*args, **kwargs)
-    except NotImplementedError:
-        if implementation == "native":
-            raise
+def native_op(op_name: str, device_type: str, implementation: str) -> Any | None:
+    """The native module's op for a functional operator's call, or None where the
+    call takes the PyTorch form.  With implementation="native" a GPU tensor that
+    no library can take raises here."""
+    if implementation not in ("native", "kernel"):
         return None
+    status = native_status()
+    if status.available and op_name in status.supported_ops and device_type in status.supported_devices:
+        return getattr(_LOADER.module, op_name)
+    if implementation == "native" and not native_disabled_by_env():
+        require_native_for_device(op_name, device_type)
+    return None
 
 
 def _native_module() -> Any:

@@ -20,7 +20,7 @@ from torch import Tensor, nn
 from torch.nn import functional as F
 
 from jakal_net.core import ImplementationMode, Layer, LayerDelta, check_implementation
-from jakal_net.native_backend import call_native, takes_native
+from jakal_net.native_backend import native_op
 
 
 def _autocast_rows(x: Tensor) -> Tensor:
@@ -34,10 +34,13 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
                implementation: ImplementationMode = "native") -> Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of ``x``."""
     check_implementation(implementation)
-    if takes_native("layer_norm", x.device.type, implementation):
-        out = call_native("layer_norm", implementation, _autocast_rows(x), weight, bias, eps)
-        if out is not None:
-            return out
+    op = native_op("layer_norm", x.device.type, implementation)
+    if op is not None:
+        try:
+            return op(_autocast_rows(x), weight, bias, eps)
+        except NotImplementedError:  # outside the library's limits
+            if implementation == "native":
+                raise
     return F.layer_norm(x, x.shape[-1:], weight, bias, eps)
 
 
@@ -46,10 +49,13 @@ def stabilize(state: Tensor, val: Tensor, weight: Tensor | None = None, bias: Te
               implementation: ImplementationMode = "native") -> tuple[Tensor, Tensor]:
     """``(tanh(scale * state), layer_norm(scale * val))`` for states ``[..., N]`` and values ``[..., N, D]``."""
     check_implementation(implementation)
-    if takes_native("stabilize", val.device.type, implementation):
-        out = call_native("stabilize", implementation, state, _autocast_rows(val), weight, bias, eps, scale)
-        if out is not None:
-            return out
+    op = native_op("stabilize", val.device.type, implementation)
+    if op is not None:
+        try:
+            return op(state, _autocast_rows(val), weight, bias, eps, scale)
+        except NotImplementedError:
+            if implementation == "native":
+                raise
     if scale != 1.0:
         state, val = state * scale, val * scale
     return torch.tanh(state), F.layer_norm(val, val.shape[-1:], weight, bias, eps)

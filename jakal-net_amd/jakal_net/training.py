@@ -15,7 +15,7 @@ from torch import Tensor
 from torch.nn import functional as F
 
 from jakal_net.core import ImplementationMode, check_implementation
-from jakal_net.native_backend import call_native, takes_native
+from jakal_net.native_backend import native_op
 
 
 def cross_entropy(logits: Tensor, target: Tensor, *, ignore_index: int = -100, reduction: str = "mean",
@@ -28,10 +28,13 @@ def cross_entropy(logits: Tensor, target: Tensor, *, ignore_index: int = -100, r
     positions the gradient 0 whatever their logits hold, and a target outside
     the classes the loss and gradient NaN."""
     check_implementation(implementation)
-    if takes_native("cross_entropy", logits.device.type, implementation):
-        out = call_native("cross_entropy", implementation, logits, target, ignore_index, reduction)
-        if out is not None:
-            return out
+    op = native_op("cross_entropy", logits.device.type, implementation)
+    if op is not None:
+        try:
+            return op(logits, target, ignore_index, reduction)
+        except NotImplementedError:  # outside the library's limits
+            if implementation == "native":
+                raise
     if target.shape != logits.shape[:-1]:
         raise RuntimeError(f"cross_entropy: logits of shape {tuple(logits.shape)} do not pair with targets of shape "
                            f"{tuple(target.shape)}.")
@@ -68,10 +71,13 @@ def grad_norm(grads: Tensor | Iterable[Tensor | None], norm_type: float = 2.0, *
     """Norm over all elements of a list of tensors (None skipped), as a scalar tensor."""
     check_implementation(implementation)
     grads = _tensors(grads)
-    if takes_native("grad_norm", _device_type(grads), implementation):
-        norm = call_native("grad_norm", implementation, grads, norm_type)
-        if norm is not None:
-            return norm
+    op = native_op("grad_norm", _device_type(grads), implementation)
+    if op is not None:
+        try:
+            return op(grads, norm_type)
+        except NotImplementedError:
+            if implementation == "native":
+                raise
     return _norm(grads, float(norm_type))
 
 
@@ -86,10 +92,13 @@ def clip_grads(grads: Tensor | Iterable[Tensor | None], max_norm: float, norm_ty
     check_implementation(implementation)
     grads = _tensors(grads)
     targets = None if out is None else _tensors(out)
-    if takes_native("clip_grads", _device_type(grads), implementation):
-        norm = call_native("clip_grads", implementation, grads, max_norm, norm_type, targets)
-        if norm is not None:
-            return norm
+    op = native_op("clip_grads", _device_type(grads), implementation)
+    if op is not None:
+        try:
+            return op(grads, max_norm, norm_type, targets)
+        except NotImplementedError:
+            if implementation == "native":
+                raise
     if not float(max_norm) >= 0.0:
         raise ValueError(f"clip_grads: max_norm must not be negative, got {max_norm}.")
     targets = grads if targets is None else targets

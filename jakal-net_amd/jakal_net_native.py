@@ -27,7 +27,6 @@ from pathlib import Path
 import torch
 from torch import Tensor
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 LIB_ENV = "JAKAL_NET_HIP_LIB"
 _HERE = Path(__file__).resolve().parent
@@ -38,7 +37,9 @@ def library_path() -> Path:
     return Path(override) if override else _HERE / "lib" / "libjakal_net_hip.so"
 
 
-_LIB = ctypes.CDLL(str(library_path()))
+# global symbols: the PyTorch operators of libjakal_net_torch.so call this library
+_LIB = ctypes.CDLL(str(library_path()), mode=ctypes.RTLD_GLOBAL)
+torch.ops.load_library(str(_HERE / "lib" / "libjakal_net_torch.so"))
 
 _P, _I64, _I32, _F, _SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_size_t
 
@@ -209,7 +210,7 @@ _declare("jn_layer_norm_forward", [_P] * 4 + [_I64] * 2 + [_F] * 2 + [_I32] * 3 
 _declare("jn_layer_norm_backward_workspace_bytes", [_I64] * 2, _SZ)
 _declare("jn_layer_norm_backward",
          [_P] * 6 + [_I64] * 2 + [_F] + [_I32] * 3 + [_P] * 4 + [_P, _SZ, _P])
-_declare("jn_cross_entropy_forward", [_P] * 2 + [_I64] * 3 + [_I32] * 2 + [_P] * 4)
+_declare("jn_cross_entropy_forward", [_P] * 2 + [_I64] * 3 + [_I32] * 2 + [_P] * 5)
 _declare("jn_cross_entropy_backward", [_P] * 5 + [_I64] * 3 + [_I32] * 2 + [_P] * 2)
 _declare("jn_grads_workspace_bytes", [_I64], _SZ)
 _declare("jn_grads_norm", [_P] * 3 + [_I64, _I32] + [_P, _P, _SZ, _P])
@@ -1966,207 +1967,53 @@ def low_rank_pairwise_topk_backward_cuda(query_val: Tensor, source_val: Tensor, 
 # ---------------------------------------------------------------------------
 # operators of a training step beside the propagation ops
 # ---------------------------------------------------------------------------
-_TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _type_code(what: str, t: Tensor) -> int:
-    code = _TYPE_CODES.get(t.dtype)
-    if code is None:
-        raise NotImplementedError(f"{what} takes fp32, bf16 and fp16 tensors, got {t.dtype}.")
-    return code
-
-
-class _RowNorm(torch.autograd.Function):
-    """Layer norm of the rows of scale * x, and tanh(scale * state) where a state
-    is given (jn_layer_norm_*).  Contiguous inputs; weight and bias (or None) of
-    one type, fp32 or x's.  Keeps x and two floats a row for the backward."""
-
-    @staticmethod
-    def forward(ctx, state, x, weight, bias, eps: float, scale: float):
-        dim = x.shape[-1]
-        rows = x.numel() // dim
-        p = weight if weight is not None else bias
-        types = (_TYPE_CODES[x.dtype], 0 if state is None else _TYPE_CODES[state.dtype],
-                 0 if p is None else _TYPE_CODES[p.dtype])
-        dev = x.device
-        with _on(dev):
-            y = torch.empty_like(x)
-            out = None if state is None else torch.empty_like(state)
-            stats = None
-            if any(ctx.needs_input_grad[1:4]):
-                stats = torch.empty(rows, 2, device=dev, dtype=torch.float32)
-            _check(_LIB.jn_layer_norm_forward(_ptr(state), _ptr(x), _ptr(weight), _ptr(bias), rows, dim, scale, eps,
-                                              *types, _ptr(out), _ptr(y), _ptr(stats), _stream(dev)))
-        ctx.save_for_backward(state, x, weight, stats)
-        ctx.meta = (types, scale, None if bias is None else bias.dtype)
-        ctx.set_materialize_grads(False)
-        return y if state is None else (out, y)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
-        state, x, weight, stats = ctx.saved_tensors
-        types, scale, bias_dtype = ctx.meta
-        g_state, g = grads if state is not None else (None, grads[0])
-        need = list(ctx.needs_input_grad[:4])
-        dim = x.shape[-1]
-        rows = x.numel() // dim
-        dev = x.device
-        need[0] = need[0] and g_state is not None
-        if g is None:  # the values reach nothing
-            need[1:] = [False] * 3
-        with _on(dev):
-            gs = torch.empty_like(state) if need[0] else None
-            gx = torch.empty_like(x) if need[1] else None
-            gw = torch.empty_like(weight) if need[2] else None
-            gb = torch.empty(dim, device=dev, dtype=bias_dtype) if need[3] else None
-            if rows == 0:
-                for t in (gw, gb):
-                    if t is not None:
-                        t.zero_()
-            elif any(need):
-                ws_bytes = int(_LIB.jn_layer_norm_backward_workspace_bytes(rows, dim)) if need[2] or need[3] else 0
-                ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
-                g_state = g_state.to(state.dtype).contiguous() if need[0] else None
-                g = g.to(x.dtype).contiguous() if any(need[1:]) else None
-                _check(_LIB.jn_layer_norm_backward(
-                    _ptr(state), _ptr(x), _ptr(weight), _ptr(stats), _ptr(g_state), _ptr(g), rows, dim, scale, *types,
-                    _ptr(gs), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), ws_bytes, _stream(dev)))
-        return gs, gx, gw, gb, None, None
-
-
-def _norm_params(x: Tensor, weight: Tensor | None, bias: Tensor | None) -> tuple[Tensor | None, Tensor | None]:
-    """weight and bias contiguous and of one type: x's where both are, else fp32."""
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if tuple(p.shape) != (x.shape[-1],):
-            raise RuntimeError(f"layer norm {name} must be shaped [{x.shape[-1]}], got {tuple(p.shape)}.")
-        _type_code(f"layer norm {name}", p)
-    if any(p is not None and p.dtype != x.dtype for p in (weight, bias)):
-        weight, bias = _f32(weight), _f32(bias)
-    return (None if weight is None else weight.contiguous()), (None if bias is None else bias.contiguous())
-
-
-def _check_norm(x: Tensor, eps: float) -> None:
-    _type_code("layer norm", x)
-    if x.dim() < 1 or not 1 <= x.shape[-1] < 1 << 28:
-        raise RuntimeError(f"layer norm needs a last axis of 1 to 2^28 - 1 elements, got shape {tuple(x.shape)}.")
-    if not eps >= 0.0:
-        raise RuntimeError(f"layer norm eps must not be negative, got {eps}.")
+# Their checks, allocations and autograd nodes are C++ (csrc/jn_torch.cpp).
+_OPS = torch.ops.jakal_net_hip
+_layer_norm = _OPS.layer_norm.default
+_stabilize = _OPS.stabilize.default
+_cross_entropy = _OPS.cross_entropy.default
+_grad_norm = _OPS.grad_norm.default
+_clip_grads = _OPS.clip_grads.default
 
 
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5) -> Tensor:
-    """Layer norm over the last axis of x (fp32, bf16 or fp16), differentiable:
+    """Layer norm over the last axis of x (fp32, bf16 or fp16), differentiable once:
     (x - mean) / sqrt(var + eps) * weight + bias, computed in fp32 and returned
     in x's type.  weight and bias [dim] may be None."""
-    _check_norm(x, eps)
-    _require_gpu(x, weight, bias)
-    weight, bias = _norm_params(x, weight, bias)
-    return _run(_RowNorm, None, x.contiguous(), weight, bias, float(eps), 1.0)
+    return _layer_norm(x, weight, bias, eps)
 
 
 def stabilize(state: Tensor, val: Tensor, weight: Tensor | None = None, bias: Tensor | None = None,
               eps: float = 1e-5, scale: float = 1.0) -> tuple[Tensor, Tensor]:
     """The end of a layer update: (tanh(scale * state), layer_norm(scale * val))
     for states [..., nodes] and values [..., nodes, dim], one launch forward;
-    differentiable in the tensors.  Each output has its input's type."""
-    _check_norm(val, eps)
-    _type_code("stabilize", state)
-    if state.shape != val.shape[:-1]:
-        raise RuntimeError(f"stabilize: values of shape {tuple(val.shape)} do not pair with states of shape "
-                           f"{tuple(state.shape)}.")
-    _require_gpu(state, val, weight, bias)
-    weight, bias = _norm_params(val, weight, bias)
-    return _run(_RowNorm, state.contiguous(), val.contiguous(), weight, bias, float(eps), float(scale))
+    differentiable once in the tensors.  Each output has its input's type."""
+    return _stabilize(state, val, weight, bias, eps, scale)
 
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
-class _CrossEntropy(torch.autograd.Function):
-    """Cross entropy of contiguous logits [..., classes] against int64 targets
-    [...] (jn_cross_entropy_*).  Keeps the logits and two floats a row."""
-
-    @staticmethod
-    def forward(ctx, logits, target, ignore_index: int, reduction: int):
-        classes = logits.shape[-1]
-        rows = target.numel()
-        dev = logits.device
-        with _on(dev):
-            f32 = dict(device=dev, dtype=torch.float32)
-            loss = torch.empty(target.shape, **f32)
-            reduced = torch.empty(2, **f32) if reduction else None
-            stats = torch.empty(rows, 2, **f32) if ctx.needs_input_grad[0] else None
-            if rows:
-                _check(_LIB.jn_cross_entropy_forward(_ptr(logits), _ptr(target), rows, classes, ignore_index,
-                                                     reduction, _TYPE_CODES[logits.dtype], _ptr(loss), _ptr(stats),
-                                                     _ptr(reduced), _stream(dev)))
-            elif reduction:
-                reduced.fill_(float("nan") if reduction == 2 else 0.0)
-        ctx.save_for_backward(logits, target, stats, reduced)
-        ctx.meta = (ignore_index, reduction)
-        return reduced[0] if reduction else loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        logits, target, stats, reduced = ctx.saved_tensors
-        ignore_index, reduction = ctx.meta
-        dev = logits.device
-        with _on(dev):
-            grad = torch.empty_like(logits)
-            if target.numel():
-                g = _f32(g)
-                _check(_LIB.jn_cross_entropy_backward(_ptr(logits), _ptr(target), _ptr(stats), _ptr(reduced), _ptr(g),
-                                                      target.numel(), logits.shape[-1], ignore_index, reduction,
-                                                      _TYPE_CODES[logits.dtype], _ptr(grad), _stream(dev)))
-        return grad, None, None, None
-
-
 def cross_entropy(logits: Tensor, target: Tensor, ignore_index: int = -100, reduction: str = "mean") -> Tensor:
     """Cross entropy of logits [..., classes] (fp32, bf16 or fp16) against class
-    indices target [...] (int64 or int32), differentiable in the logits.  The
-    loss is fp32: one value a target ("none"), their sum, or their mean over the
-    targets that are not ignore_index (NaN where none is).  Ignored positions
+    indices target [...] (int64 or int32), differentiable once in the logits.
+    The loss is fp32: one value a target ("none"), their sum, or their mean over
+    the targets that are not ignore_index (NaN where none is).  Ignored positions
     have loss 0 and gradient 0 whatever their logits hold; a target outside the
     classes has loss and gradient NaN."""
     if reduction not in _REDUCTIONS:
         raise RuntimeError(f"cross_entropy reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}.")
-    _type_code("cross_entropy", logits)
-    if logits.dim() < 1 or target.shape != logits.shape[:-1]:
-        raise RuntimeError(f"cross_entropy: logits [..., classes] of shape {tuple(logits.shape)} do not pair with "
-                           f"targets of shape {tuple(target.shape)}.")
-    if not 1 <= logits.shape[-1] < 1 << 31:
-        raise RuntimeError(f"cross_entropy needs 1 to 2^31 - 1 classes, got {logits.shape[-1]}.")
-    if target.dtype not in (torch.int64, torch.int32):
-        raise RuntimeError(f"cross_entropy targets are int64 or int32 class indices, got {target.dtype}.")
-    _require_gpu(logits, target)
-    return _run(_CrossEntropy, logits.contiguous(), target.to(torch.int64).contiguous(), int(ignore_index),
-                _REDUCTIONS[reduction])
+    return _cross_entropy(logits, target, ignore_index, _REDUCTIONS[reduction])
+
+
+_NORM_KINDS = {2.0: 0, float("inf"): 1}
 
 
 def _norm_kind(norm_type: float) -> int:
-    kinds = {2.0: 0, float("inf"): 1}
-    if float(norm_type) not in kinds:
+    kind = _NORM_KINDS.get(float(norm_type))
+    if kind is None:
         raise NotImplementedError(f"the gradient norm is the Euclidean (2) or the maximum norm (inf), got {norm_type}.")
-    return kinds[float(norm_type)]
-
-
-def _dense_list(what: str, tensors: list) -> torch.device:
-    """The device of a non-empty list of strided tensors of the supported types."""
-    for t in tensors:
-        if t.layout is not torch.strided:
-            raise NotImplementedError(f"{what} takes dense tensors, got layout {t.layout}.")
-        _type_code(what, t)
-    return _require_gpu(*tensors)
-
-
-def _pointer_args(tensors: list) -> tuple:
-    n = len(tensors)
-    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]),
-            (ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
-            (ctypes.c_int32 * n)(*[_TYPE_CODES[t.dtype] for t in tensors]))
+    return kind
 
 
 def _as_list(tensors) -> list:
@@ -2178,33 +2025,7 @@ def grad_norm(grads, norm_type: float = 2.0) -> Tensor:
     skipped), of any mix of fp32, bf16 and fp16: sqrt(sum g^2) for norm_type 2,
     max |g| for inf, as an fp32 scalar on their device; the sum of squares is
     taken in 64 bits.  0 where there is nothing to sum."""
-    kind = _norm_kind(norm_type)
-    grads = [t for t in _as_list(grads) if t is not None]
-    if not grads:
-        return torch.zeros(())
-    dev = _dense_list("grad_norm", grads)
-    with _on(dev), torch.no_grad():
-        grads = [t.contiguous() for t in grads]
-        norm = torch.empty((), device=dev, dtype=torch.float32)
-        ws_bytes = int(_LIB.jn_grads_workspace_bytes(len(grads)))
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-        _check(_LIB.jn_grads_norm(*_pointer_args(grads), len(grads), kind, _ptr(norm), _ptr(ws), ws_bytes,
-                                  _stream(dev)))
-    return norm
-
-
-def _in_order_of(g: Tensor, o: Tensor) -> Tensor:
-    """g (itself where it can be) with its elements in memory in the order that o,
-    which has to fill its memory, has them in."""
-    step = 1
-    for stride, size in sorted((s, n) for n, s in zip(o.shape, o.stride()) if n != 1):
-        if stride != step and o.numel():
-            raise NotImplementedError(f"clip_grads writes tensors that fill their memory, got strides {o.stride()} for "
-                                      f"shape {tuple(o.shape)}.")
-        step *= size
-    if g.stride() == o.stride():
-        return g
-    return torch.empty_strided(o.shape, o.stride(), device=g.device, dtype=g.dtype).copy_(g)
+    return _grad_norm([t for t in _as_list(grads) if t is not None], _norm_kind(norm_type))
 
 
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tensor:
@@ -2217,39 +2038,15 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
     of the same shapes and of any supported type, each its gradient itself or
     apart in memory from every other tensor given.  What is written to fills its
     memory (contiguous up to the order of its axes).  Nothing is waited for."""
-    kind = _norm_kind(norm_type)
-    max_norm = float(max_norm)
-    if not max_norm >= 0.0:
-        raise ValueError(f"clip_grads: max_norm must not be negative, got {max_norm}.")
     grads = _as_list(grads)
     if out is None:
-        grads = targets = [t for t in grads if t is not None]
+        grads = out = [t for t in grads if t is not None]
     else:
-        targets = _as_list(out)
-        if len(targets) != len(grads):
-            raise ValueError(f"clip_grads: {len(grads)} gradients but {len(targets)} outputs.")
-        targets = [o for o, g in zip(targets, grads) if g is not None]
-        grads = [g for g in grads if g is not None]
-        for g, o in zip(grads, targets):
-            if o is None or o.shape != g.shape:
-                raise ValueError(f"clip_grads: a gradient of shape {tuple(g.shape)} needs an output of that shape, got "
-                                 f"{None if o is None else tuple(o.shape)}.")
-            if o.requires_grad and o.is_leaf and o is not g:
-                raise ValueError("clip_grads: an output requires grad.")
-    if not grads:
-        return torch.zeros(())
-    dev = _dense_list("clip_grads", grads if out is None else grads + targets)
-    with _on(dev), torch.no_grad():
-        reads = [g if g.is_contiguous() and o.is_contiguous() else _in_order_of(g, o) for g, o in zip(grads, targets)]
-        norm = torch.empty((), device=dev, dtype=torch.float32)
-        n = len(reads)
-        ws_bytes = int(_LIB.jn_grads_workspace_bytes(n))
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-        read_ptrs, counts, types = _pointer_args(reads)
-        write_ptrs, write_types = read_ptrs, types
-        if out is not None:
-            write_ptrs, _, write_types = _pointer_args(targets)
-        _check(_LIB.jn_grads_clip(read_ptrs, write_ptrs, counts, types, write_types, n, max_norm, kind, _ptr(norm),
-                                  _ptr(ws), ws_bytes, _stream(dev)))
-    torch.autograd.graph.increment_version(targets)
-    return norm
+        out = _as_list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"clip_grads: {len(grads)} gradients but {len(out)} outputs.")
+        pairs = [(g, o) for g, o in zip(grads, out) if g is not None]
+        grads, out = [g for g, _ in pairs], [o for _, o in pairs]
+        if any(o is None for o in out):
+            raise ValueError("clip_grads: a gradient without an output.")
+    return _clip_grads(grads, out, float(max_norm), _norm_kind(norm_type))

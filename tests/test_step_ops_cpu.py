@@ -175,17 +175,18 @@ def test_c_abi_loss_checks():
     lib = _lib()
     p = ctypes.c_void_p(4096)
 
-    def forward(rows=4, classes=8, reduction=2, kind=0, z=p, t=p, loss=p, reduced=p):
-        return lib.jn_cross_entropy_forward(z, t, rows, classes, -100, reduction, kind, loss, None, reduced, None)
+    def forward(rows=4, classes=8, reduction=2, kind=0, z=p, t=p, loss=p, reduced=p, count=p):
+        return lib.jn_cross_entropy_forward(z, t, rows, classes, -100, reduction, kind, loss, None, reduced, count, None)
 
     for bad in (dict(rows=0), dict(classes=0), dict(classes=1 << 31), dict(reduction=3), dict(reduction=-1),
-                dict(kind=3), dict(z=None), dict(t=None), dict(loss=None), dict(reduced=None), dict(rows=1 << 40)):
+                dict(kind=3), dict(z=None), dict(t=None), dict(loss=None), dict(reduced=None), dict(count=None),
+                dict(rows=1 << 40)):
         assert forward(**bad) == 1, bad
 
-    def backward(stats=p, reduced=p, g=p, dz=p, reduction=2):
-        return lib.jn_cross_entropy_backward(p, p, stats, reduced, g, 4, 8, -100, reduction, 0, dz, None)
+    def backward(stats=p, count=p, g=p, dz=p, reduction=2):
+        return lib.jn_cross_entropy_backward(p, p, stats, count, g, 4, 8, -100, reduction, 0, dz, None)
 
-    for bad in (dict(stats=None), dict(reduced=None), dict(g=None), dict(dz=None), dict(reduction=5)):
+    for bad in (dict(stats=None), dict(count=None), dict(g=None), dict(dz=None), dict(reduction=5)):
         assert backward(**bad) == 1, bad
 
 

@@ -56,6 +56,212 @@ __device__ __forceinline__ float param(const void* p, int64_t i, int code, float
   return p ? load_any(p, i, code) : none;
 }
 
+// ---- rows held in registers ---------------------------------------------------
+// A group of GW waves takes a row: thread t of it the packs t, t + 64 GW, ... of
+// W elements (16 bytes; single elements where rows do not start on 16), NP packs
+// at most.  A row is read once, and its mean, centred squares and gradient sums
+// come from registers; the next row's packs load while this one is reduced.
+constexpr int kGroupThreads = 256;
+
+template <int W, int NP, int GW>
+struct RowGroup {
+  static constexpr int kThreads = GW * kWave;
+  static constexpr int kItems = W * NP;  // elements of a thread
+
+  __device__ static int thread() { return GW == 1 ? lane_id() : (int)threadIdx.x; }
+  __device__ static int64_t element(int p) { return (int64_t)(p * kThreads + thread()) * W; }
+};
+
+template <typename T, int W, int NP, int GW>
+__device__ __forceinline__ void load_row(const void* base, int64_t row, int64_t dim, Raw<T, W> (&raw)[NP]) {
+  const T* p = static_cast<const T*>(base) + row * dim;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int64_t e = RowGroup<W, NP, GW>::element(i);
+    if (e < dim) raw[i].load(p + e);
+    else raw[i].clear();
+  }
+}
+
+template <typename T, int W, int NP, int GW>
+__device__ __forceinline__ void load_params(const void* base, int type, int64_t dim, float none,
+                                            float (&v)[W * NP]) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int64_t e = RowGroup<W, NP, GW>::element(i);
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[i * W + j] = none;
+    if (!base || e >= dim) continue;
+    if (sizeof(T) != 4 && type != kTypeF32) {
+      Raw<T, W> raw;
+      raw.load(static_cast<const T*>(base) + e);
+      raw.unpack(v + i * W);
+    } else {
+      const float* p = static_cast<const float*>(base) + e;
+      if constexpr (W == 1) {
+        v[i] = p[0];
+      } else {
+#pragma unroll
+        for (int j = 0; j < W; j += 4) {
+          Raw<float, 4> raw;
+          raw.load(p + j);
+          raw.unpack(v + i * W + j);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int W, int NP, int GW>
+__global__ __launch_bounds__(kGroupThreads) void norm_forward_kernel(NormArgs a) {
+  using G = RowGroup<W, NP, GW>;
+  constexpr int kGroups = kGroupThreads / G::kThreads;
+  __shared__ float lds[GW];
+  const int64_t groups = (int64_t)gridDim.x * kGroups;
+  const int64_t first = (int64_t)blockIdx.x * kGroups + (GW == 1 ? wave_id() : 0);
+  const float n = (float)a.dim;
+  Raw<T, W> next[NP];
+  if (first < a.rows) load_row<T, W, NP, GW>(a.x, first, a.dim, next);
+  float w[G::kItems], b[G::kItems];
+  load_params<T, W, NP, GW>(a.w, a.param_type, a.dim, 1.0f, w);
+  load_params<T, W, NP, GW>(a.b, a.param_type, a.dim, 0.0f, b);
+  for (int64_t row = first; row < a.rows; row += groups) {
+    float v[G::kItems];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) next[i].unpack(v + i * W);
+    if (row + groups < a.rows) load_row<T, W, NP, GW>(a.x, row + groups, a.dim, next);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < G::kItems; ++i) {
+      v[i] *= a.scale;
+      s += v[i];
+    }
+    const float m = group_sum<GW>(s, lds) / n;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      if (G::element(i) >= a.dim) continue;  // (the clears there are not elements)
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        v[i * W + j] -= m;
+        s += v[i * W + j] * v[i * W + j];
+      }
+    }
+    const float r = 1.0f / sqrtf(group_sum<GW>(s, lds) / n + a.eps);
+    T* y = static_cast<T*>(a.y) + row * a.dim;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      if (G::element(i) >= a.dim) continue;
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[i * W + j] = v[i * W + j] * r * w[i * W + j] + b[i * W + j];
+      store_raw<T, W>(y + G::element(i), v + i * W);
+    }
+    if (a.stats && G::thread() == 0) {
+      a.stats[2 * row] = m;
+      a.stats[2 * row + 1] = r;
+    }
+  }
+  if (a.state) {
+    for (int64_t i = (int64_t)blockIdx.x * kGroupThreads + threadIdx.x; i < a.rows;
+         i += (int64_t)gridDim.x * kGroupThreads)
+      state_forward(a, i);
+  }
+}
+
+// A workgroup of WPB waves also keeps the column sums of its rows: each thread
+// its own columns' in registers, joined over the groups in LDS at the end.
+template <typename T, int W, int NP, int GW, int WPB>
+__global__ __launch_bounds__(WPB* kWave) void norm_backward_kernel(NormArgs a) {
+  using G = RowGroup<W, NP, GW>;
+  constexpr int kThreads = WPB * kWave, kGroups = WPB / GW;
+  __shared__ float lds[GW];
+  extern __shared__ float sums[];  // [kGroups][dim]
+  const int64_t groups = (int64_t)gridDim.x * kGroups;
+  const int64_t first = (int64_t)blockIdx.x * kGroups + (GW == 1 ? wave_id() : 0);
+  const float n = (float)a.dim;
+  float dw[G::kItems], db[G::kItems];
+#pragma unroll
+  for (int i = 0; i < G::kItems; ++i) dw[i] = db[i] = 0.f;
+  if (a.dx || a.partial) {
+    Raw<T, W> next_x[NP], next_g[NP];
+    if (first < a.rows) {
+      load_row<T, W, NP, GW>(a.x, first, a.dim, next_x);
+      load_row<T, W, NP, GW>(a.g, first, a.dim, next_g);
+    }
+    float w[G::kItems];
+    load_params<T, W, NP, GW>(a.w, a.param_type, a.dim, 1.0f, w);
+    for (int64_t row = first; row < a.rows; row += groups) {
+      const float m = a.stats[2 * row], r = a.stats[2 * row + 1];
+      float h[G::kItems], g[G::kItems];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        next_x[i].unpack(h + i * W);
+        next_g[i].unpack(g + i * W);
+      }
+      if (row + groups < a.rows) {
+        load_row<T, W, NP, GW>(a.x, row + groups, a.dim, next_x);
+        load_row<T, W, NP, GW>(a.g, row + groups, a.dim, next_g);
+      }
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (G::element(i) >= a.dim) continue;
+#pragma unroll
+        for (int j = i * W; j < i * W + W; ++j) {
+          h[j] = (a.scale * h[j] - m) * r;
+          dw[j] += g[j] * h[j];
+          db[j] += g[j];
+          g[j] *= w[j];
+          s1 += g[j];
+          s2 += g[j] * h[j];
+        }
+      }
+      if (!a.dx) continue;
+      s1 = group_sum<GW>(s1, lds) / n;
+      s2 = group_sum<GW>(s2, lds) / n;
+      const float sr = a.scale * r;
+      T* dx = static_cast<T*>(a.dx) + row * a.dim;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (G::element(i) >= a.dim) continue;
+#pragma unroll
+        for (int j = i * W; j < i * W + W; ++j) h[j] = sr * (g[j] - s1 - h[j] * s2);
+        store_raw<T, W>(dx + G::element(i), h + i * W);
+      }
+    }
+  }
+  if (a.dstate) {
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < a.rows; i += (int64_t)gridDim.x * kThreads)
+      state_backward(a, i);
+  }
+  if (!a.partial) return;
+  float* out = a.partial + (int64_t)blockIdx.x * 2 * a.dim;
+  const int group = kGroups == 1 ? 0 : wave_id();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (k) __syncthreads();  // the sums before are read
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int64_t e = G::element(i);
+      if (e >= a.dim) continue;
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const float v = k ? db[i * W + j] : dw[i * W + j];
+        if (kGroups == 1) out[k * a.dim + e + j] = v;
+        else sums[group * a.dim + e + j] = v;
+      }
+    }
+    if (kGroups == 1) continue;
+    __syncthreads();
+    for (int64_t c = threadIdx.x; c < a.dim; c += kThreads) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) s += sums[i * a.dim + c];
+      out[k * a.dim + c] = s;
+    }
+  }
+}
+
 // Rows of any width and alignment: a workgroup a row, three passes over it.
 constexpr int kAnyThreads = 256;
 constexpr int kAnyWaves = kAnyThreads / kWave;
@@ -146,22 +352,81 @@ __global__ __launch_bounds__(kAnyThreads) void norm_columns_any_kernel(NormArgs 
   }
 }
 
-// The slabs' partial sums, in slab order.
-__global__ __launch_bounds__(kAnyThreads) void norm_columns_finish_kernel(NormArgs a, int slabs) {
-  const int64_t c = (int64_t)blockIdx.x * kAnyThreads + threadIdx.x;
-  if (c >= a.dim) return;
-  float sw = 0.f, sb = 0.f;
-  for (int s = 0; s < slabs; ++s) {
-    sw += a.partial[(int64_t)s * 2 * a.dim + c];
-    sb += a.partial[((int64_t)s * 2 + 1) * a.dim + c];
+// The partial sums of all workgroups or slabs: 32 columns a workgroup, each by
+// 32 threads that take every 32nd partial.
+constexpr int kFinishColumns = 32, kFinishLanes = 32;
+__global__ __launch_bounds__(kFinishColumns* kFinishLanes) void norm_columns_finish_kernel(NormArgs a, int parts) {
+  __shared__ float lds[kFinishLanes][kFinishColumns + 1];
+  const int col = threadIdx.x % kFinishColumns, lane = threadIdx.x / kFinishColumns;
+  const int64_t c = (int64_t)blockIdx.x * kFinishColumns + col;  // of dw's columns and then db's
+  float s = 0.f;
+  if (c < 2 * a.dim) {
+#pragma unroll 4
+    for (int p = lane; p < parts; p += kFinishLanes) s += a.partial[(int64_t)p * 2 * a.dim + c];
   }
-  if (a.dw) store_any(a.dw, c, a.param_type, sw);
-  if (a.db) store_any(a.db, c, a.param_type, sb);
+  lds[lane][col] = s;
+  for (int step = kFinishLanes / 2; step > 0; step /= 2) {
+    __syncthreads();
+    if (lane < step) lds[lane][col] += lds[lane + step][col];
+  }
+  if (lane == 0 && c < 2 * a.dim) {
+    void* out = c < a.dim ? a.dw : a.db;
+    if (out) store_any(out, c < a.dim ? c : c - a.dim, a.param_type, lds[0][col]);
+  }
 }
 
-// Row slabs of the column sums.
+// ---- which kernel ---------------------------------------------------------------
+// The register kernels' shapes: packs of 16 bytes where every row and parameter
+// starts on 16, else single elements.  A wave takes rows of up to 16 elements a
+// lane, four waves rows of up to 16 a thread; wider rows take the kernels that
+// pass over memory.
+struct RowShape {
+  int width, packs, waves;  // W, NP, GW; packs = 0: none fits
+};
+
+RowShape row_shape(int64_t dim, bool aligned, int elem_bytes) {
+  const int w = aligned ? 16 / elem_bytes : 1;
+  for (const int waves : {1, 4}) {
+    for (const int items : {4, 8, 16}) {
+      if (items < w) continue;
+      if (dim <= (int64_t)items * waves * kWave) return {w, items / w, waves};
+    }
+  }
+  return {w, 0, 0};
+}
+
+// Calls f with a shape's packs of W elements as a constant; MOST: the most elements of a thread (8 or 16).
+template <int W, int MOST, typename F>
+int with_packs(int packs, F f) {
+  if constexpr (W <= 4) {
+    if (packs * W == 4) return f(std::integral_constant<int, 4 / W>{});
+  }
+  if constexpr (MOST >= 16) {
+    if (packs * W == 16) return f(std::integral_constant<int, 16 / W>{});
+  }
+  return f(std::integral_constant<int, 8 / W>{});
+}
+
+// Workgroups of the backward, each of which leaves one row of partial sums.
+constexpr int64_t kMaxParts = 512;
+constexpr int64_t kManyRows = 2048;
+
+// Sixteen waves a workgroup for many rows: fewer partial sums to join.  (At 16
+// elements a lane they would not have the registers.)
+int backward_waves(const RowShape& s, int64_t rows) {
+  return s.waves == 1 && s.width * s.packs <= 8 && rows >= kManyRows ? 16 : 4;
+}
+int64_t backward_groups(const RowShape& s, int64_t rows) {
+  const int64_t per = backward_waves(s, rows) / s.waves;
+  return std::min((rows + per - 1) / per, kMaxParts);
+}
+
+// Row slabs of the column sums of wide rows.
 constexpr int64_t kSlabs = 64;
 int64_t slab_count(int64_t rows) { return std::min<int64_t>(kSlabs, (rows + 15) / 16); }
+
+// Workgroups of the wave-a-row forward: eight of four waves a CU.
+constexpr int64_t kForwardGroups = 2048;
 
 int64_t row_groups(int64_t rows) { return std::min<int64_t>(rows, 1 << 20); }
 
@@ -175,6 +440,102 @@ int check_norm(const NormArgs& a, int32_t type, int32_t state_type, int32_t para
              "layer norm needs rows >= 0, 1 <= dim < 2^28 and at most 2^40 elements (rows=%lld, dim=%lld)",
              (long long)a.rows, (long long)a.dim);
   return kOk;
+}
+
+template <typename T>
+bool aligned_rows(const NormArgs& a) {
+  if (a.dim % (16 / sizeof(T)) != 0) return false;
+  for (const void* p : {a.x, static_cast<const void*>(a.y), a.g, static_cast<const void*>(a.dx), a.w, a.b}) {
+    if (!aligned16(p)) return false;
+  }
+  return true;
+}
+
+template <typename T>
+int launch_norm_forward(const NormArgs& a, hipStream_t s) {
+  const bool aligned = aligned_rows<T>(a);
+  const RowShape shape = row_shape(a.dim, aligned, sizeof(T));
+  if (!shape.packs) {
+    JN_PROFILE("norm_forward_any_kernel", s);
+    hipLaunchKernelGGL(norm_forward_any_kernel<T>, dim3((unsigned)row_groups(a.rows)), dim3(kAnyThreads), 0, s, a);
+    JN_LAUNCH_CHECK();
+    return kOk;
+  }
+  const int64_t per = kGroupThreads / kWave / shape.waves;
+  const unsigned grid = (unsigned)std::min<int64_t>((a.rows + per - 1) / per, kForwardGroups);
+  const auto run = [&](auto width, auto waves) {
+    constexpr int W = decltype(width)::value, GW = decltype(waves)::value;
+    return with_packs<W, 16>(shape.packs, [&](auto packs) -> int {
+      JN_PROFILE("norm_forward_kernel", s);
+      hipLaunchKernelGGL((norm_forward_kernel<T, W, decltype(packs)::value, GW>), dim3(grid), dim3(kGroupThreads), 0, s,
+                         a);
+      JN_LAUNCH_CHECK();
+      return kOk;
+    });
+  };
+  constexpr int V = 16 / sizeof(T);
+  using One = std::integral_constant<int, 1>;
+  using Four = std::integral_constant<int, 4>;
+  using Pack = std::integral_constant<int, V>;
+  if (aligned) return shape.waves == 1 ? run(Pack{}, One{}) : run(Pack{}, Four{});
+  return shape.waves == 1 ? run(One{}, One{}) : run(One{}, Four{});
+}
+
+int launch_columns_finish(const NormArgs& a, int64_t parts, hipStream_t s) {
+  JN_PROFILE("norm_columns_finish_kernel", s);
+  hipLaunchKernelGGL(norm_columns_finish_kernel, dim3((unsigned)((2 * a.dim + kFinishColumns - 1) / kFinishColumns)),
+                     dim3(kFinishColumns * kFinishLanes), 0, s, a, (int)parts);
+  JN_LAUNCH_CHECK();
+  return kOk;
+}
+
+template <typename T>
+int launch_norm_backward(NormArgs a, hipStream_t s) {
+  const bool columns = a.dw || a.db;
+  if (!columns) a.partial = nullptr;
+  const bool aligned = aligned_rows<T>(a);
+  const RowShape shape = row_shape(a.dim, aligned, sizeof(T));
+  if (!shape.packs) {
+    if (a.dx || a.dstate) {
+      JN_PROFILE("norm_backward_any_kernel", s);
+      hipLaunchKernelGGL(norm_backward_any_kernel<T>, dim3((unsigned)row_groups(a.rows)), dim3(kAnyThreads), 0, s, a);
+      JN_LAUNCH_CHECK();
+    }
+    if (!columns) return kOk;
+    const int64_t slabs = slab_count(a.rows);
+    {
+      JN_PROFILE("norm_columns_any_kernel", s);
+      hipLaunchKernelGGL(norm_columns_any_kernel<T>, dim3((unsigned)((a.dim + kWave - 1) / kWave), (unsigned)slabs),
+                         dim3(kAnyThreads), 0, s, a, (a.rows + slabs - 1) / slabs);
+      JN_LAUNCH_CHECK();
+    }
+    return launch_columns_finish(a, slabs, s);
+  }
+  const int64_t grid = backward_groups(shape, a.rows);
+  const auto run = [&](auto width, auto waves, auto block) {
+    constexpr int W = decltype(width)::value, GW = decltype(waves)::value, WPB = decltype(block)::value;
+    const size_t lds = a.partial && WPB > GW ? (size_t)(WPB / GW) * a.dim * sizeof(float) : 0;
+    return with_packs<W, WPB == 16 ? 8 : 16>(shape.packs, [&](auto packs) -> int {
+      JN_PROFILE("norm_backward_kernel", s);
+      hipLaunchKernelGGL((norm_backward_kernel<T, W, decltype(packs)::value, GW, WPB>), dim3((unsigned)grid),
+                         dim3(WPB * kWave), lds, s, a);
+      JN_LAUNCH_CHECK();
+      return kOk;
+    });
+  };
+  constexpr int V = 16 / sizeof(T);
+  using One = std::integral_constant<int, 1>;
+  using Four = std::integral_constant<int, 4>;
+  using Sixteen = std::integral_constant<int, 16>;
+  using Pack = std::integral_constant<int, V>;
+  const bool many = backward_waves(shape, a.rows) == 16;
+  const auto sized = [&](auto width) {
+    if (shape.waves == 4) return run(width, Four{}, Four{});
+    return many ? run(width, One{}, Sixteen{}) : run(width, One{}, Four{});
+  };
+  const int rc = aligned ? sized(Pack{}) : sized(One{});
+  if (rc || !columns) return rc;
+  return launch_columns_finish(a, grid, s);
 }
 
 }  // namespace
@@ -195,18 +556,12 @@ int jn_layer_norm_forward(const void* state, const void* x, const void* weight, 
   if (rows == 0) return kOk;
   JN_REQUIRE(x && y && (!state || state_out), kInvalidArgument, "null tensor pointer");
   const auto s = static_cast<hipStream_t>(stream);
-  return with_type(type, [&](auto* t) -> int {
-    using T = std::remove_pointer_t<decltype(t)>;
-    JN_PROFILE("norm_forward_any_kernel", s);
-    hipLaunchKernelGGL(norm_forward_any_kernel<T>, dim3((unsigned)row_groups(rows)), dim3(kAnyThreads), 0, s, a);
-    JN_LAUNCH_CHECK();
-    return kOk;
-  });
+  return with_type(type, [&](auto* t) -> int { return launch_norm_forward<std::remove_pointer_t<decltype(t)>>(a, s); });
 }
 
 size_t jn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t dim) {
   if (rows < 1 || dim < 1 || dim >= (1LL << 28)) return 0;
-  return (size_t)slab_count(rows) * 2 * dim * sizeof(float);
+  return (size_t)std::min(rows, kMaxParts) * 2 * dim * sizeof(float);  // no more parts or slabs than rows
 }
 
 int jn_layer_norm_backward(const void* state, const void* x, const void* weight, const float* stats,
@@ -228,29 +583,8 @@ int jn_layer_norm_backward(const void* state, const void* x, const void* weight,
   JN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), kWorkspaceTooSmall,
              "layer norm backward needs %zu workspace bytes, got %zu", need, workspace_bytes);
   const auto s = static_cast<hipStream_t>(stream);
-  return with_type(type, [&](auto* t) -> int {
-    using T = std::remove_pointer_t<decltype(t)>;
-    if (grad_x || grad_state) {
-      JN_PROFILE("norm_backward_any_kernel", s);
-      hipLaunchKernelGGL(norm_backward_any_kernel<T>, dim3((unsigned)row_groups(rows)), dim3(kAnyThreads), 0, s, a);
-      JN_LAUNCH_CHECK();
-    }
-    if (columns) {
-      const int64_t slabs = slab_count(rows);
-      const int64_t slab_rows = (rows + slabs - 1) / slabs;
-      {
-        JN_PROFILE("norm_columns_any_kernel", s);
-        hipLaunchKernelGGL(norm_columns_any_kernel<T>, dim3((unsigned)((dim + kWave - 1) / kWave), (unsigned)slabs),
-                           dim3(kAnyThreads), 0, s, a, slab_rows);
-        JN_LAUNCH_CHECK();
-      }
-      JN_PROFILE("norm_columns_finish_kernel", s);
-      hipLaunchKernelGGL(norm_columns_finish_kernel, dim3((unsigned)((dim + kAnyThreads - 1) / kAnyThreads)),
-                         dim3(kAnyThreads), 0, s, a, (int)slabs);
-      JN_LAUNCH_CHECK();
-    }
-    return kOk;
-  });
+  return with_type(type,
+                   [&](auto* t) -> int { return launch_norm_backward<std::remove_pointer_t<decltype(t)>>(a, s); });
 }
 
 }  // extern "C"

@@ -3,6 +3,8 @@
 // in fp32.
 #pragma once
 
+#include <type_traits>
+
 #include "jn_common.hpp"
 
 namespace jakal {
@@ -33,6 +35,42 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, int code, float v)
   else if (code == kTypeBf16) static_cast<bf16_t*>(p)[i] = (bf16_t)v;
   else static_cast<f16_t*>(p)[i] = (f16_t)v;
 }
+
+// W elements of T as one load: 16 bytes, or a single element.
+template <typename T, int W>
+struct Raw {
+  static_assert(W == 1 || W * sizeof(T) == 16, "a pack is one element or 16 bytes");
+  using type = std::conditional_t<W == 1, T, uint4>;
+  type bits;
+
+  __device__ __forceinline__ void load(const T* p) { bits = *reinterpret_cast<const type*>(p); }
+  __device__ __forceinline__ void clear() { bits = type{}; }
+  __device__ __forceinline__ void unpack(float* v) const {
+    if constexpr (W == 1) {
+      v[0] = (float)bits;
+    } else {
+      typedef T vec __attribute__((ext_vector_type(W)));
+      const vec x = __builtin_bit_cast(vec, bits);
+#pragma unroll
+      for (int i = 0; i < W; ++i) v[i] = (float)x[i];
+    }
+  }
+};
+
+template <typename T, int W>
+__device__ __forceinline__ void store_raw(T* p, const float* v) {
+  if constexpr (W == 1) {
+    *p = (T)v[0];
+  } else {
+    typedef T vec __attribute__((ext_vector_type(W)));
+    vec x;
+#pragma unroll
+    for (int i = 0; i < W; ++i) x[i] = (T)v[i];
+    *reinterpret_cast<uint4*>(p) = __builtin_bit_cast(uint4, x);
+  }
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Sum over a workgroup of WAVES waves, the same in every thread (fixed order).
 // `lds` holds WAVES floats and may be reused after the next barrier.

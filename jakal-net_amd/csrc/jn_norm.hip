@@ -61,11 +61,10 @@ __device__ __forceinline__ float param(const void* p, int64_t i, int code, float
 // W elements (16 bytes; single elements where rows do not start on 16), NP packs
 // at most.  A row is read once, and its mean, centred squares and gradient sums
 // come from registers; the next row's packs load while this one is reduced.
-constexpr int kGroupThreads = 256;
-
 template <int W, int NP, int GW>
 struct RowGroup {
   static constexpr int kThreads = GW * kWave;
+  static constexpr int kBlock = (GW > 4 ? GW : 4) * kWave;  // of the forward: four waves, or one group
   static constexpr int kItems = W * NP;  // elements of a thread
 
   __device__ static int thread() { return GW == 1 ? lane_id() : (int)threadIdx.x; }
@@ -113,9 +112,9 @@ __device__ __forceinline__ void load_params(const void* base, int type, int64_t 
 }
 
 template <typename T, int W, int NP, int GW>
-__global__ __launch_bounds__(kGroupThreads) void norm_forward_kernel(NormArgs a) {
+__global__ __launch_bounds__((GW > 4 ? GW : 4) * kWave) void norm_forward_kernel(NormArgs a) {
   using G = RowGroup<W, NP, GW>;
-  constexpr int kGroups = kGroupThreads / G::kThreads;
+  constexpr int kGroups = G::kBlock / G::kThreads;
   __shared__ float lds[GW];
   const int64_t groups = (int64_t)gridDim.x * kGroups;
   const int64_t first = (int64_t)blockIdx.x * kGroups + (GW == 1 ? wave_id() : 0);
@@ -162,8 +161,7 @@ __global__ __launch_bounds__(kGroupThreads) void norm_forward_kernel(NormArgs a)
     }
   }
   if (a.state) {
-    for (int64_t i = (int64_t)blockIdx.x * kGroupThreads + threadIdx.x; i < a.rows;
-         i += (int64_t)gridDim.x * kGroupThreads)
+    for (int64_t i = (int64_t)blockIdx.x * G::kBlock + threadIdx.x; i < a.rows; i += (int64_t)gridDim.x * G::kBlock)
       state_forward(a, i);
   }
 }
@@ -175,7 +173,7 @@ __global__ __launch_bounds__(WPB* kWave) void norm_backward_kernel(NormArgs a) {
   using G = RowGroup<W, NP, GW>;
   constexpr int kThreads = WPB * kWave, kGroups = WPB / GW;
   __shared__ float lds[GW];
-  extern __shared__ float sums[];  // [kGroups][dim]
+  extern __shared__ float sums[];  // [kGroups][dim], at most 32 KB
   const int64_t groups = (int64_t)gridDim.x * kGroups;
   const int64_t first = (int64_t)blockIdx.x * kGroups + (GW == 1 ? wave_id() : 0);
   const float n = (float)a.dim;
@@ -352,9 +350,9 @@ __global__ __launch_bounds__(kAnyThreads) void norm_columns_any_kernel(NormArgs 
   }
 }
 
-// The partial sums of all workgroups or slabs: 32 columns a workgroup, each by
-// 32 threads that take every 32nd partial.
-constexpr int kFinishColumns = 32, kFinishLanes = 32;
+// The partial sums of all workgroups or slabs: 16 columns a workgroup, each by
+// 64 threads that take every 64th partial (512 x 1024 sums in 3.9 us).
+constexpr int kFinishColumns = 16, kFinishLanes = 64;
 __global__ __launch_bounds__(kFinishColumns* kFinishLanes) void norm_columns_finish_kernel(NormArgs a, int parts) {
   __shared__ float lds[kFinishLanes][kFinishColumns + 1];
   const int col = threadIdx.x % kFinishColumns, lane = threadIdx.x / kFinishColumns;
@@ -378,43 +376,56 @@ __global__ __launch_bounds__(kFinishColumns* kFinishLanes) void norm_columns_fin
 // ---- which kernel ---------------------------------------------------------------
 // The register kernels' shapes: packs of 16 bytes where every row and parameter
 // starts on 16, else single elements.  A wave takes rows of up to 16 elements a
-// lane, four waves rows of up to 16 a thread; wider rows take the kernels that
-// pass over memory.
+// lane, four waves rows of up to 16 a thread, sixteen rows of up to 8 a thread
+// (they would not have the registers for more); wider rows take the kernels
+// that pass over memory.
 struct RowShape {
   int width, packs, waves;  // W, NP, GW; packs = 0: none fits
 };
 
 RowShape row_shape(int64_t dim, bool aligned, int elem_bytes) {
   const int w = aligned ? 16 / elem_bytes : 1;
-  for (const int waves : {1, 4}) {
+  for (const int waves : {1, 4, 16}) {
     for (const int items : {4, 8, 16}) {
-      if (items < w) continue;
+      if (items < w || (waves == 16 && items != 8)) continue;
       if (dim <= (int64_t)items * waves * kWave) return {w, items / w, waves};
     }
   }
   return {w, 0, 0};
 }
 
-// Calls f with a shape's packs of W elements as a constant; MOST: the most elements of a thread (8 or 16).
-template <int W, int MOST, typename F>
-int with_packs(int packs, F f) {
-  if constexpr (W <= 4) {
-    if (packs * W == 4) return f(std::integral_constant<int, 4 / W>{});
-  }
-  if constexpr (MOST >= 16) {
-    if (packs * W == 16) return f(std::integral_constant<int, 16 / W>{});
-  }
-  return f(std::integral_constant<int, 8 / W>{});
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// Calls f(W, NP, GW) with a shape's numbers as constants.
+template <int V, typename F>
+int with_shape(const RowShape& s, F f) {
+  const auto packed = [&](auto width) -> int {
+    constexpr int W = decltype(width)::value;
+    const auto grouped = [&](auto waves) -> int {
+      if constexpr (W <= 4) {
+        if (s.packs * W == 4) return f(width, Int<4 / W>{}, waves);
+      }
+      if (s.packs * W == 16) return f(width, Int<16 / W>{}, waves);
+      return f(width, Int<8 / W>{}, waves);
+    };
+    if (s.waves == 16) return f(width, Int<8 / W>{}, Int<16>{});
+    return s.waves == 4 ? grouped(Int<4>{}) : grouped(Int<1>{});
+  };
+  return s.width == 1 ? packed(Int<1>{}) : packed(Int<V>{});
 }
 
-// Workgroups of the backward, each of which leaves one row of partial sums.
+// Waves a workgroup of the backward, and its workgroups, each of which leaves
+// one row of partial sums.  65,536 x 512 bf16 with the join: eight waves and up
+// to 512 workgroups 42 us, sixteen and 512 46, sixteen and 256 43, four and
+// 512 59, four and 1024 44; 8,192 x 512 fp32: 15.9, 19.2, 16.9, 15.7 and 16.4;
+// 4,593 x 383: 13.2, 15.4, 12.8, 13.6 and 14.5.  Fewer rows take four, so that
+// the workgroups fill the CUs.
 constexpr int64_t kMaxParts = 512;
 constexpr int64_t kManyRows = 2048;
 
-// Sixteen waves a workgroup for many rows: fewer partial sums to join.  (At 16
-// elements a lane they would not have the registers.)
 int backward_waves(const RowShape& s, int64_t rows) {
-  return s.waves == 1 && s.width * s.packs <= 8 && rows >= kManyRows ? 16 : 4;
+  return s.waves == 16 ? 16 : s.waves == 1 && rows >= kManyRows ? 8 : 4;
 }
 int64_t backward_groups(const RowShape& s, int64_t rows) {
   const int64_t per = backward_waves(s, rows) / s.waves;
@@ -461,24 +472,15 @@ int launch_norm_forward(const NormArgs& a, hipStream_t s) {
     JN_LAUNCH_CHECK();
     return kOk;
   }
-  const int64_t per = kGroupThreads / kWave / shape.waves;
-  const unsigned grid = (unsigned)std::min<int64_t>((a.rows + per - 1) / per, kForwardGroups);
-  const auto run = [&](auto width, auto waves) {
-    constexpr int W = decltype(width)::value, GW = decltype(waves)::value;
-    return with_packs<W, 16>(shape.packs, [&](auto packs) -> int {
-      JN_PROFILE("norm_forward_kernel", s);
-      hipLaunchKernelGGL((norm_forward_kernel<T, W, decltype(packs)::value, GW>), dim3(grid), dim3(kGroupThreads), 0, s,
-                         a);
-      JN_LAUNCH_CHECK();
-      return kOk;
-    });
-  };
-  constexpr int V = 16 / sizeof(T);
-  using One = std::integral_constant<int, 1>;
-  using Four = std::integral_constant<int, 4>;
-  using Pack = std::integral_constant<int, V>;
-  if (aligned) return shape.waves == 1 ? run(Pack{}, One{}) : run(Pack{}, Four{});
-  return shape.waves == 1 ? run(One{}, One{}) : run(One{}, Four{});
+  return with_shape<16 / sizeof(T)>(shape, [&](auto width, auto packs, auto waves) -> int {
+    constexpr int W = decltype(width)::value, NP = decltype(packs)::value, GW = decltype(waves)::value;
+    constexpr int kBlock = RowGroup<W, NP, GW>::kBlock, per = kBlock / (GW * kWave);
+    const unsigned grid = (unsigned)std::min<int64_t>((a.rows + per - 1) / per, kForwardGroups);
+    JN_PROFILE("norm_forward_kernel", s);
+    hipLaunchKernelGGL((norm_forward_kernel<T, W, NP, GW>), dim3(grid), dim3(kBlock), 0, s, a);
+    JN_LAUNCH_CHECK();
+    return kOk;
+  });
 }
 
 int launch_columns_finish(const NormArgs& a, int64_t parts, hipStream_t s) {
@@ -512,28 +514,19 @@ int launch_norm_backward(NormArgs a, hipStream_t s) {
     return launch_columns_finish(a, slabs, s);
   }
   const int64_t grid = backward_groups(shape, a.rows);
-  const auto run = [&](auto width, auto waves, auto block) {
-    constexpr int W = decltype(width)::value, GW = decltype(waves)::value, WPB = decltype(block)::value;
-    const size_t lds = a.partial && WPB > GW ? (size_t)(WPB / GW) * a.dim * sizeof(float) : 0;
-    return with_packs<W, WPB == 16 ? 8 : 16>(shape.packs, [&](auto packs) -> int {
+  const int rc = with_shape<16 / sizeof(T)>(shape, [&](auto width, auto packs, auto waves) -> int {
+    constexpr int W = decltype(width)::value, NP = decltype(packs)::value, GW = decltype(waves)::value;
+    const auto run = [&](auto block) -> int {
+      constexpr int WPB = decltype(block)::value;
+      const size_t lds = a.partial && WPB > GW ? (size_t)(WPB / GW) * a.dim * sizeof(float) : 0;
       JN_PROFILE("norm_backward_kernel", s);
-      hipLaunchKernelGGL((norm_backward_kernel<T, W, decltype(packs)::value, GW, WPB>), dim3((unsigned)grid),
-                         dim3(WPB * kWave), lds, s, a);
+      hipLaunchKernelGGL((norm_backward_kernel<T, W, NP, GW, WPB>), dim3((unsigned)grid), dim3(WPB * kWave), lds, s, a);
       JN_LAUNCH_CHECK();
       return kOk;
-    });
-  };
-  constexpr int V = 16 / sizeof(T);
-  using One = std::integral_constant<int, 1>;
-  using Four = std::integral_constant<int, 4>;
-  using Sixteen = std::integral_constant<int, 16>;
-  using Pack = std::integral_constant<int, V>;
-  const bool many = backward_waves(shape, a.rows) == 16;
-  const auto sized = [&](auto width) {
-    if (shape.waves == 4) return run(width, Four{}, Four{});
-    return many ? run(width, One{}, Sixteen{}) : run(width, One{}, Four{});
-  };
-  const int rc = aligned ? sized(Pack{}) : sized(One{});
+    };
+    if constexpr (GW == 1) return backward_waves(shape, a.rows) == 8 ? run(Int<8>{}) : run(Int<4>{});
+    else return run(Int<GW>{});
+  });
   if (rc || !columns) return rc;
   return launch_columns_finish(a, grid, s);
 }

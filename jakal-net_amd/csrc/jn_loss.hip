@@ -16,8 +16,6 @@
 namespace jakal {
 namespace {
 
-constexpr int kLossThreads = 256;
-constexpr int kLossWaves = kLossThreads / kWave;
 constexpr int kNone = 0, kMean = 2;  // reductions (1: sum)
 
 struct LossArgs {
@@ -33,41 +31,121 @@ struct LossArgs {
   void* dz;
 };
 
-// Maximum over a workgroup, the same in every thread.
-__device__ __forceinline__ float group_max(float v, float* lds) {
-  v = wave_max_f(v);
-  __syncthreads();
-  if (lane_id() == 0) lds[wave_id()] = v;
-  __syncthreads();
-  float m = lds[0];
+// A row's elements as its memory has them: whole aligned packs of W elements,
+// and up to W - 1 single ones on either side, so that rows may start anywhere
+// (an odd vocabulary) and still move 16 bytes a lane.
+template <typename T>
+struct RowSpan {
+  static constexpr int W = 16 / sizeof(T);
+  int head, tail;  // single elements before and after the packs
+  int packs;
+  int64_t n;
+
+  __device__ RowSpan(const T* row, int64_t classes) : n(classes) {
+    const int off = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+    head = classes < off ? (int)classes : off;
+    packs = (int)((classes - head) / W);
+    tail = (int)(classes - head - (int64_t)packs * W);
+  }
+  // the single element that thread t takes, or -1: the head's by the first threads, the tail's by those from 32
+  __device__ int64_t single(int t) const {
+    if (t < head) return t;
+    return t >= 32 && t - 32 < tail ? n - tail + t - 32 : -1;
+  }
+  __device__ int64_t element(int pack) const { return head + (int64_t)pack * W; }
+};
+
+// A running maximum m and the sum s of exponentials below it.  s is 0 under a
+// maximum of -inf, and NaN once a NaN or +inf was met.
+struct LogSum {
+  float m = -INFINITY, s = 0.f;
+
+  __device__ __forceinline__ void join(float m2, float s2) {
+    const float top = fmaxf(m, m2);
+    s = (m == top ? s : s * __expf(m - top)) + (m2 == top ? s2 : s2 * __expf(m2 - top));
+    m = top;
+  }
+  __device__ __forceinline__ void add(float z) { join(fmaxf(z, -INFINITY), z == -INFINITY ? 0.f : __expf(z - z)); }
+};
+
+// One row by THREADS threads: each reads its packs kPacks at a time, takes their
+// maximum and then their exponentials from registers (one rescaling of its sum
+// for 16 kPacks bytes); the threads' pairs join at the end, in every thread.
+constexpr int kPacks = 8;
+template <typename T, int THREADS>
+__device__ __forceinline__ LogSum row_log_sum(const T* z, int64_t classes, float (*lds)[2]) {
+  constexpr int W = RowSpan<T>::W, kWaves = THREADS / kWave;
+  const int t = THREADS == kWave ? lane_id() : (int)threadIdx.x;
+  const RowSpan<T> span(z, classes);
+  LogSum sum;
+  const int64_t one = span.single(t);
+  if (one >= 0) sum.add((float)z[one]);
+  for (int first = t; first < span.packs; first += THREADS * kPacks) {
+    Raw<T, W> raw[kPacks];
 #pragma unroll
-  for (int i = 1; i < kLossWaves; ++i) m = fmaxf(m, lds[i]);
-  return m;
+    for (int i = 0; i < kPacks; ++i) {
+      if (first + i * THREADS < span.packs) raw[i].load(z + span.element(first + i * THREADS));
+    }
+    float m = sum.m;
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) {
+      if (first + i * THREADS >= span.packs) continue;
+      float v[W];
+      raw[i].unpack(v);
+#pragma unroll
+      for (int j = 0; j < W; ++j) m = fmaxf(m, v[j]);
+    }
+    const float base = m == -INFINITY ? 0.f : m;  // exp(-inf - 0) = 0
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) {
+      if (first + i * THREADS >= span.packs) continue;
+      float v[W];
+      raw[i].unpack(v);
+#pragma unroll
+      for (int j = 0; j < W; ++j) s += __expf(v[j] - base);
+    }
+    sum.join(m, s);
+  }
+  const float top = wave_max_f(sum.m);
+  sum.s = wave_sum(sum.m == top ? sum.s : sum.s * __expf(sum.m - top));
+  sum.m = top;
+  if constexpr (kWaves > 1) {
+    __syncthreads();  // an earlier row's readers are done
+    if (lane_id() == 0) {
+      lds[wave_id()][0] = sum.m;
+      lds[wave_id()][1] = sum.s;
+    }
+    __syncthreads();
+    sum = LogSum{};
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) sum.join(lds[i][0], lds[i][1]);
+  }
+  return sum;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kLossThreads) void loss_forward_any_kernel(LossArgs a) {
-  __shared__ float lds[kLossWaves];
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+// THREADS = 64: a wave a row, four rows a workgroup; else a workgroup a row.
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS == kWave ? 4 * kWave : THREADS) void loss_forward_kernel(LossArgs a) {
+  constexpr int kRows = THREADS == kWave ? 4 : 1;
+  __shared__ float lds[THREADS / kWave][2];
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  for (int64_t row = (int64_t)blockIdx.x * kRows + (kRows > 1 ? wave_id() : 0); row < a.rows; row += step) {
     const int64_t t = a.target[row];
+    const bool writes = (THREADS == kWave ? lane_id() : (int)threadIdx.x) == 0;
     if (t == a.ignore) {
-      if (threadIdx.x == 0) a.loss[row] = 0.f;
+      if (writes) a.loss[row] = 0.f;
       continue;
     }
     const T* z = static_cast<const T*>(a.z) + row * a.classes;
-    float m = -INFINITY;
-    for (int64_t i = threadIdx.x; i < a.classes; i += kLossThreads) m = fmaxf(m, (float)z[i]);
-    m = group_max(m, lds);
-    // a NaN logit, +inf, or a row of -inf alone makes the sum NaN
-    float s = 0.f;
-    for (int64_t i = threadIdx.x; i < a.classes; i += kLossThreads) s += expf((float)z[i] - m);
-    s = group_sum<kLossWaves>(s, lds);
-    if (threadIdx.x == 0) {
-      const float l = logf(s);
-      const bool inside = t >= 0 && t < a.classes;
-      a.loss[row] = inside ? l + (m - (float)z[t]) : NAN;
+    const bool inside = t >= 0 && t < a.classes;
+    const float zt = inside ? (float)z[t] : NAN;
+    const LogSum sum = row_log_sum<T, THREADS>(z, a.classes, lds);
+    if (writes) {
+      const float l = logf(sum.s);
+      a.loss[row] = l + (sum.m - zt);
       if (a.stats) {
-        a.stats[2 * row] = m;
+        a.stats[2 * row] = sum.m;
         a.stats[2 * row + 1] = inside ? l : NAN;
       }
     }
@@ -76,47 +154,96 @@ __global__ __launch_bounds__(kLossThreads) void loss_forward_any_kernel(LossArgs
 
 // The sum or mean of the rows' losses, and how many rows count (one workgroup;
 // sums in 64 bits, each thread its rows in order).
-constexpr int kReduceThreads = 1024;
+constexpr int kReduceThreads = 1024, kReduceWaves = kReduceThreads / kWave;
 __global__ __launch_bounds__(kReduceThreads) void loss_reduce_kernel(LossArgs a) {
-  __shared__ double sums[kReduceThreads];
-  __shared__ double counts[kReduceThreads];
+  __shared__ double lds[kReduceWaves][2];
   double s = 0.0, n = 0.0;
+#pragma unroll 4
   for (int64_t row = threadIdx.x; row < a.rows; row += kReduceThreads) {
     s += a.loss[row];
     n += a.target[row] != a.ignore ? 1.0 : 0.0;
   }
-  sums[threadIdx.x] = s;
-  counts[threadIdx.x] = n;
-  for (int step = kReduceThreads / 2; step > 0; step /= 2) {
-    __syncthreads();
-    if (threadIdx.x < step) {
-      sums[threadIdx.x] += sums[threadIdx.x + step];
-      counts[threadIdx.x] += counts[threadIdx.x + step];
-    }
+  for (int step = 1; step < kWave; step *= 2) {
+    s += __shfl_xor(s, step);
+    n += __shfl_xor(n, step);
   }
+  if (lane_id() == 0) {
+    lds[wave_id()][0] = s;
+    lds[wave_id()][1] = n;
+  }
+  __syncthreads();
   if (threadIdx.x == 0) {
+    s = n = 0.0;
+    for (int i = 0; i < kReduceWaves; ++i) {
+      s += lds[i][0];
+      n += lds[i][1];
+    }
     // no counted row: 0 / 0 = NaN for the mean, as its definition has it
-    *a.reduced = (float)(a.reduction == kMean ? sums[0] / counts[0] : sums[0]);
-    *a.count = (float)counts[0];
+    *a.reduced = (float)(a.reduction == kMean ? s / n : s);
+    *a.count = (float)n;
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kLossThreads) void loss_backward_any_kernel(LossArgs a) {
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+// The gradient of a stretch of a row: kPacks packs a thread (and the row's
+// single elements, with its first stretch).  W = 1 where the gradient's rows do
+// not start on 16 bytes where the logits' do.
+template <typename T, int W>
+__device__ __forceinline__ void loss_gradient(const T* z, T* dz, int64_t e, int64_t t, float m, float l, float c,
+                                              const Raw<T, W>& raw) {
+  float v[W];
+  raw.unpack(v);
+#pragma unroll
+  for (int j = 0; j < W; ++j) v[j] = __expf((v[j] - m) - l);
+  const int64_t hot = t - e;
+  if (hot >= 0 && hot < W) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] -= j == hot ? 1.0f : 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < W; ++j) v[j] *= c;
+  store_raw<T, W>(dz + e, v);
+}
+
+template <typename T, int THREADS, bool PACKED>
+__global__ __launch_bounds__(THREADS == kWave ? 4 * kWave : THREADS) void loss_backward_kernel(LossArgs a) {
+  constexpr int kRows = THREADS == kWave ? 4 : 1;
+  constexpr int W = PACKED ? RowSpan<T>::W : 1;
+  constexpr int64_t kStretch = (int64_t)THREADS * kPacks;
+  const int thread = THREADS == kWave ? lane_id() : (int)threadIdx.x;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  for (int64_t row = (int64_t)blockIdx.x * kRows + (kRows > 1 ? wave_id() : 0); row < a.rows; row += step) {
     const int64_t t = a.target[row];
     const T* z = static_cast<const T*>(a.z) + row * a.classes;
     T* dz = static_cast<T*>(a.dz) + row * a.classes;
-    if (t == a.ignore) {
-      for (int64_t i = threadIdx.x; i < a.classes; i += kLossThreads) dz[i] = (T)0.0f;
-      continue;
+    const bool ignored = t == a.ignore;
+    const float m = ignored ? 0.f : a.stats[2 * row], l = ignored ? 0.f : a.stats[2 * row + 1];
+    float c = ignored ? 0.f : a.grad[a.reduction == kNone ? row : 0];
+    if (!ignored && a.reduction == kMean) c /= *a.count;
+    const RowSpan<T> span(z, a.classes);
+    const int64_t packs = PACKED ? span.packs : a.classes, head = PACKED ? span.head : 0;
+    if (PACKED && blockIdx.y == 0) {
+      const int64_t one = span.single(thread);
+      if (one >= 0) {
+        Raw<T, 1> raw;
+        if (ignored) dz[one] = (T)0.0f;
+        else raw.load(z + one), loss_gradient<T, 1>(z, dz, one, t, m, l, c, raw);
+      }
     }
-    const float m = a.stats[2 * row], l = a.stats[2 * row + 1];
-    float c = a.grad[a.reduction == kNone ? row : 0];
-    if (a.reduction == kMean) c /= *a.count;
-    for (int64_t i = threadIdx.x; i < a.classes; i += kLossThreads) {
-      const float p = expf(((float)z[i] - m) - l);
-      dz[i] = (T)((p - (i == t ? 1.0f : 0.0f)) * c);
+    for (int64_t first = blockIdx.y * kStretch + thread; first < packs; first += gridDim.y * kStretch) {
+      Raw<T, W> raw[kPacks];
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i) {
+        const int64_t p = first + i * THREADS;
+        if (p < packs && !ignored) raw[i].load(z + head + p * W);
+        else raw[i].clear();
+      }
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i) {
+        const int64_t p = first + i * THREADS;
+        if (p >= packs) continue;
+        if (ignored) *reinterpret_cast<typename Raw<T, W>::type*>(dz + head + p * W) = raw[i].bits;
+        else loss_gradient<T, W>(z, dz, head + p * W, t, m, l, c, raw[i]);
+      }
     }
   }
 }
@@ -133,7 +260,42 @@ int check_loss(const LossArgs& a, int32_t type) {
   return kOk;
 }
 
-unsigned loss_groups(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 1 << 20); }
+// Rows of up to kWaveClasses take a wave each; longer ones a workgroup, of 1024
+// threads where there are too few rows to fill the CUs otherwise.
+constexpr int64_t kWaveClasses = 1024;
+constexpr int64_t kFewRows = 512;
+
+template <typename T>
+int launch_loss_forward(const LossArgs& a, hipStream_t s) {
+  JN_PROFILE("loss_forward_kernel", s);
+  if (a.classes <= kWaveClasses) {
+    const unsigned grid = (unsigned)std::min<int64_t>((a.rows + 3) / 4, 1 << 20);
+    hipLaunchKernelGGL((loss_forward_kernel<T, kWave>), dim3(grid), dim3(4 * kWave), 0, s, a);
+  } else if (a.rows < kFewRows) {
+    hipLaunchKernelGGL((loss_forward_kernel<T, 1024>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);
+  } else {
+    const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 1 << 20);
+    hipLaunchKernelGGL((loss_forward_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
+  }
+  JN_LAUNCH_CHECK();
+  return kOk;
+}
+
+template <typename T, bool PACKED>
+int launch_loss_backward(const LossArgs& a, hipStream_t s) {
+  JN_PROFILE("loss_backward_kernel", s);
+  if (a.classes <= kWaveClasses) {
+    const unsigned grid = (unsigned)std::min<int64_t>((a.rows + 3) / 4, 1 << 20);
+    hipLaunchKernelGGL((loss_backward_kernel<T, kWave, PACKED>), dim3(grid), dim3(4 * kWave), 0, s, a);
+  } else {
+    const int64_t stretch = 256 * kPacks * (PACKED ? RowSpan<T>::W : 1);
+    const unsigned parts = (unsigned)std::min<int64_t>((a.classes + stretch - 1) / stretch, 1024);
+    const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 1 << 20);
+    hipLaunchKernelGGL((loss_backward_kernel<T, 256, PACKED>), dim3(grid, parts), dim3(256), 0, s, a);
+  }
+  JN_LAUNCH_CHECK();
+  return kOk;
+}
 
 }  // namespace
 }  // namespace jakal
@@ -152,13 +314,8 @@ int jn_cross_entropy_forward(const void* logits, const int64_t* target, int64_t 
   if (const int rc = check_loss(a, type)) return rc;
   JN_REQUIRE(logits && target && loss && ((reduced && count) || reduction == kNone), kInvalidArgument, "null tensor pointer");
   const auto s = static_cast<hipStream_t>(stream);
-  const int rc = with_type(type, [&](auto* t) -> int {
-    using T = std::remove_pointer_t<decltype(t)>;
-    JN_PROFILE("loss_forward_any_kernel", s);
-    hipLaunchKernelGGL(loss_forward_any_kernel<T>, dim3(loss_groups(rows)), dim3(kLossThreads), 0, s, a);
-    JN_LAUNCH_CHECK();
-    return kOk;
-  });
+  const int rc = with_type(
+      type, [&](auto* t) -> int { return launch_loss_forward<std::remove_pointer_t<decltype(t)>>(a, s); });
   if (rc || reduction == kNone) return rc;
   JN_PROFILE("loss_reduce_kernel", s);
   hipLaunchKernelGGL(loss_reduce_kernel, dim3(1), dim3(kReduceThreads), 0, s, a);
@@ -177,12 +334,11 @@ int jn_cross_entropy_backward(const void* logits, const int64_t* target, const f
   JN_REQUIRE(logits && target && stats && grad_loss && grad_logits && (count || reduction != kMean),
              kInvalidArgument, "null tensor pointer");
   const auto s = static_cast<hipStream_t>(stream);
+  const bool packed =
+      ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(grad_logits)) & 15) == 0;
   return with_type(type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
-    JN_PROFILE("loss_backward_any_kernel", s);
-    hipLaunchKernelGGL(loss_backward_any_kernel<T>, dim3(loss_groups(rows)), dim3(kLossThreads), 0, s, a);
-    JN_LAUNCH_CHECK();
-    return kOk;
+    return packed ? launch_loss_backward<T, true>(a, s) : launch_loss_backward<T, false>(a, s);
   });
 }
 

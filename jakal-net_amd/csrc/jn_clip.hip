@@ -21,28 +21,36 @@ namespace jakal {
 namespace {
 
 constexpr int kClipThreads = 256;
-constexpr int kChunk = 4096;         // elements
-constexpr int kListMax = 140;        // tensors of one launch (4 KB of kernel arguments)
+constexpr int kChunk = 8192;         // elements
+constexpr int kListMax = 164;        // tensors of one launch (4 KB of kernel arguments)
 constexpr int64_t kMaxPartials = 2048;
 
 struct TensorList {
   const void* in[kListMax];
   void* out[kListMax];
-  int64_t size[kListMax];  // elements << 8 | output type << 4 | input type
-  int32_t first[kListMax]; // first chunk
-  int32_t count, chunks;
+  int32_t first[kListMax + 1];  // first chunk; behind the last tensor, all chunks
+  int32_t last[kListMax];       // elements of the last chunk | type << 16 | output type << 20
+  int32_t count;
 };
 static_assert(sizeof(TensorList) <= 4000, "kernel arguments stay within 4 KB");
 
-// The tensor that holds a chunk (uniform binary search).
-__device__ __forceinline__ int tensor_of(const TensorList& l, int chunk) {
+struct Chunk {
+  int tensor;
+  int64_t begin;
+  int size, type, out_type;
+};
+
+// A chunk's place (a uniform binary search for its tensor).
+__device__ __forceinline__ Chunk chunk_at(const TensorList& l, int c) {
   int lo = 0, hi = l.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
-    if (l.first[mid] <= chunk) lo = mid;
+    if (l.first[mid] <= c) lo = mid;
     else hi = mid - 1;
   }
-  return lo;
+  const int meta = l.last[lo];
+  return {lo, (int64_t)(c - l.first[lo]) * kChunk, c + 1 == l.first[lo + 1] ? meta & 0xffff : kChunk,
+          meta >> 16 & 15, meta >> 20};
 }
 
 // max that keeps a NaN
@@ -64,19 +72,49 @@ __device__ double group_join(double v, double* lds) {
   return lds[0];
 }
 
+// A chunk's part of a norm: 16-byte packs where the tensor starts on 16 bytes
+// (chunks are whole packs; the last one ends in single elements), else elements.
+template <bool MAX, typename T>
+__device__ __forceinline__ double chunk_norm(const T* p, int n, double s) {
+  constexpr int W = 16 / sizeof(T), kUnroll = kChunk / W / kClipThreads;
+  const auto take = [&](float v) {
+    const double d = v;
+    s = MAX ? max_nan(s, fabs(d)) : s + d * d;
+  };
+  int done = 0;
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    const int packs = n / W;
+    Raw<T, W> raw[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int k = i * kClipThreads + (int)threadIdx.x;
+      if (k < packs) raw[i].load(p + k * W);
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      if (i * kClipThreads + (int)threadIdx.x >= packs) continue;
+      float v[W];
+      raw[i].unpack(v);
+#pragma unroll
+      for (int j = 0; j < W; ++j) take(v[j]);
+    }
+    done = packs * W;
+  }
+#pragma unroll 8
+  for (int i = done + (int)threadIdx.x; i < n; i += kClipThreads) take((float)p[i]);
+  return s;
+}
+
 template <bool MAX>
 __global__ __launch_bounds__(kClipThreads) void grads_norm_kernel(TensorList l, double* partial) {
   __shared__ double lds[kClipThreads];
   double s = 0.0;
-  for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) {
-    const int t = tensor_of(l, c);
-    const int64_t begin = (int64_t)(c - l.first[t]) * kChunk;
-    const int64_t size = l.size[t] >> 8, end = begin + kChunk < size ? begin + kChunk : size;
-    const int type = (int)(l.size[t] & 15);
-    for (int64_t i = begin + threadIdx.x; i < end; i += kClipThreads) {
-      const double v = load_any(l.in[t], i, type);
-      s = MAX ? max_nan(s, fabs(v)) : s + v * v;
-    }
+  for (int i = blockIdx.x; i < l.first[l.count]; i += gridDim.x) {
+    const Chunk c = chunk_at(l, i);
+    const void* in = l.in[c.tensor];
+    if (c.type == kTypeF32) s = chunk_norm<MAX>(static_cast<const float*>(in) + c.begin, c.size, s);
+    else if (c.type == kTypeBf16) s = chunk_norm<MAX>(static_cast<const bf16_t*>(in) + c.begin, c.size, s);
+    else s = chunk_norm<MAX>(static_cast<const f16_t*>(in) + c.begin, c.size, s);
   }
   s = group_join<MAX>(s, lds);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
@@ -97,9 +135,50 @@ __global__ __launch_bounds__(kClipThreads) void grads_norm_finish_kernel(const d
   if (threadIdx.x == 0) *norm = (float)s;
 }
 
+// A chunk times the factor, in packs that are 16 bytes of the wider type, so
+// that loads and stores both run through memory without gaps; the tensors have
+// to start on 16 bytes for that, else element by element.
+template <bool STREAM, typename TI, typename TO>
+__device__ __forceinline__ void chunk_scale(const TI* p, TO* o, int n, float scale) {
+  constexpr int W = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO));
+  constexpr int kUnroll = 8;  // packs in flight
+  int done = 0;
+  if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
+    const int packs = n / W;
+    for (int first = threadIdx.x; first < packs; first += kUnroll * kClipThreads) {
+      Raw<TI, W> raw[kUnroll];
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) {
+        const int k = first + i * kClipThreads;
+        if (k < packs) raw[i].template load<STREAM>(p + k * W);
+      }
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) {
+        const int k = first + i * kClipThreads;
+        if (k >= packs) continue;
+        float v[W];
+        raw[i].unpack(v);
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] *= scale;
+        store_raw<TO, W, STREAM>(o + k * W, v);
+      }
+    }
+    done = packs * W;
+  }
+#pragma unroll 8
+  for (int i = done + (int)threadIdx.x; i < n; i += kClipThreads) o[i] = (TO)(scale * (float)p[i]);
+}
+
+template <bool STREAM, typename TI>
+__device__ __forceinline__ void chunk_scale_to(const TI* p, void* out, int64_t begin, int n, int type, float scale) {
+  if (type == kTypeF32) chunk_scale<STREAM>(p, static_cast<float*>(out) + begin, n, scale);
+  else if (type == kTypeBf16) chunk_scale<STREAM>(p, static_cast<bf16_t*>(out) + begin, n, scale);
+  else chunk_scale<STREAM>(p, static_cast<f16_t*>(out) + begin, n, scale);
+}
+
 // Every workgroup joins the norm's partials (at most kMaxPartials, in one
 // order) rather than wait for a launch that does; the first writes the norm.
-template <bool MAX>
+template <bool MAX, bool STREAM>
 __global__ __launch_bounds__(kClipThreads) void grads_scale_kernel(TensorList l, const double* partial, int n,
                                                                    double max_norm, float* norm) {
   __shared__ double lds[kClipThreads];
@@ -107,14 +186,17 @@ __global__ __launch_bounds__(kClipThreads) void grads_scale_kernel(TensorList l,
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
   const double ratio = max_norm / (total + 1e-6);
   const float scale = ratio < 1.0 || ratio != ratio ? (float)ratio : 1.0f;
-  for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) {
-    const int t = tensor_of(l, c);
-    if (scale == 1.0f && l.in[t] == l.out[t]) continue;  // unchanged in place
-    const int64_t begin = (int64_t)(c - l.first[t]) * kChunk;
-    const int64_t size = l.size[t] >> 8, end = begin + kChunk < size ? begin + kChunk : size;
-    const int in_type = (int)(l.size[t] & 15), out_type = (int)(l.size[t] >> 4 & 15);
-    for (int64_t i = begin + threadIdx.x; i < end; i += kClipThreads)
-      store_any(l.out[t], i, out_type, scale * load_any(l.in[t], i, in_type));
+  for (int i = blockIdx.x; i < l.first[l.count]; i += gridDim.x) {
+    const Chunk c = chunk_at(l, i);
+    const void* in = l.in[c.tensor];
+    void* out = l.out[c.tensor];
+    if (scale == 1.0f && in == out) continue;  // unchanged in place
+    if (c.type == kTypeF32)
+      chunk_scale_to<STREAM>(static_cast<const float*>(in) + c.begin, out, c.begin, c.size, c.out_type, scale);
+    else if (c.type == kTypeBf16)
+      chunk_scale_to<STREAM>(static_cast<const bf16_t*>(in) + c.begin, out, c.begin, c.size, c.out_type, scale);
+    else
+      chunk_scale_to<STREAM>(static_cast<const f16_t*>(in) + c.begin, out, c.begin, c.size, c.out_type, scale);
   }
 }
 
@@ -128,15 +210,15 @@ struct ListCursor {
   int64_t n, at = 0;
 
   bool next(TensorList& l) {
-    l.count = l.chunks = 0;
+    l.count = l.first[0] = 0;
     for (; at < n && l.count < kListMax; ++at) {
       const int64_t chunks = (counts[at] + kChunk - 1) / kChunk;
       if (chunks == 0) continue;
       l.in[l.count] = in[at];
       l.out[l.count] = out ? out[at] : nullptr;
-      l.size[l.count] = counts[at] << 8 | (out ? out_types[at] : 0) << 4 | types[at];
-      l.first[l.count++] = l.chunks;
-      l.chunks += (int32_t)chunks;
+      l.last[l.count] = (int32_t)(counts[at] - (chunks - 1) * kChunk) | types[at] << 16 | (out ? out_types[at] : 0) << 20;
+      l.first[l.count + 1] = l.first[l.count] + (int32_t)chunks;
+      ++l.count;
     }
     return l.count > 0;
   }
@@ -159,7 +241,7 @@ int check_list(const void* const* in, void* const* out, const int64_t* counts, c
     JN_REQUIRE(!clip || counts[i] == 0 || in[i] != out[i] || types[i] == out_types[i], kInvalidArgument,
                "tensor %lld: in place its element type stays", (long long)i);
     chunks += (counts[i] + kChunk - 1) / kChunk;
-    JN_REQUIRE(chunks < (1LL << 31), kUnsupported, "at most 2^43 elements in all");
+    JN_REQUIRE(chunks < (1LL << 31), kUnsupported, "at most 2^44 elements in all");
   }
   return kOk;
 }
@@ -201,8 +283,8 @@ int64_t total_chunks(const int64_t* counts, int64_t n) {
 
 // Workgroups of a launch: its share of kMaxPartials.
 int list_groups(const TensorList& l, int64_t total) {
-  if (total <= kMaxPartials) return l.chunks;
-  return (int)std::max<int64_t>(1, l.chunks * kMaxPartials / total);
+  const int64_t chunks = l.first[l.count];
+  return (int)(total <= kMaxPartials ? chunks : std::max<int64_t>(1, chunks * kMaxPartials / total));
 }
 
 // Launches that a list of n tensors may need; one partial at least for each.
@@ -234,10 +316,15 @@ int launch_clip(ListCursor c, int64_t total, double max_norm, float* norm, doubl
     JN_LAUNCH_CHECK();
     return kOk;
   }
+  // what is read and written (in place: written where it was read)
+  int64_t bytes = 0;
+  for (int64_t i = 0; i < c.n; ++i)
+    bytes += c.counts[i] * (type_bytes(c.types[i]) + (c.in[i] == c.out[i] ? 0 : type_bytes(c.out_types[i])));
+  const auto kernel = bytes > kCacheBytes ? grads_scale_kernel<MAX, true> : grads_scale_kernel<MAX, false>;
   do {
     JN_PROFILE("grads_scale_kernel", s);
-    hipLaunchKernelGGL(grads_scale_kernel<MAX>, dim3(list_groups(l, total)), dim3(kClipThreads), 0, s, l, partial,
-                       found, max_norm, norm);
+    hipLaunchKernelGGL(kernel, dim3(list_groups(l, total)), dim3(kClipThreads), 0, s, l, partial, found, max_norm,
+                       norm);
     JN_LAUNCH_CHECK();
     norm = nullptr;
   } while (c.next(l));

@@ -36,14 +36,26 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, int code, float v)
   else static_cast<f16_t*>(p)[i] = (f16_t)v;
 }
 
-// W elements of T as one load: 16 bytes, or a single element.
+// W elements of T as one access: 16 or 8 bytes, or a single element.  STREAM:
+// non-temporal, for data that the caches would not hold until its next use.
 template <typename T, int W>
 struct Raw {
-  static_assert(W == 1 || W * sizeof(T) == 16, "a pack is one element or 16 bytes");
-  using type = std::conditional_t<W == 1, T, uint4>;
+  static_assert(W == 1 || W * sizeof(T) == 16 || W * sizeof(T) == 8, "a pack is one element, 8 or 16 bytes");
+  using type = std::conditional_t<W == 1, T, std::conditional_t<W * sizeof(T) == 16, uint4, uint2>>;
   type bits;
 
-  __device__ __forceinline__ void load(const T* p) { bits = *reinterpret_cast<const type*>(p); }
+  template <bool STREAM = false>
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (STREAM && W * sizeof(T) == 16) bits = load_nt16(p);
+    else if constexpr (STREAM && W * sizeof(T) == 8 && W > 1) bits = load_nt8(p);
+    else bits = *reinterpret_cast<const type*>(p);
+  }
+  template <bool STREAM = false>
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (STREAM && W * sizeof(T) == 16) store_nt16(p, bits);
+    else if constexpr (STREAM && W * sizeof(T) == 8 && W > 1) store_nt8(p, bits);
+    else *reinterpret_cast<type*>(p) = bits;
+  }
   __device__ __forceinline__ void clear() { bits = type{}; }
   __device__ __forceinline__ void unpack(float* v) const {
     if constexpr (W == 1) {
@@ -55,20 +67,28 @@ struct Raw {
       for (int i = 0; i < W; ++i) v[i] = (float)x[i];
     }
   }
+  __device__ __forceinline__ void pack(const float* v) {
+    if constexpr (W == 1) {
+      bits = (T)v[0];
+    } else {
+      typedef T vec __attribute__((ext_vector_type(W)));
+      vec x;
+#pragma unroll
+      for (int i = 0; i < W; ++i) x[i] = (T)v[i];
+      bits = __builtin_bit_cast(type, x);
+    }
+  }
 };
 
-template <typename T, int W>
+template <typename T, int W, bool STREAM = false>
 __device__ __forceinline__ void store_raw(T* p, const float* v) {
-  if constexpr (W == 1) {
-    *p = (T)v[0];
-  } else {
-    typedef T vec __attribute__((ext_vector_type(W)));
-    vec x;
-#pragma unroll
-    for (int i = 0; i < W; ++i) x[i] = (T)v[i];
-    *reinterpret_cast<uint4*>(p) = __builtin_bit_cast(uint4, x);
-  }
+  Raw<T, W> raw;
+  raw.pack(v);
+  raw.template store<STREAM>(p);
 }
+
+// The card's last-level cache: calls that move more than it holds stream.
+constexpr int64_t kCacheBytes = 256LL << 20;
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

@@ -219,9 +219,8 @@ def run(state):
 
 
 def _jakal():
-    root = str(Path(__file__).resolve().parents[1] / "jakal-net_amd")
-    if root not in sys.path:
-        sys.path.insert(0, root)
+    if "jakal_net" not in sys.modules:
+        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "jakal-net_amd"))
     import jakal_net
 
     return jakal_net

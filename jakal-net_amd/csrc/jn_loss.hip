@@ -260,15 +260,28 @@ int check_loss(const LossArgs& a, int32_t type) {
   return kOk;
 }
 
-// Rows of up to kWaveClasses take a wave each; longer ones a workgroup, of 1024
-// threads where there are too few rows to fill the CUs otherwise.
+// Rows of up to kWaveClasses take a wave each; so do rows of up to `chunks` times
+// a wave's kPacks packs a lane where they are many.  Longer ones take a
+// workgroup, in the forward of 1024 threads where there are too few rows to fill
+// the CUs otherwise.  8,192 rows, wave against workgroup, forward and backward:
+// 1,100 bf16 12.6 and 11.8 us against 26.4 and 19.2, 4,096 bf16 19.9 and 28.6
+// against 32.8 and 29.8, 8,192 bf16 31.0 and 56.7 against 38.3 and 48.9 (two
+// chunks); fp32 2,048 17.6 and 28.0 against 20.8 and 28.1, 4,099 30.3 and 56.9
+// against 28.2 and 47.5 (two chunks); at 1,024 rows they are equal.
 constexpr int64_t kWaveClasses = 1024;
+constexpr int64_t kWaveRows = 1024;
 constexpr int64_t kFewRows = 512;
+
+template <typename T>
+bool wave_rows(const LossArgs& a, int chunks) {
+  return a.classes <= kWaveClasses ||
+         (a.rows >= kWaveRows && a.classes <= (int64_t)chunks * kWave * kPacks * RowSpan<T>::W);
+}
 
 template <typename T>
 int launch_loss_forward(const LossArgs& a, hipStream_t s) {
   JN_PROFILE("loss_forward_kernel", s);
-  if (a.classes <= kWaveClasses) {
+  if (wave_rows<T>(a, 4 / sizeof(T))) {
     const unsigned grid = (unsigned)std::min<int64_t>((a.rows + 3) / 4, 1 << 20);
     hipLaunchKernelGGL((loss_forward_kernel<T, kWave>), dim3(grid), dim3(4 * kWave), 0, s, a);
   } else if (a.rows < kFewRows) {
@@ -283,16 +296,17 @@ int launch_loss_forward(const LossArgs& a, hipStream_t s) {
 
 template <typename T, bool PACKED>
 int launch_loss_backward(const LossArgs& a, hipStream_t s) {
+  // the logits are read for the last time, and neither they nor the gradient stay in the cache
+  const bool stream = 2 * a.rows * a.classes * (int64_t)sizeof(T) > kCacheBytes;
   JN_PROFILE("loss_backward_kernel", s);
-  if (a.classes <= kWaveClasses) {
+  if (wave_rows<T>(a, 1)) {
     const unsigned grid = (unsigned)std::min<int64_t>((a.rows + 3) / 4, 1 << 20);
-    hipLaunchKernelGGL((loss_backward_kernel<T, kWave, PACKED, false>), dim3(grid), dim3(4 * kWave), 0, s, a);
+    const auto kernel = stream ? loss_backward_kernel<T, kWave, PACKED, PACKED> : loss_backward_kernel<T, kWave, PACKED, false>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(4 * kWave), 0, s, a);
   } else {
     const int64_t stretch = 256 * kPacks * (PACKED ? RowSpan<T>::W : 1);
     const unsigned parts = (unsigned)std::min<int64_t>((a.classes + stretch - 1) / stretch, 1024);
     const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 1 << 20);
-    // the logits are read for the last time, and neither they nor the gradient stay in the cache
-    const bool stream = 2 * a.rows * a.classes * (int64_t)sizeof(T) > kCacheBytes;
     const auto kernel = stream ? loss_backward_kernel<T, 256, PACKED, PACKED> : loss_backward_kernel<T, 256, PACKED, false>;
     hipLaunchKernelGGL(kernel, dim3(grid, parts), dim3(256), 0, s, a);
   }

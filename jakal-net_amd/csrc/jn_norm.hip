@@ -57,37 +57,67 @@ __device__ __forceinline__ float param(const void* p, int64_t i, int code, float
 }
 
 // ---- rows held in registers ---------------------------------------------------
-// A group of GW waves takes a row: thread t of it the packs t, t + 64 GW, ... of
-// W elements (16 bytes; single elements where rows do not start on 16), NP packs
-// at most.  A row is read once, and its mean, centred squares and gradient sums
-// come from registers; the next row's packs load while this one is reduced.
-template <int W, int NP, int GW>
+// TH threads take a row: thread t of them the packs t, t + TH, ... of W elements
+// (16 bytes; single elements where rows do not start on 16), NP packs and eight
+// elements at most.  A row is read once, and its mean, centred squares and
+// gradient sums come from registers; the next row's packs load while this one
+// is reduced.  A workgroup of BLOCK threads holds several such groups, which
+// step through the rows together (they share the barriers).
+template <int W, int NP, int TH, int BLOCK>
 struct RowGroup {
-  static constexpr int kThreads = GW * kWave;
-  static constexpr int kBlock = (GW > 4 ? GW : 4) * kWave;  // of the forward: four waves, or one group
+  static constexpr int kGroups = BLOCK / TH;
   static constexpr int kItems = W * NP;  // elements of a thread
 
-  __device__ static int thread() { return GW == 1 ? lane_id() : (int)threadIdx.x; }
-  __device__ static int64_t element(int p) { return (int64_t)(p * kThreads + thread()) * W; }
+  __device__ static int thread() { return TH == kWave ? lane_id() : (int)threadIdx.x % TH; }
+  // of a group in the workgroup: uniform over a wave where groups are whole waves
+  __device__ static int group() { return TH < kWave ? (int)threadIdx.x / TH : wave_id() / (TH / kWave); }
+  __device__ static int element(int p) { return (p * TH + thread()) * W; }
 };
 
-template <typename T, int W, int NP, int GW>
-__device__ __forceinline__ void load_row(const void* base, int64_t row, int64_t dim, Raw<T, W> (&raw)[NP]) {
-  const T* p = static_cast<const T*>(base) + row * dim;
+// Sums of N values over each group of TH threads, the same in all of them.
+template <int TH, int BLOCK, int N>
+__device__ __forceinline__ void group_sums(float (&v)[N], float (*lds)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = row16_sum(v[i]);
+    if constexpr (TH >= 32) v[i] += xor16_f(v[i]);
+    if constexpr (TH >= 64) v[i] += xor32_f(v[i]);
+  }
+  if constexpr (TH > kWave) {
+    constexpr int kWaves = TH / kWave;
+    __syncthreads();  // the readers before are done
+    if (lane_id() == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) lds[wave_id()][i] = v[i];
+    }
+    __syncthreads();
+    const int first = wave_id() / kWaves * kWaves;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) v[i] += lds[first + k][i];
+    }
+  }
+}
+
+template <typename T, int W, int NP, typename G>
+__device__ __forceinline__ void load_row(const void* base, int64_t row, const NormArgs& a, Raw<T, W> (&raw)[NP]) {
+  const T* p = static_cast<const T*>(base) + row * a.dim;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int64_t e = RowGroup<W, NP, GW>::element(i);
-    if (e < dim) raw[i].load(p + e);
+    const int e = G::element(i);
+    if (row < a.rows && e < a.dim) raw[i].load(p + e);
     else raw[i].clear();
   }
 }
 
-template <typename T, int W, int NP, int GW>
+template <typename T, int W, int NP, typename G>
 __device__ __forceinline__ void load_params(const void* base, int type, int64_t dim, float none,
                                             float (&v)[W * NP]) {
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int64_t e = RowGroup<W, NP, GW>::element(i);
+    const int e = G::element(i);
 #pragma unroll
     for (int j = 0; j < W; ++j) v[i * W + j] = none;
     if (!base || e >= dim) continue;
@@ -111,42 +141,46 @@ __device__ __forceinline__ void load_params(const void* base, int type, int64_t 
   }
 }
 
-template <typename T, int W, int NP, int GW>
-__global__ __launch_bounds__((GW > 4 ? GW : 4) * kWave) void norm_forward_kernel(NormArgs a) {
-  using G = RowGroup<W, NP, GW>;
-  constexpr int kGroups = G::kBlock / G::kThreads;
-  __shared__ float lds[GW];
-  const int64_t groups = (int64_t)gridDim.x * kGroups;
-  const int64_t first = (int64_t)blockIdx.x * kGroups + (GW == 1 ? wave_id() : 0);
+template <typename T, int W, int NP, int TH, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void norm_forward_kernel(NormArgs a) {
+  using G = RowGroup<W, NP, TH, BLOCK>;
+  __shared__ float lds[BLOCK / kWave][1];
+  const int64_t step = (int64_t)gridDim.x * G::kGroups;
+  int64_t base = (int64_t)blockIdx.x * G::kGroups;
+  const int group = G::group();
   const float n = (float)a.dim;
   Raw<T, W> next[NP];
-  if (first < a.rows) load_row<T, W, NP, GW>(a.x, first, a.dim, next);
+  load_row<T, W, NP, G>(a.x, base + group, a, next);
   float w[G::kItems], b[G::kItems];
-  load_params<T, W, NP, GW>(a.w, a.param_type, a.dim, 1.0f, w);
-  load_params<T, W, NP, GW>(a.b, a.param_type, a.dim, 0.0f, b);
-  for (int64_t row = first; row < a.rows; row += groups) {
+  load_params<T, W, NP, G>(a.w, a.param_type, a.dim, 1.0f, w);
+  load_params<T, W, NP, G>(a.b, a.param_type, a.dim, 0.0f, b);
+  for (; base < a.rows; base += step) {
+    const int64_t row = base + group;
     float v[G::kItems];
 #pragma unroll
     for (int i = 0; i < NP; ++i) next[i].unpack(v + i * W);
-    if (row + groups < a.rows) load_row<T, W, NP, GW>(a.x, row + groups, a.dim, next);
-    float s = 0.f;
+    if (base + step < a.rows) load_row<T, W, NP, G>(a.x, row + step, a, next);
+    float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < G::kItems; ++i) {
       v[i] *= a.scale;
-      s += v[i];
+      s[0] += v[i];
     }
-    const float m = group_sum<GW>(s, lds) / n;
-    s = 0.f;
+    group_sums<TH, BLOCK>(s, lds);
+    const float m = s[0] / n;
+    s[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       if (G::element(i) >= a.dim) continue;  // (the clears there are not elements)
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         v[i * W + j] -= m;
-        s += v[i * W + j] * v[i * W + j];
+        s[0] += v[i * W + j] * v[i * W + j];
       }
     }
-    const float r = 1.0f / sqrtf(group_sum<GW>(s, lds) / n + a.eps);
+    group_sums<TH, BLOCK>(s, lds);
+    const float r = 1.0f / sqrtf(s[0] / n + a.eps);
+    if (row >= a.rows) continue;
     T* y = static_cast<T*>(a.y) + row * a.dim;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
@@ -161,46 +195,46 @@ __global__ __launch_bounds__((GW > 4 ? GW : 4) * kWave) void norm_forward_kernel
     }
   }
   if (a.state) {
-    for (int64_t i = (int64_t)blockIdx.x * G::kBlock + threadIdx.x; i < a.rows; i += (int64_t)gridDim.x * G::kBlock)
+    for (int64_t i = (int64_t)blockIdx.x * BLOCK + threadIdx.x; i < a.rows; i += (int64_t)gridDim.x * BLOCK)
       state_forward(a, i);
   }
 }
 
-// A workgroup of WPB waves also keeps the column sums of its rows: each thread
-// its own columns' in registers, joined over the groups in LDS at the end.
-template <typename T, int W, int NP, int GW, int WPB>
-__global__ __launch_bounds__(WPB* kWave) void norm_backward_kernel(NormArgs a) {
-  using G = RowGroup<W, NP, GW>;
-  constexpr int kThreads = WPB * kWave, kGroups = WPB / GW;
-  __shared__ float lds[GW];
-  extern __shared__ float sums[];  // [kGroups][dim], at most 32 KB
-  const int64_t groups = (int64_t)gridDim.x * kGroups;
-  const int64_t first = (int64_t)blockIdx.x * kGroups + (GW == 1 ? wave_id() : 0);
+// Each thread also keeps its own columns' sums in registers; the groups of a
+// workgroup join in LDS at the end.
+template <typename T, int W, int NP, int TH, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void norm_backward_kernel(NormArgs a) {
+  using G = RowGroup<W, NP, TH, BLOCK>;
+  __shared__ float lds[BLOCK / kWave][2];
+  extern __shared__ float sums[];  // [kGroups][dim], at most 16 KB
+  const int64_t step = (int64_t)gridDim.x * G::kGroups;
+  const int group = G::group();
   const float n = (float)a.dim;
   float dw[G::kItems], db[G::kItems];
 #pragma unroll
   for (int i = 0; i < G::kItems; ++i) dw[i] = db[i] = 0.f;
   if (a.dx || a.partial) {
+    int64_t base = (int64_t)blockIdx.x * G::kGroups;
     Raw<T, W> next_x[NP], next_g[NP];
-    if (first < a.rows) {
-      load_row<T, W, NP, GW>(a.x, first, a.dim, next_x);
-      load_row<T, W, NP, GW>(a.g, first, a.dim, next_g);
-    }
+    load_row<T, W, NP, G>(a.x, base + group, a, next_x);
+    load_row<T, W, NP, G>(a.g, base + group, a, next_g);
     float w[G::kItems];
-    load_params<T, W, NP, GW>(a.w, a.param_type, a.dim, 1.0f, w);
-    for (int64_t row = first; row < a.rows; row += groups) {
-      const float m = a.stats[2 * row], r = a.stats[2 * row + 1];
+    load_params<T, W, NP, G>(a.w, a.param_type, a.dim, 1.0f, w);
+    for (; base < a.rows; base += step) {
+      const int64_t row = base + group;
+      const bool live = row < a.rows;  // (a dead row is all zeros)
+      const float m = live ? a.stats[2 * row] : 0.f, r = live ? a.stats[2 * row + 1] : 0.f;
       float h[G::kItems], g[G::kItems];
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         next_x[i].unpack(h + i * W);
         next_g[i].unpack(g + i * W);
       }
-      if (row + groups < a.rows) {
-        load_row<T, W, NP, GW>(a.x, row + groups, a.dim, next_x);
-        load_row<T, W, NP, GW>(a.g, row + groups, a.dim, next_g);
+      if (base + step < a.rows) {
+        load_row<T, W, NP, G>(a.x, row + step, a, next_x);
+        load_row<T, W, NP, G>(a.g, row + step, a, next_g);
       }
-      float s1 = 0.f, s2 = 0.f;
+      float s[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         if (G::element(i) >= a.dim) continue;
@@ -210,18 +244,17 @@ __global__ __launch_bounds__(WPB* kWave) void norm_backward_kernel(NormArgs a) {
           dw[j] += g[j] * h[j];
           db[j] += g[j];
           g[j] *= w[j];
-          s1 += g[j];
-          s2 += g[j] * h[j];
+          s[0] += g[j];
+          s[1] += g[j] * h[j];
         }
       }
       if (!a.dx) continue;
-      s1 = group_sum<GW>(s1, lds) / n;
-      s2 = group_sum<GW>(s2, lds) / n;
-      const float sr = a.scale * r;
+      group_sums<TH, BLOCK>(s, lds);
+      const float s1 = s[0] / n, s2 = s[1] / n, sr = a.scale * r;
       T* dx = static_cast<T*>(a.dx) + row * a.dim;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        if (G::element(i) >= a.dim) continue;
+        if (!live || G::element(i) >= a.dim) continue;
 #pragma unroll
         for (int j = i * W; j < i * W + W; ++j) h[j] = sr * (g[j] - s1 - h[j] * s2);
         store_raw<T, W>(dx + G::element(i), h + i * W);
@@ -229,32 +262,31 @@ __global__ __launch_bounds__(WPB* kWave) void norm_backward_kernel(NormArgs a) {
     }
   }
   if (a.dstate) {
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < a.rows; i += (int64_t)gridDim.x * kThreads)
+    for (int64_t i = (int64_t)blockIdx.x * BLOCK + threadIdx.x; i < a.rows; i += (int64_t)gridDim.x * BLOCK)
       state_backward(a, i);
   }
   if (!a.partial) return;
   float* out = a.partial + (int64_t)blockIdx.x * 2 * a.dim;
-  const int group = kGroups == 1 ? 0 : wave_id();
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     if (k) __syncthreads();  // the sums before are read
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int64_t e = G::element(i);
+      const int e = G::element(i);
       if (e >= a.dim) continue;
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         const float v = k ? db[i * W + j] : dw[i * W + j];
-        if (kGroups == 1) out[k * a.dim + e + j] = v;
-        else sums[group * a.dim + e + j] = v;
+        if (G::kGroups == 1) out[k * a.dim + e + j] = v;
+        else sums[group * (int)a.dim + e + j] = v;
       }
     }
-    if (kGroups == 1) continue;
+    if (G::kGroups == 1) continue;
     __syncthreads();
-    for (int64_t c = threadIdx.x; c < a.dim; c += kThreads) {
+    for (int c = threadIdx.x; c < (int)a.dim; c += BLOCK) {
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) s += sums[i * a.dim + c];
+      for (int i = 0; i < G::kGroups; ++i) s += sums[i * (int)a.dim + c];
       out[k * a.dim + c] = s;
     }
   }
@@ -375,60 +407,67 @@ __global__ __launch_bounds__(kFinishColumns* kFinishLanes) void norm_columns_fin
 
 // ---- which kernel ---------------------------------------------------------------
 // The register kernels' shapes: packs of 16 bytes where every row and parameter
-// starts on 16, else single elements.  A wave takes rows of up to 16 elements a
-// lane, four waves rows of up to 16 a thread, sixteen rows of up to 8 a thread
-// (they would not have the registers for more); wider rows take the kernels
-// that pass over memory.
+// starts on 16, else single elements; eight elements a thread (of sixteen the
+// backward has the registers for three waves a SIMD: 16,384 x 1,536 bf16 took
+// 59 us so, 41 now), by as few threads as hold the row, sixteen at least (a wave
+// for every row took 30 us for the backward of 65,536 x 64 fp32, sixteen lanes
+// take 16).  Rows that 1024 threads do not hold take the kernels that pass over
+// memory.
 struct RowShape {
-  int width, packs, waves;  // W, NP, GW; packs = 0: none fits
+  int width, items, threads;  // W, W * NP, TH; threads = 0: none fits
 };
 
 RowShape row_shape(int64_t dim, bool aligned, int elem_bytes) {
   const int w = aligned ? 16 / elem_bytes : 1;
-  for (const int waves : {1, 4, 16}) {
-    for (const int items : {4, 8, 16}) {
-      if (items < w || (waves == 16 && items != 8)) continue;
-      if (dim <= (int64_t)items * waves * kWave) return {w, items / w, waves};
-    }
-  }
-  return {w, 0, 0};
+  if (dim > 8 * 1024) return {w, 0, 0};
+  int threads = 16;
+  while (dim > 8 * threads) threads *= 2;
+  return {w, w <= 4 && dim <= 4 * threads ? 4 : 8, threads};
 }
 
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-// Calls f(W, NP, GW) with a shape's numbers as constants.
+// Calls f(W, NP, TH) with a shape's numbers as constants.
 template <int V, typename F>
 int with_shape(const RowShape& s, F f) {
   const auto packed = [&](auto width) -> int {
     constexpr int W = decltype(width)::value;
-    const auto grouped = [&](auto waves) -> int {
-      if constexpr (W <= 4) {
-        if (s.packs * W == 4) return f(width, Int<4 / W>{}, waves);
-      }
-      if (s.packs * W == 16) return f(width, Int<16 / W>{}, waves);
-      return f(width, Int<8 / W>{}, waves);
-    };
-    if (s.waves == 16) return f(width, Int<8 / W>{}, Int<16>{});
-    return s.waves == 4 ? grouped(Int<4>{}) : grouped(Int<1>{});
+    if constexpr (W <= 4) {
+      if (s.items == 4) return f(width, Int<4 / W>{}, Int<16>{});  // (up to 64 elements)
+    }
+    switch (s.threads) {
+      case 16:
+        return f(width, Int<8 / W>{}, Int<16>{});
+      case 32:
+        return f(width, Int<8 / W>{}, Int<32>{});
+      case 64:
+        return f(width, Int<8 / W>{}, Int<64>{});
+      case 128:
+        return f(width, Int<8 / W>{}, Int<128>{});
+      case 256:
+        return f(width, Int<8 / W>{}, Int<256>{});
+      case 512:
+        return f(width, Int<8 / W>{}, Int<512>{});
+      default:
+        return f(width, Int<8 / W>{}, Int<1024>{});
+    }
   };
   return s.width == 1 ? packed(Int<1>{}) : packed(Int<V>{});
 }
 
-// Waves a workgroup of the backward, and its workgroups, each of which leaves
-// one row of partial sums.  65,536 x 512 bf16 with the join: eight waves and up
-// to 512 workgroups 42 us, sixteen and 512 46, sixteen and 256 43, four and
-// 512 59, four and 1024 44; 8,192 x 512 fp32: 15.9, 19.2, 16.9, 15.7 and 16.4;
-// 4,593 x 383: 13.2, 15.4, 12.8, 13.6 and 14.5.  Fewer rows take four, so that
+// Threads of a workgroup of the backward, and its workgroups, each of which
+// leaves one row of partial sums.  65,536 x 512 bf16 with the join: 512 threads
+// and up to 512 workgroups 42 us, 1024 and 512 46, 1024 and 256 43, 256 and
+// 512 59, 256 and 1024 44; 8,192 x 512 fp32: 15.9, 19.2, 16.9, 15.7 and 16.4;
+// 4,593 x 383: 13.2, 15.4, 12.8, 13.6 and 14.5.  Fewer rows take 256, so that
 // the workgroups fill the CUs.
 constexpr int64_t kMaxParts = 512;
 constexpr int64_t kManyRows = 2048;
 
-int backward_waves(const RowShape& s, int64_t rows) {
-  return s.waves == 16 ? 16 : s.waves == 1 && rows >= kManyRows ? 8 : 4;
-}
+int backward_block(const RowShape& s, int64_t rows) { return std::max(s.threads, rows >= kManyRows ? 512 : 256); }
 int64_t backward_groups(const RowShape& s, int64_t rows) {
-  const int64_t per = backward_waves(s, rows) / s.waves;
+  const int64_t per = backward_block(s, rows) / s.threads;
   return std::min((rows + per - 1) / per, kMaxParts);
 }
 
@@ -436,7 +475,7 @@ int64_t backward_groups(const RowShape& s, int64_t rows) {
 constexpr int64_t kSlabs = 64;
 int64_t slab_count(int64_t rows) { return std::min<int64_t>(kSlabs, (rows + 15) / 16); }
 
-// Workgroups of the wave-a-row forward: eight of four waves a CU.
+// Workgroups of the forward: eight of four waves a CU.
 constexpr int64_t kForwardGroups = 2048;
 
 int64_t row_groups(int64_t rows) { return std::min<int64_t>(rows, 1 << 20); }
@@ -466,18 +505,18 @@ template <typename T>
 int launch_norm_forward(const NormArgs& a, hipStream_t s) {
   const bool aligned = aligned_rows<T>(a);
   const RowShape shape = row_shape(a.dim, aligned, sizeof(T));
-  if (!shape.packs) {
+  if (!shape.threads) {
     JN_PROFILE("norm_forward_any_kernel", s);
     hipLaunchKernelGGL(norm_forward_any_kernel<T>, dim3((unsigned)row_groups(a.rows)), dim3(kAnyThreads), 0, s, a);
     JN_LAUNCH_CHECK();
     return kOk;
   }
-  return with_shape<16 / sizeof(T)>(shape, [&](auto width, auto packs, auto waves) -> int {
-    constexpr int W = decltype(width)::value, NP = decltype(packs)::value, GW = decltype(waves)::value;
-    constexpr int kBlock = RowGroup<W, NP, GW>::kBlock, per = kBlock / (GW * kWave);
+  return with_shape<16 / sizeof(T)>(shape, [&](auto width, auto packs, auto threads) -> int {
+    constexpr int W = decltype(width)::value, NP = decltype(packs)::value, TH = decltype(threads)::value;
+    constexpr int kBlock = TH > 256 ? TH : 256, per = kBlock / TH;
     const unsigned grid = (unsigned)std::min<int64_t>((a.rows + per - 1) / per, kForwardGroups);
     JN_PROFILE("norm_forward_kernel", s);
-    hipLaunchKernelGGL((norm_forward_kernel<T, W, NP, GW>), dim3(grid), dim3(kBlock), 0, s, a);
+    hipLaunchKernelGGL((norm_forward_kernel<T, W, NP, TH, kBlock>), dim3(grid), dim3(kBlock), 0, s, a);
     JN_LAUNCH_CHECK();
     return kOk;
   });
@@ -497,7 +536,7 @@ int launch_norm_backward(NormArgs a, hipStream_t s) {
   if (!columns) a.partial = nullptr;
   const bool aligned = aligned_rows<T>(a);
   const RowShape shape = row_shape(a.dim, aligned, sizeof(T));
-  if (!shape.packs) {
+  if (!shape.threads) {
     if (a.dx || a.dstate) {
       JN_PROFILE("norm_backward_any_kernel", s);
       hipLaunchKernelGGL(norm_backward_any_kernel<T>, dim3((unsigned)row_groups(a.rows)), dim3(kAnyThreads), 0, s, a);
@@ -514,18 +553,18 @@ int launch_norm_backward(NormArgs a, hipStream_t s) {
     return launch_columns_finish(a, slabs, s);
   }
   const int64_t grid = backward_groups(shape, a.rows);
-  const int rc = with_shape<16 / sizeof(T)>(shape, [&](auto width, auto packs, auto waves) -> int {
-    constexpr int W = decltype(width)::value, NP = decltype(packs)::value, GW = decltype(waves)::value;
+  const int rc = with_shape<16 / sizeof(T)>(shape, [&](auto width, auto packs, auto threads) -> int {
+    constexpr int W = decltype(width)::value, NP = decltype(packs)::value, TH = decltype(threads)::value;
     const auto run = [&](auto block) -> int {
-      constexpr int WPB = decltype(block)::value;
-      const size_t lds = a.partial && WPB > GW ? (size_t)(WPB / GW) * a.dim * sizeof(float) : 0;
+      constexpr int kBlock = decltype(block)::value;
+      const size_t lds = a.partial && kBlock > TH ? (size_t)(kBlock / TH) * a.dim * sizeof(float) : 0;
       JN_PROFILE("norm_backward_kernel", s);
-      hipLaunchKernelGGL((norm_backward_kernel<T, W, NP, GW, WPB>), dim3((unsigned)grid), dim3(WPB * kWave), lds, s, a);
+      hipLaunchKernelGGL((norm_backward_kernel<T, W, NP, TH, kBlock>), dim3((unsigned)grid), dim3(kBlock), lds, s, a);
       JN_LAUNCH_CHECK();
       return kOk;
     };
-    if constexpr (GW == 1) return backward_waves(shape, a.rows) == 8 ? run(Int<8>{}) : run(Int<4>{});
-    else return run(Int<GW>{});
+    if constexpr (TH >= 512) return run(Int<TH>{});
+    else return backward_block(shape, a.rows) == 512 ? run(Int<512>{}) : run(Int<256>{});
   });
   if (rc || !columns) return rc;
   return launch_columns_finish(a, grid, s);

@@ -104,10 +104,15 @@ __device__ __forceinline__ void group_sums(float (&v)[N], float (*lds)[N]) {
 template <typename T, int W, int NP, typename G>
 __device__ __forceinline__ void load_row(const void* base, int64_t row, const NormArgs& a, Raw<T, W> (&raw)[NP]) {
   const T* p = static_cast<const T*>(base) + row * a.dim;
+  if (row >= a.rows) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) raw[i].clear();
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int e = G::element(i);
-    if (row < a.rows && e < a.dim) raw[i].load(p + e);
+    if (e < a.dim) raw[i].load(p + e);
     else raw[i].clear();
   }
 }

@@ -124,6 +124,7 @@ def test_masked_logits(dev, classes, dtype):
     O.close("masked loss", loss[keep], want["loss"][0], want["loss"][1])
     O.close("masked grad", grad[keep], want["grad"][0],
             want["grad"][1] + O.half(z.dtype) * want["grad"][0].abs() + O.floor(z.dtype))
+    loss = loss.detach()
     assert float(loss[3]) == float("inf") and bool(torch.isfinite(grad[3]).all()) and float(grad[3, 1]) == -1.0
     assert float(loss[1]) == 0.0 and not grad[1].any()
 
@@ -237,10 +238,19 @@ def test_two_captured_steps_replay_as_eager(dev):
                 assert torch.equal(a, b), f"replay {rep}"
 
 
-def test_more_than_2_31_logits(dev):
+@pytest.mark.parametrize("rows,classes", [(1030, 1100), (1024, 2048), (1500, 4096), (1201, 4099), (1025, 8192),
+                                          (511, 9000), (513, 9000)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_many_rows(dev, rows, classes, dtype):
+    z, t = _made(dev, rows, classes, O.DTYPES[dtype], seed=3)
+    t[::7] = -100
+    _case(dev, z, t, what=f"{rows}x{classes} {dtype}")
+
+
+@pytest.mark.parametrize("rows,classes", [((1 << 15) + 9, 65537), (200003, 1000), (100003, 2047)])
+def test_more_logits_than_the_cache_or_31_bits(dev, rows, classes):
     import jakal_net as J
 
-    classes, rows = 65537, (1 << 15) + 9
     z = torch.empty(rows, classes, device=dev, dtype=torch.bfloat16).normal_(std=2.0)
     t = torch.randint(0, classes, (rows,), device=dev)
     leaf = z.requires_grad_()

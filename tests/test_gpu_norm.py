@@ -68,6 +68,16 @@ def test_row_counts(dev, rows, dim):
     _norm_case(dev, rows, dim, torch.bfloat16, torch.float32)
 
 
+@pytest.mark.parametrize("rows", [3, 15, 33, 255, 2047, 2049, 9001])
+@pytest.mark.parametrize("dim", [8, 60, 64, 128, 130, 200, 1000, 3000, 8000])
+def test_groups_that_end_inside_a_workgroup(dev, rows, dim):
+    """Rows that do not fill the last workgroup's groups, few and many, for each number of threads a row."""
+    if rows * dim <= 1 << 24:
+        _norm_case(dev, rows, dim, torch.float32, torch.float32)
+        _norm_case(dev, rows, dim + 1, torch.bfloat16, torch.bfloat16)
+        _norm_case(dev, rows, dim, torch.float16, torch.float32)
+
+
 @pytest.mark.parametrize("affine", ["both", "weight", "bias", "none"])
 @pytest.mark.parametrize("dim", [100, 512, 4096, 9000])
 def test_parameters_left_out(dev, dim, affine):
@@ -328,6 +338,42 @@ def test_more_than_2_31_elements(dev):
     for n, got in (("w", gw), ("b", gb)):
         value, bound, size = sums[n]
         O.close("far grad " + n, got, value, bound + O.depth(rows) * O.U * size + O.U * value.abs())
+
+
+def test_inputs_changed_before_the_backward_raise(dev):
+    import jakal_net as J
+
+    for which in ("val", "weight", "state"):
+        t = dict(state=torch.randn(4, device=dev), val=torch.randn(4, 16, device=dev), weight=torch.ones(16, device=dev))
+        leaves = {n: v.requires_grad_() for n, v in t.items()}
+        used = {n: v * 1.0 for n, v in leaves.items()}
+        a, b = J.stabilize(**used)
+        with torch.no_grad():
+            used[which].mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            (a.sum() + b.sum()).backward()
+    x = torch.randn(4, 16, device=dev, requires_grad=True)
+    y = J.layer_norm(x)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+
+
+def test_transforms(dev):
+    """vmap runs it slice by slice; torch.func's gradients and forward mode raise."""
+    import jakal_net as J
+    from torch.autograd import forward_ad
+
+    x = torch.randn(3, 4, 8, device=dev)
+    assert torch.equal(torch.func.vmap(J.layer_norm)(x), J.layer_norm(x))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: J.layer_norm(t).pow(3).sum())(x)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(J.layer_norm, (x,), (x,))
+    with pytest.raises((RuntimeError, NotImplementedError)), forward_ad.dual_level():
+        J.layer_norm(forward_ad.make_dual(x, x))
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        J.layer_norm(x[0].to_sparse())
 
 
 def test_autocast_returns_fp32_rows(dev):

@@ -57,6 +57,7 @@ def _wide(t: Tensor) -> Tensor:
     return t.float() if t.dtype in (torch.float16, torch.bfloat16) else t
 
 
+@torch.no_grad()
 def _norm(grads: list, norm_type: float) -> Tensor:
     grads = [t for t in grads if t is not None and t.numel()]
     if not grads:
@@ -65,7 +66,6 @@ def _norm(grads: list, norm_type: float) -> Tensor:
     return torch.linalg.vector_norm(norms, norm_type)
 
 
-@torch.no_grad()
 def grad_norm(grads: Tensor | Iterable[Tensor | None], norm_type: float = 2.0, *,
               implementation: ImplementationMode = "native") -> Tensor:
     """Norm over all elements of a list of tensors (None skipped), as a scalar tensor."""
@@ -81,7 +81,6 @@ def grad_norm(grads: Tensor | Iterable[Tensor | None], norm_type: float = 2.0, *
     return _norm(grads, float(norm_type))
 
 
-@torch.no_grad()
 def clip_grads(grads: Tensor | Iterable[Tensor | None], max_norm: float, norm_type: float = 2.0, *,
                out: Tensor | Iterable[Tensor | None] | None = None,
                implementation: ImplementationMode = "native") -> Tensor:
@@ -106,9 +105,10 @@ def clip_grads(grads: Tensor | Iterable[Tensor | None], max_norm: float, norm_ty
         raise ValueError(f"clip_grads: {len(grads)} gradients but {len(targets)} outputs.")
     norm = _norm(grads, float(norm_type))
     factor = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
-    for g, o in zip(grads, targets):
-        if g is not None:
-            o.copy_(_wide(g) * factor)
+    with torch.no_grad():
+        for g, o in zip(grads, targets):
+            if g is not None:
+                o.copy_(_wide(g) * factor)
     return norm
 
 

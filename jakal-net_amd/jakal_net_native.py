@@ -2045,8 +2045,9 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
         out = _as_list(out)
         if len(out) != len(grads):
             raise ValueError(f"clip_grads: {len(grads)} gradients but {len(out)} outputs.")
-        pairs = [(g, o) for g, o in zip(grads, out) if g is not None]
-        grads, out = [g for g, _ in pairs], [o for _, o in pairs]
+        given = [i for i, g in enumerate(grads) if g is not None]
+        if len(given) != len(grads):
+            grads, out = [grads[i] for i in given], [out[i] for i in given]
         if any(o is None for o in out):
             raise ValueError("clip_grads: a gradient without an output.")
     return _clip_grads(grads, out, float(max_norm), _norm_kind(norm_type))

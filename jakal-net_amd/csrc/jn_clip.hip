@@ -72,8 +72,14 @@ __device__ double group_join(double v, double* lds) {
   return lds[0];
 }
 
-// A chunk's part of a norm: 16-byte packs where the tensor starts on 16 bytes
-// (chunks are whole packs; the last one ends in single elements), else elements.
+// Elements before the first whole pack of W: views of one flat buffer start
+// anywhere in it.
+template <int W, typename T>
+__device__ __forceinline__ int pack_head(const T* p) {
+  return (int)((0 - reinterpret_cast<uintptr_t>(p) / sizeof(T)) & (W - 1));
+}
+
+// A chunk's part of a norm: 16-byte packs, and single elements on either side.
 template <bool MAX, typename T>
 __device__ __forceinline__ double chunk_norm(const T* p, int n, double s) {
   constexpr int W = 16 / sizeof(T), kUnroll = kChunk / W / kClipThreads;
@@ -81,27 +87,22 @@ __device__ __forceinline__ double chunk_norm(const T* p, int n, double s) {
     const double d = v;
     s = MAX ? max_nan(s, fabs(d)) : s + d * d;
   };
-  int done = 0;
-  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    const int packs = n / W;
-    Raw<T, W> raw[kUnroll];
+  const int t = threadIdx.x, head = min(pack_head<W>(p), n), packs = (n - head) / W, tail = head + packs * W;
+  Raw<T, W> raw[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int k = i * kClipThreads + (int)threadIdx.x;
-      if (k < packs) raw[i].load(p + k * W);
-    }
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      if (i * kClipThreads + (int)threadIdx.x >= packs) continue;
-      float v[W];
-      raw[i].unpack(v);
-#pragma unroll
-      for (int j = 0; j < W; ++j) take(v[j]);
-    }
-    done = packs * W;
+  for (int i = 0; i < kUnroll; ++i) {
+    if (i * kClipThreads + t < packs) raw[i].load(p + head + (i * kClipThreads + t) * W);
   }
-#pragma unroll 8
-  for (int i = done + (int)threadIdx.x; i < n; i += kClipThreads) take((float)p[i]);
+  if (t < head) take((float)p[t]);
+  if (tail + t < n) take((float)p[tail + t]);
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) {
+    if (i * kClipThreads + t >= packs) continue;
+    float v[W];
+    raw[i].unpack(v);
+#pragma unroll
+    for (int j = 0; j < W; ++j) take(v[j]);
+  }
   return s;
 }
 
@@ -136,37 +137,40 @@ __global__ __launch_bounds__(kClipThreads) void grads_norm_finish_kernel(const d
 }
 
 // A chunk times the factor, in packs that are 16 bytes of the wider type, so
-// that loads and stores both run through memory without gaps; the tensors have
-// to start on 16 bytes for that, else element by element.
+// that loads and stores both run through memory without gaps; where the two
+// tensors' packs do not start at the same element, element by element.
 template <bool STREAM, typename TI, typename TO>
 __device__ __forceinline__ void chunk_scale(const TI* p, TO* o, int n, float scale) {
   constexpr int W = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO));
   constexpr int kUnroll = 8;  // packs in flight
-  int done = 0;
-  if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
-    const int packs = n / W;
-    for (int first = threadIdx.x; first < packs; first += kUnroll * kClipThreads) {
-      Raw<TI, W> raw[kUnroll];
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        const int k = first + i * kClipThreads;
-        if (k < packs) raw[i].template load<STREAM>(p + k * W);
-      }
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        const int k = first + i * kClipThreads;
-        if (k >= packs) continue;
-        float v[W];
-        raw[i].unpack(v);
-#pragma unroll
-        for (int j = 0; j < W; ++j) v[j] *= scale;
-        store_raw<TO, W, STREAM>(o + k * W, v);
-      }
-    }
-    done = packs * W;
-  }
+  const int t = threadIdx.x, head = min(pack_head<W>(p), n);
+  if (pack_head<W>(o) != pack_head<W>(p)) {
 #pragma unroll 8
-  for (int i = done + (int)threadIdx.x; i < n; i += kClipThreads) o[i] = (TO)(scale * (float)p[i]);
+    for (int i = t; i < n; i += kClipThreads) o[i] = (TO)(scale * (float)p[i]);
+    return;
+  }
+  const int packs = (n - head) / W, tail = head + packs * W;
+  if (t < head) o[t] = (TO)(scale * (float)p[t]);
+  if (tail + t < n) o[tail + t] = (TO)(scale * (float)p[tail + t]);
+  p += head, o += head;
+  for (int first = t; first < packs; first += kUnroll * kClipThreads) {
+    Raw<TI, W> raw[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int k = first + i * kClipThreads;
+      if (k < packs) raw[i].template load<STREAM>(p + k * W);
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int k = first + i * kClipThreads;
+      if (k >= packs) continue;
+      float v[W];
+      raw[i].unpack(v);
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[j] *= scale;
+      store_raw<TO, W, STREAM>(o + k * W, v);
+    }
+  }
 }
 
 template <bool STREAM, typename TI>

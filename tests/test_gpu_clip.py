@@ -87,7 +87,26 @@ def test_into_other_buffers(dev, dtype, out_dtype, offset):
         assert all(bool((p[:1 + offset] == 7).all()) and float(p[-1]) == 7.0 for p in pads)
 
 
-@pytest.mark.parametrize("count", [1, 139, 140, 141, 300, 1000])
+@pytest.mark.parametrize("phase", [(0, 0), (1, 1), (3, 3), (5, 1), (2, 6), (7, 7), (1, 0), (4, 4)])
+@pytest.mark.parametrize("dtype,out_dtype", [("fp32", "fp32"), ("bf16", "bf16"), ("bf16", "fp32"), ("fp32", "fp16")])
+def test_views_of_flat_buffers(dev, dtype, out_dtype, phase):
+    """Gradients and outputs as unpadded views of two flat buffers, at any element of them."""
+    import jakal_net as J
+
+    sizes = [5, 8192, 3, 8193, 1, 2, 20001, 16384, 7]
+    g = torch.Generator().manual_seed(6)
+    total = sum(sizes)
+    flat = (torch.randn(total + 8, generator=g) * 0.01).to(O.DTYPES[dtype]).to(dev)[phase[0]:phase[0] + total]
+    out = torch.full((total + 16,), 7.0, device=dev, dtype=O.DTYPES[out_dtype])
+    grads, outs = list(flat.split(sizes)), list(out[phase[1] + 1:phase[1] + 1 + total].split(sizes))
+    max_norm = 0.3 * O.grads_norm(grads)
+    _check(grads, outs, J.clip_grads(grads, max_norm, out=outs), max_norm, 2.0, f"phase {phase}")
+    assert bool((out[:phase[1] + 1] == 7).all()) and bool((out[phase[1] + 1 + total:] == 7).all())
+    before = [t.clone() for t in grads]
+    _check(before, grads, J.clip_grads(grads, max_norm), max_norm, 2.0, f"phase {phase} in place")
+
+
+@pytest.mark.parametrize("count", [1, 139, 140, 141, 163, 164, 165, 300, 1000])
 def test_long_lists(dev, count):
     import jakal_net as J
 

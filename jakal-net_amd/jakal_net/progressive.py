@@ -183,7 +183,8 @@ class ProgressiveBStep(nn.Module):
     the shifted targets (a start token, then targets[:-1]) as their inputs and
     predict the targets; the loss is the mean cross entropy over all slots."""
 
-    def __init__(self, cfg: ProgressiveBConfig = ProgressiveBConfig(), *, implementation: ImplementationMode = "native") -> None:
+    def __init__(self, cfg: ProgressiveBConfig = ProgressiveBConfig(), *,
+                 implementation: ImplementationMode = "native") -> None:
         super().__init__()
         d, r, k = cfg.dim, cfg.rank, cfg.topk
         self.cfg = cfg

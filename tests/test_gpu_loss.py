@@ -167,6 +167,15 @@ def test_layouts(dev, kind):
     assert torch.equal(got, want)
 
 
+def test_one_row_without_axes(dev):
+    import jakal_net as J
+
+    z, t = _made(dev, 3, 40, torch.float32)
+    loss = J.cross_entropy(z[1], t[1], reduction="none")
+    assert loss.shape == () and torch.equal(loss, J.cross_entropy(z, t, reduction="none")[1])
+    assert torch.equal(J.cross_entropy(z[1], t[1]), loss)
+
+
 def test_backward_twice_and_scaled(dev):
     import jakal_net as J
 

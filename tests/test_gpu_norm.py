@@ -127,6 +127,32 @@ def test_batch_shapes(dev, shape):
     _check("shape", ["y", "grad_x"], [y.reshape(flat.shape), gx.reshape(flat.shape)], want, [torch.float32] * 2)
 
 
+def test_stabilize_without_rows(dev):
+    import jakal_net as J
+
+    s = torch.randn(2, 0, device=dev, requires_grad=True)
+    x = torch.randn(2, 0, 12, device=dev, requires_grad=True)
+    w, b = (torch.ones(12, device=dev, requires_grad=True) for _ in range(2))
+    t, y = J.stabilize(s, x, w, b, scale=0.5)
+    gs, gx, gw, gb = torch.autograd.grad([t, y], [s, x, w, b], [torch.ones_like(t), torch.ones_like(y)])
+    assert t.shape == gs.shape == (2, 0) and y.shape == gx.shape == (2, 0, 12)
+    assert not gw.any() and not gb.any()
+
+
+@pytest.mark.parametrize("kinds", [("bf16", "fp32", "bf16"), ("fp32", "bf16", "fp32"), ("fp16", "bf16", "fp32")])
+def test_parameters_of_other_types(dev, kinds):
+    """Weight and bias of types of their own are taken in fp32, their gradients come back in their types."""
+    import jakal_net as J
+
+    kx, kw, kb = (O.DTYPES[k] for k in kinds)
+    x, gy, weight, bias = _made(dev, 21, 72, kx, torch.float32)
+    leaves = [t.to(k).requires_grad_() for t, k in ((x, kx), (weight, kw), (bias, kb))]
+    y = J.layer_norm(*leaves)
+    grads = torch.autograd.grad(y, leaves, gy)
+    want = O.norm(*(t.detach() for t in leaves), 1e-5, 1.0, gy)
+    _check(f"types {kinds}", ["y", "grad_x", "grad_weight", "grad_bias"], [y, *grads], want, [kx, kx, kw, kb])
+
+
 def test_strided_inputs_and_expanded_gradients(dev):
     import jakal_net as J
 

@@ -134,7 +134,10 @@ def test_native_module_refuses_host_tensors_and_types():
         with pytest.raises(NotImplementedError):
             call()
     for op in ("layer_norm", "stabilize", "cross_entropy", "grad_norm", "clip_grads"):
-        assert op in jn.supported_ops()
+        assert op in jn.supported_ops() and hasattr(torch.ops.jakal_net_hip, op)
+    # tensors without memory of their own reach no kernel
+    with pytest.raises(RuntimeError):
+        jn.layer_norm(torch.empty(3, 4, device="meta"))
 
 
 def _lib():

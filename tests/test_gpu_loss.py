@@ -49,7 +49,7 @@ def test_class_counts(dev, classes, dtype):
     _case(dev, z, t, what=f"{classes} {dtype}")
 
 
-@pytest.mark.parametrize("rows", [1, 2, 63, 257, 1031, 5000])
+@pytest.mark.parametrize("rows", [1, 2, 15, 17, 63, 64, 65, 257, 1031, 5000])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_rows_and_reductions(dev, rows, reduction):
     z, t = _made(dev, rows, 130, torch.float32)

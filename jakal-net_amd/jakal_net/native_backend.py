@@ -160,13 +160,17 @@ def require_native_for_device(op_name: str, device_type: str) -> None:
 
 def native_op(op_name: str, device_type: str, implementation: str) -> Any | None:
     """The native module's op for a functional operator's call, or None where the
-    call takes the PyTorch form.  With implementation="native" a GPU tensor that
-    no library can take raises here."""
+    call takes the PyTorch form.
+
+    The functional operators are additions to the reference's module contract, so
+    a module that does not list them leaves them to PyTorch.  With
+    implementation="native" a GPU tensor raises where no module is available, or
+    none for its device."""
     if implementation not in ("native", "kernel"):
         return None
     status = native_status()
-    if status.available and op_name in status.supported_ops and device_type in status.supported_devices:
-        return getattr(_LOADER.module, op_name)
+    if status.available and device_type in status.supported_devices:
+        return getattr(_LOADER.module, op_name) if op_name in status.supported_ops else None
     if implementation == "native" and not native_disabled_by_env():
         require_native_for_device(op_name, device_type)
     return None

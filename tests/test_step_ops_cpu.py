@@ -140,6 +140,28 @@ def test_native_module_refuses_host_tensors_and_types():
         jn.layer_norm(torch.empty(3, 4, device="meta"))
 
 
+def test_dispatch_of_the_functional_operators(monkeypatch):
+    from jakal_net import native_backend as nb
+
+    with_op = nb.NativeStatus(True, "m", "b", ("layer_norm",), ("cuda",), None)
+    without = nb.NativeStatus(True, "m", "b", ("propagation_topk",), ("cuda",), None)
+    missing = nb.NativeStatus(False, "m", None, (), (), "no module")
+    module = type("M", (), {"layer_norm": staticmethod(lambda *a: "here")})
+    for status, implementation, device, want in (
+            (with_op, "native", "cuda", "here"), (with_op, "kernel", "cuda", "here"), (with_op, "reference", "cuda", None),
+            (with_op, "native", "cpu", None), (without, "native", "cuda", None), (missing, "kernel", "cuda", None),
+            (missing, "native", "cpu", None)):
+        monkeypatch.setattr(nb, "native_status", lambda s=status: s)
+        monkeypatch.setattr(nb._LOADER, "module", module)
+        op = nb.native_op("layer_norm", device, implementation)
+        assert (op() if op else None) == want, (status, implementation, device)
+    monkeypatch.setattr(nb, "native_status", lambda: missing)
+    with pytest.raises(RuntimeError, match="unavailable"):
+        nb.native_op("layer_norm", "cuda", "native")
+    monkeypatch.setenv("JAKAL_NET_DISABLE_NATIVE", "1")
+    assert nb.native_op("layer_norm", "cuda", "native") is None
+
+
 def _lib():
     import jakal_net_native as jn
 

@@ -61,6 +61,13 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
 
+// t as memory holds it row by row, its lazy negation carried out (contiguous()
+// alone leaves that to the reader where there is nothing to copy).
+Tensor plain(const Tensor& t) {
+  if (!t.defined()) return t;
+  return t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous();
+}
+
 Tensor given(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 
 // Whether a call has to record a backward.  Forward-mode tangents are refused:
@@ -126,9 +133,9 @@ struct JakalRowNormBackward : torch::autograd::Node {
     Tensor gs, gx, gw, gb, ws;
     if (need[0]) {
       gs = at::empty_like(state);
-      g_state = g_state.to(state.scalar_type()).contiguous();
+      g_state = plain(g_state.to(state.scalar_type()));
     }
-    if (need[1] || sums) g = g.to(x.scalar_type()).contiguous();
+    if (need[1] || sums) g = plain(g.to(x.scalar_type()));
     if (need[1]) gx = at::empty_like(x);
     if (need[2]) gw = at::empty_like(weight);
     if (need[3]) gb = at::empty({call.dim}, x.options().dtype(bias_type));
@@ -162,7 +169,7 @@ void norm_params(const Tensor& x, Tensor& weight, Tensor& bias) {
     own = own && p->scalar_type() == x.scalar_type();
   }
   for (Tensor* p : {&weight, &bias}) {
-    if (p->defined()) *p = (own ? *p : p->to(at::kFloat)).contiguous();
+    if (p->defined()) *p = plain(own ? *p : p->to(at::kFloat));
   }
 }
 
@@ -183,7 +190,7 @@ std::tuple<Tensor, Tensor> row_norm(const Tensor& state_in, const Tensor& x_in, 
   }
   Tensor weight = given(weight_in), bias = given(bias_in);
   norm_params(x_in, weight, bias);
-  const Tensor x = x_in.contiguous(), state = state_in.defined() ? state_in.contiguous() : Tensor();
+  const Tensor x = plain(x_in), state = plain(state_in);
   call.dim = x.size(-1);
   call.rows = x.numel() / call.dim;
   call.scale = (float)scale;
@@ -255,7 +262,7 @@ struct JakalCrossEntropyBackward : torch::autograd::Node {
     const c10::DeviceGuard guard(logits.device());
     const Tensor out = at::empty_like(logits);
     if (target.numel()) {
-      const Tensor g = grads[0].to(at::kFloat).contiguous();
+      const Tensor g = plain(grads[0].to(at::kFloat));
       check(jn_cross_entropy_backward(ptr(logits), target.data_ptr<int64_t>(), fptr(stats), fptr(count), fptr(g),
                                       target.numel(), logits.size(-1), ignore_index, (int32_t)reduction,
                                       type_code("cross_entropy", logits), ptr(out), stream_of(logits)));
@@ -275,7 +282,7 @@ Tensor cross_entropy(const Tensor& logits_in, const Tensor& target_in, int64_t i
               "cross_entropy targets are int64 or int32 class indices, got ", target_in.scalar_type(), ".");
   check_gpu(logits_in, logits_in);
   check_gpu(target_in, logits_in);
-  const Tensor logits = logits_in.contiguous(), target = target_in.to(at::kLong).contiguous();
+  const Tensor logits = plain(logits_in), target = target_in.to(at::kLong).contiguous();
   std::shared_ptr<JakalCrossEntropyBackward> node;
   if (records(logits)) {
     node = make_node<JakalCrossEntropyBackward>();
@@ -317,6 +324,7 @@ void check_list(const char* what, at::TensorList tensors, const Tensor& first) {
   for (const Tensor& t : tensors) {
     TORCH_CHECK_NOT_IMPLEMENTED(t.layout() == at::kStrided, what, " takes dense tensors, got layout ", t.layout(),
                                 ".");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.is_neg(), what, " takes tensors without a pending negation (resolve_neg).");
     type_code(what, t);
     check_gpu(t, first);
   }

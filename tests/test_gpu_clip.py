@@ -239,6 +239,21 @@ def test_two_captured_calls_replay_as_eager(dev):
             assert all(torch.equal(a, b) for a, b in zip(w, [norm] + out)), f"replay {rep}"
 
 
+def test_pending_negations(dev):
+    """Tensors whose negation torch has put off are refused, and taken once it is carried out."""
+    import jakal_net as J
+
+    a, b = torch.randn(50, device=dev), torch.empty(50, device=dev)
+    late, before = torch._neg_view(a), a.clone()
+    for call in (lambda: J.grad_norm([late]), lambda: J.clip_grads([late], 1.0),
+                 lambda: J.clip_grads([late], 1.0, out=[b]), lambda: J.clip_grads([b.fill_(2.0)], 1.0, out=[late])):
+        with pytest.raises(NotImplementedError):
+            call()
+        assert torch.equal(a, before)
+    J.clip_grads([late.resolve_neg()], float("inf"), out=[b])
+    assert torch.equal(b, -a)
+
+
 def test_refusals(dev):
     import jakal_net as J
 

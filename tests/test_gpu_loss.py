@@ -188,6 +188,24 @@ def test_backward_twice_and_scaled(dev):
     assert torch.equal(one, again) and torch.equal(two, 2 * one)
 
 
+def test_pending_negations(dev):
+    """Logits whose negation torch has put off, and a loss's gradient that comes through a conjugate."""
+    import jakal_net as J
+
+    z, t = _made(dev, 9, 70, torch.float32)
+    results = []
+    for lazy in (False, True):
+        leaf = z.detach().requires_grad_()
+        loss = J.cross_entropy(torch._neg_view(leaf) if lazy else -leaf, t)
+        whole = torch.complex(torch.zeros_like(loss), loss)
+        part = whole.conj().imag if lazy else -whole.imag
+        results.append((loss, *torch.autograd.grad(part, leaf)))
+    for eager, late in zip(*results):
+        assert torch.equal(eager, late)
+    want = O.cross_entropy(-z, t, -100, "mean", None)["grad"]  # (of the logits; minus for the leaf, minus for the part)
+    O.close("grad", results[1][1], want[0], want[1] + O.U * want[0].abs() + O.floor(torch.float32))
+
+
 def test_gradient_against_differences(dev):
     """<grad, d> against the loss's own quotient of differences over 2 t."""
     import jakal_net as J

@@ -385,6 +385,24 @@ def test_inputs_changed_before_the_backward_raise(dev):
         y.sum().backward()
 
 
+def test_pending_negations(dev):
+    """Tensors whose negation torch has put off (the imaginary parts of conjugates), inputs and gradients."""
+    import jakal_net as J
+
+    _, _, weight, bias = _made(dev, 6, 40, torch.float32, torch.float32)
+    x, gy = torch.randn(6, 40, device=dev), torch.randn(6, 40, device=dev)
+    state, gs = torch.randn(6, device=dev), torch.randn(6, device=dev)
+    results = []
+    for lazy in (False, True):
+        neg = torch._neg_view if lazy else torch.neg
+        leaves = [t.detach().requires_grad_() for t in (state, x, weight, bias)]
+        out, y = J.stabilize(*(neg(t) for t in leaves), scale=0.5)
+        results.append((out, y, *torch.autograd.grad((out, y), leaves, (neg(gs), neg(gy)))))
+    assert torch._neg_view(gy).is_neg() and torch._neg_view(gy).is_contiguous()
+    for eager, late in zip(*results):
+        assert torch.equal(eager, late)
+
+
 def test_transforms(dev):
     """vmap runs it slice by slice; torch.func's gradients and forward mode raise."""
     import jakal_net as J

@@ -84,6 +84,30 @@ std::shared_ptr<Node> make_node() {
   return std::shared_ptr<Node>(new Node(), torch::autograd::deleteNode);
 }
 
+// A tensor kept for the backward, or none.  Hooks on saved tensors may give back
+// another than was saved; the kernels read what its type and size were.
+class Kept {
+ public:
+  void set(const Tensor& t) {
+    saved_ = SavedVariable(t, false);
+    if (!t.defined()) return;
+    device_ = t.device(), type_ = t.scalar_type(), count_ = t.numel();
+  }
+  Tensor get() const {
+    const Tensor t = saved_.unpack();
+    TORCH_CHECK(t.defined() ? t.device() == device_ && t.scalar_type() == type_ && t.numel() == count_ : count_ < 0,
+                "jakal_net_native: a saved tensor came back with another device, type or size.");
+    return plain(t);
+  }
+  void reset() { saved_.reset_data(); }
+
+ private:
+  SavedVariable saved_;
+  c10::Device device_ = at::kCPU;
+  at::ScalarType type_ = at::kFloat;
+  int64_t count_ = -1;  // none
+};
+
 // The gradients of a backward that is recorded itself (create_graph) raise when
 // they are differentiated: the operators have a first derivative only.
 variable_list once_differentiable(variable_list grads, bool recorded) {
@@ -104,7 +128,7 @@ struct NormCall {
 };
 
 struct JakalRowNormBackward : torch::autograd::Node {
-  SavedVariable state_, x_, weight_, stats_;
+  Kept state_, x_, weight_, stats_;
   NormCall call{};
   bool has_state = false;
   at::ScalarType bias_type = at::kFloat;
@@ -113,17 +137,17 @@ struct JakalRowNormBackward : torch::autograd::Node {
 
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    state_.reset_data();
-    x_.reset_data();
-    weight_.reset_data();
-    stats_.reset_data();
+    state_.reset();
+    x_.reset();
+    weight_.reset();
+    stats_.reset();
   }
 
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     const bool recorded = at::GradMode::is_enabled();
     const at::AutoGradMode off(false);
-    const Tensor state = state_.unpack(), x = x_.unpack(), weight = weight_.unpack(), stats = stats_.unpack();
+    const Tensor state = state_.get(), x = x_.get(), weight = weight_.get(), stats = stats_.get();
     Tensor g_state = has_state ? grads[0] : Tensor(), g = grads[has_state ? 1 : 0];
     // wanted: what something takes, of outputs that something used
     bool need[4];
@@ -214,10 +238,10 @@ std::tuple<Tensor, Tensor> row_norm(const Tensor& state_in, const Tensor& x_in, 
                                 stream_of(x)));
   }
   if (node) {
-    node->state_ = SavedVariable(state, false);
-    node->x_ = SavedVariable(x, false);
-    node->weight_ = SavedVariable(weight, false);
-    node->stats_ = SavedVariable(stats, false);
+    node->state_.set(state);
+    node->x_.set(x);
+    node->weight_.set(weight);
+    node->stats_.set(stats);
     node->call = call;
     node->has_state = state.defined();
     if (bias.defined()) node->bias_type = bias.scalar_type();
@@ -239,17 +263,17 @@ std::tuple<Tensor, Tensor> stabilize(const Tensor& state, const Tensor& val, con
 
 // ---- cross entropy ------------------------------------------------------------
 struct JakalCrossEntropyBackward : torch::autograd::Node {
-  SavedVariable logits_, target_, stats_, count_;
+  Kept logits_, target_, stats_, count_;
   int64_t ignore_index = 0, reduction = 0;
 
   std::string name() const override { return "JakalCrossEntropyBackward"; }
 
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    logits_.reset_data();
-    target_.reset_data();
-    stats_.reset_data();
-    count_.reset_data();
+    logits_.reset();
+    target_.reset();
+    stats_.reset();
+    count_.reset();
   }
 
   variable_list apply(variable_list&& grads) override {
@@ -257,8 +281,8 @@ struct JakalCrossEntropyBackward : torch::autograd::Node {
     const bool recorded = at::GradMode::is_enabled();
     const at::AutoGradMode off(false);
     if (!grads[0].defined() || !task_should_compute_output(0)) return {Tensor()};
-    const Tensor logits = logits_.unpack(), target = target_.unpack(), stats = stats_.unpack(),
-                 count = count_.unpack();
+    const Tensor logits = logits_.get(), target = target_.get(), stats = stats_.get(),
+                 count = count_.get();
     const c10::DeviceGuard guard(logits.device());
     const Tensor out = at::empty_like(logits);
     if (target.numel()) {
@@ -308,10 +332,10 @@ Tensor cross_entropy(const Tensor& logits_in, const Tensor& target_in, int64_t i
   }
   const Tensor& out = reduction ? reduced : loss;
   if (node) {
-    node->logits_ = SavedVariable(logits, false);
-    node->target_ = SavedVariable(target, false);
-    node->stats_ = SavedVariable(stats, false);
-    node->count_ = SavedVariable(count, false);
+    node->logits_.set(logits);
+    node->target_.set(target);
+    node->stats_.set(stats);
+    node->count_.set(count);
     node->ignore_index = ignore_index;
     node->reduction = reduction;
     torch::autograd::set_history(out, node);

@@ -129,3 +129,57 @@ def test_two_captured_clipped_steps_replay_as_eager(dev):
             got = [loss, norm] + [p.data for p in m.parameters()]
             assert float(norm) > 0.1, "the step has to clip"
             assert all(torch.equal(a, b) for a, b in zip(got, w)), f"replay {rep}"
+
+
+def _update_and_loss(dev):
+    """A layer update and a loss over its values, and the leaves it starts from."""
+    import jakal_net as J
+
+    g = torch.Generator().manual_seed(3)
+    leaves = [torch.randn(shape, generator=g).to(dev).requires_grad_() for shape in ((2, 9), (2, 9, 40), (40,), (40,))]
+    target = torch.randint(0, 40, (2, 9), generator=g).to(dev)
+
+    def run(state, val, weight, bias):
+        out, y = J.stabilize(state, val, weight, bias, scale=0.5)
+        return J.cross_entropy(y, target) + out.square().sum()
+
+    return run, leaves
+
+
+def _other_order(t):
+    """t, its elements in another order in memory."""
+    return t.transpose(0, -1).contiguous().transpose(0, -1) if t.dim() > 1 else t.clone()
+
+
+@pytest.mark.parametrize("kind", ["cpu", "order", "checkpoint", "reentrant checkpoint"])
+def test_saved_tensors_that_come_back(dev, kind):
+    from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
+    from torch.utils.checkpoint import checkpoint
+
+    run, leaves = _update_and_loss(dev)
+    want = torch.autograd.grad(run(*leaves), leaves)
+    if kind == "cpu":
+        with save_on_cpu():
+            loss = run(*leaves)
+    elif kind == "order":
+        with saved_tensors_hooks(lambda t: t, _other_order):
+            loss = run(*leaves)
+    else:
+        loss = checkpoint(run, *leaves, use_reentrant=kind.startswith("reentrant"))
+    loss.backward()
+    assert all(torch.equal(p.grad, g) for p, g in zip(leaves, want))
+
+
+@pytest.mark.parametrize("change", [torch.Tensor.bfloat16, torch.Tensor.cpu, lambda t: t.reshape(-1)[:1],
+                                    lambda t: t.reshape(-1).repeat(2)], ids=["type", "device", "shorter", "longer"])
+def test_saved_tensors_that_come_back_changed_raise(dev, change):
+    import jakal_net as J
+    from torch.autograd.graph import saved_tensors_hooks
+
+    _, (state, val, weight, bias) = _update_and_loss(dev)
+    target = torch.zeros(2, 9, dtype=torch.long, device=dev)
+    with saved_tensors_hooks(lambda t: t, change):
+        losses = [J.layer_norm(val, weight, bias).sum(), J.stabilize(state, val)[0].sum(), J.cross_entropy(val, target)]
+    for loss in losses:
+        with pytest.raises(RuntimeError, match="came back"):
+            loss.backward()

@@ -7,7 +7,7 @@ step, scale included, as one operator; ``layer_norm`` is its norm alone.
 
 ``implementation`` as in the operators: ``"native"`` (the default here) runs the
 HIP library for GPU tensors of fp32, bf16 or fp16 and raises where it cannot,
-CPU tensors take the PyTorch form; ``"kernel"`` takes the PyTorch form where
+CPU tensors (and a native module without these operators) take the PyTorch form; ``"kernel"`` takes the PyTorch form where
 the library declines; ``"reference"`` and ``"streaming"`` are the PyTorch form.
 The library computes in fp32 and rounds once; under autocast half-precision
 values come back in fp32, as torch's layer norm returns them.

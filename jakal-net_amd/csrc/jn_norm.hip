@@ -398,26 +398,33 @@ __global__ __launch_bounds__(kAnyThreads) void norm_columns_any_kernel(NormArgs 
   }
 }
 
-// The partial sums of all workgroups or slabs: 16 columns a workgroup, each by
-// 64 threads that take every 64th partial (512 x 1024 sums in 3.9 us).
+// The partial sums of all workgroups or slabs: 16 columns a workgroup at a time,
+// each by 64 threads that take every 64th partial (512 x 1024 sums in 3.9 us).
+// A launch has fewer than 2^32 threads along an axis, which 2^25 columns of dw
+// and db would reach in workgroups of their own, so that those step.
 constexpr int kFinishColumns = 16, kFinishLanes = 64;
+constexpr int64_t kFinishGroups = 1 << 16;
 __global__ __launch_bounds__(kFinishColumns* kFinishLanes) void norm_columns_finish_kernel(NormArgs a, int parts) {
   __shared__ float lds[kFinishLanes][kFinishColumns + 1];
   const int col = threadIdx.x % kFinishColumns, lane = threadIdx.x / kFinishColumns;
-  const int64_t c = (int64_t)blockIdx.x * kFinishColumns + col;  // of dw's columns and then db's
-  float s = 0.f;
-  if (c < 2 * a.dim) {
+  for (int64_t first = (int64_t)blockIdx.x * kFinishColumns; first < 2 * a.dim;
+       first += (int64_t)gridDim.x * kFinishColumns) {
+    const int64_t c = first + col;  // of dw's columns and then db's
+    float s = 0.f;
+    if (c < 2 * a.dim) {
 #pragma unroll 4
-    for (int p = lane; p < parts; p += kFinishLanes) s += a.partial[(int64_t)p * 2 * a.dim + c];
-  }
-  lds[lane][col] = s;
-  for (int step = kFinishLanes / 2; step > 0; step /= 2) {
+      for (int p = lane; p < parts; p += kFinishLanes) s += a.partial[(int64_t)p * 2 * a.dim + c];
+    }
+    lds[lane][col] = s;
+    for (int step = kFinishLanes / 2; step > 0; step /= 2) {
+      __syncthreads();
+      if (lane < step) lds[lane][col] += lds[lane + step][col];
+    }
+    if (lane == 0 && c < 2 * a.dim) {
+      void* out = c < a.dim ? a.dw : a.db;
+      if (out) store_any(out, c < a.dim ? c : c - a.dim, a.param_type, lds[0][col]);
+    }
     __syncthreads();
-    if (lane < step) lds[lane][col] += lds[lane + step][col];
-  }
-  if (lane == 0 && c < 2 * a.dim) {
-    void* out = c < a.dim ? a.dw : a.db;
-    if (out) store_any(out, c < a.dim ? c : c - a.dim, a.param_type, lds[0][col]);
   }
 }
 
@@ -551,9 +558,10 @@ int launch_norm_forward(const NormArgs& a, hipStream_t s) {
 }
 
 int launch_columns_finish(const NormArgs& a, int64_t parts, hipStream_t s) {
+  const int64_t groups = std::min((2 * a.dim + kFinishColumns - 1) / kFinishColumns, kFinishGroups);
   JN_PROFILE("norm_columns_finish_kernel", s);
-  hipLaunchKernelGGL(norm_columns_finish_kernel, dim3((unsigned)((2 * a.dim + kFinishColumns - 1) / kFinishColumns)),
-                     dim3(kFinishColumns * kFinishLanes), 0, s, a, (int)parts);
+  hipLaunchKernelGGL(norm_columns_finish_kernel, dim3((unsigned)groups), dim3(kFinishColumns * kFinishLanes), 0, s, a,
+                     (int)parts);
   JN_LAUNCH_CHECK();
   return kOk;
 }

@@ -308,9 +308,30 @@ __global__ __launch_bounds__(BLOCK) void norm_backward_kernel(NormArgs a) {
 }
 
 // Rows of any width and alignment: a workgroup a row, three passes over it, two of
-// them from L2 (2,048 x 16,384 fp32: forward 118 us, backward 186).
+// them from L2 (fp32, forward and backward with parameter gradients: 1,024 x 16,384
+// 53 and 94 us, 2,048 x 16,384 99 and 167, 3,000 x 16,384 128 and 287, 512 x 33,000
+// 75 and 150).
 constexpr int kAnyThreads = 256;
 constexpr int kAnyWaves = kAnyThreads / kWave;
+
+// The sum of term(i) over a row by a workgroup, the same in every thread.  A
+// thread adds 256 terms in fp32 and those sums in 64 bits: a row of 2^28 gives
+// it 2^20 terms, whose sum in fp32 alone drops digits of every term (of a constant
+// 0.1 the mean of 2^26 came out 150 times as far off as runs of 256 may be).  Eight
+// loads in flight: one at a time took 129 us for the forward of 512 x 33,000.
+constexpr int64_t kRun = 256 * kAnyThreads;  // elements
+template <typename F>
+__device__ __forceinline__ float row_sum(int64_t dim, float* lds, F term) {
+  double s = 0.0;
+  for (int64_t first = 0; first < dim; first += kRun) {
+    const int64_t end = min(dim, first + kRun);
+    float run = 0.f;
+#pragma unroll 8
+    for (int64_t i = first + threadIdx.x; i < end; i += kAnyThreads) run += term(i);
+    s += run;
+  }
+  return group_sum<kAnyWaves>((float)s, lds);
+}
 
 template <typename T>
 __global__ __launch_bounds__(kAnyThreads) void norm_forward_any_kernel(NormArgs a) {
@@ -319,15 +340,12 @@ __global__ __launch_bounds__(kAnyThreads) void norm_forward_any_kernel(NormArgs 
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.dim;
     T* y = static_cast<T*>(a.y) + row * a.dim;
-    float s = 0.f;
-    for (int64_t i = threadIdx.x; i < a.dim; i += kAnyThreads) s += a.scale * (float)x[i];
-    const float m = group_sum<kAnyWaves>(s, lds) / n;
-    s = 0.f;
-    for (int64_t i = threadIdx.x; i < a.dim; i += kAnyThreads) {
+    const float m = row_sum(a.dim, lds, [&](int64_t i) { return a.scale * (float)x[i]; }) / n;
+    const float var = row_sum(a.dim, lds, [&](int64_t i) {
       const float c = a.scale * (float)x[i] - m;
-      s += c * c;
-    }
-    const float r = 1.0f / sqrtf(group_sum<kAnyWaves>(s, lds) / n + a.eps);
+      return c * c;
+    }) / n;
+    const float r = 1.0f / sqrtf(var + a.eps);
     for (int64_t i = threadIdx.x; i < a.dim; i += kAnyThreads) {
       const float h = (a.scale * (float)x[i] - m) * r;
       y[i] = (T)(h * param(a.w, i, a.param_type, 1.0f) + param(a.b, i, a.param_type, 0.0f));
@@ -353,14 +371,19 @@ __global__ __launch_bounds__(kAnyThreads) void norm_backward_any_kernel(NormArgs
     const T* g = static_cast<const T*>(a.g) + row * a.dim;
     T* dx = static_cast<T*>(a.dx) + row * a.dim;
     const float m = a.stats[2 * row], r = a.stats[2 * row + 1];
-    float s1 = 0.f, s2 = 0.f;
-    for (int64_t i = threadIdx.x; i < a.dim; i += kAnyThreads) {
-      const float gw = (float)g[i] * param(a.w, i, a.param_type, 1.0f);
-      s1 += gw;
-      s2 += gw * ((a.scale * (float)x[i] - m) * r);
+    double d1 = 0.0, d2 = 0.0;
+    for (int64_t first = 0; first < a.dim; first += kRun) {
+      const int64_t end = min(a.dim, first + kRun);
+      float run1 = 0.f, run2 = 0.f;
+      for (int64_t i = first + threadIdx.x; i < end; i += kAnyThreads) {
+        const float gw = (float)g[i] * param(a.w, i, a.param_type, 1.0f);
+        run1 += gw;
+        run2 += gw * ((a.scale * (float)x[i] - m) * r);
+      }
+      d1 += run1, d2 += run2;
     }
-    s1 = group_sum<kAnyWaves>(s1, lds) / n;
-    s2 = group_sum<kAnyWaves>(s2, lds) / n;
+    const float s1 = group_sum<kAnyWaves>((float)d1, lds) / n;
+    const float s2 = group_sum<kAnyWaves>((float)d2, lds) / n;
     const float sr = a.scale * r;
     for (int64_t i = threadIdx.x; i < a.dim; i += kAnyThreads) {
       const float gw = (float)g[i] * param(a.w, i, a.param_type, 1.0f);

@@ -533,6 +533,14 @@ BackwardGrid backward_grid(const RowShape& s, int64_t rows, bool columns) {
 constexpr int64_t kSlabs = 64;
 int64_t slab_count(int64_t rows) { return std::min<int64_t>(kSlabs, (rows + 15) / 16); }
 
+// Rows of partial sums that a backward with parameter gradients leaves: a slab's
+// or a workgroup's each (the shape's threads go by the width alone).  A single
+// workgroup leaves none, and is given one.
+int64_t part_count(int64_t rows, int64_t dim) {
+  const RowShape shape = row_shape(dim, false, sizeof(float));
+  return shape.threads ? backward_grid(shape, rows, true).groups : slab_count(rows);
+}
+
 // Workgroups of the forward: eight of four waves a CU.
 constexpr int64_t kForwardGroups = 2048;
 
@@ -654,7 +662,7 @@ int jn_layer_norm_forward(const void* state, const void* x, const void* weight, 
 
 size_t jn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t dim) {
   if (rows < 1 || dim < 1 || dim >= (1LL << 28)) return 0;
-  return (size_t)std::min(rows, kMaxParts) * 2 * dim * sizeof(float);  // no more parts or slabs than rows
+  return (size_t)part_count(rows, dim) * 2 * dim * sizeof(float);
 }
 
 int jn_layer_norm_backward(const void* state, const void* x, const void* weight, const float* stats,

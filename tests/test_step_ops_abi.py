@@ -1,0 +1,27 @@
+"""Sizes and limits that the training-step operators' C ABI states on the host."""
+
+import pytest
+
+
+def _lib():
+    import jakal_net_native as jn
+
+    return jn._LIB
+
+
+@pytest.mark.parametrize("rows,dim", [(512, 262144), (100, 8193), (9, 33000), (1 << 20, 8200)])
+def test_norm_workspace_of_wide_rows_is_its_slabs(rows, dim):
+    """Rows beyond 8,192 elements are summed by slabs of 16 rows or more, 64 at most."""
+    slabs = min(64, (rows + 15) // 16)
+    assert _lib().jn_layer_norm_backward_workspace_bytes(rows, dim) == slabs * 2 * dim * 4
+
+
+@pytest.mark.parametrize("dim", [1, 8, 100, 512, 1000, 4096, 8192])
+def test_norm_workspace_of_register_rows_is_its_workgroups(dim):
+    """One row of partial sums a workgroup, which has 256 threads at least and takes a row by 16 to 1024 of them."""
+    threads = 16
+    while dim > 8 * threads:
+        threads *= 2
+    for rows in (1, 4, 70, 1000, 2047, 2048, 70000, 1 << 24):
+        parts, rest = divmod(_lib().jn_layer_norm_backward_workspace_bytes(rows, dim), 2 * dim * 4)
+        assert rest == 0 and 1 <= parts <= min(512, -(-rows // max(1, 256 // threads)))

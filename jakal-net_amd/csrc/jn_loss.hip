@@ -57,6 +57,12 @@ struct RowSpan {
 
 // A running maximum m and the sum s of exponentials below it.  s is 0 under a
 // maximum of -inf, and NaN once a NaN or +inf was met.
+//
+// The sums take the hardware's 2^t of t = x log2(e), whose rounding makes |x| / 2
+// ulps of a term.  Of log s that is 2^-24 times the mean of |x| under the softmax
+// at most, and that mean is log(classes) at most: an ulp of the loss where all
+// terms round the same way, less where they differ.  8,192 rows of 16,384 bf16
+// classes, a fifth ignored, take 41 us so, 68 with expf() and 52 with exp_of().
 struct LogSum {
   float m = -INFINITY, s = 0.f;
 
@@ -234,6 +240,22 @@ __global__ __launch_bounds__(kReduceThreads) void loss_reduce_kernel(LossArgs a)
   }
 }
 
+// e^x for x <= 0 (or NaN), to 1.2 ulps: the hardware's 2^t of t = x log2(e),
+// times e^(what the rounding of t lost), which is 1 + that; without it x = -80
+// is off by 40 ulps.  Below -150 the result is 0, and -inf has no rounding to
+// give back.  The fp32 gradient takes this (8,192 x 2,048 in 19.1 us either way,
+// 1,531 x 4,099 in 9.1 against 8.7; expf() 19.5 and 9.1).  Half-precision ones
+// round to 2^-8 or 2^-11 of their value behind it, a hundred times what __expf
+// loses at -80, and would pay 11.4 us instead of 9.5 at 1,024 x 16,384 bf16.
+__device__ __forceinline__ float exp_of(float x) {
+  constexpr float kLog2E = 0x1.715476p+0f, kLog2ELow = 0x1.4ae0cp-26f, kLn2 = 0x1.62e43p-1f;  // log2(e) = the two's sum
+  x = x < -150.0f ? -150.0f : x;
+  const float t = x * kLog2E;
+  const float lost = fmaf(x, kLog2ELow, fmaf(x, kLog2E, -t));
+  const float p = __builtin_amdgcn_exp2f(t);
+  return fmaf(p, lost * kLn2, p);
+}
+
 // The gradient of a stretch of a row: kPacks packs a thread (and the row's
 // single elements, with its first stretch).  W = 1 where the gradient's rows do
 // not start on 16 bytes where the logits' do.  The logits are read for the last
@@ -248,7 +270,10 @@ __device__ __forceinline__ void loss_gradient(const T* z, T* dz, int64_t e, int6
   float v[W];
   raw.unpack(v);
 #pragma unroll
-  for (int j = 0; j < W; ++j) v[j] = __expf((v[j] - m) - l);
+  for (int j = 0; j < W; ++j) {
+    const float x = (v[j] - m) - l;
+    v[j] = std::is_same_v<T, float> ? exp_of(x) : __expf(x);
+  }
   const int64_t hot = t - e;
   if (hot >= 0 && hot < W) {
 #pragma unroll

@@ -265,7 +265,7 @@ __device__ __forceinline__ float exp_of(float x) {
 // 149 and 173, 8,192 339 and 386.  By itself 8,192 rows, a fifth ignored, take
 // 67 us (485 MB, 7.3 TB/s).
 template <typename T, int W>
-__device__ __forceinline__ void loss_gradient(const T* z, T* dz, int64_t e, int64_t t, float m, float l, float c,
+__device__ __forceinline__ void loss_gradient(T* dz, int64_t e, int64_t t, float m, float l, float c,
                                               const Raw<T, W>& raw) {
   float v[W];
   raw.unpack(v);
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(THREADS == kWave ? 4 * kWave : THREADS) void loss_b
       if (one >= 0) {
         Raw<T, 1> raw;
         if (ignored) dz[one] = (T)0.0f;
-        else raw.load(z + one), loss_gradient<T, 1>(z, dz, one, t, m, l, c, raw);
+        else raw.load(z + one), loss_gradient<T, 1>(dz, one, t, m, l, c, raw);
       }
     }
     for (int64_t first = blockIdx.y * kStretch + thread; first < packs; first += gridDim.y * kStretch) {
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(THREADS == kWave ? 4 * kWave : THREADS) void loss_b
         const int64_t p = first + i * THREADS;
         if (p >= packs) continue;
         if (ignored) raw[i].template store<true>(dz + head + p * W);
-        else loss_gradient<T, W>(z, dz, head + p * W, t, m, l, c, raw[i]);
+        else loss_gradient<T, W>(dz, head + p * W, t, m, l, c, raw[i]);
       }
     }
   }

@@ -39,7 +39,7 @@ typedef void* jn_stream_t;
 /* Message of the last failing call on this host thread ("" if none). */
 const char* jn_last_error(void);
 
-/* ABI revision of this header (bumped on any signature or accepted-range change); this is 18. */
+/* ABI revision of this header (bumped on any signature or accepted-range change); this is 19. */
 int jn_abi_version(void);
 
 /*
@@ -944,6 +944,17 @@ int jn_layer_norm_backward(const void* state, const void* x, const void* weight,
 int jn_cross_entropy_forward(const void* logits, const int64_t* target, int64_t rows, int64_t classes,
                              int64_t ignore_index, int32_t reduction, int32_t type, float* loss, float* stats,
                              float* reduced, float* count, jn_stream_t stream);
+
+/*
+ * The reduction of a forward's losses by itself, for many rows: after
+ * jn_cross_entropy_forward with reduction 0, *reduced and *count as with
+ * reduction 1 or 2.  That call's own reduction is one workgroup's whatever the
+ * rows; this one takes many where the size query is not 0.
+ */
+size_t jn_cross_entropy_reduce_workspace_bytes(int64_t rows);
+int jn_cross_entropy_reduce(const float* loss, const int64_t* target, int64_t rows, int64_t ignore_index,
+                            int32_t reduction, float* reduced, float* count, void* workspace, size_t workspace_bytes,
+                            jn_stream_t stream);
 
 /*
  * grad_logits = (softmax(z) - onehot(target)) * c, 0 in ignored rows; c is

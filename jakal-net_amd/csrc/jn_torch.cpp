@@ -325,9 +325,16 @@ Tensor cross_entropy(const Tensor& logits_in, const Tensor& target_in, int64_t i
     }
     if (node) stats = at::empty({rows, 2}, f32);
     if (rows) {
+      // the losses of many rows are reduced by many workgroups, in a call of its own
+      const size_t bytes = reduction ? jn_cross_entropy_reduce_workspace_bytes(rows) : 0;
       check(jn_cross_entropy_forward(ptr(logits), target.data_ptr<int64_t>(), rows, logits.size(-1), ignore_index,
-                                     (int32_t)reduction, type, fptr(loss), fptr(stats), fptr(reduced), fptr(count),
-                                     stream_of(logits)));
+                                     bytes ? 0 : (int32_t)reduction, type, fptr(loss), fptr(stats), fptr(reduced),
+                                     fptr(count), stream_of(logits)));
+      if (bytes) {
+        const Tensor ws = at::empty({(int64_t)bytes}, f32.dtype(at::kByte));
+        check(jn_cross_entropy_reduce(fptr(loss), target.data_ptr<int64_t>(), rows, ignore_index, (int32_t)reduction,
+                                      fptr(reduced), fptr(count), ptr(ws), bytes, stream_of(logits)));
+      }
     }
   }
   const Tensor& out = reduction ? reduced : loss;

@@ -211,6 +211,8 @@ _declare("jn_layer_norm_backward_workspace_bytes", [_I64] * 2, _SZ)
 _declare("jn_layer_norm_backward",
          [_P] * 6 + [_I64] * 2 + [_F] + [_I32] * 3 + [_P] * 4 + [_P, _SZ, _P])
 _declare("jn_cross_entropy_forward", [_P] * 2 + [_I64] * 3 + [_I32] * 2 + [_P] * 5)
+_declare("jn_cross_entropy_reduce_workspace_bytes", [_I64], _SZ)
+_declare("jn_cross_entropy_reduce", [_P] * 2 + [_I64] * 2 + [_I32] + [_P] * 2 + [_P, _SZ, _P])
 _declare("jn_cross_entropy_backward", [_P] * 5 + [_I64] * 3 + [_I32] * 2 + [_P] * 2)
 _declare("jn_grads_workspace_bytes", [_I64], _SZ)
 _declare("jn_grads_norm", [_P] * 3 + [_I64, _I32] + [_P, _P, _SZ, _P])

@@ -1,5 +1,7 @@
 """Sizes and limits that the training-step operators' C ABI states on the host."""
 
+import ctypes
+
 import pytest
 
 
@@ -25,3 +27,19 @@ def test_norm_workspace_of_register_rows_is_its_workgroups(dim):
     for rows in (1, 4, 70, 1000, 2047, 2048, 70000, 1 << 24):
         parts, rest = divmod(_lib().jn_layer_norm_backward_workspace_bytes(rows, dim), 2 * dim * 4)
         assert rest == 0 and 1 <= parts <= min(512, -(-rows // max(1, 256 // threads)))
+
+
+def test_loss_reduction_checks():
+    lib = _lib()
+    p = ctypes.c_void_p(4096)  # never read: every call below fails
+    size = lib.jn_cross_entropy_reduce_workspace_bytes
+    assert [size(n) for n in (-1, 0, 1, 32768)] == [0] * 4 and size(32769) == 9 * 16 and size(1 << 40) == 256 * 16
+
+    def call(loss=p, target=p, rows=100000, reduction=2, reduced=p, count=p, ws=p, ws_bytes=1 << 20):
+        return lib.jn_cross_entropy_reduce(loss, target, rows, -100, reduction, reduced, count, ws, ws_bytes, None)
+
+    for bad in (dict(loss=None), dict(target=None), dict(rows=0), dict(rows=(1 << 40) + 1), dict(reduction=0),
+                dict(reduction=3), dict(reduced=None), dict(count=None)):
+        assert call(**bad) == 1, bad
+    for bad in (dict(ws=None), dict(ws_bytes=size(100000) - 1)):
+        assert call(**bad) == 4, bad

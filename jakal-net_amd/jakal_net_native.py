@@ -14,7 +14,9 @@ rows, the top-k scores run on bf16 MFMAs, and the outputs and value gradients
 come back in bf16.  Gradients come from
 ``torch.autograd.Function`` wrappers whose backward calls the library's
 backward entry points.  Importing this module fails if the library cannot be
-loaded; nothing here computes on the CPU.
+loaded; nothing here computes on the CPU.  The operators of a training step
+are C++ PyTorch operators in ``lib/libjakal_net_torch.so``; where that cannot
+be loaded they raise, and the rest runs.
 """
 
 from __future__ import annotations
@@ -39,7 +41,14 @@ def library_path() -> Path:
 
 # global symbols: the PyTorch operators of libjakal_net_torch.so call this library
 _LIB = ctypes.CDLL(str(library_path()), mode=ctypes.RTLD_GLOBAL)
-torch.ops.load_library(str(_HERE / "lib" / "libjakal_net_torch.so"))
+# That one is bound to the torch it was built against.  Without it the ops over
+# ctypes run all the same, and its operators raise what kept it from loading.
+_TORCH_LIB = _HERE / "lib" / "libjakal_net_torch.so"
+_torch_lib_error: str | None = None
+try:
+    torch.ops.load_library(str(_TORCH_LIB))
+except OSError as exc:
+    _torch_lib_error = str(exc)
 
 _P, _I64, _I32, _F, _SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_size_t
 
@@ -1970,12 +1979,19 @@ def low_rank_pairwise_topk_backward_cuda(query_val: Tensor, source_val: Tensor, 
 # operators of a training step beside the propagation ops
 # ---------------------------------------------------------------------------
 # Their checks, allocations and autograd nodes are C++ (csrc/jn_torch.cpp).
-_OPS = torch.ops.jakal_net_hip
-_layer_norm = _OPS.layer_norm.default
-_stabilize = _OPS.stabilize.default
-_cross_entropy = _OPS.cross_entropy.default
-_grad_norm = _OPS.grad_norm.default
-_clip_grads = _OPS.clip_grads.default
+def _torch_op(name: str):
+    if _torch_lib_error is None:
+        return getattr(torch.ops.jakal_net_hip, name).default
+
+    def missing(*args):
+        raise NotImplementedError(f"jakal_net_native.{name} needs {_TORCH_LIB.name}, which did not load: "
+                                  f"{_torch_lib_error}")
+
+    return missing
+
+
+_layer_norm, _stabilize, _cross_entropy, _grad_norm, _clip_grads = map(
+    _torch_op, ("layer_norm", "stabilize", "cross_entropy", "grad_norm", "clip_grads"))
 
 
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5) -> Tensor:

@@ -169,18 +169,18 @@ __device__ __forceinline__ void write_reduced(const LossArgs& a, double s, doubl
 }
 
 // Few logits in one launch: a workgroup of sixteen waves takes all rows, a wave
-// every sixteenth, and reduces their losses.
+// each, and reduces their losses.
 constexpr int kSmallWaves = 16;
 template <typename T>
 __global__ __launch_bounds__(kSmallWaves* kWave) void loss_small_kernel(LossArgs a) {
   __shared__ double lds[kSmallWaves][2];
   double s = 0.0, n = 0.0;
-  for (int64_t row = wave_id(); row < a.rows; row += kSmallWaves) {
+  if (const int row = wave_id(); row < a.rows) {
     const int64_t t = a.target[row];
     const bool counts = t != a.ignore, inside = t >= 0 && t < a.classes;
     float loss = 0.f;
     if (counts) {
-      const T* z = static_cast<const T*>(a.z) + row * a.classes;
+      const T* z = static_cast<const T*>(a.z) + (int64_t)row * a.classes;
       const float zt = inside ? (float)z[t] : NAN;
       const LogSum sum = row_log_sum<T, kWave>(z, a.classes, nullptr);
       const float l = logf(sum.s);
@@ -191,8 +191,8 @@ __global__ __launch_bounds__(kSmallWaves* kWave) void loss_small_kernel(LossArgs
       }
     }
     if (lane_id() == 0) a.loss[row] = loss;
-    s += loss;
-    n += counts ? 1.0 : 0.0;
+    s = loss;
+    n = counts ? 1.0 : 0.0;
   }
   if (lane_id() == 0) {
     lds[wave_id()][0] = s;
@@ -391,10 +391,15 @@ int check_loss(const LossArgs& a, int32_t type) {
 // against 32.8 and 29.8, 8,192 bf16 31.0 and 56.7 against 38.3 and 48.9 (two
 // chunks); fp32 2,048 17.6 and 28.0 against 20.8 and 28.1, 4,099 30.3 and 56.9
 // against 28.2 and 47.5 (two chunks); at 1,024 rows they are equal.
-// One workgroup takes 16 x 64 fp32 logits and their mean in 3.1 us, 64 x 1,000 in
-// 8.4, 8 x 8,000 in 6.0; two launches take 6 to 7 and the host 4 more.
-constexpr int64_t kSmallRows = 64;
+// One launch by one workgroup where each of its waves has one row at most, short
+// enough for a wave (a captured call, one launch against two, fp32 and bf16: 16 x
+// 64 2.9 and 3.7 against 4.9 and 5.6 us, 16 x 4,000 5.5 and 5.3 against 6.4 and
+// 6.5, 8 x 8,000 5.9 and 5.8 against 6.4 and 6.9; two rows a wave, 32 x 1,000,
+// 5.1 and 6.3 against 5.1 and 5.3, 64 x 1,000 8.5 and 10.5 against 5.1 and 5.3;
+// longer rows, 4 x 16,000, 8.5 and 7.1 against 6.6 and 6.9, 1 x 64,000 27 and 20
+// against 8.4 and 8.1).  The second launch costs the host 4 us.
 constexpr int64_t kSmallBytes = 256 << 10;
+constexpr int64_t kSmallRowBytes = 32 << 10;
 constexpr int64_t kWaveClasses = 1024;
 constexpr int64_t kWaveRows = 1024;
 constexpr int64_t kFewRows = 512;
@@ -455,7 +460,9 @@ int jn_cross_entropy_forward(const void* logits, const int64_t* target, int64_t 
   JN_REQUIRE(logits && target && loss && ((reduced && count) || reduction == kNone), kInvalidArgument,
              "null tensor pointer");
   const auto s = static_cast<hipStream_t>(stream);
-  const bool small = reduction != kNone && rows <= kSmallRows && rows * classes * type_bytes(type) <= kSmallBytes;
+  const int64_t row_bytes = classes * type_bytes(type);
+  const bool small = reduction != kNone && rows <= kSmallWaves && row_bytes <= kSmallRowBytes &&
+                     rows * row_bytes <= kSmallBytes;
   const int rc = with_type(type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
     if (!small) return launch_loss_forward<T>(a, s);

@@ -510,11 +510,13 @@ int with_shape(const RowShape& s, F f) {
 // the workgroups fill the CUs.
 constexpr int64_t kMaxParts = 512;
 constexpr int64_t kManyRows = 2048;
-constexpr int64_t kFewSteps = 4;
+constexpr int64_t kFewSteps = 2;
 
-// A workgroup that has all rows in a few steps needs no partial sums and no
-// second launch: 32 x 512 fp32 in 6.6 us, 4 x 4,096 in 8.2, against 7 to 8 in two
-// launches that cost the host 4 more (sixteen steps: 18 and 22).
+// A workgroup that has all rows in two steps needs no partial sums and no second
+// launch (fp32, captured, one launch against two: one step 8 x 512 3.9 against 6.0
+// us, 32 x 64 3.3 and 5.0; two steps 16 x 512 4.8 and 6.1, 2 x 4,096 6.0 and 7.8;
+// four 32 x 512 6.6 and 6.2, 16 x 1,024 7.7 and 6.6, 4 x 4,096 8.2 and 7.8).  The
+// second launch costs the host 4 us.
 bool one_workgroup(const RowShape& s, int64_t rows) { return rows <= kFewSteps * std::max(512 / s.threads, 1); }
 
 struct BackwardGrid {

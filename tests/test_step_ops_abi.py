@@ -43,3 +43,11 @@ def test_loss_reduction_checks():
         assert call(**bad) == 1, bad
     for bad in (dict(ws=None), dict(ws_bytes=size(100000) - 1)):
         assert call(**bad) == 4, bad
+
+
+@pytest.mark.parametrize("dim,step", [(64, 32), (512, 8), (4096, 1), (8192, 1)])
+def test_norm_rows_of_two_steps_stay_in_one_workgroup(dim, step):
+    """step: the rows that a workgroup of 512 threads (1024 for the widest) has at a time."""
+    size = _lib().jn_layer_norm_backward_workspace_bytes
+    one = 2 * dim * 4
+    assert size(1, dim) == size(2 * step, dim) == one and size(2 * step + 1, dim) > one

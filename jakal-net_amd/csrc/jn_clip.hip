@@ -23,7 +23,7 @@ namespace {
 constexpr int kClipThreads = 256;
 constexpr int kChunk = 8192;         // elements
 constexpr int kListMax = 164;        // tensors of one launch (4 KB of kernel arguments)
-constexpr int64_t kMaxPartials = 2048;
+constexpr int64_t kMaxPartials = 2048;  // shared out over the launches; beyond it one for each further launch
 
 struct TensorList {
   const void* in[kListMax];
@@ -183,8 +183,8 @@ __device__ __forceinline__ void chunk_scale_to(const TI* p, void* out, int64_t b
   else chunk_scale<STREAM>(p, static_cast<f16_t*>(out) + begin, n, scale);
 }
 
-// Every workgroup joins the norm's partials (at most kMaxPartials, in one
-// order) rather than wait for a launch that does; the first writes the norm.
+// Every workgroup joins the norm's partials (in one order; partial_count bounds
+// them) rather than wait for a launch that does; the first writes the norm.
 // 145 tensors of 45.6M elements, fp32 into fp32: 57 us, 365 MB, 6.4 TB/s (with
 // ordinary stores 68, and the next norm 47 instead of 32: it has their lines to
 // write back); bf16 into fp32 42 us.
@@ -292,13 +292,15 @@ int64_t total_chunks(const int64_t* counts, int64_t n) {
   return s;
 }
 
-// Workgroups of a launch: its share of kMaxPartials.
+// Workgroups of a launch, a partial each: its share of kMaxPartials rounded
+// down, and one at least.
 int list_groups(const TensorList& l, int64_t total) {
   const int64_t chunks = l.first[l.count];
   return (int)(total <= kMaxPartials ? chunks : std::max<int64_t>(1, chunks * kMaxPartials / total));
 }
 
-// Launches that a list of n tensors may need; one partial at least for each.
+// The most partials that a list of n tensors leaves: the shares come to
+// kMaxPartials, and launches whose share is none add one each.
 int64_t partial_count(int64_t n) { return kMaxPartials + n / kListMax + 1; }
 
 template <bool MAX>
@@ -327,10 +329,13 @@ int launch_clip(ListCursor c, int64_t total, double max_norm, float* norm, doubl
     JN_LAUNCH_CHECK();
     return kOk;
   }
-  // What is read and written (in place: written where it was read).  Streaming
-  // beyond the cache is a fifth faster by itself; with a pass that reads the
-  // outputs 256 MB took 121 us so and 107 with ordinary accesses, 384 MB 176 and
-  // 178, 512 MB 232 and 245, 800 MB 362 and 388.
+  // What is read and written (in place: written where it was read).  Beyond the
+  // cache it streams.  fp32 into fp32, streaming and with ordinary accesses, alone
+  // and with a fused AdamW over the outputs behind it: 256 MB 72 and 73, 665 and
+  // 683 us; 365 MB 97 and 105, 737 and 757; 512 MB 133 and 165, 839 and 865; in
+  // place 365 MB 85 and 87, 872 and 878.  (A pass that does nothing but read the
+  // outputs behind it finds more of them after ordinary accesses up to 384 MB:
+  // 256 MB 121 and 107, 384 MB 176 and 178, 512 MB 232 and 245.)
   int64_t bytes = 0;
   for (int64_t i = 0; i < c.n; ++i)
     bytes += c.counts[i] * (type_bytes(c.types[i]) + (c.in[i] == c.out[i] ? 0 : type_bytes(c.out_types[i])));

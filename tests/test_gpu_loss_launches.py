@@ -23,9 +23,10 @@ def _kernels(call):
 
 
 @pytest.mark.parametrize("rows,classes,dtype,one", [(1, 10, "fp32", True), (16, 4000, "fp32", True),
-                                                    (16, 8000, "bf16", True), (17, 10, "fp32", False), (64, 1000, "bf16", False),
-                                                    (1, 8192, "fp32", True), (1, 8193, "fp32", False),
-                                                    (1, 64000, "bf16", False), (16, 4100, "fp32", False)])
+                                                    (16, 8000, "bf16", True), (17, 10, "fp32", False),
+                                                    (64, 1000, "bf16", False), (1, 8192, "fp32", True),
+                                                    (1, 8193, "fp32", False), (1, 64000, "bf16", False),
+                                                    (16, 4100, "fp32", False)])
 def test_one_launch_for_a_row_a_wave(rows, classes, dtype, one):
     import jakal_net as J
 

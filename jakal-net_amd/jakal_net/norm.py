@@ -7,8 +7,9 @@ step, scale included, as one operator; ``layer_norm`` is its norm alone.
 
 ``implementation`` as in the operators: ``"native"`` (the default here) runs the
 HIP library for GPU tensors of fp32, bf16 or fp16 and raises where it cannot,
-CPU tensors (and a native module without these operators) take the PyTorch form; ``"kernel"`` takes the PyTorch form where
-the library declines; ``"reference"`` and ``"streaming"`` are the PyTorch form.
+CPU tensors (and a native module without these operators) take the PyTorch form;
+``"kernel"`` takes the PyTorch form where the library declines; ``"reference"``
+and ``"streaming"`` are the PyTorch form.
 The library computes in fp32 and rounds once; under autocast half-precision
 values come back in fp32, as torch's layer norm returns them.
 """
@@ -78,11 +79,22 @@ class LayerNorm(nn.LayerNorm):
         return layer_norm(x, self.weight, self.bias, eps=self.eps, implementation=self.implementation)
 
 
-def stabilize_layer(layer: Layer, norm: nn.LayerNorm, delta: LayerDelta | None = None, scale: float = 1.0) -> Layer:
+def _is_called(norm: nn.Module) -> bool:
+    """Whether a norm module has to be called: another class than a layer norm, a forward of its own, or hooks on it."""
+    return (type(norm) not in (LayerNorm, nn.LayerNorm) or "forward" in vars(norm) or bool(norm._forward_hooks)
+            or bool(norm._forward_pre_hooks) or bool(norm._backward_hooks) or bool(norm._backward_pre_hooks))
+
+
+def stabilize_layer(layer: Layer, norm: nn.Module, delta: LayerDelta | None = None, scale: float = 1.0) -> Layer:
     """The layer after an update: replaced by ``scale`` times the delta, where one
     is given, then stabilised with the norm's parameters.  The path is that of
-    the norm's ``implementation`` (the PyTorch form for a plain nn.LayerNorm)."""
+    the norm's ``implementation`` (the PyTorch form for a plain nn.LayerNorm); a
+    norm of another class, or with hooks, is called on the scaled values instead."""
     state, val = (layer.state, layer.val) if delta is None else (delta.delta_state, delta.delta_val)
+    if _is_called(norm):
+        if scale != 1.0:
+            state, val = state * scale, val * scale
+        return layer.with_tensors(state=torch.tanh(state), val=norm(val))
     if val.shape[-1:] != norm.normalized_shape:
         raise RuntimeError(f"stabilize_layer: a norm over {tuple(norm.normalized_shape)} for values of width "
                            f"{val.shape[-1]}.")

@@ -2,8 +2,9 @@
 
 ``implementation`` as in the operators: ``"native"`` (the default here) runs the
 HIP library for GPU tensors of fp32, bf16 or fp16 and raises where it cannot,
-CPU tensors (and a native module without these operators) take the PyTorch form; ``"kernel"`` takes the PyTorch form where
-the library declines; ``"reference"`` and ``"streaming"`` are the PyTorch form.
+CPU tensors (and a native module without these operators) take the PyTorch form;
+``"kernel"`` takes the PyTorch form where the library declines; ``"reference"``
+and ``"streaming"`` are the PyTorch form.
 """
 
 from __future__ import annotations

@@ -64,12 +64,12 @@ __device__ __forceinline__ float param(const void* p, int64_t i, int code, float
 // is reduced.  A workgroup of BLOCK threads holds several such groups, which
 // step through the rows together (they share the barriers).
 //
-// The forward is bound by HBM once rows fill the chip (65,536 x 512: bf16 28 to 30
-// us, 4.5 TB/s of read and write; fp32 49 us, 5.5 TB/s), by one launch's latency
-// below (64 x 512: 3.2 us); so is the backward (36 us, 5.7 TB/s; 78 us, 5.1 TB/s;
-// 8,192 x 512 fp32 12 us).  Rows of single elements move 4.8 TB/s in fp32 and 3.2
-// in bf16 (65,536 x 383); 16-byte accesses at any element took the latter from
-// 31 to 71 us.
+// The forward is bound by HBM once rows fill the chip (65,536 x 512: bf16 30 us,
+// 4.4 TB/s of read and write; fp32 43 us, 6.2 TB/s), by one launch's latency below
+// (64 x 512: 3.2 us); so is the backward (36 us, 5.7 TB/s; 78 us, 5.2 TB/s; 8,192 x
+// 512 fp32 12 us).  Rows of single elements move 5.3 TB/s in fp32 and 3.1 in bf16
+// (65,536 x 383 forward); 16-byte accesses at any element took the latter from 31
+// to 71 us.
 template <int W, int NP, int TH, int BLOCK>
 struct RowGroup {
   static constexpr int kGroups = BLOCK / TH;
@@ -308,9 +308,9 @@ __global__ __launch_bounds__(BLOCK) void norm_backward_kernel(NormArgs a) {
 }
 
 // Rows of any width and alignment: a workgroup a row, three passes over it, two of
-// them from L2 (fp32, forward and backward with parameter gradients: 1,024 x 16,384
-// 53 and 94 us, 2,048 x 16,384 99 and 167, 3,000 x 16,384 128 and 287, 512 x 33,000
-// 75 and 150).
+// them from L2 (fp32, forward and input gradient: 1,024 x 16,384 74 and 74 us,
+// 2,048 x 16,384 116 and 125, 512 x 33,000 106 and 130; the column sums take 22,
+// 51 and 28 more, the join 8 to 14).
 constexpr int kAnyThreads = 256;
 constexpr int kAnyWaves = kAnyThreads / kWave;
 
@@ -318,7 +318,7 @@ constexpr int kAnyWaves = kAnyThreads / kWave;
 // thread adds 256 terms in fp32 and those sums in 64 bits: a row of 2^28 gives
 // it 2^20 terms, whose sum in fp32 alone drops digits of every term (of a constant
 // 0.1 the mean of 2^26 came out 150 times as far off as runs of 256 may be).  Eight
-// loads in flight: one at a time took 129 us for the forward of 512 x 33,000.
+// loads in flight: one at a time the three forwards took 100, 116 and 163 us.
 constexpr int64_t kRun = 256 * kAnyThreads;  // elements
 template <typename F>
 __device__ __forceinline__ float row_sum(int64_t dim, float* lds, F term) {
@@ -455,9 +455,9 @@ __global__ __launch_bounds__(kFinishColumns* kFinishLanes) void norm_columns_fin
 // The register kernels' shapes: packs of 16 bytes where every row and parameter
 // starts on 16, else single elements; eight elements a thread (of sixteen the
 // backward has the registers for three waves a SIMD: 16,384 x 1,536 bf16 took
-// 59 us so, 41 now), by as few threads as hold the row, sixteen at least (a wave
+// 59 us so, 39 now), by as few threads as hold the row, sixteen at least (a wave
 // for every row took 30 us for the backward of 65,536 x 64 fp32, sixteen lanes
-// take 16).  Rows that 1024 threads do not hold take the kernels that pass over
+// take 11).  Rows that 1024 threads do not hold take the kernels that pass over
 // memory.
 struct RowShape {
   int width, items, threads;  // W, W * NP, TH; threads = 0: none fits

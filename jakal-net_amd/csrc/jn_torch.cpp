@@ -278,7 +278,7 @@ NormGrads row_norm_backward(const std::optional<Tensor>& g_state_in, const std::
 struct JakalRowNormBackward : torch::autograd::Node {
   Kept state_, x_, weight_, stats_;
   double scale = 1.0;
-  bool has_state = false;
+  int state_at = -1, y_at = -1;  // the outputs' places, or -1: no gradient comes through it
   at::ScalarType bias_type = at::kFloat;
 
   std::string name() const override { return "JakalRowNormBackward"; }
@@ -296,7 +296,7 @@ struct JakalRowNormBackward : torch::autograd::Node {
     const bool recorded = at::GradMode::is_enabled();
     const at::AutoGradMode off(false);
     const Tensor state = state_.get(), x = x_.get(), weight = weight_.get(), stats = stats_.get();
-    const Tensor g_state = has_state ? grads[0] : Tensor(), g = grads[has_state ? 1 : 0];
+    const Tensor g_state = state_at < 0 ? Tensor() : grads[state_at], g = y_at < 0 ? Tensor() : grads[y_at];
     // wanted: what something takes, of outputs that something used
     std::array<bool, 4> need;
     bool any = false;
@@ -337,10 +337,17 @@ std::tuple<Tensor, Tensor> row_norm(const Tensor& state_in, const Tensor& x_in, 
     node->weight_.set(weight);
     node->stats_.set(stats);
     node->scale = scale;
-    node->has_state = state.defined();
     if (bias.defined()) node->bias_type = bias.scalar_type();
-    if (state.defined()) torch::autograd::set_history(out, node);
-    torch::autograd::set_history(y, node);
+    // an output is differentiable where its own inputs are
+    int places = 0;
+    if (torch::autograd::compute_requires_grad(state)) {
+      node->state_at = places++;
+      torch::autograd::set_history(out, node);
+    }
+    if (torch::autograd::compute_requires_grad(x, weight, bias)) {
+      node->y_at = places++;
+      torch::autograd::set_history(y, node);
+    }
   }
   return {out, y};
 }

@@ -54,3 +54,13 @@ def test_lists_of_fake_tensors():
             assert norm.shape == () and norm.dtype is torch.float32 and norm.device.type == "cuda"
         with pytest.raises(ValueError):
             J.clip_grads(grads, 1.0, out=out[::-1])
+
+
+def test_history_of_fake_outputs():
+    import jakal_net as J
+
+    with FakeTensorMode():
+        state, val = torch.empty(4, device="cuda"), torch.empty(4, 8, device="cuda")
+        for a, b in ((True, False), (False, True), (True, True), (False, False)):
+            t, y = J.stabilize(state.detach().requires_grad_(a), val.detach().requires_grad_(b))
+            assert (t.requires_grad, y.requires_grad) == (a, b)

@@ -80,9 +80,11 @@ class LayerNorm(nn.LayerNorm):
 
 
 def _is_called(norm: nn.Module) -> bool:
-    """Whether a norm module has to be called: another class than a layer norm, a forward of its own, or hooks on it."""
-    return (type(norm) not in (LayerNorm, nn.LayerNorm) or "forward" in vars(norm) or bool(norm._forward_hooks)
-            or bool(norm._forward_pre_hooks) or bool(norm._backward_hooks) or bool(norm._backward_pre_hooks))
+    """Whether a norm module has to be called: another class than a layer norm, one over several axes, a forward of
+    its own, or hooks on it."""
+    return (type(norm) not in (LayerNorm, nn.LayerNorm) or len(norm.normalized_shape) != 1 or "forward" in vars(norm)
+            or bool(norm._forward_hooks) or bool(norm._forward_pre_hooks) or bool(norm._backward_hooks)
+            or bool(norm._backward_pre_hooks))
 
 
 def stabilize_layer(layer: Layer, norm: nn.Module, delta: LayerDelta | None = None, scale: float = 1.0) -> Layer:

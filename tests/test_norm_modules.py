@@ -27,8 +27,8 @@ class _Doubled(nn.Module):
 def _norms():
     parametrised = J.LayerNorm(12)
     nn.utils.parametrize.register_parametrization(parametrised, "weight", _Doubled())
-    return dict(identity=nn.Identity(), axes=nn.LayerNorm((5, 12)), rms=nn.RMSNorm(12), chain=nn.Sequential(nn.LayerNorm(12), nn.Tanh()),
-                subclass=_Shifted(12), parametrised=parametrised)
+    return dict(identity=nn.Identity(), axes=nn.LayerNorm((5, 12)), rms=nn.RMSNorm(12),
+                chain=nn.Sequential(nn.LayerNorm(12), nn.Tanh()), subclass=_Shifted(12), parametrised=parametrised)
 
 
 @pytest.mark.parametrize("kind", list(_norms()))

@@ -1,0 +1,441 @@
+"""Operators on microscaled numbers: activations kept in 8 bits, products in 4.
+
+A microscaled tensor holds runs of 32 elements of its last axis as short floats
+(e4m3: 8 bits, largest 448; e2m1: 4 bits, largest 6) times a power of two, the
+smallest that keeps the run's largest element in range.  Two things are made of
+them.  A training step keeps what its layers save for the backward in e4m3
+(``saved="e4m3"``): the forward is unchanged, the gradients are taken at the
+kept values.  A model that answers multiplies by frozen e2m1 weights
+(``mx_linear``), the activations microscaled on the way in.
+
+``run`` computes them in plain torch operations in 32 bits, or, where ``own`` is
+true, through ``jakal_net``.  Inputs are what the model meets: activations near
+unit variance with a few wide rows, weights at their initial scale, gradients at
+the scale a mean loss leaves.
+"""
+
+from __future__ import annotations
+
+import math
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+BLOCK = 32
+# largest exponent, largest significand, mantissa bits, smallest normal exponent
+FORMATS = {"e4m3": (8, 1.75, 3, -6), "e2m1": (2, 1.5, 1, 0)}
+EPS = 1e-5
+
+
+def _quantize(rows, dim, form, dtype="fp32"):
+    """rows x dim elements microscaled, and the values they stand for."""
+    return dict(op="quantize", rows=rows, dim=dim, form=form, dtype=dtype)
+
+
+def _product(rows, dim, out, acts, dtype="bf16", bias=True, train=False):
+    """rows x dim activations by out x dim e2m1 weights; acts: the activations' form; train: their gradient too."""
+    return dict(op="product", rows=rows, dim=dim, out=out, acts=acts, dtype=dtype, bias=bias, train=train)
+
+
+def _linear(rows, dim, out, dtype="fp32", bias=True):
+    """A linear layer's training step over rows x dim activations, which are kept in e4m3."""
+    return dict(op="linear", rows=rows, dim=dim, out=out, dtype=dtype, bias=bias)
+
+
+def _gelu(rows, dim, dtype="fp32"):
+    """The activation between two linear layers, its input kept in e4m3."""
+    return dict(op="gelu", rows=rows, dim=dim, dtype=dtype)
+
+
+def _stabilize(batch, nodes, dim, scale, dtype="fp32"):
+    """The end of a layer update over [batch, nodes, dim] values, which are kept in e4m3."""
+    return dict(op="stabilize", batch=batch, nodes=nodes, dim=dim, scale=scale, dtype=dtype)
+
+
+def listed():
+    return [
+        # the 64 query slots of one sequence: latency only
+        dict(name="quantize_query_e4m3", **_quantize(64, 512, "e4m3")),
+        # the vocabulary weights as they are made ready for answering
+        dict(name="quantize_head_e2m1", **_quantize(16384, 2048, "e2m1", dtype="bf16")),
+        # the head's last product for one token
+        dict(name="product_token", **_product(1, 2048, 16384, "e2m1")),
+        # the head's first product for the query slots of one sequence
+        dict(name="product_query", **_product(64, 512, 2048, "e4m3", dtype="fp32")),
+        # logits of every prefix position of 16 sequences: the largest
+        dict(name="product_prefix", **_product(16 * 512, 2048, 16384, "e2m1")),
+        # odd sizes, with the gradient that goes on below a frozen head
+        dict(name="product_ragged_train", **_product(1531, 383, 4099, "e4m3", dtype="fp32", train=True)),
+        # the vocabulary product of a training step over 16 sequences of 64 query slots, as bf16 autocast has it
+        dict(name="linear_head_train", **_linear(16 * 64, 2048, 16384, dtype="bf16")),
+        # odd sizes in fp32
+        dict(name="linear_ragged_train", **_linear(1531, 383, 1000)),
+        # the head's activation for one sequence: latency only
+        dict(name="gelu_query_train", **_gelu(64, 2048)),
+        # and over every prefix position of 16
+        dict(name="gelu_prefix_train", **_gelu(16 * 512, 2048, dtype="bf16")),
+        # the update of the sequence layer in a training step: the model makes about twenty such calls
+        dict(name="stabilize_sequence_train", **_stabilize(16, 512, 512, 0.25)),
+        # odd nodes and an odd width
+        dict(name="stabilize_ragged_train", **_stabilize(3, 1531, 383, 0.15, dtype="bf16")),
+    ]
+
+
+ELEMENTS = 16384 * 2048
+PRODUCTS = 16 * 512 * 2048 * 16384
+
+
+def _spread(rng, low, high):
+    """A whole number between low and high, even over the logarithm."""
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def _width(rng, low, high):
+    """A row length: mostly a multiple of 32, else any."""
+    d = _spread(rng, low, high)
+    return max(low, d // 32 * 32) if rng.random() < 0.6 else d
+
+
+def draw(rng):
+    op = rng.choice(["quantize", "product", "product", "product", "linear", "linear", "gelu", "stabilize"])
+    dtype = rng.choice(["fp32", "bf16", "bf16", "fp16"])
+    if op == "quantize":
+        dim = _width(rng, 8, 8192)
+        return _quantize(_spread(rng, 1, min(65536, ELEMENTS // dim)), dim, rng.choice(["e4m3", "e2m1"]), dtype)
+    if op == "product":
+        train = rng.random() < 0.4
+        dim, out = _width(rng, 32, 8192), _width(rng, 32, 16384)
+        most = PRODUCTS // (16 if train else 1)
+        rows = _spread(rng, 1, min(8192, most // (dim * out)))
+        return _product(rows, dim, out, rng.choice(["e2m1", "e4m3"]), dtype, rng.random() < 0.5, train)
+    if op == "linear":
+        dim, out = _width(rng, 32, 4096), _width(rng, 32, 16384)
+        rows = _spread(rng, 1, min(8192, PRODUCTS // 16 // (dim * out)))
+        return _linear(rows, dim, out, dtype, rng.random() < 0.7)
+    if op == "gelu":
+        dim = _width(rng, 8, 8192)
+        return _gelu(_spread(rng, 1, min(65536, ELEMENTS // dim)), dim, dtype)
+    dim = _width(rng, 16, 1024)
+    batch = _spread(rng, 1, 16)
+    nodes = _spread(rng, 1, min(4096, ELEMENTS // (dim * batch)))
+    return _stabilize(batch, nodes, dim, round(rng.uniform(0.02, 1.0), 3), dtype)
+
+
+# ---------------------------------------------------------------------------
+# inputs
+# ---------------------------------------------------------------------------
+def _generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _normal(g, *shape, scale=1.0, mean=0.0, dtype=torch.float32):
+    return (torch.randn(shape, generator=g, device="cuda") * scale + mean).to(dtype)
+
+
+def _activations(g, rows, dim, dtype):
+    """Rows near unit variance, a few of them several times wider."""
+    wide = torch.exp(0.5 * torch.randn(rows, 1, generator=g, device="cuda"))
+    return (torch.randn(rows, dim, generator=g, device="cuda") * wide).to(dtype)
+
+
+def prepare(case, seed):
+    g = _generator(seed)
+    dtype = DTYPES[case["dtype"]]
+    op = case["op"]
+    state = dict(case=case)
+    if op == "stabilize":
+        lead, dim = (case["batch"], case["nodes"]), case["dim"]
+        state.update(
+            state=_normal(g, *lead, scale=2.0, dtype=dtype).requires_grad_(),
+            val=_normal(g, *lead, dim, scale=1.3, mean=0.2, dtype=dtype).requires_grad_(),
+            weight=_normal(g, dim, scale=0.1, mean=1.0, dtype=dtype).requires_grad_(),
+            bias=_normal(g, dim, scale=0.1, dtype=dtype).requires_grad_(),
+            grad_state=_normal(g, *lead, scale=0.1, dtype=dtype), grad=_normal(g, *lead, dim, scale=0.1, dtype=dtype))
+        return state
+    rows, dim = case["rows"], case["dim"]
+    x = _activations(g, rows, dim, dtype)
+    if op == "quantize":
+        return dict(state, x=x)
+    if op == "gelu":
+        return dict(state, x=x.requires_grad_(), grad=_normal(g, rows, dim, scale=0.1, dtype=dtype))
+    out = case["out"]
+    # a linear layer's initial scale
+    w = (torch.rand(out, dim, generator=g, device="cuda") * 2.0 - 1.0) * dim ** -0.5
+    bias = _normal(g, out, scale=0.02, dtype=dtype) if case["bias"] else None
+    if op == "linear":
+        state.update(x=x.requires_grad_(), weight=w.to(dtype).requires_grad_(),
+                     bias=None if bias is None else bias.requires_grad_())
+    else:
+        values, exponents = _microscale(w, "e2m1")
+        state.update(x=x.requires_grad_(case["train"]), bias=bias, codes=_nibbles(values, exponents, dim),
+                     scales=(exponents + 127).to(torch.uint8))
+    if op == "linear" or case["train"]:
+        state["grad"] = _normal(g, rows, out, scale=0.1, dtype=dtype)
+    return state
+
+
+def _nibbles(values, exponents, dim):
+    """The e2m1 codes of microscaled values, two a byte, the first of them in the low half; runs are whole."""
+    pad = -dim % BLOCK
+    v = torch.nn.functional.pad(values, (0, pad)).unflatten(-1, (-1, BLOCK)) * _two_to(-exponents).unsqueeze(-1)
+    size = v.abs()
+    code = torch.zeros_like(size, dtype=torch.uint8)
+    for bound in (0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0):
+        code += (size >= bound).to(torch.uint8)
+    code += 8 * torch.signbit(v).to(torch.uint8)
+    code = code.flatten(-2)
+    return code[..., 0::2] | (code[..., 1::2] << 4)
+
+
+# ---------------------------------------------------------------------------
+# one pass
+# ---------------------------------------------------------------------------
+def run(state):
+    case = state["case"]
+    kind = case["op"]
+    if own:
+        return {"quantize": _own_quantize, "product": _own_product, "linear": _own_linear, "gelu": _own_gelu,
+                "stabilize": _own_stabilize}[kind](state, case)
+    with torch.no_grad():
+        return {"quantize": _plain_quantize, "product": _plain_product, "linear": _plain_linear, "gelu": _plain_gelu,
+                "stabilize": _plain_stabilize}[kind](state, case)
+
+
+def _jakal():
+    if "jakal_net" not in sys.modules:
+        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "jakal-net_amd"))
+    import jakal_net
+
+    return jakal_net
+
+
+def _own_quantize(state, case):
+    J = _jakal()
+    q = J.mx_quantize(state["x"], case["form"], implementation="native")
+    return {"values": J.mx_dequantize(q, implementation="native"), "scales": q.scales}
+
+
+def _own_product(state, case):
+    J = _jakal()
+    weight = J.MXTensor(state["codes"], state["scales"], "e2m1", case["dim"])
+    y = J.mx_linear(state["x"], weight, state["bias"], activations=case["acts"], implementation="native")
+    out = {"y": y.detach()}
+    if case["train"]:
+        out["grad_x"] = torch.autograd.grad(y, state["x"], state["grad"])[0]
+    return out
+
+
+def _grads(out, ends, seeds, state, names):
+    names = [n for n in names if state[n] is not None]
+    grads = torch.autograd.grad(ends, [state[n] for n in names], seeds)
+    out.update({"grad_" + n: t for n, t in zip(names, grads)})
+    return out
+
+
+def _own_linear(state, case):
+    y = _jakal().linear(state["x"], state["weight"], state["bias"], saved="e4m3", implementation="native")
+    return _grads({"y": y.detach()}, [y], [state["grad"]], state, ("x", "weight", "bias"))
+
+
+def _own_gelu(state, case):
+    y = _jakal().gelu(state["x"], saved="e4m3", implementation="native")
+    return _grads({"y": y.detach()}, [y], [state["grad"]], state, ("x",))
+
+
+def _own_stabilize(state, case):
+    t, y = _jakal().stabilize(state["state"], state["val"], state["weight"], state["bias"], eps=EPS,
+                              scale=case["scale"], saved="e4m3", implementation="native")
+    return _grads({"state": t.detach(), "y": y.detach()}, [t, y], [state["grad_state"], state["grad"]], state,
+                  ("state", "val", "weight", "bias"))
+
+
+def _two_to(exponents):
+    """2^e in fp32, exactly, for -126 <= e <= 127."""
+    return ((exponents.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def _microscale(x, form):
+    """(the values that x stands for microscaled, the exponents of its runs), of finite x in fp32."""
+    top, significand, bits, least = FORMATS[form]
+    dim = x.shape[-1]
+    v = torch.nn.functional.pad(x, (0, -dim % BLOCK)).unflatten(-1, (-1, BLOCK))
+    part, e = torch.frexp(v.abs().amax(-1))  # in [0.5, 1)
+    e = torch.where(part == 0, -126, e - 1 - top + (2.0 * part > significand)).clamp(min=-126)
+    v = v * _two_to(-e).unsqueeze(-1)
+    step = _two_to(((v.abs().view(torch.int32) >> 23) - 127).clamp(min=least) - bits)
+    v = torch.round(v / step) * step * _two_to(e).unsqueeze(-1)
+    return v.flatten(-2)[..., :dim], e
+
+
+def _decoded(state, case):
+    """The e2m1 weights' values in fp32."""
+    table = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device="cuda")
+    table = torch.cat([table, -table])
+    codes = state["codes"].int()
+    v = table[torch.stack([codes & 15, codes >> 4], -1)].flatten(-2).unflatten(-1, (-1, BLOCK))
+    return (v * _two_to(state["scales"].int() - 127).unsqueeze(-1)).flatten(-2)[..., :case["dim"]]
+
+
+def _plain_quantize(state, case):
+    values, e = _microscale(state["x"].float(), case["form"])
+    return {"values": values.to(state["x"].dtype), "scales": (e + 127).to(torch.uint8)}
+
+
+def _plain_product(state, case):
+    x, w = state["x"], _decoded(state, case)
+    y = _microscale(x.float(), case["acts"])[0] @ w.t()
+    if state["bias"] is not None:
+        y = y + state["bias"].float()
+    out = {"y": y.to(x.dtype)}
+    if case["train"]:
+        out["grad_x"] = (state["grad"].float() @ w).to(x.dtype)
+    return out
+
+
+def _plain_linear(state, case):
+    x, weight, g = state["x"], state["weight"], state["grad"].float()
+    y = x.float() @ weight.float().t()
+    if state["bias"] is not None:
+        y = y + state["bias"].float()
+    kept = _microscale(x.float(), "e4m3")[0]
+    out = {"y": y.to(x.dtype), "grad_x": (g @ weight.float()).to(x.dtype), "grad_weight": (g.t() @ kept).to(x.dtype)}
+    if state["bias"] is not None:
+        out["grad_bias"] = g.sum(0).to(x.dtype)
+    return out
+
+
+def _plain_gelu(state, case):
+    x = state["x"].float()
+    kept = _microscale(x, "e4m3")[0]
+    y = 0.5 * x * (1.0 + torch.erf(x * math.sqrt(0.5)))
+    slope = 0.5 * (1.0 + torch.erf(kept * math.sqrt(0.5))) + kept * torch.exp(-0.5 * kept * kept) / math.sqrt(2 * math.pi)
+    return {"y": y.to(state["x"].dtype), "grad_x": (state["grad"].float() * slope).to(state["x"].dtype)}
+
+
+def _plain_stabilize(state, case):
+    scale, dtype = case["scale"], state["val"].dtype
+    weight = state["weight"].float()
+    t = torch.tanh(state["state"].float() * scale)
+    v = state["val"].float()
+    kept = _microscale(v, "e4m3")[0] * scale
+    v = v * scale
+    mean = v.mean(-1, keepdim=True)
+    v = v - mean
+    r = 1.0 / torch.sqrt((v * v).mean(-1, keepdim=True) + EPS)
+    y = v * r * weight + state["bias"].float()
+    h = (kept - mean) * r
+    g = state["grad"].float()
+    gw = g * weight
+    dx = scale * r * (gw - gw.mean(-1, keepdim=True) - h * (gw * h).mean(-1, keepdim=True))
+    return {"state": t.to(dtype), "y": y.to(dtype),
+            "grad_state": (scale * (1.0 - t * t) * state["grad_state"].float()).to(dtype), "grad_val": dx.to(dtype),
+            "grad_weight": (g * h).sum((0, 1)).to(dtype), "grad_bias": g.sum((0, 1)).to(dtype)}
+
+
+# ---------------------------------------------------------------------------
+# what a pass cannot do without, and its definition in 64 bits
+# ---------------------------------------------------------------------------
+SIZE = {"fp32": 4, "bf16": 2, "fp16": 2}
+
+
+def _packed(rows, dim, form):
+    """Bytes of a microscaled tensor."""
+    return rows * dim * (1 if form == "e4m3" else 0.5) + rows * math.ceil(dim / BLOCK)
+
+
+def work(case):
+    e, op, dim = SIZE[case["dtype"]], case["op"], case["dim"]
+    if op == "quantize":
+        rows = case["rows"]
+        return {"bytes": 2 * rows * dim * e + 2 * _packed(rows, dim, case["form"]), "flops": 4 * rows * dim}
+    if op == "gelu":
+        rows = case["rows"]
+        return {"bytes": 4 * rows * dim * e + 2 * _packed(rows, dim, "e4m3"), "flops": 40 * rows * dim}
+    if op == "stabilize":
+        rows = case["batch"] * case["nodes"]
+        return {"bytes": 4 * rows * (dim + 1) * e + 2 * _packed(rows, dim, "e4m3") + 6 * dim * e,
+                "flops": 26 * rows * dim}
+    rows, out = case["rows"], case["out"]
+    bias = out * e if case["bias"] else 0
+    if op == "product":
+        times = 2 if case["train"] else 1
+        return {"bytes": times * ((rows * dim + rows * out) * e + _packed(out, dim, "e2m1")) + bias,
+                "flops": times * 2 * rows * dim * out}
+    return {"bytes": 2 * (rows * dim + dim * out) * e + 2 * rows * out * e + 2 * _packed(rows, dim, "e4m3") + 2 * bias,
+            "flops": 3 * 2 * rows * dim * out}
+
+
+def _grid(form):
+    """All magnitudes of a format, rising, in 64 bits; a tie between two goes to the one of even place."""
+    bits, least, last = (3, -6, 126) if form == "e4m3" else (1, 0, 7)
+    places = torch.arange(last + 1, device="cuda", dtype=torch.float64)
+    exponent = torch.floor(places / 2 ** bits).clamp(min=1.0)
+    lead = (places >= 2 ** bits).double()
+    return (lead + torch.remainder(places, 2 ** bits) / 2 ** bits) * torch.exp2(exponent - 1.0 + least)
+
+
+def _kept(x, form):
+    """x microscaled, in 64 bits: the nearest of the format's magnitudes times the run's power of two."""
+    grid = _grid(form)
+    x = x.detach().double()
+    dim = x.shape[-1]
+    out, powers = torch.empty_like(x), []
+    for at in range(0, dim, BLOCK):
+        run_ = x[..., at:at + BLOCK]
+        most = run_.abs().amax(-1, keepdim=True)
+        e = torch.ceil(torch.log2(most / grid[-1])).clamp(min=-126.0)
+        size = run_.abs() * torch.exp2(-e)
+        high = torch.searchsorted(grid, size.contiguous()).clamp(max=len(grid) - 1)
+        low = (high - 1).clamp(min=0)
+        up, down = grid[high] - size, size - grid[low]
+        place = torch.where((up < down) | ((up == down) & (high % 2 == 0)), high, low)
+        out[..., at:at + BLOCK] = torch.copysign(grid[place] * torch.exp2(e), run_)
+        powers.append(e)
+    return out, torch.cat(powers, -1)
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    op = case["op"]
+    if op == "quantize":
+        values, e = _kept(state["x"], case["form"])
+        return {"values": values, "scales": (e + 127.0).to(torch.uint8)}
+    if op == "gelu":
+        x, k, g = state["x"].detach().double(), _kept(state["x"], "e4m3")[0], state["grad"].double()
+        half = torch.special.ndtr
+        return {"y": x * half(x), "grad_x": g * (half(k) + k * torch.exp(-k * k / 2.0) * (2.0 * math.pi) ** -0.5)}
+    if op == "stabilize":
+        s, r = case["scale"], {n: state[n].detach().double() for n in ("state", "val", "weight", "bias")}
+        t = torch.tanh(s * r["state"])
+        var, mean = torch.var_mean(s * r["val"], -1, correction=0, keepdim=True)
+        inv = torch.rsqrt(var + EPS)
+        h = (s * _kept(state["val"], "e4m3")[0] - mean) * inv
+        g = state["grad"].double()
+        gh = g * r["weight"]
+        centred = gh - gh.mean(-1, keepdim=True)
+        return {"state": t, "y": (s * r["val"] - mean) * inv * r["weight"] + r["bias"],
+                "grad_state": s * state["grad_state"].double() / torch.cosh(s * r["state"]) ** 2,
+                "grad_val": s * inv * (centred - h * (gh * h).mean(-1, keepdim=True)),
+                "grad_weight": (g * h).sum((0, 1)), "grad_bias": g.sum((0, 1))}
+    bias = 0.0 if state["bias"] is None else state["bias"].detach().double()
+    if op == "product":
+        grid = _grid("e2m1")
+        w = torch.empty(case["out"], 2 * state["codes"].shape[-1], dtype=torch.float64, device="cuda")
+        for half, part in enumerate((state["codes"] % 16, state["codes"] // 16)):
+            w[:, half::2] = grid[(part % 8).long()] * (1.0 - 2.0 * (part // 8).double())
+        w *= torch.exp2(state["scales"].double() - 127.0).repeat_interleave(BLOCK, -1)
+        w = w[:, :case["dim"]]
+        out = {"y": torch.matmul(_kept(state["x"], case["acts"])[0], w.t()) + bias}
+        if case["train"]:
+            out["grad_x"] = torch.matmul(state["grad"].double(), w)
+        return out
+    x, w, g = state["x"].detach().double(), state["weight"].detach().double(), state["grad"].double()
+    out = {"y": torch.matmul(x, w.t()) + bias, "grad_x": torch.matmul(g, w),
+           "grad_weight": torch.matmul(g.t(), _kept(state["x"], "e4m3")[0])}
+    if state["bias"] is not None:
+        out["grad_bias"] = g.sum(0)
+    return out

@@ -6,7 +6,7 @@ smallest that keeps the run's largest element in range.  Two things are made of
 them.  A training step keeps what its layers save for the backward in e4m3
 (``saved="e4m3"``): the forward is unchanged, the gradients are taken at the
 kept values.  A model that answers multiplies by frozen e2m1 weights
-(``mx_linear``), the activations microscaled on the way in.
+(``mx_linear``), the activations as they are or microscaled on the way in.
 
 ``run`` computes them in plain torch operations in 32 bits, or, where ``own`` is
 true, through ``jakal_net``.  Inputs are what the model meets: activations near
@@ -37,7 +37,8 @@ def _quantize(rows, dim, form, dtype="fp32"):
 
 
 def _product(rows, dim, out, acts, dtype="bf16", bias=True, train=False):
-    """rows x dim activations by out x dim e2m1 weights; acts: the activations' form; train: their gradient too."""
+    """rows x dim activations by out x dim e2m1 weights; acts: e2m1, or none for the activations as they are; train:
+    their gradient too."""
     return dict(op="product", rows=rows, dim=dim, out=out, acts=acts, dtype=dtype, bias=bias, train=train)
 
 
@@ -65,11 +66,11 @@ def listed():
         # the head's last product for one token
         dict(name="product_token", **_product(1, 2048, 16384, "e2m1")),
         # the head's first product for the query slots of one sequence
-        dict(name="product_query", **_product(64, 512, 2048, "e4m3", dtype="fp32")),
+        dict(name="product_query", **_product(64, 512, 2048, "none", dtype="fp32")),
         # logits of every prefix position of 16 sequences: the largest
         dict(name="product_prefix", **_product(16 * 512, 2048, 16384, "e2m1")),
         # odd sizes, with the gradient that goes on below a frozen head
-        dict(name="product_ragged_train", **_product(1531, 383, 4099, "e4m3", dtype="fp32", train=True)),
+        dict(name="product_ragged_train", **_product(1531, 383, 4099, "none", dtype="fp32", train=True)),
         # the vocabulary product of a training step over 16 sequences of 64 query slots, as bf16 autocast has it
         dict(name="linear_head_train", **_linear(16 * 64, 2048, 16384, dtype="bf16")),
         # odd sizes in fp32
@@ -111,7 +112,7 @@ def draw(rng):
         dim, out = _width(rng, 32, 8192), _width(rng, 32, 16384)
         most = PRODUCTS // (16 if train else 1)
         rows = _spread(rng, 1, min(8192, most // (dim * out)))
-        return _product(rows, dim, out, rng.choice(["e2m1", "e4m3"]), dtype, rng.random() < 0.5, train)
+        return _product(rows, dim, out, rng.choice(["e2m1", "none"]), dtype, rng.random() < 0.5, train)
     if op == "linear":
         dim, out = _width(rng, 32, 4096), _width(rng, 32, 16384)
         rows = _spread(rng, 1, min(8192, PRODUCTS // 16 // (dim * out)))
@@ -222,7 +223,8 @@ def _own_quantize(state, case):
 def _own_product(state, case):
     J = _jakal()
     weight = J.MXTensor(state["codes"], state["scales"], "e2m1", case["dim"])
-    y = J.mx_linear(state["x"], weight, state["bias"], activations=case["acts"], implementation="native")
+    acts = None if case["acts"] == "none" else case["acts"]
+    y = J.mx_linear(state["x"], weight, state["bias"], activations=acts, implementation="native")
     out = {"y": y.detach()}
     if case["train"]:
         out["grad_x"] = torch.autograd.grad(y, state["x"], state["grad"])[0]
@@ -287,7 +289,7 @@ def _plain_quantize(state, case):
 
 def _plain_product(state, case):
     x, w = state["x"], _decoded(state, case)
-    y = _microscale(x.float(), case["acts"])[0] @ w.t()
+    y = (x.float() if case["acts"] == "none" else _microscale(x.float(), case["acts"])[0]) @ w.t()
     if state["bias"] is not None:
         y = y + state["bias"].float()
     out = {"y": y.to(x.dtype)}
@@ -429,7 +431,8 @@ def exact(case, seed):
             w[:, half::2] = grid[(part % 8).long()] * (1.0 - 2.0 * (part // 8).double())
         w *= torch.exp2(state["scales"].double() - 127.0).repeat_interleave(BLOCK, -1)
         w = w[:, :case["dim"]]
-        out = {"y": torch.matmul(_kept(state["x"], case["acts"])[0], w.t()) + bias}
+        x = state["x"].detach().double() if case["acts"] == "none" else _kept(state["x"], case["acts"])[0]
+        out = {"y": torch.matmul(x, w.t()) + bias}
         if case["train"]:
             out["grad_x"] = torch.matmul(state["grad"].double(), w)
         return out

@@ -4,8 +4,8 @@ A microscaled tensor holds runs of 32 elements of its last axis as short floats
 (e4m3: 8 bits, largest 448; e2m1: 4 bits, largest 6) times a power of two, the
 smallest that keeps the run's largest element in range.  Two things are made of
 them.  A training step keeps what its layers save for the backward in e4m3
-(``saved="e4m3"``): the forward is unchanged, the gradients are taken at the
-kept values.  A model that answers multiplies by frozen e2m1 weights
+(``saved="e4m3"``; a norm, its centred input): the forward is unchanged, the
+gradients are taken at the kept values.  A model that answers multiplies by frozen e2m1 weights
 (``mx_linear``), the activations as they are or microscaled on the way in.
 
 ``run`` computes them in plain torch operations in 32 bits, or, where ``own`` is
@@ -53,7 +53,7 @@ def _gelu(rows, dim, dtype="fp32"):
 
 
 def _stabilize(batch, nodes, dim, scale, dtype="fp32"):
-    """The end of a layer update over [batch, nodes, dim] values, which are kept in e4m3."""
+    """The end of a layer update over [batch, nodes, dim] values, which are kept, centred, in e4m3."""
     return dict(op="stabilize", batch=batch, nodes=nodes, dim=dim, scale=scale, dtype=dtype)
 
 
@@ -323,13 +323,14 @@ def _plain_stabilize(state, case):
     weight = state["weight"].float()
     t = torch.tanh(state["state"].float() * scale)
     v = state["val"].float()
-    kept = _microscale(v, "e4m3")[0] * scale
+    # the mean in 64 bits, so that what is kept lies on the same side of every border whatever the order of summing
+    kept = _microscale(v - state["val"].double().mean(-1, keepdim=True).float(), "e4m3")[0] * scale
     v = v * scale
     mean = v.mean(-1, keepdim=True)
     v = v - mean
     r = 1.0 / torch.sqrt((v * v).mean(-1, keepdim=True) + EPS)
     y = v * r * weight + state["bias"].float()
-    h = (kept - mean) * r
+    h = kept * r
     g = state["grad"].float()
     gw = g * weight
     dx = scale * r * (gw - gw.mean(-1, keepdim=True) - h * (gw * h).mean(-1, keepdim=True))
@@ -415,7 +416,9 @@ def exact(case, seed):
         t = torch.tanh(s * r["state"])
         var, mean = torch.var_mean(s * r["val"], -1, correction=0, keepdim=True)
         inv = torch.rsqrt(var + EPS)
-        h = (s * _kept(state["val"], "e4m3")[0] - mean) * inv
+        # what is kept is an fp32 number: the value less the row's mean
+        centre = torch.mean(state["val"].detach().double(), -1, keepdim=True).float()
+        h = s * _kept(state["val"].detach().float() - centre, "e4m3")[0] * inv
         g = state["grad"].double()
         gh = g * r["weight"]
         centred = gh - gh.mean(-1, keepdim=True)

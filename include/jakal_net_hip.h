@@ -39,7 +39,7 @@ typedef void* jn_stream_t;
 /* Message of the last failing call on this host thread ("" if none). */
 const char* jn_last_error(void);
 
-/* ABI revision of this header (bumped on any signature or accepted-range change); this is 19. */
+/* ABI revision of this header (bumped on any signature or accepted-range change); this is 20. */
 int jn_abi_version(void);
 
 /*
@@ -979,6 +979,84 @@ int jn_grads_norm(const void* const* grads, const int64_t* counts, const int32_t
 int jn_grads_clip(const void* const* grads, void* const* out, const int64_t* counts, const int32_t* types,
                   const int32_t* out_types, int64_t tensors, double max_norm, int32_t norm_kind, float* norm,
                   void* workspace, size_t workspace_bytes, jn_stream_t stream);
+
+/*
+ * Microscaled tensors: rows of `dim` elements in runs of 32 (the last may be
+ * short), each run one power of two times short floats.
+ *   JN_E4M3: 8 bits, largest 448;  JN_E2M1: 4 bits, largest 6 (0 .5 1 1.5 2 3 4 6)
+ *   scale s of a run: 2^(s - 127), the smallest power of two >= 2^-126 that keeps
+ *   the run's largest magnitude within the format; 255 (the whole run is NaN)
+ *   where the run holds an infinity or a NaN
+ *   code of an element: x / 2^(s - 127) rounded to the nearest, ties to even
+ * codes: rows of ceil(dim / 32) * 32 bytes (e4m3) or * 16 (e2m1, two codes a
+ * byte, the first in the low half), zeros past dim, starting on 16 bytes; scales:
+ * rows of ceil(dim / 32) bytes.  Dequantising gives the values, rounded to `type`
+ * (exact in fp32 and bf16 but below 2^-126).
+ */
+#define JN_E4M3 0
+#define JN_E2M1 1
+#define JN_PLAIN (-1)
+int jn_mx_quantize(const void* x, int64_t rows, int64_t dim, int32_t type, int32_t format, void* codes, void* scales,
+                   jn_stream_t stream);
+int jn_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t dim, int32_t format, int32_t type,
+                     void* x, jn_stream_t stream);
+
+/*
+ * y [rows, out] = x . W^T + bias with W [out, dim] in JN_E2M1 and x [rows, dim] as
+ * it is (activations JN_PLAIN) or microscaled on the way in (JN_E2M1); products are
+ * exact, sums fp32, one rounding to `type` (of x, bias and y; bias [out] may be
+ * null).  y starts on 16 bytes.
+ * grad_x [rows, dim] = grad_y . W: the rounding of x passes the gradient through.
+ */
+size_t jn_mx_linear_forward_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t activations);
+int jn_mx_linear_forward(const void* x, const void* weight_codes, const void* weight_scales, const void* bias,
+                         int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t activations, void* y,
+                         void* workspace, size_t workspace_bytes, jn_stream_t stream);
+size_t jn_mx_linear_backward_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type);
+int jn_mx_linear_backward(const void* grad_y, const void* weight_codes, const void* weight_scales, int64_t rows,
+                          int64_t dim, int64_t out, int32_t type, void* grad_x, void* workspace,
+                          size_t workspace_bytes, jn_stream_t stream);
+
+/*
+ * Weight gradient of a linear layer from its input kept in JN_E4M3:
+ *   grad_weight [out, dim] = grad_y^T . x,  grad_bias [out] = sum over rows of grad_y
+ * grad_y [rows, out], grad_weight and grad_bias (may be null) are of `type`;
+ * grad_weight starts on 16 bytes.  Exact products, fp32 sums in a fixed order.
+ */
+size_t jn_mx_weight_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t bias);
+int jn_mx_weight_grad(const void* grad_y, const void* codes, const void* scales, int64_t rows, int64_t dim,
+                      int64_t out, int32_t type, void* grad_weight, void* grad_bias, void* workspace,
+                      size_t workspace_bytes, jn_stream_t stream);
+
+/* sums [dim] of `type`: the sums over rows of x [rows, dim], fp32 in a fixed order. */
+size_t jn_column_sums_workspace_bytes(int64_t rows, int64_t dim);
+int jn_column_sums(const void* x, int64_t rows, int64_t dim, int32_t type, void* sums, void* workspace,
+                   size_t workspace_bytes, jn_stream_t stream);
+
+/*
+ * jn_layer_norm_forward that also keeps, in JN_E4M3, c = x - p with p the row's mean
+ * in 64 bits rounded to fp32 (codes and scales of the rows), and its gradients from
+ * what was kept: h = scale r times the kept c, r being x's own (stats).  A row with
+ * an infinity or a NaN is kept as NaN.  The workspace is jn_layer_norm_backward's.
+ */
+int jn_layer_norm_forward_kept(const void* state, const void* x, const void* weight, const void* bias, int64_t rows,
+                               int64_t dim, float scale, float eps, int32_t type, int32_t state_type,
+                               int32_t param_type, void* state_out, void* y, float* stats, void* codes, void* scales,
+                               jn_stream_t stream);
+int jn_layer_norm_backward_kept(const void* state, const void* codes, const void* scales, const void* weight,
+                                const float* stats, const void* grad_state_out, const void* grad_y, int64_t rows,
+                                int64_t dim, float scale, int32_t type, int32_t state_type, int32_t param_type,
+                                void* grad_state, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                                size_t workspace_bytes, jn_stream_t stream);
+
+/*
+ * y = x Phi(x), with x kept in JN_E4M3 where codes and scales are given (both or
+ * neither); grad_x = grad_y (Phi(x) + x phi(x)) at the kept x.
+ */
+int jn_gelu_forward(const void* x, int64_t rows, int64_t dim, int32_t type, void* y, void* codes, void* scales,
+                    jn_stream_t stream);
+int jn_gelu_backward(const void* codes, const void* scales, const void* grad_y, int64_t rows, int64_t dim,
+                     int32_t type, void* grad_x, jn_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,672 @@
+// Products with a microscaled operand (jn_mx_linear_*, jn_mx_weight_grad).
+//
+//   forward      y[m, n] = sum_k x[m, k] W[n, k] + b[n], W microscaled along k; x as it
+//                is (mx_mixed_kernel), or microscaled along k too on its way in
+//                (mx_linear_kernel, on the scaled matrix instructions)
+//   gradients    c[m, n] = sum_r A(m, r) B[r, n] with B [r, n] microscaled along n
+//                and A of ordinary numbers (mx_mixed_kernel): a frozen weight's input
+//                gradient (A = grad_y [m, r], B = W) and a layer's weight gradient from
+//                its kept input (A = grad_y^T, grad_y [r, m], B = x)
+#include "../../include/jakal_net_hip.h"
+#include "jn_internal.hpp"
+#include "jn_mx.hpp"
+
+namespace jakal {
+
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef int intx8 __attribute__((ext_vector_type(8)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
+
+// Tiles of a product's output over the workgroups: contiguous ranges per XCD,
+// bands of 8 row tiles sweeping the columns.
+struct TilePlace {
+  int split, mi, ni;
+  __device__ TilePlace(int tiles_m, int tiles_n) {
+    const int id = xcd_swizzle(blockIdx.x, gridDim.x);
+    const int per = tiles_m * tiles_n;
+    split = id / per;
+    const int t = id - split * per;
+    constexpr int kBand = 8;
+    const int band = t / (kBand * tiles_n);
+    const int bm = min(kBand, tiles_m - band * kBand);
+    const int tb = t - band * kBand * tiles_n;
+    mi = band * kBand + tb % bm;
+    ni = tb / bm;
+  }
+};
+
+// ---- ordinary numbers by microscaled ones ---------------------------------------
+// v_mfma_f32_16x16x32_bf16 over tiles of 128 x 128: microscaled values are bf16
+// values (at most four significant bits), and A is one, two or three bf16 terms
+// that add up to it exactly (bf16, fp16, fp32), so every product is exact and the
+// sums are fp32.  Both operands pass through registers on their way into LDS.  An
+// operand whose rows run along r lies there as it does in memory ([row][r]); one
+// whose rows run along m or n lies as [r][128] and is read transposed
+// (ds_read_b64_tr_b16).
+enum Product { kForward, kInputGrad, kWeightGrad };
+
+struct MixedArgs {
+  const void* a;          // [m][lda], or [r][lda] (weight gradient)
+  const uint8_t* codes;   // B: [n][pitch] along r (forward), or [r][pitch] along n
+  const uint8_t* scales;  // a byte a run, in the same order
+  const void* bias;       // [n] or null (forward)
+  void* out;              // [m][n] of the element type, or null: partial sums
+  float* partial;         // [splits][m][ldp]
+  void* bias_grad;        // [m]: sums of A over r (weight gradient), or null
+  float* bias_partial;    // [splits][m]
+  int64_t m, n, r;
+  int64_t lda, ldp, pitch, runs;
+  int64_t chunk;          // of r a split, a multiple of the slice
+  int tiles_m, tiles_n;
+};
+
+constexpr int kTile = 128;
+constexpr int kPlain = -1;  // activations that are not microscaled
+
+template <typename T>
+constexpr int kTerms = sizeof(T) == 4 ? 3 : std::is_same_v<T, f16_t> ? 2 : 1;
+template <typename T>
+constexpr int kSlice = kTerms<T> == 1 ? 64 : 32;
+
+// The bf16 terms of two numbers, each pair in a word.
+template <typename T>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[kTerms<T>]) {
+  if constexpr (kTerms<T> == 3) {
+    uint32_t h[2], m[2], l[2];
+    const uint32_t u[2] = {__float_as_uint(a), __float_as_uint(b)};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x3_split(u[i], h[i], m[i], l[i]);
+      // an infinity or a NaN has no remainder, and a NaN must not lose its low bits
+      if ((u[i] & 0x7F800000u) == 0x7F800000u) {
+        m[i] = l[i] = 0;
+        if (u[i] & 0x7FFFFFu) h[i] |= 0x400000u;
+      }
+    }
+    w[0] = x3_pair(h[0], h[1]), w[1] = x3_pair(m[0], m[1]), w[2] = x3_pair(l[0], l[1]);
+  } else {  // fp16: eight bits and the other three
+    const uint32_t h0 = __float_as_uint(a) & 0xFFFF0000u, h1 = __float_as_uint(b) & 0xFFFF0000u;
+    const bool f0 = fabsf(a) < __builtin_inff(), f1 = fabsf(b) < __builtin_inff();
+    const uint32_t l0 = f0 ? __float_as_uint(a - __uint_as_float(h0)) : 0;
+    const uint32_t l1 = f1 ? __float_as_uint(b - __uint_as_float(h1)) : 0;
+    const uint32_t q0 = a != a ? 0x400000u : 0u, q1 = b != b ? 0x400000u : 0u;
+    w[0] = x3_pair(h0 | q0, h1 | q1), w[1] = x3_pair(l0, l1);
+  }
+}
+
+// Places in LDS, in bf16 elements, so that the lanes of one read fall on all banks.
+// [row][SLICE] with the slice along the row: 16-byte chunks permuted by the row.
+template <int SLICE>
+__device__ __forceinline__ int lds_kc(int row, int chunk) {
+  if constexpr (SLICE == 64) return row * 64 + ((chunk ^ (row >> 1)) & 7) * 8;
+  else return row * 32 + ((chunk ^ (row >> 2)) & 3) * 8;
+}
+// [r][128]: 32-byte chunks permuted by the row.
+__device__ __forceinline__ int lds_tr(int r, int chunk32) {
+  return r * kTile + ((chunk32 ^ ((r & 3) | ((r >> 1) & 4))) & 7) * 16;
+}
+
+__device__ __forceinline__ shortx4 read_tr(const bf16_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) shortx4*)(const_cast<bf16_t*>(p)));
+}
+
+// Eight consecutive r from r0 on of column c16 * 16 + (lane & 15), for lane group g: r0 = 8 g.
+__device__ __forceinline__ bf16x8v fragment_tr(const bf16_t* plane, int r0, int c16, int lane) {
+  const int i = lane & 15;
+  const shortx4 a = read_tr(plane + lds_tr(r0 + (i >> 2), c16) + (i & 3) * 4);
+  const shortx4 b = read_tr(plane + lds_tr(r0 + 4 + (i >> 2), c16) + (i & 3) * 4);
+  typedef short shortx8 __attribute__((ext_vector_type(8)));
+  return __builtin_bit_cast(bf16x8v, (shortx8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Four consecutive elements of an output row of n elements, from element c on.
+template <typename T>
+__device__ __forceinline__ void store_quad(T* p, int64_t c, int64_t n, const float (&v)[4]) {
+  if (n % 4 == 0) {
+    store_raw<T, 4>(p, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (c + q < n) p[q] = (T)v[q];
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void load_bias(const T* bias, int64_t c, int64_t n, float (&b)[4]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) b[q] = bias && c + q < n ? (float)bias[c + q] : 0.f;
+}
+
+// Two elements of e4m3 or e2m1 as bf16, times the run's scale: one instruction.
+template <int FORM, int WORD_HALF>
+__device__ __forceinline__ uint32_t decode_pair(uint32_t code, float scale) {
+  if constexpr (FORM == kE4m3)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code, scale, WORD_HALF));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, scale, WORD_HALF));
+}
+
+template <typename T, Product P, bool PACKED>
+__global__ __launch_bounds__(256, 2) void mx_mixed_kernel(MixedArgs g) {
+  constexpr int FORM = P == kWeightGrad ? kE4m3 : kE2m1;
+  constexpr bool A_R = P != kWeightGrad, B_R = P == kForward;  // rows along r
+  constexpr int TERMS = kTerms<T>, SLICE = kSlice<T>;
+  constexpr int kPlane = kTile * SLICE;            // elements of a plane
+  constexpr int kStage = (TERMS + 1) * kPlane;
+  constexpr int kUnits = kPlane / 8 / 256;         // units of eight elements a thread: of A, and of B
+  __shared__ __align__(16) bf16_t smem[2 * kStage];
+
+  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
+  const int grp = lane >> 4, col = lane & 15;
+  const int wm = wave >> 1, wn = wave & 1;
+  const TilePlace at(g.tiles_m, g.tiles_n);
+  const int64_t m0 = (int64_t)at.mi * kTile, n0 = (int64_t)at.ni * kTile;
+  const int64_t rbeg = at.split * g.chunk, rend = min(g.r, rbeg + g.chunk);
+  const T* abase = static_cast<const T*>(g.a);
+  const bool sums = P == kWeightGrad && g.bias_partial && at.ni == 0;
+
+  // one slice in registers
+  constexpr int W = PACKED ? 16 / sizeof(T) : 1;
+  Raw<T, W> ra[kUnits][8 / W];
+  uint2 rb[kUnits];
+  int rs[kUnits];
+
+  auto load = [&](int64_t r0) {
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int id = tid + 256 * u;
+      const int64_t row = A_R ? m0 + id / (SLICE / 8) : r0 + id / (kTile / 8);
+      const int64_t c = A_R ? r0 + id % (SLICE / 8) * 8 : m0 + id % (kTile / 8) * 8;
+      const int64_t rows = A_R ? g.m : rend, cols = A_R ? rend : g.m;
+      const T* p = abase + row * g.lda + c;
+#pragma unroll
+      for (int j = 0; j < 8 / W; ++j) {
+        if (row < rows && c + j * W < cols) ra[u][j].load(p + j * W);
+        else ra[u][j].clear();
+      }
+      const int64_t brow = B_R ? n0 + id / (SLICE / 8) : r0 + id / (kTile / 8);
+      const int64_t e = B_R ? r0 + id % (SLICE / 8) * 8 : n0 + id % (kTile / 8) * 8;
+      rb[u] = uint2{0, 0}, rs[u] = 127;
+      if (brow < (B_R ? g.n : rend) && e < g.runs * kMxRun) {
+        if constexpr (FORM == kE4m3) rb[u] = *reinterpret_cast<const uint2*>(g.codes + brow * g.pitch + e);
+        else rb[u].x = *reinterpret_cast<const uint32_t*>(g.codes + brow * g.pitch + e / 2);
+        rs[u] = g.scales[brow * g.runs + e / kMxRun];
+      }
+    }
+  };
+  float total[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto store = [&](bf16_t* stage) {
+    bf16_t* sb = stage + TERMS * kPlane;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int id = tid + 256 * u;
+      const int along = lds_kc<SLICE>(id / (SLICE / 8), id % (SLICE / 8));
+      const int across = lds_tr(id / (kTile / 8), id % (kTile / 8) / 2) + id % 2 * 8;
+      const int place = A_R ? along : across;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8 / W; ++j) ra[u][j].unpack(v + j * W);
+      if (sums) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) total[j] += v[j];
+      }
+      if constexpr (TERMS == 1) {
+        uint4 w;
+        if constexpr (PACKED) w = ra[u][0].bits;
+        else w = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+        *reinterpret_cast<uint4*>(stage + place) = w;
+      } else {
+        uint32_t w[4][TERMS];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_pair<T>(v[2 * j], v[2 * j + 1], w[j]);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+          *reinterpret_cast<uint4*>(stage + t * kPlane + place) = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
+      }
+      const float scale = mx_scale(rs[u]);
+      uint4 d;
+      if constexpr (FORM == kE4m3)
+        d = make_uint4(decode_pair<FORM, 0>(rb[u].x, scale), decode_pair<FORM, 1>(rb[u].x, scale),
+                       decode_pair<FORM, 0>(rb[u].y, scale), decode_pair<FORM, 1>(rb[u].y, scale));
+      else
+        d = make_uint4(decode_pair<FORM, 0>(rb[u].x, scale), decode_pair<FORM, 1>(rb[u].x, scale),
+                       decode_pair<FORM, 2>(rb[u].x, scale), decode_pair<FORM, 3>(rb[u].x, scale));
+      *reinterpret_cast<uint4*>(sb + (B_R ? along : across)) = d;
+    }
+  };
+
+  floatx4 acc[4][4];  // [n][m] tiles of 16
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  const int slices = rend > rbeg ? (int)((rend - rbeg + SLICE - 1) / SLICE) : 0;
+  if (slices > 0) {
+    load(rbeg);
+    store(smem);
+  }
+  __syncthreads();
+  for (int s = 0; s < slices; ++s) {
+    const bf16_t* stage = smem + (s & 1) * kStage;
+    if (s + 1 < slices) load(rbeg + (int64_t)(s + 1) * SLICE);
+#pragma unroll
+    for (int k = 0; k < SLICE / 32; ++k) {
+      bf16x8v b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (B_R)
+          b[i] = *reinterpret_cast<const bf16x8v*>(stage + TERMS * kPlane +
+                                                   lds_kc<SLICE>(wn * 64 + i * 16 + col, k * 4 + grp));
+        else
+          b[i] = fragment_tr(stage + TERMS * kPlane, k * 32 + grp * 8, wn * 4 + i, lane);
+      }
+#pragma unroll
+      for (int t = TERMS - 1; t >= 0; --t) {  // the smallest terms first
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          bf16x8v a;
+          if constexpr (A_R)
+            a = *reinterpret_cast<const bf16x8v*>(stage + t * kPlane +
+                                                  lds_kc<SLICE>(wm * 64 + j * 16 + col, k * 4 + grp));
+          else
+            a = fragment_tr(stage + t * kPlane, k * 32 + grp * 8, wm * 4 + j, lane);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[i], a, acc[i][j], 0, 0, 0);
+        }
+      }
+    }
+    if (s + 1 < slices) store(smem + ((s + 1) & 1) * kStage);
+    __syncthreads();
+  }
+
+  // a lane holds four consecutive n of one m in each tile
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = n0 + wn * 64 + i * 16 + grp * 4;
+    if (n >= g.n) continue;
+    float bias[4] = {0.f, 0.f, 0.f, 0.f};
+    if (P == kForward && g.out) load_bias(static_cast<const T*>(g.bias), n, g.n, bias);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t m = m0 + wm * 64 + j * 16 + col;
+      if (m >= g.m) continue;
+      if (g.out) {
+        const float v[4] = {acc[i][j][0] + bias[0], acc[i][j][1] + bias[1], acc[i][j][2] + bias[2],
+                            acc[i][j][3] + bias[3]};
+        store_quad(static_cast<T*>(g.out) + m * g.n + n, n, g.n, v);
+      } else {
+        *reinterpret_cast<floatx4*>(g.partial + ((int64_t)at.split * g.m + m) * g.ldp + n) = acc[i][j];
+      }
+    }
+  }
+  if (sums) {  // the 16 threads that had the same eight columns, in order
+    float* lds = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) lds[(tid / 16) * kTile + tid % 16 * 8 + j] = total[j];
+    __syncthreads();
+    if (tid < kTile && m0 + tid < g.m) {
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t += lds[i * kTile + tid];
+      g.bias_partial[(int64_t)at.split * g.m + m0 + tid] = t;
+    }
+  }
+}
+
+// The splits' sums in order, rounded once.  One thread four elements of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void mx_sum_kernel(MixedArgs g, int splits) {
+  const int64_t quads = g.ldp / 4, total = g.partial ? g.m * quads : 0;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id < total) {
+    const int64_t m = id / quads, n = (id - m * quads) * 4;
+    floatx4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s)
+      v += *reinterpret_cast<const floatx4*>(g.partial + ((int64_t)s * g.m + m) * g.ldp + n);
+    float w[4];
+    load_bias(static_cast<const T*>(g.bias), n, g.n, w);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w[q] += v[q];
+    store_quad(static_cast<T*>(g.out) + m * g.n + n, n, g.n, w);
+  } else if (g.bias_partial && id - total < g.m) {
+    const int64_t m = id - total;
+    float t = 0.f;
+    for (int s = 0; s < splits; ++s) t += g.bias_partial[(int64_t)s * g.m + m];
+    static_cast<T*>(g.bias_grad)[m] = (T)t;
+  }
+}
+
+// Splits of the sum: workgroups enough for two a CU, slices enough for each.
+struct MixedPlan {
+  int tiles_m, tiles_n, splits;
+  int64_t chunk, ldp;
+  size_t partial_bytes, bias_bytes;
+
+  MixedPlan(int64_t m, int64_t n, int64_t r, int32_t type, bool bias) {
+    const int slice = type == kTypeBf16 ? kSlice<bf16_t> : kSlice<float>;
+    tiles_m = (int)((m + kTile - 1) / kTile), tiles_n = (int)((n + kTile - 1) / kTile);
+    const int64_t tiles = (int64_t)tiles_m * tiles_n, slices = std::max<int64_t>(1, (r + slice - 1) / slice);
+    const int64_t want = std::min<int64_t>({(512 + tiles - 1) / tiles, std::max<int64_t>(1, slices / 4), 64});
+    const int64_t each = (slices + want - 1) / want;
+    splits = (int)std::max<int64_t>(1, (slices + each - 1) / each);
+    chunk = each * slice;
+    ldp = (n + 3) / 4 * 4;
+    partial_bytes = splits > 1 ? (size_t)splits * m * ldp * sizeof(float) : 0;
+    bias_bytes = bias ? (size_t)splits * m * sizeof(float) : 0;
+  }
+  size_t bytes() const { return (partial_bytes + 255) / 256 * 256 + bias_bytes; }
+};
+
+template <Product P>
+int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size_t workspace_bytes,
+             hipStream_t s) {
+  const MixedPlan plan(g.m, g.n, g.r, type, g.bias_grad != nullptr);
+  JN_REQUIRE(plan.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes()),
+             kWorkspaceTooSmall, "%s: needs %zu workspace bytes on a 16-byte address, got %zu", what, plan.bytes(),
+             workspace_bytes);
+  JN_REQUIRE((int64_t)plan.tiles_m * plan.tiles_n * plan.splits < (int64_t(1) << 31), kUnsupported,
+             "%s: too many output tiles", what);
+  void* const out = g.out;
+  g.tiles_m = plan.tiles_m, g.tiles_n = plan.tiles_n, g.chunk = plan.chunk, g.ldp = plan.ldp;
+  const int64_t along = P == kForward ? g.r : g.n;
+  g.runs = mx_runs(along), g.pitch = mx_pitch(along, P == kWeightGrad ? kE4m3 : kE2m1);
+  if (plan.partial_bytes) g.out = nullptr, g.partial = static_cast<float*>(workspace);
+  if (g.bias_grad)
+    g.bias_partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + (plan.partial_bytes + 255) / 256 * 256);
+  const dim3 grid((unsigned)((int64_t)plan.tiles_m * plan.tiles_n * plan.splits));
+  return with_type(type, [&](auto* t) -> int {
+    using T = std::remove_pointer_t<decltype(t)>;
+    const bool packed = aligned16(g.a) && g.lda * sizeof(T) % 16 == 0;
+    {
+      JN_PROFILE(P == kForward ? "mx_forward_kernel" : P == kInputGrad ? "mx_input_grad_kernel" : "mx_weight_grad_kernel", s);
+      if (packed) hipLaunchKernelGGL((mx_mixed_kernel<T, P, true>), grid, dim3(256), 0, s, g);
+      else hipLaunchKernelGGL((mx_mixed_kernel<T, P, false>), grid, dim3(256), 0, s, g);
+      JN_LAUNCH_CHECK();
+    }
+    if (g.partial || g.bias_partial) {
+      JN_PROFILE("mx_sum_kernel", s);
+      g.out = out;
+      const int64_t threads = (g.partial ? g.m * (g.ldp / 4) : 0) + (g.bias_partial ? g.m : 0);
+      hipLaunchKernelGGL(mx_sum_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, g,
+                         plan.splits);
+      JN_LAUNCH_CHECK();
+    }
+    return kOk;
+  });
+}
+
+// ---- sums over rows -------------------------------------------------------------
+// A thread sums one column over a slab of rows, a second launch the slabs in order.
+constexpr int64_t kSlabRows = 64, kSlabs = 256;
+
+int64_t sum_slabs(int64_t rows) { return std::min(kSlabs, (rows + kSlabRows - 1) / kSlabRows); }
+
+template <typename T>
+__global__ __launch_bounds__(256) void column_sums_kernel(const T* x, int64_t rows, int64_t dim, int64_t each,
+                                                          float* partial) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= dim) return;
+  const int64_t beg = blockIdx.y * each, end = min(rows, beg + each);
+  float t = 0.f;
+  for (int64_t r = beg; r < end; ++r) t += (float)x[r * dim + c];
+  partial[blockIdx.y * dim + c] = t;
+}
+
+// ---- forward: microscaled by microscaled --------------------------------------
+// v_mfma_scale_f32_16x16x128_f8f6f4 on e2m1 by e2m1: four runs of k an instruction,
+// their scales a byte a lane.  A run's products span eight bits, so its sum is exact,
+// and the runs' sums are added in fp32.  (With e4m3 the instruction drops what lies
+// 14 bits below the run's largest product; x is e2m1 here or not microscaled at all.)
+// Tiles of 128 x 128, slices of 256 k, LDS double buffered.
+struct LinearArgs {
+  const uint8_t* x;   // [m][pitch]
+  const uint8_t* xs;  // [m][runs]
+  const uint8_t* w;   // [n][pitch]
+  const uint8_t* ws;  // [n][runs]
+  const void* bias;   // [n] or null
+  void* y;            // [m][n]
+  int64_t m, n, runs, pitch;
+  int tiles_m, tiles_n;
+};
+
+constexpr int kMxSlice = 256;                   // elements of k
+constexpr int kSliceRuns = kMxSlice / kMxRun;   // 8
+
+// Rows of 8 chunks of 16 bytes, permuted by the row.
+__device__ __forceinline__ int lds_row(int row, int chunk) { return row * 128 + ((chunk ^ (row >> 1)) & 7) * 16; }
+
+template <typename T>
+__global__ __launch_bounds__(256) void mx_linear_kernel(LinearArgs g) {
+  constexpr int C = 8;  // 16-byte chunks of a row's slice
+  constexpr int kX = kTile * C * 16, kS = kTile * kSliceRuns;
+  constexpr int kStage = 2 * (kX + kS);
+  __shared__ __align__(16) uint8_t smem[2 * kStage];
+
+  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
+  const int grp = lane >> 4, col = lane & 15;
+  const int wm = wave >> 1, wn = wave & 1;
+  const TilePlace at(g.tiles_m, g.tiles_n);
+  const int64_t m0 = (int64_t)at.mi * kTile, n0 = (int64_t)at.ni * kTile;
+
+  uint4 rx[C / 2], rw[C / 2];
+  uint64_t rs;
+  auto load = [&](int64_t k0) {  // in runs
+#pragma unroll
+    for (int u = 0; u < C / 2; ++u) {
+      const int id = tid + 256 * u, row = id / C;
+      const int64_t byte = k0 * 16 + id % C * 16;
+      rx[u] = m0 + row < g.m && byte < g.pitch ? *reinterpret_cast<const uint4*>(g.x + (m0 + row) * g.pitch + byte)
+                                               : make_uint4(0, 0, 0, 0);
+      rw[u] = n0 + row < g.n && byte < g.pitch ? *reinterpret_cast<const uint4*>(g.w + (n0 + row) * g.pitch + byte)
+                                               : make_uint4(0, 0, 0, 0);
+    }
+    // a row's eight scales a thread: of X, then of W; 2^0 past the end
+    const bool is_x = tid < kTile;
+    const int64_t row = is_x ? m0 + tid : n0 + tid - kTile;
+    const uint8_t* p = (is_x ? g.xs : g.ws) + row * g.runs + k0;
+    rs = 0;
+#pragma unroll
+    for (int i = 0; i < kSliceRuns; ++i) {
+      const uint64_t s = row < (is_x ? g.m : g.n) && k0 + i < g.runs ? p[i] : 127;
+      rs |= s << (8 * i);
+    }
+  };
+  auto store = [&](uint8_t* stage) {
+#pragma unroll
+    for (int u = 0; u < C / 2; ++u) {
+      const int id = tid + 256 * u;
+      *reinterpret_cast<uint4*>(stage + lds_row(id / C, id % C)) = rx[u];
+      *reinterpret_cast<uint4*>(stage + kX + lds_row(id / C, id % C)) = rw[u];
+    }
+    *reinterpret_cast<uint64_t*>(stage + 2 * kX + tid * 8) = rs;
+  };
+
+  floatx4 acc[4][4];  // [n][m] tiles of 16
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  const int slices = (int)((g.runs + kSliceRuns - 1) / kSliceRuns);
+  load(0);
+  store(smem);
+  __syncthreads();
+  for (int s = 0; s < slices; ++s) {
+    const uint8_t* stage = smem + (s & 1) * kStage;
+    if (s + 1 < slices) load((int64_t)(s + 1) * kSliceRuns);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      intx8 x[4], w[4];
+      int xs[4], ws[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // a lane has the run 4 k + grp of its row
+        const int xr = wm * 64 + i * 16 + col, wr = wn * 64 + i * 16 + col;
+        const uint4 a = *reinterpret_cast<const uint4*>(stage + lds_row(xr, 4 * k + grp));
+        const uint4 b = *reinterpret_cast<const uint4*>(stage + kX + lds_row(wr, 4 * k + grp));
+        x[i] = intx8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+        w[i] = intx8{(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+        xs[i] = (int)(*reinterpret_cast<const uint32_t*>(stage + 2 * kX + xr * 8 + k * 4) >> (8 * grp));
+        ws[i] = (int)(*reinterpret_cast<const uint32_t*>(stage + 2 * kX + kS + wr * 8 + k * 4) >> (8 * grp));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x[j], acc[i][j], 4, 4, 0, ws[i], 0, xs[j]);
+    }
+    if (s + 1 < slices) store(smem + ((s + 1) & 1) * kStage);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = n0 + wn * 64 + i * 16 + grp * 4;
+    if (n >= g.n) continue;
+    float b[4];
+    load_bias(static_cast<const T*>(g.bias), n, g.n, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t m = m0 + wm * 64 + j * 16 + col;
+      if (m >= g.m) continue;
+      const float v[4] = {acc[i][j][0] + b[0], acc[i][j][1] + b[1], acc[i][j][2] + b[2], acc[i][j][3] + b[3]};
+      store_quad(static_cast<T*>(g.y) + m * g.n + n, n, g.n, v);
+    }
+  }
+}
+
+size_t linear_codes_bytes(int64_t rows, int64_t dim) { return (size_t)(rows * mx_pitch(dim, kE2m1) + 255) / 256 * 256; }
+
+int check_product(const char* what, int64_t rows, int64_t dim, int64_t out, int32_t type) {
+  JN_REQUIRE(known_type(type), kInvalidArgument, "%s: unknown element type %d", what, type);
+  JN_REQUIRE(rows >= 1 && dim >= 1 && out >= 1 && rows < (int64_t(1) << 31) && dim < (int64_t(1) << 24) &&
+                 out < (int64_t(1) << 24),
+             kInvalidArgument, "%s: needs 1 to 2^31 - 1 rows and 1 to 2^24 - 1 inputs and outputs, got %lld, %lld, %lld",
+             what, (long long)rows, (long long)dim, (long long)out);
+  return kOk;
+}
+
+}  // namespace
+}  // namespace jakal
+
+using namespace jakal;
+
+extern "C" {
+
+size_t jn_mx_linear_forward_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t activations) {
+  if (check_product("mx_linear", rows, dim, out, type)) return 0;
+  if (activations == kPlain) return MixedPlan(rows, out, dim, type, false).bytes();
+  return linear_codes_bytes(rows, dim) + (size_t)(rows * mx_runs(dim));
+}
+
+int jn_mx_linear_forward(const void* x, const void* weight_codes, const void* weight_scales, const void* bias,
+                         int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t activations, void* y,
+                         void* workspace, size_t workspace_bytes, jn_stream_t stream) {
+  if (const int rc = check_product("mx_linear", rows, dim, out, type)) return rc;
+  JN_REQUIRE(activations == kE2m1 || activations == kPlain, kInvalidArgument,
+             "mx_linear: activations are e2m1 (1) or as they are (-1), got %d", activations);
+  JN_REQUIRE(x && weight_codes && weight_scales && y, kInvalidArgument, "null tensor pointer");
+  JN_REQUIRE(aligned16(weight_codes) && aligned16(y), kInvalidArgument,
+             "mx_linear: weight codes and outputs must start on 16 bytes");
+  const auto s = static_cast<hipStream_t>(stream);
+  if (activations == kPlain) {
+    MixedArgs g{};
+    g.a = x, g.codes = static_cast<const uint8_t*>(weight_codes), g.scales = static_cast<const uint8_t*>(weight_scales);
+    g.bias = bias, g.out = y, g.m = rows, g.n = out, g.r = dim, g.lda = dim;
+    return run_mixed<kForward>("mx_linear", g, type, workspace, workspace_bytes, s);
+  }
+  const size_t need = jn_mx_linear_forward_workspace_bytes(rows, dim, out, type, activations);
+  JN_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, kWorkspaceTooSmall,
+             "mx_linear: needs %zu workspace bytes on a 16-byte address, got %zu", need, workspace_bytes);
+  LinearArgs g{};
+  uint8_t* const codes = static_cast<uint8_t*>(workspace);
+  uint8_t* const scales = codes + linear_codes_bytes(rows, dim);
+  g.x = codes, g.xs = scales;
+  g.w = static_cast<const uint8_t*>(weight_codes), g.ws = static_cast<const uint8_t*>(weight_scales);
+  g.bias = bias, g.y = y, g.m = rows, g.n = out, g.runs = mx_runs(dim), g.pitch = mx_pitch(dim, kE2m1);
+  g.tiles_m = (int)((rows + kTile - 1) / kTile), g.tiles_n = (int)((out + kTile - 1) / kTile);
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
+  JN_REQUIRE(tiles < (int64_t(1) << 31), kUnsupported, "mx_linear: too many output tiles");
+  if (const int rc = launch_mx_quantize(x, rows, dim, type, kE2m1, codes, scales, s)) return rc;
+  return with_type(type, [&](auto* t) -> int {
+    using T = std::remove_pointer_t<decltype(t)>;
+    JN_PROFILE("mx_linear_kernel", s);
+    hipLaunchKernelGGL(mx_linear_kernel<T>, dim3((unsigned)tiles), dim3(256), 0, s, g);
+    JN_LAUNCH_CHECK();
+    return kOk;
+  });
+}
+
+size_t jn_mx_linear_backward_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type) {
+  if (check_product("mx_linear backward", rows, dim, out, type)) return 0;
+  return MixedPlan(rows, dim, out, type, false).bytes();
+}
+
+int jn_mx_linear_backward(const void* grad_y, const void* weight_codes, const void* weight_scales, int64_t rows,
+                          int64_t dim, int64_t out, int32_t type, void* grad_x, void* workspace,
+                          size_t workspace_bytes, jn_stream_t stream) {
+  if (const int rc = check_product("mx_linear backward", rows, dim, out, type)) return rc;
+  JN_REQUIRE(grad_y && weight_codes && weight_scales && grad_x, kInvalidArgument, "null tensor pointer");
+  JN_REQUIRE(aligned16(weight_codes) && aligned16(grad_x), kInvalidArgument,
+             "mx_linear backward: weight codes and grad_x must start on 16 bytes");
+  MixedArgs g{};
+  g.a = grad_y, g.codes = static_cast<const uint8_t*>(weight_codes);
+  g.scales = static_cast<const uint8_t*>(weight_scales);
+  g.out = grad_x, g.m = rows, g.n = dim, g.r = out, g.lda = out;
+  return run_mixed<kInputGrad>("mx_linear backward", g, type, workspace, workspace_bytes,
+                        static_cast<hipStream_t>(stream));
+}
+
+size_t jn_mx_weight_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t bias) {
+  if (check_product("mx_weight_grad", rows, dim, out, type)) return 0;
+  return MixedPlan(out, dim, rows, type, bias != 0).bytes();
+}
+
+int jn_mx_weight_grad(const void* grad_y, const void* codes, const void* scales, int64_t rows, int64_t dim,
+                      int64_t out, int32_t type, void* grad_weight, void* grad_bias, void* workspace,
+                      size_t workspace_bytes, jn_stream_t stream) {
+  if (const int rc = check_product("mx_weight_grad", rows, dim, out, type)) return rc;
+  JN_REQUIRE(grad_y && codes && scales && grad_weight, kInvalidArgument, "null tensor pointer");
+  JN_REQUIRE(aligned16(codes) && aligned16(grad_weight), kInvalidArgument,
+             "mx_weight_grad: codes and grad_weight must start on 16 bytes");
+  MixedArgs g{};
+  g.a = grad_y, g.codes = static_cast<const uint8_t*>(codes), g.scales = static_cast<const uint8_t*>(scales);
+  g.out = grad_weight, g.bias_grad = grad_bias, g.m = out, g.n = dim, g.r = rows, g.lda = out;
+  return run_mixed<kWeightGrad>("mx_weight_grad", g, type, workspace, workspace_bytes,
+                         static_cast<hipStream_t>(stream));
+}
+
+size_t jn_column_sums_workspace_bytes(int64_t rows, int64_t dim) {
+  return rows < 1 || dim < 1 ? 0 : (size_t)(sum_slabs(rows) * dim) * sizeof(float);
+}
+
+int jn_column_sums(const void* x, int64_t rows, int64_t dim, int32_t type, void* sums, void* workspace,
+                   size_t workspace_bytes, jn_stream_t stream) {
+  if (const int rc = check_product("column_sums", rows, 1, dim, type)) return rc;
+  JN_REQUIRE(x && sums, kInvalidArgument, "null tensor pointer");
+  const size_t need = jn_column_sums_workspace_bytes(rows, dim);
+  JN_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, kWorkspaceTooSmall,
+             "column_sums: needs %zu workspace bytes on a 16-byte address, got %zu", need, workspace_bytes);
+  const auto s = static_cast<hipStream_t>(stream);
+  const int64_t slabs = sum_slabs(rows), each = (rows + slabs - 1) / slabs;
+  const unsigned columns = (unsigned)((dim + 255) / 256);
+  MixedArgs g{};
+  g.bias_partial = static_cast<float*>(workspace), g.bias_grad = sums, g.m = dim;
+  return with_type(type, [&](auto* t) -> int {
+    using T = std::remove_pointer_t<decltype(t)>;
+    JN_PROFILE("column_sums_kernel", s);
+    hipLaunchKernelGGL(column_sums_kernel<T>, dim3(columns, (unsigned)slabs), dim3(256), 0, s,
+                       static_cast<const T*>(x), rows, dim, each, g.bias_partial);
+    JN_LAUNCH_CHECK();
+    hipLaunchKernelGGL(mx_sum_kernel<T>, dim3(columns), dim3(256), 0, s, g, (int)slabs);
+    JN_LAUNCH_CHECK();
+    return kOk;
+  });
+}
+
+}  // extern "C"

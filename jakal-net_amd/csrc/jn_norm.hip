@@ -7,9 +7,15 @@
 //   g_w = g w;  dx = scale r (g_w - mean(g_w) - h mean(g_w h))
 //   dw = sum over rows of g h,  db = sum over rows of g
 //   dstate = scale (1 - tanh^2) g_state
+//
+// Or keeping c = x - p in e4m3 for the backward (jn_layer_norm_*_kept), p being the
+// mean of x in 64 bits rounded to fp32: the forward is the same, h in the gradients
+// is scale r times the kept c.  What is kept is centred so that its rounding is
+// relative to h whatever the mean is; the mean in 64 bits is the same number in any
+// order of summing, and with it the codes are.
 #include "../../include/jakal_net_hip.h"
 #include "jn_internal.hpp"
-#include "jn_rows.hpp"
+#include "jn_mx.hpp"
 
 namespace jakal {
 namespace {
@@ -34,6 +40,9 @@ struct NormArgs {
   float* partial;   // [slabs][2][dim], or null: one workgroup has all sums, and writes dw and db
   void* dw;         // or null
   void* db;         // or null
+  // the centred x in e4m3: written beside y, or read in x's place; or null
+  uint8_t* codes;
+  uint8_t* scales;
 };
 
 // tanh and its slope 1 - tanh^2 = 4 e / (1 + e)^2 with e = exp(-2 |v|), which
@@ -124,6 +133,174 @@ __device__ __forceinline__ void load_row(const void* base, int64_t row, const No
   }
 }
 
+// W elements of a row kept in e4m3, and their run's scale.
+template <int W>
+struct KeptPack {
+  std::conditional_t<W == 1, uint8_t, std::conditional_t<W == 4, uint32_t, uint2>> code;
+  uint8_t scale;
+
+  __device__ __forceinline__ void clear() { code = {}, scale = 127; }
+  __device__ __forceinline__ void unpack(float* v) const {
+    const float f = mx_scale(scale);
+    if constexpr (W == 1) {
+      v[0] = __builtin_amdgcn_cvt_f32_fp8((int)code, 0) * f;
+    } else {
+      uint32_t words[2] = {0, 0};
+      if constexpr (W == 4) words[0] = code;
+      else words[0] = code.x, words[1] = code.y;
+#pragma unroll
+      for (int i = 0; i < W; i += 2) {
+        const floatx2_t x = i % 4 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)words[i / 4], true)
+                                  : __builtin_amdgcn_cvt_pk_f32_fp8((int)words[i / 4], false);
+        v[i] = x[0] * f, v[i + 1] = x[1] * f;
+      }
+    }
+  }
+};
+
+template <typename T, int W, int NP, typename G>
+__device__ __forceinline__ void load_row(const NormArgs& a, int64_t row, KeptPack<W> (&kept)[NP]) {
+  const uint8_t* codes = a.codes + row * mx_pitch(a.dim, kE4m3);
+  const uint8_t* scales = a.scales + row * mx_runs(a.dim);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int e = G::element(i);
+    if (row < a.rows && e < a.dim) {
+      kept[i].code = *reinterpret_cast<const decltype(kept[i].code)*>(codes + e);
+      kept[i].scale = scales[e / kMxRun];
+    } else {
+      kept[i].clear();
+    }
+  }
+}
+template <typename T, int W, int NP, typename G>
+__device__ __forceinline__ void load_row(const NormArgs& a, int64_t row, Raw<T, W> (&raw)[NP]) {
+  load_row<T, W, NP, G>(a.x, row, a, raw);
+}
+
+// The sum of a value over each group of TH threads in 64 bits, in all of them.
+template <int TH, int BLOCK>
+__device__ __forceinline__ double group_sum_64(double v, double* lds) {
+#pragma unroll
+  for (int i = 1; i < (TH < kWave ? TH : kWave); i *= 2) v += __shfl_xor(v, i);
+  if constexpr (TH > kWave) {
+    constexpr int kWaves = TH / kWave;
+    __syncthreads();  // the readers before are done
+    if (lane_id() == 0) lds[wave_id()] = v;
+    __syncthreads();
+    const int first = wave_id() / kWaves * kWaves;
+    v = 0.0;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) v += lds[first + k];
+  }
+  return v;
+}
+
+// Keeps a row, centred, in e4m3: the largest of a run's elements over the 32 / W lanes
+// that hold it (two packs of sixteen lanes where rows of single elements have no more).
+template <int W, int NP, int TH, int BLOCK, typename G>
+__device__ __forceinline__ void keep_row(const NormArgs& a, int64_t row, const float* x, double* lds) {
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < W * NP; ++i) sum += x[i];  // (zeros past the row's end)
+  const float p = (float)(group_sum_64<TH, BLOCK>(sum, lds) / (double)a.dim);
+  float v[W * NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+#pragma unroll
+    for (int j = i * W; j < i * W + W; ++j) v[j] = G::element(i) < a.dim ? x[j] - p : 0.f;
+  }
+  uint32_t most[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    most[i] = 0;
+#pragma unroll
+    for (int j = 0; j < W; ++j) most[i] = max(most[i], __float_as_uint(v[i * W + j]) & 0x7FFFFFFFu);
+  }
+  constexpr bool kPairs = W == 1 && TH == 16;
+  static_assert(!kPairs || NP % 2 == 0, "a run is two packs");
+  if constexpr (kPairs) {
+#pragma unroll
+    for (int i = 0; i < NP; i += 2) most[i] = most[i + 1] = max(most[i], most[i + 1]);
+  }
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    most[i] = quad_max(most[i]);
+    if constexpr (W <= 4)  // eight lanes
+      most[i] = max(most[i], (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most[i], 0x141, 0xF, 0xF, true));
+    if constexpr (W == 1) {  // sixteen, and 32
+      most[i] = max(most[i], (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most[i], 0x140, 0xF, 0xF, true));
+      if constexpr (!kPairs) most[i] = max(most[i], (uint32_t)xor16_i((int)most[i]));
+    }
+  }
+  if (row >= a.rows) return;
+  const int64_t pitch = mx_pitch(a.dim, kE4m3);
+  uint8_t* codes = a.codes + row * pitch;
+  uint8_t* scales = a.scales + row * mx_runs(a.dim);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int e = G::element(i);
+    if (e >= pitch) continue;
+    const int s = mx_scale_code<kE4m3>(most[i]);
+    const float inv = __uint_as_float((uint32_t)(254 - min(s, 253)) << 23);
+    uint32_t words[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < W; j += 2) {
+      const float x = v[i * W + j] * inv, y = W > 1 ? v[i * W + (W > 1 ? j + 1 : j)] * inv : 0.f;
+      words[j / 4] = j % 4 ? __builtin_amdgcn_cvt_pk_fp8_f32(x, y, (int)words[j / 4], true)
+                           : __builtin_amdgcn_cvt_pk_fp8_f32(x, y, (int)words[j / 4], false);
+    }
+    if (s == 255) words[0] = words[1] = 0x7F7F7F7Fu;
+    if constexpr (W == 1) codes[e] = (uint8_t)words[0];
+    else if constexpr (W == 4) *reinterpret_cast<uint32_t*>(codes + e) = words[0];
+    else *reinterpret_cast<uint2*>(codes + e) = make_uint2(words[0], words[1]);
+    if (e % kMxRun == 0) scales[e / kMxRun] = (uint8_t)s;
+  }
+}
+
+// The same for rows of any width: a workgroup a row.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_keep_any_kernel(NormArgs a) {
+  __shared__ double lds[4];
+  const int64_t units = mx_runs(a.dim) * 4;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.dim;
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < a.dim; i += 256) sum += (double)(float)x[i];
+    const float p = (float)(group_sum_64<256, 256>(sum, lds) / (double)a.dim);
+    for (int64_t u = threadIdx.x; u < units; u += 256) {  // whole quads
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = u * 8 + j < a.dim ? (float)x[u * 8 + j] - p : 0.f;
+      uint32_t code[2];
+      const int s = mx_encode<kE4m3>(v, code);
+      mx_store<kE4m3>(a.codes, a.scales, row * units + u, code, s);
+    }
+  }
+}
+
+// h of element i of a row: from x, or from what was kept of it.
+template <typename T, bool KEPT>
+struct RowReader {
+  const T* x;
+  const uint8_t* codes;
+  const uint8_t* scales;
+  float scale, m, r;
+
+  __device__ RowReader(const NormArgs& a, int64_t row) {
+    if constexpr (KEPT) codes = a.codes + row * mx_pitch(a.dim, kE4m3), scales = a.scales + row * mx_runs(a.dim);
+    else x = static_cast<const T*>(a.x) + row * a.dim;
+    scale = a.scale, m = a.stats[2 * row], r = a.stats[2 * row + 1];
+  }
+  __device__ __forceinline__ float operator[](int64_t i) const {
+    if constexpr (KEPT) {
+      return scale * (__builtin_amdgcn_cvt_f32_fp8((int)codes[i], 0) * mx_scale(scales[i / kMxRun])) * r;
+    } else {
+      return (scale * (float)x[i] - m) * r;
+    }
+  }
+};
+
 template <typename T, int W, int NP, typename G>
 __device__ __forceinline__ void load_params(const void* base, int type, int64_t dim, float none,
                                             float (&v)[W * NP]) {
@@ -153,10 +330,11 @@ __device__ __forceinline__ void load_params(const void* base, int type, int64_t 
   }
 }
 
-template <typename T, int W, int NP, int TH, int BLOCK>
+template <typename T, int W, int NP, int TH, int BLOCK, bool KEEP>
 __global__ __launch_bounds__(BLOCK) void norm_forward_kernel(NormArgs a) {
   using G = RowGroup<W, NP, TH, BLOCK>;
   __shared__ float lds[BLOCK / kWave][1];
+  __shared__ double lds64[KEEP ? BLOCK / kWave : 1];
   const int64_t step = (int64_t)gridDim.x * G::kGroups;
   int64_t base = (int64_t)blockIdx.x * G::kGroups;
   const int group = G::group();
@@ -172,6 +350,7 @@ __global__ __launch_bounds__(BLOCK) void norm_forward_kernel(NormArgs a) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) next[i].unpack(v + i * W);
     if (base + step < a.rows) load_row<T, W, NP, G>(a.x, row + step, a, next);
+    if constexpr (KEEP) keep_row<W, NP, TH, BLOCK, G>(a, row, v, lds64);
     float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < G::kItems; ++i) {
@@ -214,7 +393,7 @@ __global__ __launch_bounds__(BLOCK) void norm_forward_kernel(NormArgs a) {
 
 // Each thread also keeps its own columns' sums in registers; the groups of a
 // workgroup join in LDS at the end.
-template <typename T, int W, int NP, int TH, int BLOCK>
+template <typename T, int W, int NP, int TH, int BLOCK, bool KEPT>
 __global__ __launch_bounds__(BLOCK) void norm_backward_kernel(NormArgs a) {
   using G = RowGroup<W, NP, TH, BLOCK>;
   __shared__ float lds[BLOCK / kWave][2];
@@ -227,8 +406,9 @@ __global__ __launch_bounds__(BLOCK) void norm_backward_kernel(NormArgs a) {
   for (int i = 0; i < G::kItems; ++i) dw[i] = db[i] = 0.f;
   if (a.dx || a.dw || a.db) {
     int64_t base = (int64_t)blockIdx.x * G::kGroups;
-    Raw<T, W> next_x[NP], next_g[NP];
-    load_row<T, W, NP, G>(a.x, base + group, a, next_x);
+    std::conditional_t<KEPT, KeptPack<W>, Raw<T, W>> next_x[NP];
+    Raw<T, W> next_g[NP];
+    load_row<T, W, NP, G>(a, base + group, next_x);
     load_row<T, W, NP, G>(a.g, base + group, a, next_g);
     float w[G::kItems];
     load_params<T, W, NP, G>(a.w, a.param_type, a.dim, 1.0f, w);
@@ -243,7 +423,7 @@ __global__ __launch_bounds__(BLOCK) void norm_backward_kernel(NormArgs a) {
         next_g[i].unpack(g + i * W);
       }
       if (base + step < a.rows) {
-        load_row<T, W, NP, G>(a.x, row + step, a, next_x);
+        load_row<T, W, NP, G>(a, row + step, next_x);
         load_row<T, W, NP, G>(a.g, row + step, a, next_g);
       }
       float s[2] = {0.f, 0.f};
@@ -252,7 +432,7 @@ __global__ __launch_bounds__(BLOCK) void norm_backward_kernel(NormArgs a) {
         if (G::element(i) >= a.dim) continue;
 #pragma unroll
         for (int j = i * W; j < i * W + W; ++j) {
-          h[j] = (a.scale * h[j] - m) * r;
+          h[j] = KEPT ? a.scale * h[j] * r : (a.scale * h[j] - m) * r;
           dw[j] += g[j] * h[j];
           db[j] += g[j];
           g[j] *= w[j];
@@ -360,17 +540,16 @@ __global__ __launch_bounds__(kAnyThreads) void norm_forward_any_kernel(NormArgs 
   }
 }
 
-template <typename T>
+template <typename T, bool KEPT>
 __global__ __launch_bounds__(kAnyThreads) void norm_backward_any_kernel(NormArgs a) {
   __shared__ float lds[kAnyWaves];
   const float n = (float)a.dim;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     if (a.dstate && threadIdx.x == 0) state_backward(a, row);
     if (!a.dx) continue;
-    const T* x = static_cast<const T*>(a.x) + row * a.dim;
+    const RowReader<T, KEPT> h(a, row);
     const T* g = static_cast<const T*>(a.g) + row * a.dim;
     T* dx = static_cast<T*>(a.dx) + row * a.dim;
-    const float m = a.stats[2 * row], r = a.stats[2 * row + 1];
     double d1 = 0.0, d2 = 0.0;
     for (int64_t first = 0; first < a.dim; first += kRun) {
       const int64_t end = min(a.dim, first + kRun);
@@ -378,24 +557,23 @@ __global__ __launch_bounds__(kAnyThreads) void norm_backward_any_kernel(NormArgs
       for (int64_t i = first + threadIdx.x; i < end; i += kAnyThreads) {
         const float gw = (float)g[i] * param(a.w, i, a.param_type, 1.0f);
         run1 += gw;
-        run2 += gw * ((a.scale * (float)x[i] - m) * r);
+        run2 += gw * h[i];
       }
       d1 += run1, d2 += run2;
     }
     const float s1 = group_sum<kAnyWaves>((float)d1, lds) / n;
     const float s2 = group_sum<kAnyWaves>((float)d2, lds) / n;
-    const float sr = a.scale * r;
+    const float sr = a.scale * h.r;
     for (int64_t i = threadIdx.x; i < a.dim; i += kAnyThreads) {
       const float gw = (float)g[i] * param(a.w, i, a.param_type, 1.0f);
-      const float h = (a.scale * (float)x[i] - m) * r;
-      dx[i] = (T)(sr * (gw - s1 - h * s2));
+      dx[i] = (T)(sr * (gw - s1 - h[i] * s2));
     }
   }
 }
 
 // Partial column sums of g h and g: a workgroup takes 64 columns of a slab of
 // rows, its four waves every fourth row.
-template <typename T>
+template <typename T, bool KEPT>
 __global__ __launch_bounds__(kAnyThreads) void norm_columns_any_kernel(NormArgs a, int64_t slab_rows) {
   __shared__ float lds[2][kAnyWaves][kWave];
   const int64_t c = (int64_t)blockIdx.x * kWave + lane_id();
@@ -405,8 +583,7 @@ __global__ __launch_bounds__(kAnyThreads) void norm_columns_any_kernel(NormArgs 
   if (c < a.dim) {
     for (int64_t row = r0 + wave_id(); row < r1; row += kAnyWaves) {
       const float g = (float)static_cast<const T*>(a.g)[row * a.dim + c];
-      const float x = (float)static_cast<const T*>(a.x)[row * a.dim + c];
-      sw += g * ((a.scale * x - a.stats[2 * row]) * a.stats[2 * row + 1]);
+      sw += g * RowReader<T, KEPT>(a, row)[c];
       sb += g;
     }
   }
@@ -569,14 +746,21 @@ bool aligned_rows(const NormArgs& a) {
   return true;
 }
 
-template <typename T>
+template <typename T, bool KEEP>
 int launch_norm_forward(const NormArgs& a, hipStream_t s) {
   const bool aligned = aligned_rows<T>(a);
   const RowShape shape = row_shape(a.dim, aligned, sizeof(T));
   if (!shape.threads) {
-    JN_PROFILE("norm_forward_any_kernel", s);
-    hipLaunchKernelGGL(norm_forward_any_kernel<T>, dim3((unsigned)row_groups(a.rows)), dim3(kAnyThreads), 0, s, a);
-    JN_LAUNCH_CHECK();
+    {
+      JN_PROFILE("norm_forward_any_kernel", s);
+      hipLaunchKernelGGL(norm_forward_any_kernel<T>, dim3((unsigned)row_groups(a.rows)), dim3(kAnyThreads), 0, s, a);
+      JN_LAUNCH_CHECK();
+    }
+    if constexpr (KEEP) {
+      JN_PROFILE("norm_keep_any_kernel", s);
+      hipLaunchKernelGGL(norm_keep_any_kernel<T>, dim3((unsigned)row_groups(a.rows)), dim3(256), 0, s, a);
+      JN_LAUNCH_CHECK();
+    }
     return kOk;
   }
   return with_shape<16 / sizeof(T)>(shape, [&](auto width, auto packs, auto threads) -> int {
@@ -584,7 +768,7 @@ int launch_norm_forward(const NormArgs& a, hipStream_t s) {
     constexpr int kBlock = TH > 256 ? TH : 256, per = kBlock / TH;
     const unsigned grid = (unsigned)std::min<int64_t>((a.rows + per - 1) / per, kForwardGroups);
     JN_PROFILE("norm_forward_kernel", s);
-    hipLaunchKernelGGL((norm_forward_kernel<T, W, NP, TH, kBlock>), dim3(grid), dim3(kBlock), 0, s, a);
+    hipLaunchKernelGGL((norm_forward_kernel<T, W, NP, TH, kBlock, KEEP>), dim3(grid), dim3(kBlock), 0, s, a);
     JN_LAUNCH_CHECK();
     return kOk;
   });
@@ -599,7 +783,7 @@ int launch_columns_finish(const NormArgs& a, int64_t parts, hipStream_t s) {
   return kOk;
 }
 
-template <typename T>
+template <typename T, bool KEPT>
 int launch_norm_backward(NormArgs a, hipStream_t s) {
   const bool columns = a.dw || a.db;
   if (!columns && !a.dx && !a.dstate) return kOk;
@@ -608,14 +792,15 @@ int launch_norm_backward(NormArgs a, hipStream_t s) {
   if (!shape.threads) {
     if (a.dx || a.dstate) {
       JN_PROFILE("norm_backward_any_kernel", s);
-      hipLaunchKernelGGL(norm_backward_any_kernel<T>, dim3((unsigned)row_groups(a.rows)), dim3(kAnyThreads), 0, s, a);
+      hipLaunchKernelGGL((norm_backward_any_kernel<T, KEPT>), dim3((unsigned)row_groups(a.rows)), dim3(kAnyThreads), 0, s,
+                         a);
       JN_LAUNCH_CHECK();
     }
     if (!columns) return kOk;
     const int64_t slabs = slab_count(a.rows);
     {
       JN_PROFILE("norm_columns_any_kernel", s);
-      hipLaunchKernelGGL(norm_columns_any_kernel<T>, dim3((unsigned)((a.dim + kWave - 1) / kWave), (unsigned)slabs),
+      hipLaunchKernelGGL((norm_columns_any_kernel<T, KEPT>), dim3((unsigned)((a.dim + kWave - 1) / kWave), (unsigned)slabs),
                          dim3(kAnyThreads), 0, s, a, (a.rows + slabs - 1) / slabs);
       JN_LAUNCH_CHECK();
     }
@@ -629,8 +814,8 @@ int launch_norm_backward(NormArgs a, hipStream_t s) {
       constexpr int kBlock = decltype(block)::value;
       const size_t lds = columns && kBlock > TH ? (size_t)(kBlock / TH) * a.dim * sizeof(float) : 0;
       JN_PROFILE("norm_backward_kernel", s);
-      hipLaunchKernelGGL((norm_backward_kernel<T, W, NP, TH, kBlock>), dim3((unsigned)grid.groups), dim3(kBlock), lds, s,
-                         a);
+      hipLaunchKernelGGL((norm_backward_kernel<T, W, NP, TH, kBlock, KEPT>), dim3((unsigned)grid.groups), dim3(kBlock),
+                         lds, s, a);
       JN_LAUNCH_CHECK();
       return kOk;
     };
@@ -646,20 +831,72 @@ int launch_norm_backward(NormArgs a, hipStream_t s) {
 
 using namespace jakal;
 
+namespace {
+
+int forward(const void* state, const void* x, const void* weight, const void* bias, int64_t rows, int64_t dim,
+            float scale, float eps, int32_t type, int32_t state_type, int32_t param_type, void* state_out, void* y,
+            float* stats, bool keep, void* codes, void* scales, jn_stream_t stream) {
+  NormArgs a{};
+  a.x = x, a.w = weight, a.b = bias, a.state = state, a.rows = rows, a.dim = dim, a.scale = scale, a.eps = eps;
+  a.state_type = state_type, a.param_type = param_type, a.y = y, a.state_out = state_out, a.stats = stats;
+  a.codes = static_cast<uint8_t*>(codes), a.scales = static_cast<uint8_t*>(scales);
+  if (const int rc = check_norm(a, type, state_type, param_type)) return rc;
+  JN_REQUIRE(eps >= 0.0f, kInvalidArgument, "layer norm: eps must not be negative");
+  if (rows == 0) return kOk;
+  JN_REQUIRE(x && y && (!state || state_out), kInvalidArgument, "null tensor pointer");
+  JN_REQUIRE(!keep || (codes && scales && aligned16(codes)), kInvalidArgument,
+             "layer norm: codes and scales to keep x in, the codes on a 16-byte address");
+  const auto s = static_cast<hipStream_t>(stream);
+  return with_type(type, [&](auto* t) -> int {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return keep ? launch_norm_forward<T, true>(a, s) : launch_norm_forward<T, false>(a, s);
+  });
+}
+
+int backward(const void* state, const void* x, const void* weight, const float* stats, const void* grad_state_out,
+             const void* grad_y, int64_t rows, int64_t dim, float scale, int32_t type, int32_t state_type,
+             int32_t param_type, void* grad_state, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+             size_t workspace_bytes, bool kept, const void* codes, const void* scales, jn_stream_t stream) {
+  NormArgs a{};
+  a.x = x, a.w = weight, a.state = state, a.rows = rows, a.dim = dim, a.scale = scale;
+  a.state_type = state_type, a.param_type = param_type, a.stats = const_cast<float*>(stats);
+  a.g = grad_y, a.g_state = grad_state_out, a.dx = grad_x, a.dstate = grad_state;
+  a.partial = static_cast<float*>(workspace), a.dw = grad_weight, a.db = grad_bias;
+  a.codes = static_cast<uint8_t*>(const_cast<void*>(codes)), a.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
+  if (const int rc = check_norm(a, type, state_type, param_type)) return rc;
+  JN_REQUIRE(rows >= 1, kInvalidArgument, "layer norm backward needs at least one row");
+  const bool columns = grad_weight || grad_bias;
+  JN_REQUIRE(!grad_state || (state && grad_state_out), kInvalidArgument, "null tensor pointer");
+  JN_REQUIRE((!grad_x && !columns) || ((kept ? codes && scales : x != nullptr) && stats && grad_y), kInvalidArgument,
+             "null tensor pointer");
+  JN_REQUIRE(!kept || aligned16(codes), kInvalidArgument, "layer norm: codes must start on 16 bytes");
+  const size_t need = columns ? jn_layer_norm_backward_workspace_bytes(rows, dim) : 0;
+  JN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), kWorkspaceTooSmall,
+             "layer norm backward needs %zu workspace bytes, got %zu", need, workspace_bytes);
+  const auto s = static_cast<hipStream_t>(stream);
+  return with_type(type, [&](auto* t) -> int {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return kept ? launch_norm_backward<T, true>(a, s) : launch_norm_backward<T, false>(a, s);
+  });
+}
+
+}  // namespace
+
 extern "C" {
 
 int jn_layer_norm_forward(const void* state, const void* x, const void* weight, const void* bias, int64_t rows,
                           int64_t dim, float scale, float eps, int32_t type, int32_t state_type, int32_t param_type,
                           void* state_out, void* y, float* stats, jn_stream_t stream) {
-  NormArgs a{};
-  a.x = x, a.w = weight, a.b = bias, a.state = state, a.rows = rows, a.dim = dim, a.scale = scale, a.eps = eps;
-  a.state_type = state_type, a.param_type = param_type, a.y = y, a.state_out = state_out, a.stats = stats;
-  if (const int rc = check_norm(a, type, state_type, param_type)) return rc;
-  JN_REQUIRE(eps >= 0.0f, kInvalidArgument, "layer norm: eps must not be negative");
-  if (rows == 0) return kOk;
-  JN_REQUIRE(x && y && (!state || state_out), kInvalidArgument, "null tensor pointer");
-  const auto s = static_cast<hipStream_t>(stream);
-  return with_type(type, [&](auto* t) -> int { return launch_norm_forward<std::remove_pointer_t<decltype(t)>>(a, s); });
+  return forward(state, x, weight, bias, rows, dim, scale, eps, type, state_type, param_type, state_out, y, stats,
+                 false, nullptr, nullptr, stream);
+}
+
+int jn_layer_norm_forward_kept(const void* state, const void* x, const void* weight, const void* bias, int64_t rows,
+                               int64_t dim, float scale, float eps, int32_t type, int32_t state_type,
+                               int32_t param_type, void* state_out, void* y, float* stats, void* codes, void* scales,
+                               jn_stream_t stream) {
+  return forward(state, x, weight, bias, rows, dim, scale, eps, type, state_type, param_type, state_out, y, stats,
+                 true, codes, scales, stream);
 }
 
 size_t jn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t dim) {
@@ -672,22 +909,18 @@ int jn_layer_norm_backward(const void* state, const void* x, const void* weight,
                            int32_t type, int32_t state_type, int32_t param_type, void* grad_state, void* grad_x,
                            void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
                            jn_stream_t stream) {
-  NormArgs a{};
-  a.x = x, a.w = weight, a.state = state, a.rows = rows, a.dim = dim, a.scale = scale;
-  a.state_type = state_type, a.param_type = param_type, a.stats = const_cast<float*>(stats);
-  a.g = grad_y, a.g_state = grad_state_out, a.dx = grad_x, a.dstate = grad_state;
-  a.partial = static_cast<float*>(workspace), a.dw = grad_weight, a.db = grad_bias;
-  if (const int rc = check_norm(a, type, state_type, param_type)) return rc;
-  JN_REQUIRE(rows >= 1, kInvalidArgument, "layer norm backward needs at least one row");
-  const bool columns = grad_weight || grad_bias;
-  JN_REQUIRE(!grad_state || (state && grad_state_out), kInvalidArgument, "null tensor pointer");
-  JN_REQUIRE((!grad_x && !columns) || (x && stats && grad_y), kInvalidArgument, "null tensor pointer");
-  const size_t need = columns ? jn_layer_norm_backward_workspace_bytes(rows, dim) : 0;
-  JN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), kWorkspaceTooSmall,
-             "layer norm backward needs %zu workspace bytes, got %zu", need, workspace_bytes);
-  const auto s = static_cast<hipStream_t>(stream);
-  return with_type(type,
-                   [&](auto* t) -> int { return launch_norm_backward<std::remove_pointer_t<decltype(t)>>(a, s); });
+  return backward(state, x, weight, stats, grad_state_out, grad_y, rows, dim, scale, type, state_type, param_type,
+                  grad_state, grad_x, grad_weight, grad_bias, workspace, workspace_bytes, false, nullptr, nullptr,
+                  stream);
+}
+
+int jn_layer_norm_backward_kept(const void* state, const void* codes, const void* scales, const void* weight,
+                                const float* stats, const void* grad_state_out, const void* grad_y, int64_t rows,
+                                int64_t dim, float scale, int32_t type, int32_t state_type, int32_t param_type,
+                                void* grad_state, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                                size_t workspace_bytes, jn_stream_t stream) {
+  return backward(state, nullptr, weight, stats, grad_state_out, grad_y, rows, dim, scale, type, state_type, param_type,
+                  grad_state, grad_x, grad_weight, grad_bias, workspace, workspace_bytes, true, codes, scales, stream);
 }
 
 }  // extern "C"

@@ -12,6 +12,11 @@ CPU tensors (and a native module without these operators) take the PyTorch form;
 and ``"streaming"`` are the PyTorch form.
 The library computes in fp32 and rounds once; under autocast half-precision
 values come back in fp32, as torch's layer norm returns them.
+
+``saved="e4m3"`` keeps for the backward the centred values in 8 bits
+(``jakal_net.mx``): the outputs are the same, and the gradients are the norm's
+formulas with ``h = scale * r * kept``, the inverse deviation r being that of the
+values themselves.
 """
 
 from __future__ import annotations
@@ -21,6 +26,7 @@ from torch import Tensor, nn
 from torch.nn import functional as F
 
 from jakal_net.core import ImplementationMode, Layer, LayerDelta, check_implementation
+from jakal_net.mx import check_saved, layer_norm_saved
 from jakal_net.native_backend import native_op
 
 
@@ -32,31 +38,38 @@ def _autocast_rows(x: Tensor) -> Tensor:
 
 
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, *, eps: float = 1e-5,
-               implementation: ImplementationMode = "native") -> Tensor:
+               saved: str | None = None, implementation: ImplementationMode = "native") -> Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of ``x``."""
     check_implementation(implementation)
-    op = native_op("layer_norm", x.device.type, implementation)
+    check_saved(saved)
+    op = native_op("layer_norm" if saved is None else "layer_norm_saved", x.device.type, implementation)
     if op is not None:
         try:
             return op(_autocast_rows(x), weight, bias, eps)
         except NotImplementedError:  # outside the library's limits
             if implementation == "native":
                 raise
+    if saved is not None:
+        return layer_norm_saved(_autocast_rows(x), weight, bias, eps, 1.0)
     return F.layer_norm(x, x.shape[-1:], weight, bias, eps)
 
 
 def stabilize(state: Tensor, val: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, *,
-              eps: float = 1e-5, scale: float = 1.0,
+              eps: float = 1e-5, scale: float = 1.0, saved: str | None = None,
               implementation: ImplementationMode = "native") -> tuple[Tensor, Tensor]:
     """``(tanh(scale * state), layer_norm(scale * val))`` for states ``[..., N]`` and values ``[..., N, D]``."""
     check_implementation(implementation)
-    op = native_op("stabilize", val.device.type, implementation)
+    check_saved(saved)
+    op = native_op("stabilize" if saved is None else "stabilize_saved", val.device.type, implementation)
     if op is not None:
         try:
             return op(state, _autocast_rows(val), weight, bias, eps, scale)
         except NotImplementedError:
             if implementation == "native":
                 raise
+    if saved is not None:
+        return (torch.tanh(state if scale == 1.0 else state * scale),
+                layer_norm_saved(_autocast_rows(val), weight, bias, eps, scale))
     if scale != 1.0:
         state, val = state * scale, val * scale
     return torch.tanh(state), F.layer_norm(val, val.shape[-1:], weight, bias, eps)
@@ -65,18 +78,24 @@ def stabilize(state: Tensor, val: Tensor, weight: Tensor | None = None, bias: Te
 class LayerNorm(nn.LayerNorm):
     """``nn.LayerNorm`` over one axis (its parameters, names and initialisation) on ``layer_norm``."""
 
+    saved: str | None = None
+
     def __init__(self, dim: int, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True, *,
-                 implementation: ImplementationMode = "native", device=None, dtype=None) -> None:
+                 saved: str | None = None, implementation: ImplementationMode = "native", device=None,
+                 dtype=None) -> None:
         check_implementation(implementation)
+        check_saved(saved)
         super().__init__(dim, eps, elementwise_affine, bias, device=device, dtype=dtype)
         if len(self.normalized_shape) != 1:
             raise ValueError(f"LayerNorm takes one axis, got {self.normalized_shape}.")
+        self.saved = saved
         self.implementation = implementation
 
     def forward(self, x: Tensor) -> Tensor:
         if x.shape[-1:] != self.normalized_shape:
             raise RuntimeError(f"LayerNorm over {self.normalized_shape[0]} elements got rows of {x.shape[-1]}.")
-        return layer_norm(x, self.weight, self.bias, eps=self.eps, implementation=self.implementation)
+        return layer_norm(x, self.weight, self.bias, eps=self.eps, saved=self.saved,
+                          implementation=self.implementation)
 
 
 def _is_called(norm: nn.Module) -> bool:
@@ -101,5 +120,6 @@ def stabilize_layer(layer: Layer, norm: nn.Module, delta: LayerDelta | None = No
         raise RuntimeError(f"stabilize_layer: a norm over {tuple(norm.normalized_shape)} for values of width "
                            f"{val.shape[-1]}.")
     state, val = stabilize(state, val, norm.weight, norm.bias, eps=norm.eps, scale=scale,
+                           saved=getattr(norm, "saved", None),
                            implementation=getattr(norm, "implementation", "streaming"))
     return layer.with_tensors(state=state, val=val)

@@ -29,6 +29,12 @@ that with implementation="native" each operator runs on the HIP library:
   LayerNorm, Linear(d, 4d), GELU, Linear(4d, vocab); the loss is the mean cross
   entropy (compute_next_token_loss with front weight 1, :2997-3006).
 
+Two options are this build's own.  ``activations="e4m3"`` keeps in 8 bits what the
+norms, the feedback's and the head's linears and the head's GELU save for the
+backward (``jakal_net.mx``); the forward, the parameters and their names are
+unchanged.  ``quantize_head`` gives a trained model's head 4-bit weights to answer
+with.
+
 Options this step does not take (dropouts, route-concentration and diversity
 losses, stats tracking, the pre-norm position, residual merges) are the
 reference's off-by-default ones.  The compressed adapter (a dense bilinear
@@ -47,6 +53,7 @@ from torch import Tensor, nn
 
 from jakal_net.core import ImplementationMode, Layer, LayerDelta
 from jakal_net.modules import LowRankBilinearPairwise, LowRankBilinearRoute
+from jakal_net.mx import GELU, Linear, MXLinear, check_saved
 from jakal_net.norm import LayerNorm, stabilize_layer
 from jakal_net.propagation import SparsePropagation
 from jakal_net.training import clip_grad_norm_, cross_entropy
@@ -130,12 +137,14 @@ class _JointBlock(nn.Module):
     the sequence, expanded and compressed pairwise modules are shared by all blocks."""
 
     def __init__(self, cfg: ProgressiveBConfig, stage: tuple[float, float, float], s_pairwise: nn.Module,
-                 exp_pairwise: nn.Module, cmp_pairwise: nn.Module, implementation: str) -> None:
+                 exp_pairwise: nn.Module, cmp_pairwise: nn.Module, implementation: str,
+                 activations: str | None = None) -> None:
         super().__init__()
         d, r, k = cfg.dim, cfg.rank, cfg.topk
         self.cfg = cfg
         self.alpha_b, self.beta_s_to_b, self.beta_b_to_s = stage
-        self.s_norm, self.exp_norm, self.cmp_norm = (LayerNorm(d, implementation=implementation) for _ in range(3))
+        self.s_norm, self.exp_norm, self.cmp_norm = (
+            LayerNorm(d, saved=activations, implementation=implementation) for _ in range(3))
         self.exp_slot_state = nn.Parameter(0.02 * torch.randn(cfg.expanded))
         self.exp_slot_val = nn.Parameter(0.02 * torch.randn(cfg.expanded, d))
         self.cmp_slot_state = nn.Parameter(0.02 * torch.randn(cfg.compressed))
@@ -181,11 +190,24 @@ class ProgressiveBStep(nn.Module):
 
     prefix_ids [B, prefix], target_ids [B, query] (int64).  The query slots see
     the shifted targets (a start token, then targets[:-1]) as their inputs and
-    predict the targets; the loss is the mean cross entropy over all slots."""
+    predict the targets; the loss is the mean cross entropy over all slots.
+    ``activations``: how norms, linears and the GELU keep their inputs for the
+    backward, None (as they are) or "e4m3"."""
 
     def __init__(self, cfg: ProgressiveBConfig = ProgressiveBConfig(), *,
-                 implementation: ImplementationMode = "native") -> None:
+                 implementation: ImplementationMode = "native", activations: str | None = None) -> None:
         super().__init__()
+        check_saved(activations)
+        self.activations = activations
+
+        def norm() -> LayerNorm:
+            return LayerNorm(cfg.dim, saved=activations, implementation=implementation)
+
+        def linear(inputs: int, outputs: int) -> nn.Linear:
+            if activations is None:
+                return nn.Linear(inputs, outputs)
+            return Linear(inputs, outputs, saved=activations, implementation=implementation)
+
         d, r, k = cfg.dim, cfg.rank, cfg.topk
         self.cfg = cfg
         self.implementation = implementation
@@ -194,11 +216,11 @@ class ProgressiveBStep(nn.Module):
         self.state_init = nn.Linear(d, 1)
         nn.init.zeros_(self.state_init.weight)
         nn.init.zeros_(self.state_init.bias)
-        self.s_norm = LayerNorm(d, implementation=implementation)
+        self.s_norm = norm()
         # one pairwise module per layer family, shared by every operator of the family
         s_pairwise, exp_pairwise = LowRankBilinearPairwise(d, r), LowRankBilinearPairwise(d, r)
         cmp_pairwise, q_pairwise = LowRankBilinearPairwise(d, r), LowRankBilinearPairwise(d, r)
-        self.q_norm = LayerNorm(d, implementation=implementation)
+        self.q_norm = norm()
         self.q_transition = SparseTransition(LowRankBilinearRoute(d, d, rank=r), topk=k, implementation=implementation)
         # the query propagation runs as a causal window of query - 1 over the slots
         self.q_prop = SparsePropagation(q_pairwise, sparse_type="window", window=cfg.query - 1,
@@ -207,16 +229,27 @@ class ProgressiveBStep(nn.Module):
             SparsePropagation(s_pairwise, sparse_type="window", window=cfg.s_window, implementation=implementation)
             for _ in range(cfg.warmup))
         self.blocks = nn.ModuleList(
-            _JointBlock(cfg, cfg.stage(i), s_pairwise, exp_pairwise, cmp_pairwise, implementation)
+            _JointBlock(cfg, cfg.stage(i), s_pairwise, exp_pairwise, cmp_pairwise, implementation,
+                        activations)
             for i in range(cfg.blocks))
         self.refine = nn.ModuleList(
             SparsePropagation(s_pairwise, sparse_type="window", window=cfg.s_window, implementation=implementation)
             for _ in range(cfg.refine))
-        self.head_norm = LayerNorm(d, implementation=implementation)
-        self.feedback_norm = LayerNorm(d, implementation=implementation)
-        self.feedback_proj = nn.Linear(d, d)
-        self.head = nn.Sequential(nn.Linear(d, 4 * d), nn.GELU(), nn.Linear(4 * d, cfg.vocab))
+        self.head_norm = norm()
+        self.feedback_norm = norm()
+        self.feedback_proj = linear(d, d)
+        act = nn.GELU() if activations is None else GELU(saved=activations, implementation=implementation)
+        self.head = nn.Sequential(linear(d, 4 * d), act, linear(4 * d, cfg.vocab))
         self.start_token = cfg.vocab - 1
+
+    def quantize_head(self, activations: str | None = None) -> ProgressiveBStep:
+        """Gives the head frozen 4-bit weights, to answer with; ``activations="e2m1"``:
+        its two products microscale their inputs too.  Gradients still reach what
+        comes before the head."""
+        self.head = nn.Sequential(*(
+            MXLinear.from_linear(m, activations=activations, implementation=self.implementation)
+            if isinstance(m, nn.Linear) else m for m in self.head))
+        return self
 
     def encode_prefix(self, prefix_ids: Tensor) -> Layer:
         c = self.cfg

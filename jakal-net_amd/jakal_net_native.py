@@ -227,6 +227,22 @@ _declare("jn_grads_workspace_bytes", [_I64], _SZ)
 _declare("jn_grads_norm", [_P] * 3 + [_I64, _I32] + [_P, _P, _SZ, _P])
 _declare("jn_grads_clip", [_P] * 5 + [_I64, ctypes.c_double, _I32] + [_P, _P, _SZ, _P])
 
+_declare("jn_mx_quantize", [_P] + [_I64] * 2 + [_I32] * 2 + [_P] * 3)
+_declare("jn_mx_dequantize", [_P] * 2 + [_I64] * 2 + [_I32] * 2 + [_P] * 2)
+_declare("jn_mx_linear_forward_workspace_bytes", [_I64] * 3 + [_I32] * 2, _SZ)
+_declare("jn_mx_linear_forward", [_P] * 4 + [_I64] * 3 + [_I32] * 2 + [_P] * 2 + [_SZ, _P])
+_declare("jn_mx_linear_backward_workspace_bytes", [_I64] * 3 + [_I32], _SZ)
+_declare("jn_mx_linear_backward", [_P] * 3 + [_I64] * 3 + [_I32] + [_P] * 2 + [_SZ, _P])
+_declare("jn_mx_weight_grad_workspace_bytes", [_I64] * 3 + [_I32] * 2, _SZ)
+_declare("jn_mx_weight_grad", [_P] * 3 + [_I64] * 3 + [_I32] + [_P] * 3 + [_SZ, _P])
+_declare("jn_column_sums_workspace_bytes", [_I64] * 2, _SZ)
+_declare("jn_column_sums", [_P] + [_I64] * 2 + [_I32] + [_P] * 2 + [_SZ, _P])
+_declare("jn_layer_norm_forward_kept", [_P] * 4 + [_I64] * 2 + [_F] * 2 + [_I32] * 3 + [_P] * 6)
+_declare("jn_layer_norm_backward_kept",
+         [_P] * 7 + [_I64] * 2 + [_F] + [_I32] * 3 + [_P] * 4 + [_P, _SZ, _P])
+_declare("jn_gelu_forward", [_P] + [_I64] * 2 + [_I32] + [_P] * 4)
+_declare("jn_gelu_backward", [_P] * 3 + [_I64] * 2 + [_I32] + [_P] * 2)
+
 _declare("jn_unit_scale_forward", [_P, _I64, _I64, _F, _P, _P])
 _declare("jn_unit_scale_backward", [_P, _P, _I64, _I64, _F, _P, _P])
 
@@ -272,6 +288,13 @@ _SUPPORTED_OPS = (
     "cross_entropy",
     "grad_norm",
     "clip_grads",
+    "mx_quantize",
+    "mx_dequantize",
+    "mx_linear",
+    "linear_saved",
+    "gelu_saved",
+    "layer_norm_saved",
+    "stabilize_saved",
 )
 _ROUTE_COMPRESS_KINDS = {"softmax": 0, "signed_abs_softmax": 1, "signed_entmax15": 2}
 MAX_ROUTE_TOPK = 64  # routes over every destination (more run dense); the raw pairwise op's k range
@@ -2069,3 +2092,71 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
         if any(o is None for o in out):
             raise ValueError("clip_grads: a gradient without an output.")
     return _clip_grads(grads, out, float(max_norm), _norm_kind(norm_type))
+
+
+# ---------------------------------------------------------------------------
+# microscaled tensors: activations kept in 8 bits, products by 4-bit weights
+# ---------------------------------------------------------------------------
+# Checks, allocations and autograd nodes are C++ (csrc/jn_torch_mx.cpp).
+(_mx_quantize, _mx_dequantize, _mx_linear, _linear_saved, _gelu_saved, _layer_norm_saved, _stabilize_saved) = map(
+    _torch_op, ("mx_quantize", "mx_dequantize", "mx_linear", "linear_saved", "gelu_saved", "layer_norm_saved",
+                "stabilize_saved"))
+
+_FORMATS = {"e4m3": 0, "e2m1": 1}
+
+
+def _format(name: str) -> int:
+    code = _FORMATS.get(name)
+    if code is None:
+        raise ValueError(f"a microscaled format is one of {sorted(_FORMATS)}, got {name!r}.")
+    return code
+
+
+def mx_quantize(x: Tensor, format: str) -> tuple[Tensor, Tensor]:
+    """x (fp32, bf16 or fp16) microscaled along its last axis: (codes, scales), uint8.
+    Runs of 32 elements, the last may be short; a run's scale is 2**(s - 127), the
+    smallest power of two from 2**-126 on that keeps its largest magnitude within
+    the format (448 for "e4m3", 6 for "e2m1"), its elements are rounded to nearest,
+    ties to even.  A run with an infinity or a NaN has the scale 255: it is NaN."""
+    return _mx_quantize(x, _format(format))
+
+
+def mx_dequantize(codes: Tensor, scales: Tensor, format: str, size: int, dtype: torch.dtype = torch.float32) -> Tensor:
+    """The values of microscaled rows of `size` elements, rounded to dtype."""
+    return _mx_dequantize(codes, scales, _format(format), size, dtype)
+
+
+def mx_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Tensor | None = None,
+              activations: str | None = None) -> Tensor:
+    """x @ W.T + bias: W [outputs, inputs] the e2m1 tensor of codes and scales, x [...,
+    inputs] as it is (None) or microscaled on the way in ("e2m1"), bias [outputs] of
+    x's type; exact products, fp32 sums, the result in x's type.  Differentiable once
+    in x (grad @ W: the rounding passes it through) and bias."""
+    if activations not in (None, "e2m1"):
+        raise ValueError(f"mx_linear takes activations as they are (None) or 'e2m1', got {activations!r}.")
+    return _mx_linear(x, codes, scales, bias, -1 if activations is None else 1)
+
+
+def linear_saved(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor:
+    """x @ weight.T + bias with x kept in e4m3: the weight's gradient is grad.T @ (kept
+    x), the others are the plain layer's.  Differentiable once; one type for all."""
+    return _linear_saved(x, weight, bias)
+
+
+def gelu_saved(x: Tensor) -> Tensor:
+    """x * Phi(x) with x kept in e4m3: the gradient is grad * (Phi + x phi) at the kept
+    x.  Differentiable once."""
+    return _gelu_saved(x)
+
+
+def layer_norm_saved(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5) -> Tensor:
+    """layer_norm with x - mean(x) kept in e4m3: the gradients are the layer norm's
+    formulas with h = r times what was kept, r being x's own."""
+    return _layer_norm_saved(x, weight, bias, eps)
+
+
+def stabilize_saved(state: Tensor, val: Tensor, weight: Tensor | None = None, bias: Tensor | None = None,
+                    eps: float = 1e-5, scale: float = 1.0) -> tuple[Tensor, Tensor]:
+    """stabilize with the values kept as layer_norm_saved keeps them (the states are kept
+    as they are)."""
+    return _stabilize_saved(state, val, weight, bias, eps, scale)

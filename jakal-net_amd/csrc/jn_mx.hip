@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void gelu_backward_kernel(UnitArgs a) {
 }
 
 int unit_args(const char* what, const void* x, void* y, const void* codes, const void* scales, int64_t rows,
-              int64_t dim, int32_t type, UnitArgs& a) {
+              int64_t dim, int32_t type, UnitArgs& a, int64_t runs = 0) {
   JN_REQUIRE(known_type(type), kInvalidArgument, "%s: unknown element type %d", what, type);
   JN_REQUIRE(rows >= 1 && dim >= 1 && dim < (int64_t(1) << 31) && rows <= (int64_t(1) << 36) / mx_runs(dim),
              kInvalidArgument, "%s: needs rows and dim >= 1, dim < 2^31 and at most 2^36 runs, got %lld x %lld", what,
@@ -103,8 +103,9 @@ int unit_args(const char* what, const void* x, void* y, const void* codes, const
   a.x = x, a.y = y;
   a.codes = static_cast<uint8_t*>(const_cast<void*>(codes));
   a.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
-  a.row_units = mx_runs(dim) * 4, a.units = rows * a.row_units;
-  const bool flat = dim % kMxRun == 0;
+  if (runs == 0) runs = mx_runs(dim);
+  a.row_units = runs * 4, a.units = rows * a.row_units;
+  const bool flat = dim == runs * kMxRun;
   a.rows = flat ? 1 : rows, a.dim = flat ? rows * dim : dim;
   return kOk;
 }
@@ -128,9 +129,9 @@ dim3 unit_grid(const UnitArgs& a) { return dim3((unsigned)((a.units + 255) / 256
 }  // namespace
 
 int launch_mx_quantize(const void* x, int64_t rows, int64_t dim, int32_t type, int32_t form, void* codes, void* scales,
-                       hipStream_t s) {
+                       hipStream_t s, int64_t runs) {
   UnitArgs a{};
-  if (const int rc = unit_args("mx_quantize", x, nullptr, codes, scales, rows, dim, type, a)) return rc;
+  if (const int rc = unit_args("mx_quantize", x, nullptr, codes, scales, rows, dim, type, a, runs)) return rc;
   return with_type(type, [&](auto* t) -> int {
     return with_form(form, [&](auto f) -> int {
       return with_packs(packed_rows(a, type), [&](auto p) -> int {

@@ -158,8 +158,9 @@ __device__ __forceinline__ void store_unit(T* row, int64_t e, int64_t dim, const
   }
 }
 
-// jn_mx_quantize's launch, for the kernels that microscale an operand of their own.
+// jn_mx_quantize's launch, for the kernels that microscale an operand of their own:
+// rows of `runs` runs where given, the surplus zeros.
 int launch_mx_quantize(const void* x, int64_t rows, int64_t dim, int32_t type, int32_t form, void* codes, void* scales,
-                       hipStream_t s);
+                       hipStream_t s, int64_t runs = 0);
 
 }  // namespace jakal

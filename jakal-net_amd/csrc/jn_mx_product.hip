@@ -103,7 +103,7 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[kTerm
 template <int SLICE>
 __device__ __forceinline__ int lds_kc(int row, int chunk) {
   if constexpr (SLICE == 64) return row * 64 + ((chunk ^ (row >> 1)) & 7) * 8;
-  else return row * 32 + ((chunk ^ (row >> 2)) & 3) * 8;
+  else return row * 32 + ((chunk ^ -(row >> 2)) & 3) * 8;
 }
 // [r][128]: 32-byte chunks permuted by the row.
 __device__ __forceinline__ int lds_tr(int r, int chunk32) {
@@ -423,116 +423,187 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const T* x, int64_t ro
 // their scales a byte a lane.  A run's products span eight bits, so its sum is exact,
 // and the runs' sums are added in fp32.  (With e4m3 the instruction drops what lies
 // 14 bits below the run's largest product; x is e2m1 here or not microscaled at all.)
-// Tiles of 128 x 128, slices of 256 k, LDS double buffered.
 struct LinearArgs {
-  const uint8_t* x;   // [m][pitch]
-  const uint8_t* xs;  // [m][runs]
+  const uint8_t* x;   // [m][x_pitch], rows padded with zeros to whole steps
+  const uint8_t* xs;  // [m][x_runs]
   const uint8_t* w;   // [n][pitch]
-  const uint8_t* ws;  // [n][runs]
+  const uint8_t* ws;  // [n][x_runs]
   const void* bias;   // [n] or null
   void* y;            // [m][n]
-  int64_t m, n, runs, pitch;
+  int64_t m, n, x_runs, pitch, x_pitch;
   int tiles_m, tiles_n;
 };
 
-constexpr int kMxSlice = 256;                   // elements of k
-constexpr int kSliceRuns = kMxSlice / kMxRun;   // 8
+constexpr int kStepRuns = 8, kStepBytes = 128;  // of a row in a step of 256 k: a cache line of codes
 
-// Rows of 8 chunks of 16 bytes, permuted by the row.
+// Rows of 8 chunks of 16 bytes, permuted so that the 16 lanes of a read that are served
+// together (0-3, 12-15 and 20-27 of the first 32, and so on) fall on all 64 banks.
 __device__ __forceinline__ int lds_row(int row, int chunk) { return row * 128 + ((chunk ^ (row >> 1)) & 7) * 16; }
 
-template <typename T>
-__global__ __launch_bounds__(256) void mx_linear_kernel(LinearArgs g) {
-  constexpr int C = 8;  // 16-byte chunks of a row's slice
-  constexpr int kX = kTile * C * 16, kS = kTile * kSliceRuns;
-  constexpr int kStage = 2 * (kX + kS);
+// An e2m1 operand: four of the instruction's eight words.
+__device__ __forceinline__ intx8 wide(u32x4_nt v) { return intx8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; }
+
+// Loads straight into LDS, 16 or 4 bytes a lane, at `base` + lane * BYTES.  In assembly,
+// since the compiler would wait for all of them before any later read of LDS: whoever
+// reads waits itself (wait_loads, then the barrier).  They have no result registers.
+typedef __attribute__((address_space(3))) const uint8_t lds_byte;
+typedef int intx4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t lds_offset(const uint8_t* p) { return (uint32_t)(uintptr_t)(lds_byte*)p; }
+
+// The resource over [base, base + bytes), or its first 2^32 - 1 bytes: a tile's rows reach no further.
+__device__ __forceinline__ intx4 rows_rsrc(const uint8_t* base, int64_t bytes) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  return intx4{__builtin_amdgcn_readfirstlane((int)(uint32_t)p),
+               __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xFFFFu)),
+               __builtin_amdgcn_readfirstlane((int)(uint32_t)min(bytes, (int64_t)0xFFFFFFFF)), 0x00020000};
+}
+
+// `base`, `at` and the resource are uniform over the wave.
+template <int BYTES>
+__device__ __forceinline__ void load_lds(intx4 rs, uint32_t base, uint32_t offset, uint32_t at) {
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(base), "v"(offset),
+                 "s"(rs), "s"(at)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(base), "v"(offset),
+                 "s"(rs), "s"(at)
+                 : "memory", "m0");
+}
+
+// Until the wave's loads have landed and its reads of LDS are done.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+// Tiles of TM x TN over WM x WN waves in steps of 256 k, LDS double buffered: a step's
+// loads go there directly while the step before is multiplied.  Rows past the operands'
+// ends are their last rows (their outputs are not written); past a row's end x is zeros,
+// so that W may be anything finite there.
+template <typename T, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(WM* WN* kWave, 2) void mx_linear_kernel(LinearArgs g) {
+  constexpr int WAVES = WM * WN;
+  constexpr int MT = TM / WM / 16, NT = TN / WN / 16;          // 16-wide tiles of a wave
+  constexpr int XU = TM / (8 * WAVES), WU = TN / (8 * WAVES);  // 16-byte loads a lane and step, eight rows each
+  constexpr int kX = TM * kStepBytes, kW = TN * kStepBytes;
+  constexpr int kXS = TM * kStepRuns, kWS = TN * kStepRuns;
+  constexpr int kStage = kX + kW + kXS + kWS;
+  constexpr int kXSL = kXS / 256, kWSL = kWS / 256;            // 4-byte loads of the scales
+  static_assert(WAVES % kXSL == 0 && WAVES % kWSL == 0, "a wave loads scales once");
   __shared__ __align__(16) uint8_t smem[2 * kStage];
 
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
   const int grp = lane >> 4, col = lane & 15;
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / WN, wn = wave % WN;
   const TilePlace at(g.tiles_m, g.tiles_n);
-  const int64_t m0 = (int64_t)at.mi * kTile, n0 = (int64_t)at.ni * kTile;
+  const int64_t m0 = (int64_t)at.mi * TM, n0 = (int64_t)at.ni * TN;
+  const int mrows = (int)min((int64_t)TM, g.m - m0), nrows = (int)min((int64_t)TN, g.n - n0);
 
-  uint4 rx[C / 2], rw[C / 2];
-  uint64_t rs;
-  auto load = [&](int64_t k0) {  // in runs
+  const auto rx = rows_rsrc(g.x + m0 * g.x_pitch, (g.m - m0) * g.x_pitch);
+  const auto rw = rows_rsrc(g.w + n0 * g.pitch, (g.n - n0) * g.pitch);
+  const auto rxs = rows_rsrc(g.xs + m0 * g.x_runs, (g.m - m0) * g.x_runs);
+  const auto rws = rows_rsrc(g.ws + n0 * g.x_runs, (g.n - n0) * g.x_runs);
+  // the lane's chunk of its row is the one that belongs in its place
+  uint32_t ox[XU], ow[WU];
 #pragma unroll
-    for (int u = 0; u < C / 2; ++u) {
-      const int id = tid + 256 * u, row = id / C;
-      const int64_t byte = k0 * 16 + id % C * 16;
-      rx[u] = m0 + row < g.m && byte < g.pitch ? *reinterpret_cast<const uint4*>(g.x + (m0 + row) * g.pitch + byte)
-                                               : make_uint4(0, 0, 0, 0);
-      rw[u] = n0 + row < g.n && byte < g.pitch ? *reinterpret_cast<const uint4*>(g.w + (n0 + row) * g.pitch + byte)
-                                               : make_uint4(0, 0, 0, 0);
-    }
-    // a row's eight scales a thread: of X, then of W; 2^0 past the end
-    const bool is_x = tid < kTile;
-    const int64_t row = is_x ? m0 + tid : n0 + tid - kTile;
-    const uint8_t* p = (is_x ? g.xs : g.ws) + row * g.runs + k0;
-    rs = 0;
+  for (int u = 0; u < XU; ++u) {
+    const int row = (u * WAVES + wave) * 8 + lane / 8;
+    ox[u] = __umul24(min(row, mrows - 1), (uint32_t)g.x_pitch) + ((lane ^ (row >> 1)) & 7) * 16;
+  }
 #pragma unroll
-    for (int i = 0; i < kSliceRuns; ++i) {
-      const uint64_t s = row < (is_x ? g.m : g.n) && k0 + i < g.runs ? p[i] : 127;
-      rs |= s << (8 * i);
-    }
+  for (int u = 0; u < WU; ++u) {
+    const int row = (u * WAVES + wave) * 8 + lane / 8;
+    ow[u] = __umul24(min(row, nrows - 1), (uint32_t)g.pitch) + ((lane ^ (row >> 1)) & 7) * 16;
+  }
+  const int xsrow = tid / 2 % TM, wsrow = tid / 2 % TN;
+  const uint32_t oxs = __umul24(min(xsrow, mrows - 1), (uint32_t)g.x_runs) + tid % 2 * 4;
+  const uint32_t ows = __umul24(min(wsrow, nrows - 1), (uint32_t)g.x_runs) + tid % 2 * 4;
+
+  const uint32_t lds = lds_offset(smem);
+  // (past the last step out of range, which reads nothing: without a branch the loop below is one block)
+  const int steps = (int)(g.x_runs / kStepRuns);
+  auto load = [&](int step, uint32_t stage) {
+    const uint32_t k = step < steps ? (uint32_t)step * kStepBytes : kOobOffset;
+    const uint32_t run = step < steps ? (uint32_t)step * kStepRuns : kOobOffset;
+#pragma unroll
+    for (int u = 0; u < XU; ++u) load_lds<16>(rx, lds + stage + (u * WAVES + wave) * 1024, ox[u], k);
+#pragma unroll
+    for (int u = 0; u < WU; ++u) load_lds<16>(rw, lds + stage + kX + (u * WAVES + wave) * 1024, ow[u], k);
+    load_lds<4>(rxs, lds + stage + kX + kW + wave % kXSL * 256, oxs, run);
+    load_lds<4>(rws, lds + stage + kX + kW + kXS + wave % kWSL * 256, ows, run);
   };
-  auto store = [&](uint8_t* stage) {
+
+  floatx4 acc[NT][MT];
 #pragma unroll
-    for (int u = 0; u < C / 2; ++u) {
-      const int id = tid + 256 * u;
-      *reinterpret_cast<uint4*>(stage + lds_row(id / C, id % C)) = rx[u];
-      *reinterpret_cast<uint4*>(stage + kX + lds_row(id / C, id % C)) = rw[u];
-    }
-    *reinterpret_cast<uint64_t*>(stage + 2 * kX + tid * 8) = rs;
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  // one half step's operands; a lane has the run 4 k + grp of its rows
+  u32x4_nt x[MT], w[NT];
+  int xs[MT], ws[NT];
+  // (a tile's rows are sixteen further on, where the chunks are permuted alike, and the
+  // other half step's chunks four: one address an operand, and constants)
+  const int xat = lds_row(wm * (TM / WM) + col, grp), wat = kX + lds_row(wn * (TN / WN) + col, grp);
+  const int xsat = kX + kW + (wm * (TM / WM) + col) * kStepRuns + grp;
+  const int wsat = kX + kW + kXS + (wn * (TN / WN) + col) * kStepRuns + grp;
+  auto read_x = [&](uint32_t stage, int k, int j) {
+    x[j] = *reinterpret_cast<const u32x4_nt*>(smem + stage + (xat ^ (64 * k)) + j * 16 * kStepBytes);
+    xs[j] = smem[stage + xsat + 4 * k + j * 16 * kStepRuns];
   };
-
-  floatx4 acc[4][4];  // [n][m] tiles of 16
+  auto read_w = [&](uint32_t stage, int k, int i) {
+    w[i] = *reinterpret_cast<const u32x4_nt*>(smem + stage + (wat ^ (64 * k)) + i * 16 * kStepBytes);
+    ws[i] = smem[stage + wsat + 4 * k + i * 16 * kStepRuns];
+  };
+  // A half step's products.  An operand is read anew, for the half step after (from `next`),
+  // as soon as its last product is under way; `then` follows the first row of products.
+  auto half = [&](uint32_t next, int k, auto then) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NT; ++i) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-
-  const int slices = (int)((g.runs + kSliceRuns - 1) / kSliceRuns);
-  load(0);
-  store(smem);
-  __syncthreads();
-  for (int s = 0; s < slices; ++s) {
-    const uint8_t* stage = smem + (s & 1) * kStage;
-    if (s + 1 < slices) load((int64_t)(s + 1) * kSliceRuns);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      intx8 x[4], w[4];
-      int xs[4], ws[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // a lane has the run 4 k + grp of its row
-        const int xr = wm * 64 + i * 16 + col, wr = wn * 64 + i * 16 + col;
-        const uint4 a = *reinterpret_cast<const uint4*>(stage + lds_row(xr, 4 * k + grp));
-        const uint4 b = *reinterpret_cast<const uint4*>(stage + kX + lds_row(wr, 4 * k + grp));
-        x[i] = intx8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
-        w[i] = intx8{(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-        xs[i] = (int)(*reinterpret_cast<const uint32_t*>(stage + 2 * kX + xr * 8 + k * 4) >> (8 * grp));
-        ws[i] = (int)(*reinterpret_cast<const uint32_t*>(stage + 2 * kX + kS + wr * 8 + k * 4) >> (8 * grp));
+      for (int j = 0; j < MT; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[i]), wide(x[j]), acc[i][j], 4, 4, 0, ws[i], 0,
+                                                                     xs[j]);
+        if (i == NT - 1) {
+          read_x(next, k, j);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], x[j], acc[i][j], 4, 4, 0, ws[i], 0, xs[j]);
+      if (i == 0) then();
+      read_w(next, k, i);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (s + 1 < slices) store(smem + ((s + 1) & 1) * kStage);
-    __syncthreads();
+  };
+
+  load(0, 0);
+  wait_loads();
+  __builtin_amdgcn_s_barrier();
+  load(1, kStage);
+#pragma unroll
+  for (int j = 0; j < MT; ++j) read_x(0, 0, j);
+#pragma unroll
+  for (int i = 0; i < NT; ++i) read_w(0, 0, i);
+  for (int s = 0; s < steps; ++s) {
+    const uint32_t cur = (s & 1) * kStage;
+    half(cur, 1, [] {});
+    // (the last step reads on into the other stage, for nothing)
+    half(kStage - cur, 0, [&] {
+      // the next step has landed, and every wave has all of this one's operands in
+      // registers: its stage is free for the step after the next
+      wait_loads();
+      __builtin_amdgcn_s_barrier();
+      load(s + 2, cur);
+    });
   }
 
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = n0 + wn * 64 + i * 16 + grp * 4;
+  for (int i = 0; i < NT; ++i) {
+    const int64_t n = n0 + wn * (TN / WN) + i * 16 + grp * 4;
     if (n >= g.n) continue;
     float b[4];
     load_bias(static_cast<const T*>(g.bias), n, g.n, b);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + wm * 64 + j * 16 + col;
+    for (int j = 0; j < MT; ++j) {
+      const int64_t m = m0 + wm * (TM / WM) + j * 16 + col;
       if (m >= g.m) continue;
       const float v[4] = {acc[i][j][0] + b[0], acc[i][j][1] + b[1], acc[i][j][2] + b[2], acc[i][j][3] + b[3]};
       store_quad(static_cast<T*>(g.y) + m * g.n + n, n, g.n, v);
@@ -540,7 +611,32 @@ __global__ __launch_bounds__(256) void mx_linear_kernel(LinearArgs g) {
   }
 }
 
-size_t linear_codes_bytes(int64_t rows, int64_t dim) { return (size_t)(rows * mx_pitch(dim, kE2m1) + 255) / 256 * 256; }
+// W's scales with rows of whole steps, 2^0 past their ends: for weights whose rows are not.
+__global__ __launch_bounds__(256) void mx_pad_scales_kernel(const uint8_t* scales, int64_t rows, int64_t runs,
+                                                            int64_t padded, uint8_t* out) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t words = padded / 4, row = id / words, run = (id - row * words) * 4;
+  if (row >= rows) return;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w |= (run + i < runs ? (uint32_t)scales[row * runs + run + i] : 127u) << (8 * i);
+  reinterpret_cast<uint32_t*>(out)[id] = w;
+}
+
+// x microscaled for this product: rows of whole steps.
+int64_t step_runs(int64_t dim) { return (mx_runs(dim) + kStepRuns - 1) / kStepRuns * kStepRuns; }
+size_t linear_codes_bytes(int64_t rows, int64_t dim) { return (size_t)(rows * step_runs(dim) * 16); }
+
+template <typename T, int TM, int TN, int WM, int WN>
+int launch_linear(LinearArgs g, hipStream_t s) {
+  g.tiles_m = (int)((g.m + TM - 1) / TM), g.tiles_n = (int)((g.n + TN - 1) / TN);
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
+  JN_REQUIRE(tiles < (int64_t(1) << 31), kUnsupported, "mx_linear: too many output tiles");
+  JN_PROFILE("mx_linear_kernel", s);
+  hipLaunchKernelGGL((mx_linear_kernel<T, TM, TN, WM, WN>), dim3((unsigned)tiles), dim3(WM * WN * kWave), 0, s, g);
+  JN_LAUNCH_CHECK();
+  return kOk;
+}
 
 int check_product(const char* what, int64_t rows, int64_t dim, int64_t out, int32_t type) {
   JN_REQUIRE(known_type(type), kInvalidArgument, "%s: unknown element type %d", what, type);
@@ -561,7 +657,7 @@ extern "C" {
 size_t jn_mx_linear_forward_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t activations) {
   if (check_product("mx_linear", rows, dim, out, type)) return 0;
   if (activations == kPlain) return MixedPlan(rows, out, dim, type, false).bytes();
-  return linear_codes_bytes(rows, dim) + (size_t)(rows * mx_runs(dim));
+  return linear_codes_bytes(rows, dim) + (size_t)((rows + (mx_runs(dim) % kStepRuns ? out : 0)) * step_runs(dim));
 }
 
 int jn_mx_linear_forward(const void* x, const void* weight_codes, const void* weight_scales, const void* bias,
@@ -583,22 +679,31 @@ int jn_mx_linear_forward(const void* x, const void* weight_codes, const void* we
   const size_t need = jn_mx_linear_forward_workspace_bytes(rows, dim, out, type, activations);
   JN_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, kWorkspaceTooSmall,
              "mx_linear: needs %zu workspace bytes on a 16-byte address, got %zu", need, workspace_bytes);
+  JN_REQUIRE((reinterpret_cast<uintptr_t>(weight_scales) & 3) == 0 || mx_runs(dim) % kStepRuns, kInvalidArgument,
+             "mx_linear: weight scales must start on 4 bytes");
   LinearArgs g{};
   uint8_t* const codes = static_cast<uint8_t*>(workspace);
   uint8_t* const scales = codes + linear_codes_bytes(rows, dim);
   g.x = codes, g.xs = scales;
   g.w = static_cast<const uint8_t*>(weight_codes), g.ws = static_cast<const uint8_t*>(weight_scales);
-  g.bias = bias, g.y = y, g.m = rows, g.n = out, g.runs = mx_runs(dim), g.pitch = mx_pitch(dim, kE2m1);
-  g.tiles_m = (int)((rows + kTile - 1) / kTile), g.tiles_n = (int)((out + kTile - 1) / kTile);
-  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
-  JN_REQUIRE(tiles < (int64_t(1) << 31), kUnsupported, "mx_linear: too many output tiles");
-  if (const int rc = launch_mx_quantize(x, rows, dim, type, kE2m1, codes, scales, s)) return rc;
+  g.bias = bias, g.y = y, g.m = rows, g.n = out, g.pitch = mx_pitch(dim, kE2m1);
+  g.x_runs = step_runs(dim), g.x_pitch = g.x_runs * 16;
+  if (mx_runs(dim) % kStepRuns) {
+    uint8_t* const padded = scales + rows * g.x_runs;
+    const int64_t words = out * g.x_runs / 4;
+    JN_PROFILE("mx_pad_scales_kernel", s);
+    hipLaunchKernelGGL(mx_pad_scales_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, g.ws, out,
+                       mx_runs(dim), g.x_runs, padded);
+    JN_LAUNCH_CHECK();
+    g.ws = padded;
+  }
+  if (const int rc = launch_mx_quantize(x, rows, dim, type, kE2m1, codes, scales, s, g.x_runs)) return rc;
   return with_type(type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
-    JN_PROFILE("mx_linear_kernel", s);
-    hipLaunchKernelGGL(mx_linear_kernel<T>, dim3((unsigned)tiles), dim3(256), 0, s, g);
-    JN_LAUNCH_CHECK();
-    return kOk;
+    const auto tiles = [&](int64_t tm, int64_t tn) { return (rows + tm - 1) / tm * ((out + tn - 1) / tn); };
+    if (tiles(256, 256) >= 256) return launch_linear<T, 256, 256, 2, 4>(g, s);
+    if (tiles(128, 128) >= 256) return launch_linear<T, 128, 128, 2, 2>(g, s);
+    return launch_linear<T, 64, 64, 2, 2>(g, s);
   });
 }
 

@@ -172,7 +172,7 @@ Tensor mx_product_meta(const Tensor& x, const Tensor& codes, const Tensor&, cons
 Tensor mx_product(const Tensor& x_in, const Tensor& codes_in, const Tensor& scales_in,
                   const std::optional<Tensor>& bias_in, int64_t acts) {
   check_mx_linear(x_in, codes_in, scales_in, given(bias_in), acts);
-  const Tensor x = plain(x_in), codes = aligned(codes_in), scales = plain(scales_in), bias = plain(given(bias_in));
+  const Tensor x = plain(x_in), codes = aligned(codes_in), scales = aligned(scales_in), bias = plain(given(bias_in));
   const c10::DeviceGuard guard(x.device());
   const Tensor y = mx_product_meta(x, codes, scales, bias_in, acts);
   const int64_t dim = x.size(-1), rows = x.numel() / dim;

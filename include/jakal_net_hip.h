@@ -1028,6 +1028,16 @@ int jn_mx_weight_grad(const void* grad_y, const void* codes, const void* scales,
                       int64_t out, int32_t type, void* grad_weight, void* grad_bias, void* workspace,
                       size_t workspace_bytes, jn_stream_t stream);
 
+/*
+ * grad_x [rows, dim] = grad_y [rows, out] . weight [out, dim] of a plain linear layer,
+ * JN_BF16, for the sizes that jn_linear_input_grad_fits answers 1 to (few output tiles
+ * over a long sum); exact products, fp32 sums in a fixed order.  All start on 16 bytes.
+ */
+int32_t jn_linear_input_grad_fits(int64_t rows, int64_t dim, int64_t out, int32_t type);
+size_t jn_linear_input_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type);
+int jn_linear_input_grad(const void* grad_y, const void* weight, int64_t rows, int64_t dim, int64_t out, int32_t type,
+                         void* grad_x, void* workspace, size_t workspace_bytes, jn_stream_t stream);
+
 /* sums [dim] of `type`: the sums over rows of x [rows, dim], fp32 in a fixed order. */
 size_t jn_column_sums_workspace_bytes(int64_t rows, int64_t dim);
 int jn_column_sums(const void* x, int64_t rows, int64_t dim, int32_t type, void* sums, void* workspace,

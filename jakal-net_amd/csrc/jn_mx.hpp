@@ -50,6 +50,15 @@ __device__ __forceinline__ float mx_scale(int s) {
   return __uint_as_float(s == 255 ? 0x7FC00000u : s == 0 ? 0x00400000u : (uint32_t)s << 23);
 }
 
+// Eight e2m1 codes of numbers within the format.
+__device__ __forceinline__ uint32_t e2m1_word(const float (&v)[8]) {
+  uint32_t a = 0;
+  a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[0], v[1], 1.0f, 0);
+  a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[2], v[3], 1.0f, 1);
+  a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[4], v[5], 1.0f, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[6], v[7], 1.0f, 3);
+}
+
 // The codes of a lane's eight elements (e4m3: two words; e2m1: one) and its run's
 // scale code.  |v| * 2^(127 - s) is within the format, so nothing saturates; the
 // product is exact but where it falls below 2^-126, far under half the least code.
@@ -69,12 +78,10 @@ __device__ __forceinline__ int mx_encode(const float (&v)[8], uint32_t (&code)[2
     code[0] = s == 255 ? 0x7F7F7F7Fu : (uint32_t)a;
     code[1] = s == 255 ? 0x7F7F7F7Fu : (uint32_t)b;
   } else {
-    uint32_t a = 0;
-    a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[0] * inv, v[1] * inv, 1.0f, 0);
-    a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[2] * inv, v[3] * inv, 1.0f, 1);
-    a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[4] * inv, v[5] * inv, 1.0f, 2);
-    a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[6] * inv, v[7] * inv, 1.0f, 3);
-    code[0] = s == 255 ? 0u : a;
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = v[i] * inv;
+    code[0] = s == 255 ? 0u : e2m1_word(f);
     code[1] = 0;
   }
   return s;

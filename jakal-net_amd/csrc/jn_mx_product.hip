@@ -47,7 +47,7 @@ struct TilePlace {
 // operand whose rows run along r lies there as it does in memory ([row][r]); one
 // whose rows run along m or n lies as [r][128] and is read transposed
 // (ds_read_b64_tr_b16).
-enum Product { kForward, kInputGrad, kWeightGrad };
+enum Product { kForward, kInputGrad, kWeightGrad, kPlainGrad };
 
 struct MixedArgs {
   const void* a;          // [m][lda], or [r][lda] (weight gradient)
@@ -64,7 +64,6 @@ struct MixedArgs {
   int tiles_m, tiles_n;
 };
 
-constexpr int kTile = 128;
 constexpr int kPlain = -1;  // activations that are not microscaled
 
 template <typename T>
@@ -105,9 +104,10 @@ __device__ __forceinline__ int lds_kc(int row, int chunk) {
   if constexpr (SLICE == 64) return row * 64 + ((chunk ^ (row >> 1)) & 7) * 8;
   else return row * 32 + ((chunk ^ -(row >> 2)) & 3) * 8;
 }
-// [r][128]: 32-byte chunks permuted by the row.
+// [r][WIDTH]: the 32-byte chunks of each 256 bytes permuted by the row.
+template <int WIDTH>
 __device__ __forceinline__ int lds_tr(int r, int chunk32) {
-  return r * kTile + ((chunk32 ^ ((r & 3) | ((r >> 1) & 4))) & 7) * 16;
+  return r * WIDTH + (chunk32 & ~7) * 16 + ((chunk32 ^ ((r & 3) | ((r >> 1) & 4))) & 7) * 16;
 }
 
 __device__ __forceinline__ shortx4 read_tr(const bf16_t* p) {
@@ -115,11 +115,18 @@ __device__ __forceinline__ shortx4 read_tr(const bf16_t* p) {
       (__attribute__((address_space(3))) shortx4*)(const_cast<bf16_t*>(p)));
 }
 
+// The wide kernel's [r][256]: rows of 32 bytes more, and 128 more every eight rows, so
+// that four rows and those eight further on fall on different banks.  Sums of what a row
+// and a column add, where a permutation would take an address for every tile.
+constexpr int kPadRow = 256 + 16, kPadEight = 64, kPadPlane = 64 * kPadRow + 8 * kPadEight;
+__device__ __forceinline__ int lds_pad(int r, int c) { return r * kPadRow + (r >> 3) * kPadEight + c; }
+
 // Eight consecutive r from r0 on of column c16 * 16 + (lane & 15), for lane group g: r0 = 8 g.
+template <int WIDTH>
 __device__ __forceinline__ bf16x8v fragment_tr(const bf16_t* plane, int r0, int c16, int lane) {
   const int i = lane & 15;
-  const shortx4 a = read_tr(plane + lds_tr(r0 + (i >> 2), c16) + (i & 3) * 4);
-  const shortx4 b = read_tr(plane + lds_tr(r0 + 4 + (i >> 2), c16) + (i & 3) * 4);
+  const shortx4 a = read_tr(plane + lds_tr<WIDTH>(r0 + (i >> 2), c16) + (i & 3) * 4);
+  const shortx4 b = read_tr(plane + lds_tr<WIDTH>(r0 + 4 + (i >> 2), c16) + (i & 3) * 4);
   typedef short shortx8 __attribute__((ext_vector_type(8)));
   return __builtin_bit_cast(bf16x8v, (shortx8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
@@ -151,83 +158,98 @@ __device__ __forceinline__ uint32_t decode_pair(uint32_t code, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, scale, WORD_HALF));
 }
 
-template <typename T, Product P, bool PACKED>
-__global__ __launch_bounds__(256, 2) void mx_mixed_kernel(MixedArgs g) {
+// Eight elements of a row, `left` of them inside it (at most eight count): one access
+// where they all are, whatever the row's alignment; zeros past the end.
+template <typename T>
+struct Eight {
+  typedef T vec __attribute__((ext_vector_type(8)));
+  typedef vec loose __attribute__((aligned(sizeof(T))));
+  vec v;
+
+  __device__ __forceinline__ void load(const T* p, int64_t left) {
+    if (left >= 8) {
+      v = *reinterpret_cast<const loose*>(p);
+    } else {
+      v = vec{};
+#pragma unroll
+      for (int i = 0; i < 7; ++i) {
+        if (i < left) v[i] = p[i];
+      }
+    }
+  }
+};
+
+// Tiles of TM x TN over WM x WN waves, LDS double buffered with the next slice in registers.
+template <typename T, Product P, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(WM* WN* kWave, 2) void mx_mixed_kernel(MixedArgs g) {
   constexpr int FORM = P == kWeightGrad ? kE4m3 : kE2m1;
   constexpr bool A_R = P != kWeightGrad, B_R = P == kForward;  // rows along r
-  constexpr int TERMS = kTerms<T>, SLICE = kSlice<T>;
-  constexpr int kPlane = kTile * SLICE;            // elements of a plane
-  constexpr int kStage = (TERMS + 1) * kPlane;
-  constexpr int kUnits = kPlane / 8 / 256;         // units of eight elements a thread: of A, and of B
+  constexpr int TERMS = kTerms<T>, SLICE = kSlice<T>, THREADS = WM * WN * kWave;
+  constexpr int kA = TM * SLICE, kB = TN * SLICE;  // elements of a plane
+  constexpr int kStage = TERMS * kA + kB;
+  constexpr int UA = kA / 8 / THREADS, UB = kB / 8 / THREADS;  // units of eight elements a thread
+  constexpr int MT = TM / WM / 16, NT = TN / WN / 16;
   __shared__ __align__(16) bf16_t smem[2 * kStage];
 
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
   const int grp = lane >> 4, col = lane & 15;
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / WN, wn = wave % WN;
   const TilePlace at(g.tiles_m, g.tiles_n);
-  const int64_t m0 = (int64_t)at.mi * kTile, n0 = (int64_t)at.ni * kTile;
+  const int64_t m0 = (int64_t)at.mi * TM, n0 = (int64_t)at.ni * TN;
   const int64_t rbeg = at.split * g.chunk, rend = min(g.r, rbeg + g.chunk);
   const T* abase = static_cast<const T*>(g.a);
   const bool sums = P == kWeightGrad && g.bias_partial && at.ni == 0;
 
   // one slice in registers
-  constexpr int W = PACKED ? 16 / sizeof(T) : 1;
-  Raw<T, W> ra[kUnits][8 / W];
-  uint2 rb[kUnits];
-  int rs[kUnits];
-
+  Eight<T> ra[UA];
+  uint2 rb[UB];
+  int rs[UB];
   auto load = [&](int64_t r0) {
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int id = tid + 256 * u;
-      const int64_t row = A_R ? m0 + id / (SLICE / 8) : r0 + id / (kTile / 8);
-      const int64_t c = A_R ? r0 + id % (SLICE / 8) * 8 : m0 + id % (kTile / 8) * 8;
-      const int64_t rows = A_R ? g.m : rend, cols = A_R ? rend : g.m;
-      const T* p = abase + row * g.lda + c;
+    for (int u = 0; u < UA; ++u) {
+      const int id = tid + THREADS * u;
+      const int64_t row = A_R ? m0 + id / (SLICE / 8) : r0 + id / (TM / 8);
+      const int64_t c = A_R ? r0 + id % (SLICE / 8) * 8 : m0 + id % (TM / 8) * 8;
+      ra[u].load(abase + row * g.lda + c, row < (A_R ? g.m : rend) ? (A_R ? rend : g.m) - c : 0);
+    }
 #pragma unroll
-      for (int j = 0; j < 8 / W; ++j) {
-        if (row < rows && c + j * W < cols) ra[u][j].load(p + j * W);
-        else ra[u][j].clear();
-      }
-      const int64_t brow = B_R ? n0 + id / (SLICE / 8) : r0 + id / (kTile / 8);
-      const int64_t e = B_R ? r0 + id % (SLICE / 8) * 8 : n0 + id % (kTile / 8) * 8;
+    for (int u = 0; u < UB; ++u) {
+      const int id = tid + THREADS * u;
+      const int64_t row = B_R ? n0 + id / (SLICE / 8) : r0 + id / (TN / 8);
+      const int64_t e = B_R ? r0 + id % (SLICE / 8) * 8 : n0 + id % (TN / 8) * 8;
       rb[u] = uint2{0, 0}, rs[u] = 127;
-      if (brow < (B_R ? g.n : rend) && e < g.runs * kMxRun) {
-        if constexpr (FORM == kE4m3) rb[u] = *reinterpret_cast<const uint2*>(g.codes + brow * g.pitch + e);
-        else rb[u].x = *reinterpret_cast<const uint32_t*>(g.codes + brow * g.pitch + e / 2);
-        rs[u] = g.scales[brow * g.runs + e / kMxRun];
+      if (row < (B_R ? g.n : rend) && e < g.runs * kMxRun) {
+        if constexpr (FORM == kE4m3) rb[u] = *reinterpret_cast<const uint2*>(g.codes + row * g.pitch + e);
+        else rb[u].x = *reinterpret_cast<const uint32_t*>(g.codes + row * g.pitch + e / 2);
+        rs[u] = g.scales[row * g.runs + e / kMxRun];
       }
     }
   };
   float total[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   auto store = [&](bf16_t* stage) {
-    bf16_t* sb = stage + TERMS * kPlane;
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int id = tid + 256 * u;
-      const int along = lds_kc<SLICE>(id / (SLICE / 8), id % (SLICE / 8));
-      const int across = lds_tr(id / (kTile / 8), id % (kTile / 8) / 2) + id % 2 * 8;
-      const int place = A_R ? along : across;
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8 / W; ++j) ra[u][j].unpack(v + j * W);
+    for (int u = 0; u < UA; ++u) {
+      const int id = tid + THREADS * u;
+      bf16_t* p = stage + (A_R ? lds_kc<SLICE>(id / (SLICE / 8), id % (SLICE / 8))
+                               : lds_tr<TM>(id / (TM / 8), id % (TM / 8) / 2) + id % 2 * 8);
       if (sums) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) total[j] += v[j];
+        for (int j = 0; j < 8; ++j) total[j] += (float)ra[u].v[j];
       }
       if constexpr (TERMS == 1) {
-        uint4 w;
-        if constexpr (PACKED) w = ra[u][0].bits;
-        else w = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-        *reinterpret_cast<uint4*>(stage + place) = w;
+        *reinterpret_cast<typename Eight<T>::vec*>(p) = ra[u].v;
       } else {
         uint32_t w[4][TERMS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split_pair<T>(v[2 * j], v[2 * j + 1], w[j]);
+        for (int j = 0; j < 4; ++j) split_pair<T>((float)ra[u].v[2 * j], (float)ra[u].v[2 * j + 1], w[j]);
 #pragma unroll
         for (int t = 0; t < TERMS; ++t)
-          *reinterpret_cast<uint4*>(stage + t * kPlane + place) = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
+          *reinterpret_cast<uint4*>(p + t * kA) = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
       }
+    }
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const int id = tid + THREADS * u;
       const float scale = mx_scale(rs[u]);
       uint4 d;
       if constexpr (FORM == kE4m3)
@@ -236,15 +258,17 @@ __global__ __launch_bounds__(256, 2) void mx_mixed_kernel(MixedArgs g) {
       else
         d = make_uint4(decode_pair<FORM, 0>(rb[u].x, scale), decode_pair<FORM, 1>(rb[u].x, scale),
                        decode_pair<FORM, 2>(rb[u].x, scale), decode_pair<FORM, 3>(rb[u].x, scale));
-      *reinterpret_cast<uint4*>(sb + (B_R ? along : across)) = d;
+      *reinterpret_cast<uint4*>(stage + TERMS * kA +
+                                (B_R ? lds_kc<SLICE>(id / (SLICE / 8), id % (SLICE / 8))
+                                     : lds_tr<TN>(id / (TN / 8), id % (TN / 8) / 2) + id % 2 * 8)) = d;
     }
   };
 
-  floatx4 acc[4][4];  // [n][m] tiles of 16
+  floatx4 acc[NT][MT];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < MT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   const int slices = rend > rbeg ? (int)((rend - rbeg + SLICE - 1) / SLICE) : 0;
   if (slices > 0) {
@@ -257,27 +281,27 @@ __global__ __launch_bounds__(256, 2) void mx_mixed_kernel(MixedArgs g) {
     if (s + 1 < slices) load(rbeg + (int64_t)(s + 1) * SLICE);
 #pragma unroll
     for (int k = 0; k < SLICE / 32; ++k) {
-      bf16x8v b[4];
+      bf16x8v b[NT];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NT; ++i) {
         if constexpr (B_R)
-          b[i] = *reinterpret_cast<const bf16x8v*>(stage + TERMS * kPlane +
-                                                   lds_kc<SLICE>(wn * 64 + i * 16 + col, k * 4 + grp));
+          b[i] = *reinterpret_cast<const bf16x8v*>(stage + TERMS * kA +
+                                                   lds_kc<SLICE>(wn * (TN / WN) + i * 16 + col, k * 4 + grp));
         else
-          b[i] = fragment_tr(stage + TERMS * kPlane, k * 32 + grp * 8, wn * 4 + i, lane);
+          b[i] = fragment_tr<TN>(stage + TERMS * kA, k * 32 + grp * 8, wn * NT + i, lane);
       }
 #pragma unroll
       for (int t = TERMS - 1; t >= 0; --t) {  // the smallest terms first
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < MT; ++j) {
           bf16x8v a;
           if constexpr (A_R)
-            a = *reinterpret_cast<const bf16x8v*>(stage + t * kPlane +
-                                                  lds_kc<SLICE>(wm * 64 + j * 16 + col, k * 4 + grp));
+            a = *reinterpret_cast<const bf16x8v*>(stage + t * kA +
+                                                  lds_kc<SLICE>(wm * (TM / WM) + j * 16 + col, k * 4 + grp));
           else
-            a = fragment_tr(stage + t * kPlane, k * 32 + grp * 8, wm * 4 + j, lane);
+            a = fragment_tr<TM>(stage + t * kA, k * 32 + grp * 8, wm * MT + j, lane);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[i], a, acc[i][j], 0, 0, 0);
+          for (int i = 0; i < NT; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[i], a, acc[i][j], 0, 0, 0);
         }
       }
     }
@@ -287,14 +311,14 @@ __global__ __launch_bounds__(256, 2) void mx_mixed_kernel(MixedArgs g) {
 
   // a lane holds four consecutive n of one m in each tile
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = n0 + wn * 64 + i * 16 + grp * 4;
+  for (int i = 0; i < NT; ++i) {
+    const int64_t n = n0 + wn * (TN / WN) + i * 16 + grp * 4;
     if (n >= g.n) continue;
     float bias[4] = {0.f, 0.f, 0.f, 0.f};
     if (P == kForward && g.out) load_bias(static_cast<const T*>(g.bias), n, g.n, bias);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + wm * 64 + j * 16 + col;
+    for (int j = 0; j < MT; ++j) {
+      const int64_t m = m0 + wm * (TM / WM) + j * 16 + col;
       if (m >= g.m) continue;
       if (g.out) {
         const float v[4] = {acc[i][j][0] + bias[0], acc[i][j][1] + bias[1], acc[i][j][2] + bias[2],
@@ -305,16 +329,200 @@ __global__ __launch_bounds__(256, 2) void mx_mixed_kernel(MixedArgs g) {
       }
     }
   }
-  if (sums) {  // the 16 threads that had the same eight columns, in order
+  if (sums) {  // the threads that had the same eight columns, in order
     float* lds = reinterpret_cast<float*>(smem);
+    constexpr int kSame = THREADS / (TM / 8);
+    static_assert(UA == 0 || THREADS % (TM / 8) == 0, "a thread keeps its columns");
 #pragma unroll
-    for (int j = 0; j < 8; ++j) lds[(tid / 16) * kTile + tid % 16 * 8 + j] = total[j];
+    for (int j = 0; j < 8; ++j) lds[(tid / (TM / 8)) * TM + tid % (TM / 8) * 8 + j] = total[j];
     __syncthreads();
-    if (tid < kTile && m0 + tid < g.m) {
+    if (tid < TM && m0 + tid < g.m) {
       float t = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) t += lds[i * kTile + tid];
+      for (int i = 0; i < kSame; ++i) t += lds[i * TM + tid];
       g.bias_partial[(int64_t)at.split * g.m + m0 + tid] = t;
+    }
+  }
+}
+
+// The same for bf16 A with rows of whole, aligned 16-byte packs, where the output has
+// wide tiles enough: 256 x 256 over 2 x 4 waves.  A slice is two half steps of 32 r.  Its
+// operands are read from LDS while the half step before is multiplied, each as soon as
+// its register is free; the slice after lies in registers by then and goes to the other
+// stage meanwhile, and the one after that is on its way from memory.  B may be plain bf16
+// too (kPlainGrad: a linear layer's input gradient).
+template <Product P>
+__global__ __launch_bounds__(512, 2) void mx_wide_kernel(MixedArgs g) {
+  constexpr int FORM = P == kWeightGrad ? kE4m3 : kE2m1;
+  constexpr bool A_R = P != kWeightGrad, B_R = P == kForward, B_PLAIN = P == kPlainGrad;
+  constexpr int TILE = 256, SLICE = 64, U = TILE * SLICE / 8 / 512;  // units of eight elements a thread
+  constexpr int kA = A_R ? TILE * SLICE : kPadPlane, kB = B_R ? TILE * SLICE : kPadPlane, kStage = kA + kB;
+  constexpr int MT = 8, NT = 4;
+  static_assert(U == NT, "a unit is stored after each row of products");
+  __shared__ __align__(16) bf16_t smem[2 * kStage];
+
+  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
+  const int grp = lane >> 4, col = lane & 15;
+  const int wm = wave >> 2, wn = wave & 3;
+  const TilePlace at(g.tiles_m, g.tiles_n);
+  const int64_t m0 = (int64_t)at.mi * TILE, n0 = (int64_t)at.ni * TILE;
+  const int64_t rbeg = at.split * g.chunk, rend = min(g.r, rbeg + g.chunk);
+  const int slices = rend > rbeg ? (int)((rend - rbeg + SLICE - 1) / SLICE) : 0;
+
+  // A thread's units of a slice are `kStep` rows apart: rows of m or n (ROWS_R) or of r.
+  // What lies past the last row, or past r's end, is out of range and reads as zeros; m
+  // and n past the end within rows of r are the next row's numbers (their outputs are
+  // not written).
+  constexpr int UR = SLICE / 8, UT = TILE / 8;  // units of a row along r, and across
+  const int urow = tid / UR, uunit = tid % UR, trow = tid / UT, tunit = tid % UT;
+  constexpr int kStepR = 512 / UR, kStepT = 512 / UT;
+  uint4 ra[U];
+  u32x4_nt rb[U];
+  uint32_t rs[U];
+  // `first`: the operand's first row and first unit here, `bytes` a row's, `unit` a unit's
+  const auto place = [&](bool rows_r, const void* base, int64_t rows, int64_t first, int64_t c, int64_t bytes, int left) {
+    const int64_t skip = first * bytes + c;
+    const int64_t end = rows_r ? rows * bytes : min(rows, first + left) * bytes;
+    return make_rsrc(static_cast<const char*>(base) + skip, (uint32_t)max((int64_t)0, min(end - skip, (int64_t)0x7FFFFFFF)));
+  };
+  auto load = [&](int s) {
+    // (strides that the compiler takes for new in every slice: it would keep the offsets
+    // of all units in registers that the operands need)
+    const auto fresh = [](int64_t v) {
+      uint32_t x = (uint32_t)v;
+      asm volatile("" : "+s"(x));
+      return x;
+    };
+    const int64_t r0 = rbeg + (int64_t)s * SLICE;
+    const int left = (int)max((int64_t)0, min((int64_t)SLICE, rend - r0));  // of r in the slice
+    const uint32_t skip = uunit * 8 < left ? 0u : kOobOffset;               // of a unit along r
+    const auto rsa = A_R ? place(true, g.a, g.m, m0, r0 * 2, g.lda * 2, left) : place(false, g.a, g.r, r0, m0 * 2, g.lda * 2, left);
+    const uint32_t lda = fresh(g.lda * 2);
+    const uint32_t oa = A_R ? (uint32_t)urow * lda + uunit * 16 + skip : (uint32_t)trow * lda + tunit * 16;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      ra[u] = __builtin_bit_cast(
+          uint4, __builtin_amdgcn_raw_buffer_load_b128(rsa, oa + u * (A_R ? kStepR : kStepT) * lda, 0, 0));
+    if constexpr (B_PLAIN) {
+      const uint32_t ldb = fresh(g.n * 2), ob = (uint32_t)trow * ldb + tunit * 16;
+      const auto rsb = place(false, g.codes, g.r, r0, n0 * 2, g.n * 2, left);
+#pragma unroll
+      for (int u = 0; u < U; ++u) rb[u] = __builtin_amdgcn_raw_buffer_load_b128(rsb, ob + u * kStepT * ldb, 0, 0);
+    } else {
+      constexpr int UNIT = FORM == kE4m3 ? 8 : 4;  // bytes of a unit's codes
+      const uint32_t pitch = fresh(g.pitch), runs = fresh(g.runs);
+      const auto rsb = B_R ? place(true, g.codes, g.n, n0, r0 / 8 * UNIT, g.pitch, left)
+                           : place(false, g.codes, g.r, r0, n0 / 8 * UNIT, g.pitch, left);
+      const auto rss = B_R ? place(true, g.scales, g.n, n0, r0 / kMxRun, g.runs, left)
+                           : place(false, g.scales, g.r, r0, n0 / kMxRun, g.runs, left);
+      const uint32_t ob = B_R ? (uint32_t)urow * pitch + uunit * UNIT + skip : (uint32_t)trow * pitch + tunit * UNIT;
+      const uint32_t os = B_R ? (uint32_t)urow * runs + uunit / 4 + skip : (uint32_t)trow * runs + tunit / 4;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t step = u * (B_R ? kStepR : kStepT);
+        if constexpr (FORM == kE4m3) {
+          const auto v = __builtin_amdgcn_raw_buffer_load_b64(rsb, ob + step * pitch, 0, 0);
+          rb[u][0] = v[0], rb[u][1] = v[1];
+        } else {
+          rb[u][0] = __builtin_amdgcn_raw_buffer_load_b32(rsb, ob + step * pitch, 0, 0);
+        }
+        rs[u] = __builtin_amdgcn_raw_buffer_load_b8(rss, os + step * runs, 0, 0);
+      }
+    }
+  };
+  // (a unit's row is a whole number of eight rows and of the chunks' permutation further on)
+  const int along = lds_kc<SLICE>(urow, uunit), across = lds_pad(trow, tunit * 8);
+  constexpr int kAlong = kStepR * SLICE, kAcross = kStepT * kPadRow + kStepT / 8 * kPadEight;
+  static_assert(kStepR % 16 == 0 && kStepT % 8 == 0, "a unit's place is the first one's and a constant");
+  auto store = [&](int stage, int u) {
+    *reinterpret_cast<uint4*>(smem + stage + (A_R ? along + u * kAlong : across + u * kAcross)) = ra[u];
+    uint4 d;
+    if constexpr (B_PLAIN) {
+      d = make_uint4(rb[u][0], rb[u][1], rb[u][2], rb[u][3]);
+    } else {
+      const float scale = mx_scale((int)rs[u]);
+      if constexpr (FORM == kE4m3)
+        d = make_uint4(decode_pair<FORM, 0>(rb[u][0], scale), decode_pair<FORM, 1>(rb[u][0], scale),
+                       decode_pair<FORM, 0>(rb[u][1], scale), decode_pair<FORM, 1>(rb[u][1], scale));
+      else
+        d = make_uint4(decode_pair<FORM, 0>(rb[u][0], scale), decode_pair<FORM, 1>(rb[u][0], scale),
+                       decode_pair<FORM, 2>(rb[u][0], scale), decode_pair<FORM, 3>(rb[u][0], scale));
+    }
+    *reinterpret_cast<uint4*>(smem + stage + kA + (B_R ? along + u * kAlong : across + u * kAcross)) = d;
+  };
+
+  bf16x8v a[MT], b[NT];  // one half step's operands
+  // one address an operand and constants: sixteen rows further on the chunks are permuted
+  // alike, and the other half step's are four chunks further on
+  const auto read = [&](bool rows_r, int origin, int base, int k, int t) -> bf16x8v {
+    if (rows_r) return *reinterpret_cast<const bf16x8v*>(smem + origin + (base ^ (32 * k)) + t * 16 * SLICE);
+    const bf16_t* p = smem + origin + base + k * (32 * kPadRow + 4 * kPadEight) + t * 16;
+    const shortx4 lo = read_tr(p), hi = read_tr(p + 4 * kPadRow);
+    typedef short shortx8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(bf16x8v, (shortx8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  const int abase = A_R ? lds_kc<SLICE>(wm * 128 + col, grp) : lds_pad(grp * 8 + (col >> 2), wm * 128 + (col & 3) * 4);
+  const int bbase = B_R ? lds_kc<SLICE>(wn * 64 + col, grp) : lds_pad(grp * 8 + (col >> 2), wn * 64 + (col & 3) * 4);
+  auto read_a = [&](int stage, int k, int j) { a[j] = read(A_R, stage, abase, k, j); };
+  auto read_b = [&](int stage, int k, int i) { b[i] = read(B_R, stage + kA, bbase, k, i); };
+  floatx4 acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  auto half = [&](int next, int k, auto then) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[i], a[j], acc[i][j], 0, 0, 0);
+        if (i == NT - 1) read_a(next, k, j);
+      }
+      then(i);
+      read_b(next, k, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if (slices > 0) {
+    load(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) store(0, u);
+    load(1);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < MT; ++j) read_a(0, 0, j);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) read_b(0, 0, i);
+  }
+  for (int s = 0; s < slices; ++s) {
+    const int cur = (s & 1) * kStage, next = kStage - cur;
+    half(cur, 1, [&](int i) { store(next, i); });
+    load(s + 2);  // (nothing past the last)
+    // every wave has this slice's operands in registers, and has stored its part of the next
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    half(next, 0, [](int) {});
+  }
+
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int64_t n = n0 + wn * 64 + i * 16 + grp * 4;
+    if (n >= g.n) continue;
+    float bias[4] = {0.f, 0.f, 0.f, 0.f};
+    if (P == kForward && g.out) load_bias(static_cast<const bf16_t*>(g.bias), n, g.n, bias);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      const int64_t m = m0 + wm * 128 + j * 16 + col;
+      if (m >= g.m) continue;
+      if (g.out) {
+        const float v[4] = {acc[i][j][0] + bias[0], acc[i][j][1] + bias[1], acc[i][j][2] + bias[2],
+                            acc[i][j][3] + bias[3]};
+        store_quad(static_cast<bf16_t*>(g.out) + m * g.n + n, n, g.n, v);
+      } else {
+        *reinterpret_cast<floatx4*>(g.partial + ((int64_t)at.split * g.m + m) * g.ldp + n) = acc[i][j];
+      }
     }
   }
 }
@@ -327,6 +535,7 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(MixedArgs g, int splits) {
   if (id < total) {
     const int64_t m = id / quads, n = (id - m * quads) * 4;
     floatx4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s)
       v += *reinterpret_cast<const floatx4*>(g.partial + ((int64_t)s * g.m + m) * g.ldp + n);
     float w[4];
@@ -342,31 +551,119 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(MixedArgs g, int splits) {
   }
 }
 
-// Splits of the sum: workgroups enough for two a CU, slices enough for each.
+// ---- sums over rows -------------------------------------------------------------
+// A thread sums one column, or a 16-byte pack of them, over a slab of rows, a second
+// launch the slabs in order.
+constexpr int64_t kSlabRows = 32, kSlabs = 256;
+
+int64_t sum_slabs(int64_t rows) { return std::min(kSlabs, (rows + kSlabRows - 1) / kSlabRows); }
+
+template <typename T, int W>
+__global__ __launch_bounds__(256) void column_sums_kernel(const T* x, int64_t rows, int64_t dim, int64_t each,
+                                                          float* partial) {
+  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * W;
+  if (c >= dim) return;
+  const int64_t beg = blockIdx.y * each, end = min(rows, beg + each);
+  float t[W] = {};
+#pragma unroll 8
+  for (int64_t r = beg; r < end; ++r) {
+    Raw<T, W> raw;
+    raw.load(x + r * dim + c);
+    float v[W];
+    raw.unpack(v);
+#pragma unroll
+    for (int i = 0; i < W; ++i) t[i] += v[i];
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i) partial[blockIdx.y * dim + c + i] = t[i];
+}
+
+// 64 columns a workgroup, its waves a quarter of the slabs each (256 slabs by one thread a
+// column took 60 us).
+template <typename T>
+__global__ __launch_bounds__(256) void columns_join_kernel(const float* partial, int64_t dim, int slabs, T* sums) {
+  __shared__ float lds[4][kWave];
+  const int64_t c = (int64_t)blockIdx.x * kWave + lane_id();
+  float t = 0.f;
+  if (c < dim) {
+#pragma unroll 16
+    for (int s = wave_id(); s < slabs; s += 4) t += partial[s * dim + c];
+  }
+  lds[wave_id()][lane_id()] = t;
+  __syncthreads();
+  if (wave_id() == 0 && c < dim) sums[c] = (T)(((lds[0][lane_id()] + lds[1][lane_id()]) + lds[2][lane_id()]) + lds[3][lane_id()]);
+}
+
+template <typename T>
+int launch_column_sums(const void* x, int64_t rows, int64_t dim, float* partial, void* sums, hipStream_t s) {
+  const int64_t slabs = sum_slabs(rows), each = (rows + slabs - 1) / slabs;
+  JN_PROFILE("column_sums_kernel", s);
+  constexpr int W = 16 / sizeof(T);
+  const T* const p = static_cast<const T*>(x);
+  if (dim % W == 0 && aligned16(x))
+    hipLaunchKernelGGL((column_sums_kernel<T, W>), dim3((unsigned)((dim / W + 255) / 256), (unsigned)slabs), dim3(256), 0,
+                       s, p, rows, dim, each, partial);
+  else
+    hipLaunchKernelGGL((column_sums_kernel<T, 1>), dim3((unsigned)((dim + 255) / 256), (unsigned)slabs), dim3(256), 0, s,
+                       p, rows, dim, each, partial);
+  JN_LAUNCH_CHECK();
+  hipLaunchKernelGGL(columns_join_kernel<T>, dim3((unsigned)((dim + kWave - 1) / kWave)), dim3(256), 0, s, partial, dim,
+                     (int)slabs, static_cast<T*>(sums));
+  JN_LAUNCH_CHECK();
+  return kOk;
+}
+
+// Splits of the narrow tiles' sum by what they were measured to cost: a slice's time with
+// one workgroup on a CU and with two, and for more than one split a second launch and the
+// partial sums' way to memory and back (in us).
+int64_t narrow_splits(int32_t type, int64_t outputs, int64_t tiles, int64_t slices) {
+  const double one = type == kTypeBf16 ? 1.2 : 1.3, two = type == kTypeF32 ? 2.2 : type == kTypeF16 ? 1.9 : 1.5;
+  int64_t best = 1;
+  double least = 0.0;
+  for (int64_t s = 1; s <= std::min<int64_t>(64, slices); ++s) {
+    const int64_t groups = tiles * s, each = (slices + s - 1) / s;
+    const double time = (groups <= 256 ? one : two * (double)((groups + 511) / 512)) * (double)each +
+                        (s > 1 ? 4.0 + (double)s * (double)outputs * 8.0 / 6e6 : 0.0);
+    if (s == 1 || time < least) best = s, least = time;
+  }
+  return best;
+}
+
+// Which tiles, and how many splits of the sum.
 struct MixedPlan {
-  int tiles_m, tiles_n, splits;
+  int tile, tiles_m, tiles_n, splits;
   int64_t chunk, ldp;
   size_t partial_bytes, bias_bytes;
 
-  MixedPlan(int64_t m, int64_t n, int64_t r, int32_t type, bool bias) {
+  MixedPlan(Product p, int64_t m, int64_t n, int64_t r, int32_t type, bool bias) {
+    // A's rows of whole packs of 16 bytes, and offsets of a tile's rows below 2^31
+    const int64_t lda = p == kWeightGrad ? m : r;
+    const bool packed = lda % 8 == 0 && lda < (1 << 21) && n < (1 << 21) && (p != kPlainGrad || n % 8 == 0);
     const int slice = type == kTypeBf16 ? kSlice<bf16_t> : kSlice<float>;
-    tiles_m = (int)((m + kTile - 1) / kTile), tiles_n = (int)((n + kTile - 1) / kTile);
-    const int64_t tiles = (int64_t)tiles_m * tiles_n, slices = std::max<int64_t>(1, (r + slice - 1) / slice);
-    const int64_t want = std::min<int64_t>({(512 + tiles - 1) / tiles, std::max<int64_t>(1, slices / 4), 64});
+    const auto tiles = [&](int64_t t) { return (m + t - 1) / t * ((n + t - 1) / t); };
+    const int64_t slices = std::max<int64_t>(1, (r + slice - 1) / slice);
+    // wide tiles where they, split at most eight slices deep, keep three quarters of the CUs
+    // busy (one workgroup each)
+    const int64_t deep = std::max<int64_t>(1, std::min<int64_t>({256 / tiles(256), slices / 8, 64}));
+    const bool wide = type == kTypeBf16 && packed && tiles(256) * deep >= 192;
+    tile = wide ? 256 : 128;
+    tiles_m = (int)((m + tile - 1) / tile), tiles_n = (int)((n + tile - 1) / tile);
+    const int64_t want = wide ? deep : narrow_splits(type, m * n, tiles(128), slices);
     const int64_t each = (slices + want - 1) / want;
     splits = (int)std::max<int64_t>(1, (slices + each - 1) / each);
     chunk = each * slice;
     ldp = (n + 3) / 4 * 4;
     partial_bytes = splits > 1 ? (size_t)splits * m * ldp * sizeof(float) : 0;
-    bias_bytes = bias ? (size_t)splits * m * sizeof(float) : 0;
+    bias_bytes = bias ? (size_t)(wide ? sum_slabs(r) : splits) * m * sizeof(float) : 0;
   }
   size_t bytes() const { return (partial_bytes + 255) / 256 * 256 + bias_bytes; }
 };
 
 template <Product P>
 int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size_t workspace_bytes,
-             hipStream_t s) {
-  const MixedPlan plan(g.m, g.n, g.r, type, g.bias_grad != nullptr);
+              hipStream_t s) {
+  const MixedPlan plan(P, g.m, g.n, g.r, type, g.bias_grad != nullptr);
+  JN_REQUIRE(plan.tile != 256 || aligned16(g.a), kInvalidArgument, "%s: the operand must start on 16 bytes", what);
   JN_REQUIRE(plan.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes()),
              kWorkspaceTooSmall, "%s: needs %zu workspace bytes on a 16-byte address, got %zu", what, plan.bytes(),
              workspace_bytes);
@@ -382,40 +679,32 @@ int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size
   const dim3 grid((unsigned)((int64_t)plan.tiles_m * plan.tiles_n * plan.splits));
   return with_type(type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
-    const bool packed = aligned16(g.a) && g.lda * sizeof(T) % 16 == 0;
+    if (plan.tile == 256 && g.bias_grad) {  // (the wide tiles have no registers for them)
+      if (const int rc = launch_column_sums<T>(g.a, g.r, g.m, g.bias_partial, g.bias_grad, s)) return rc;
+      g.bias_grad = nullptr, g.bias_partial = nullptr;
+    }
     {
-      JN_PROFILE(P == kForward ? "mx_forward_kernel" : P == kInputGrad ? "mx_input_grad_kernel" : "mx_weight_grad_kernel", s);
-      if (packed) hipLaunchKernelGGL((mx_mixed_kernel<T, P, true>), grid, dim3(256), 0, s, g);
-      else hipLaunchKernelGGL((mx_mixed_kernel<T, P, false>), grid, dim3(256), 0, s, g);
+      JN_PROFILE(P == kForward ? "mx_forward_kernel"
+                 : P == kInputGrad ? "mx_input_grad_kernel"
+                 : P == kWeightGrad ? "mx_weight_grad_kernel"
+                                    : "linear_input_grad_kernel",
+                 s);
+      if (plan.tile == 256) {
+        hipLaunchKernelGGL(mx_wide_kernel<P>, grid, dim3(512), 0, s, g);
+      } else if constexpr (P != kPlainGrad) {
+        hipLaunchKernelGGL((mx_mixed_kernel<T, P, 128, 128, 2, 2>), grid, dim3(256), 0, s, g);
+      }
       JN_LAUNCH_CHECK();
     }
     if (g.partial || g.bias_partial) {
       JN_PROFILE("mx_sum_kernel", s);
       g.out = out;
       const int64_t threads = (g.partial ? g.m * (g.ldp / 4) : 0) + (g.bias_partial ? g.m : 0);
-      hipLaunchKernelGGL(mx_sum_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, g,
-                         plan.splits);
+      hipLaunchKernelGGL(mx_sum_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, g, plan.splits);
       JN_LAUNCH_CHECK();
     }
     return kOk;
   });
-}
-
-// ---- sums over rows -------------------------------------------------------------
-// A thread sums one column over a slab of rows, a second launch the slabs in order.
-constexpr int64_t kSlabRows = 64, kSlabs = 256;
-
-int64_t sum_slabs(int64_t rows) { return std::min(kSlabs, (rows + kSlabRows - 1) / kSlabRows); }
-
-template <typename T>
-__global__ __launch_bounds__(256) void column_sums_kernel(const T* x, int64_t rows, int64_t dim, int64_t each,
-                                                          float* partial) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= dim) return;
-  const int64_t beg = blockIdx.y * each, end = min(rows, beg + each);
-  float t = 0.f;
-  for (int64_t r = beg; r < end; ++r) t += (float)x[r * dim + c];
-  partial[blockIdx.y * dim + c] = t;
 }
 
 // ---- forward: microscaled by microscaled --------------------------------------
@@ -451,24 +740,23 @@ typedef int intx4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ uint32_t lds_offset(const uint8_t* p) { return (uint32_t)(uintptr_t)(lds_byte*)p; }
 
-// The resource over [base, base + bytes), or its first 2^32 - 1 bytes: a tile's rows reach no further.
+// The resource over [base, base + bytes), or its first 2^32 - 1 bytes: a tile's rows
+// reach no further.  Empty where bytes is negative.
 __device__ __forceinline__ intx4 rows_rsrc(const uint8_t* base, int64_t bytes) {
   const uint64_t p = reinterpret_cast<uint64_t>(base);
   return intx4{__builtin_amdgcn_readfirstlane((int)(uint32_t)p),
                __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xFFFFu)),
-               __builtin_amdgcn_readfirstlane((int)(uint32_t)min(bytes, (int64_t)0xFFFFFFFF)), 0x00020000};
+               __builtin_amdgcn_readfirstlane((int)(uint32_t)max((int64_t)0, min(bytes, (int64_t)0xFFFFFFFF))), 0x00020000};
 }
 
-// `base`, `at` and the resource are uniform over the wave.
+// `base` and the resource are uniform over the wave.
 template <int BYTES>
-__device__ __forceinline__ void load_lds(intx4 rs, uint32_t base, uint32_t offset, uint32_t at) {
+__device__ __forceinline__ void load_lds(intx4 rs, uint32_t base, uint32_t offset) {
   if constexpr (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(base), "v"(offset),
-                 "s"(rs), "s"(at)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(base), "v"(offset), "s"(rs)
                  : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(base), "v"(offset),
-                 "s"(rs), "s"(at)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(base), "v"(offset), "s"(rs)
                  : "memory", "m0");
 }
 
@@ -498,10 +786,6 @@ __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_linear_kernel(LinearArgs 
   const int64_t m0 = (int64_t)at.mi * TM, n0 = (int64_t)at.ni * TN;
   const int mrows = (int)min((int64_t)TM, g.m - m0), nrows = (int)min((int64_t)TN, g.n - n0);
 
-  const auto rx = rows_rsrc(g.x + m0 * g.x_pitch, (g.m - m0) * g.x_pitch);
-  const auto rw = rows_rsrc(g.w + n0 * g.pitch, (g.n - n0) * g.pitch);
-  const auto rxs = rows_rsrc(g.xs + m0 * g.x_runs, (g.m - m0) * g.x_runs);
-  const auto rws = rows_rsrc(g.ws + n0 * g.x_runs, (g.n - n0) * g.x_runs);
   // the lane's chunk of its row is the one that belongs in its place
   uint32_t ox[XU], ow[WU];
 #pragma unroll
@@ -519,17 +803,25 @@ __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_linear_kernel(LinearArgs 
   const uint32_t ows = __umul24(min(wsrow, nrows - 1), (uint32_t)g.x_runs) + tid % 2 * 4;
 
   const uint32_t lds = lds_offset(smem);
-  // (past the last step out of range, which reads nothing: without a branch the loop below is one block)
+  // The step is in the resources' bases, since a scalar offset is no part of the range
+  // check; past the last step all is out of range, which reads nothing (without a branch
+  // the loop below is one block).
   const int steps = (int)(g.x_runs / kStepRuns);
   auto load = [&](int step, uint32_t stage) {
-    const uint32_t k = step < steps ? (uint32_t)step * kStepBytes : kOobOffset;
-    const uint32_t run = step < steps ? (uint32_t)step * kStepRuns : kOobOffset;
+    const auto at_step = [&](const uint8_t* rows, int64_t bytes, int each) {
+      const int64_t k = (int64_t)step * each;
+      return rows_rsrc(rows + k, step < steps ? bytes - k : 0);
+    };
+    const auto rx = at_step(g.x + m0 * g.x_pitch, (g.m - m0) * g.x_pitch, kStepBytes);
+    const auto rw = at_step(g.w + n0 * g.pitch, (g.n - n0) * g.pitch, kStepBytes);
+    const auto rxs = at_step(g.xs + m0 * g.x_runs, (g.m - m0) * g.x_runs, kStepRuns);
+    const auto rws = at_step(g.ws + n0 * g.x_runs, (g.n - n0) * g.x_runs, kStepRuns);
 #pragma unroll
-    for (int u = 0; u < XU; ++u) load_lds<16>(rx, lds + stage + (u * WAVES + wave) * 1024, ox[u], k);
+    for (int u = 0; u < XU; ++u) load_lds<16>(rx, lds + stage + (u * WAVES + wave) * 1024, ox[u]);
 #pragma unroll
-    for (int u = 0; u < WU; ++u) load_lds<16>(rw, lds + stage + kX + (u * WAVES + wave) * 1024, ow[u], k);
-    load_lds<4>(rxs, lds + stage + kX + kW + wave % kXSL * 256, oxs, run);
-    load_lds<4>(rws, lds + stage + kX + kW + kXS + wave % kWSL * 256, ows, run);
+    for (int u = 0; u < WU; ++u) load_lds<16>(rw, lds + stage + kX + (u * WAVES + wave) * 1024, ow[u]);
+    load_lds<4>(rxs, lds + stage + kX + kW + wave % kXSL * 256, oxs);
+    load_lds<4>(rws, lds + stage + kX + kW + kXS + wave % kWSL * 256, ows);
   };
 
   floatx4 acc[NT][MT];
@@ -623,6 +915,146 @@ __global__ __launch_bounds__(256) void mx_pad_scales_kernel(const uint8_t* scale
   reinterpret_cast<uint32_t*>(out)[id] = w;
 }
 
+// ---- forward of few rows --------------------------------------------------------
+// Up to 64 rows of x read W once: a workgroup takes NT tiles of sixteen outputs, its
+// waves every WAVES-th step of 128 k, straight from memory into registers (a lane has a
+// run of 32 k of its row of W, and the same run of its rows of x); their sums join in
+// LDS in order.  FORM e2m1: a lane microscales its run of x itself.  Plain x: W's run is
+// four bf16 operands of eight, x's as many of each of its terms.
+struct RowsArgs {
+  const void* x;      // [m][dim]
+  const uint8_t* w;   // [n][pitch]
+  const uint8_t* ws;  // [n][runs]
+  const void* bias;   // [n] or null
+  void* y;            // [m][n]
+  int64_t m, n, dim, runs, pitch;
+};
+
+template <typename T, bool SCALED, int MT, int NT, int WAVES>
+__global__ __launch_bounds__(WAVES* kWave) void mx_rows_kernel(RowsArgs g) {
+  __shared__ __align__(16) float sums[WAVES][NT * MT][256];
+  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
+  const int grp = lane >> 4, col = lane & 15;
+  const int64_t n0 = (int64_t)blockIdx.x * NT * 16, m0 = (int64_t)blockIdx.y * MT * 16;
+  const T* x = static_cast<const T*>(g.x);
+  constexpr int TERMS = kTerms<T>;
+
+  floatx4 acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  const int64_t steps = (g.runs + 3) / 4;
+#pragma unroll 2
+  for (int64_t s = wave; s < steps; s += WAVES) {
+    const int64_t run = s * 4 + grp;
+    u32x4_nt w[NT];
+    int ws[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int64_t n = min(n0 + i * 16 + col, g.n - 1);  // (past the end: the last row, not written)
+      w[i] = u32x4_nt{0, 0, 0, 0}, ws[i] = 127;
+      if (run < g.runs) {
+        w[i] = *reinterpret_cast<const u32x4_nt*>(g.w + n * g.pitch + run * 16);
+        ws[i] = g.ws[n * g.runs + run];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      const int64_t m = m0 + j * 16 + col, e = run * kMxRun;
+      Eight<T> v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q].load(x + m * g.dim + e + q * 8, m < g.m ? g.dim - e - q * 8 : 0);
+      if constexpr (SCALED) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int q = 0; q < 32; ++q) most = max(most, __float_as_uint((float)v[q / 8].v[q % 8]) & 0x7FFFFFFFu);
+        const int xs = mx_scale_code<kE2m1>(most);
+        const float inv = __uint_as_float((uint32_t)(254 - min(xs, 253)) << 23);
+        u32x4_nt c;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float f[8];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) f[t] = (float)v[q].v[t] * inv;
+          c[q] = xs == 255 ? 0u : e2m1_word(f);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[i]), wide(c), acc[i][j], 4, 4, 0, ws[i], 0, xs);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          bf16x8v xt[TERMS];
+          if constexpr (TERMS == 1) {
+            xt[0] = v[q].v;
+          } else {
+            uint32_t t[4][TERMS];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) split_pair<T>((float)v[q].v[2 * p], (float)v[q].v[2 * p + 1], t[p]);
+#pragma unroll
+            for (int p = 0; p < TERMS; ++p)
+              xt[p] = __builtin_bit_cast(bf16x8v, make_uint4(t[0][p], t[1][p], t[2][p], t[3][p]));
+          }
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const float scale = mx_scale(ws[i]);
+            const bf16x8v wt = __builtin_bit_cast(
+                bf16x8v, make_uint4(decode_pair<kE2m1, 0>(w[i][q], scale), decode_pair<kE2m1, 1>(w[i][q], scale),
+                                    decode_pair<kE2m1, 2>(w[i][q], scale), decode_pair<kE2m1, 3>(w[i][q], scale)));
+#pragma unroll
+            for (int p = TERMS - 1; p >= 0; --p)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wt, xt[p], acc[i][j], 0, 0, 0);
+          }
+        }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) *reinterpret_cast<floatx4*>(&sums[wave][i * MT + j][col * 16 + grp * 4]) = acc[i][j];
+  __syncthreads();
+  for (int id = tid; id < NT * MT * 256; id += WAVES * kWave) {  // [m][n] of the workgroup's outputs
+    const int c = id % (NT * 16), row = id / (NT * 16);
+    const int64_t n = n0 + c, m = m0 + row;
+    if (m >= g.m || n >= g.n) continue;
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) t += sums[w][(c / 16) * MT + row / 16][(row % 16) * 16 + c % 16];
+    if (g.bias) t += (float)static_cast<const T*>(g.bias)[n];
+    static_cast<T*>(g.y)[m * g.n + n] = (T)t;
+  }
+}
+
+template <typename T, bool SCALED, int MT, int NT>
+int launch_rows(const RowsArgs& g, hipStream_t s) {
+  const dim3 grid((unsigned)((g.n + NT * 16 - 1) / (NT * 16)), (unsigned)((g.m + MT * 16 - 1) / (MT * 16)));
+  JN_PROFILE("mx_rows_kernel", s);
+  if (g.runs > 16) hipLaunchKernelGGL((mx_rows_kernel<T, SCALED, MT, NT, 8>), grid, dim3(8 * kWave), 0, s, g);
+  else hipLaunchKernelGGL((mx_rows_kernel<T, SCALED, MT, NT, 4>), grid, dim3(4 * kWave), 0, s, g);
+  JN_LAUNCH_CHECK();
+  return kOk;
+}
+
+// Tiles of outputs a workgroup, and tiles of rows: as many as leave a workgroup for every
+// CU (x's way into registers is the most of the work of many rows; 64 x 2,048 x 16,384
+// bf16 with one, two and four tiles of outputs 27.9, 22.8 and 17.3 us, one row 8.2 to 8.7).
+template <typename T, bool SCALED>
+int run_rows(const RowsArgs& g, hipStream_t s) {
+  const int64_t rows = (g.m + 15) / 16, outs = (g.n + 15) / 16;
+  if (rows == 1) return outs >= 1024 ? launch_rows<T, SCALED, 1, 4>(g, s) : launch_rows<T, SCALED, 1, 1>(g, s);
+  if (outs >= 1024) return rows == 2 ? launch_rows<T, SCALED, 2, 4>(g, s) : launch_rows<T, SCALED, 4, 4>(g, s);
+  if (outs >= 256) return rows == 2 ? launch_rows<T, SCALED, 2, 1>(g, s) : launch_rows<T, SCALED, 4, 1>(g, s);
+  return rows > 2 && outs >= 128 ? launch_rows<T, SCALED, 2, 1>(g, s) : launch_rows<T, SCALED, 1, 1>(g, s);
+}
+
+// Few rows: microscaling x apart costs more than it does here until it is shared by
+// more workgroups (bf16, 2,048 x 16,384: 64 rows 17.6 us, 65 in two launches 13.3).
+bool few_rows(int64_t rows, int32_t activations) { return rows <= (activations == kPlain ? 64 : 32); }
+
 // x microscaled for this product: rows of whole steps.
 int64_t step_runs(int64_t dim) { return (mx_runs(dim) + kStepRuns - 1) / kStepRuns * kStepRuns; }
 size_t linear_codes_bytes(int64_t rows, int64_t dim) { return (size_t)(rows * step_runs(dim) * 16); }
@@ -655,8 +1087,8 @@ using namespace jakal;
 extern "C" {
 
 size_t jn_mx_linear_forward_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t activations) {
-  if (check_product("mx_linear", rows, dim, out, type)) return 0;
-  if (activations == kPlain) return MixedPlan(rows, out, dim, type, false).bytes();
+  if (check_product("mx_linear", rows, dim, out, type) || few_rows(rows, activations)) return 0;
+  if (activations == kPlain) return MixedPlan(kForward, rows, out, dim, type, false).bytes();
   return linear_codes_bytes(rows, dim) + (size_t)((rows + (mx_runs(dim) % kStepRuns ? out : 0)) * step_runs(dim));
 }
 
@@ -670,6 +1102,15 @@ int jn_mx_linear_forward(const void* x, const void* weight_codes, const void* we
   JN_REQUIRE(aligned16(weight_codes) && aligned16(y), kInvalidArgument,
              "mx_linear: weight codes and outputs must start on 16 bytes");
   const auto s = static_cast<hipStream_t>(stream);
+  if (few_rows(rows, activations)) {
+    RowsArgs g{};
+    g.x = x, g.w = static_cast<const uint8_t*>(weight_codes), g.ws = static_cast<const uint8_t*>(weight_scales);
+    g.bias = bias, g.y = y, g.m = rows, g.n = out, g.dim = dim, g.runs = mx_runs(dim), g.pitch = mx_pitch(dim, kE2m1);
+    return with_type(type, [&](auto* t) -> int {
+      using T = std::remove_pointer_t<decltype(t)>;
+      return activations == kPlain ? run_rows<T, false>(g, s) : run_rows<T, true>(g, s);
+    });
+  }
   if (activations == kPlain) {
     MixedArgs g{};
     g.a = x, g.codes = static_cast<const uint8_t*>(weight_codes), g.scales = static_cast<const uint8_t*>(weight_scales);
@@ -709,7 +1150,7 @@ int jn_mx_linear_forward(const void* x, const void* weight_codes, const void* we
 
 size_t jn_mx_linear_backward_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type) {
   if (check_product("mx_linear backward", rows, dim, out, type)) return 0;
-  return MixedPlan(rows, dim, out, type, false).bytes();
+  return MixedPlan(kInputGrad, rows, dim, out, type, false).bytes();
 }
 
 int jn_mx_linear_backward(const void* grad_y, const void* weight_codes, const void* weight_scales, int64_t rows,
@@ -729,7 +1170,7 @@ int jn_mx_linear_backward(const void* grad_y, const void* weight_codes, const vo
 
 size_t jn_mx_weight_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t bias) {
   if (check_product("mx_weight_grad", rows, dim, out, type)) return 0;
-  return MixedPlan(out, dim, rows, type, bias != 0).bytes();
+  return MixedPlan(kWeightGrad, out, dim, rows, type, bias != 0).bytes();
 }
 
 int jn_mx_weight_grad(const void* grad_y, const void* codes, const void* scales, int64_t rows, int64_t dim,
@@ -746,6 +1187,34 @@ int jn_mx_weight_grad(const void* grad_y, const void* codes, const void* scales,
                          static_cast<hipStream_t>(stream));
 }
 
+int32_t jn_linear_input_grad_fits(int64_t rows, int64_t dim, int64_t out, int32_t type) {
+  if (check_product("linear backward", rows, dim, out, type)) return 0;
+  // Measured with the library's product (us): 1,024 x 2,048 outputs over 16,384 83 and 112,
+  // 32,768 138 and 284, 8,192 60 and 68, 4,096 42 and 35; 512 x 1,024 over 16,384 42 and 65,
+  // 2,048 x 2,048 139 and 146; 4,096 x 2,048 266 and 245, 8,192 x 4,096 over 4,096 250 and 210.
+  const MixedPlan plan(kPlainGrad, rows, dim, out, type, false);
+  return plan.tile == 256 && out >= 8192 && (int64_t)plan.tiles_m * plan.tiles_n <= 64;
+}
+
+size_t jn_linear_input_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type) {
+  if (check_product("linear backward", rows, dim, out, type)) return 0;
+  return MixedPlan(kPlainGrad, rows, dim, out, type, false).bytes();
+}
+
+int jn_linear_input_grad(const void* grad_y, const void* weight, int64_t rows, int64_t dim, int64_t out, int32_t type,
+                         void* grad_x, void* workspace, size_t workspace_bytes, jn_stream_t stream) {
+  if (const int rc = check_product("linear backward", rows, dim, out, type)) return rc;
+  JN_REQUIRE(grad_y && weight && grad_x, kInvalidArgument, "null tensor pointer");
+  JN_REQUIRE(aligned16(weight) && aligned16(grad_x), kInvalidArgument,
+             "linear backward: weight and grad_x must start on 16 bytes");
+  JN_REQUIRE(jn_linear_input_grad_fits(rows, dim, out, type), kUnsupported,
+             "linear backward: these sizes are left to a library product");
+  MixedArgs g{};
+  g.a = grad_y, g.codes = static_cast<const uint8_t*>(weight), g.out = grad_x;
+  g.m = rows, g.n = dim, g.r = out, g.lda = out;
+  return run_mixed<kPlainGrad>("linear backward", g, type, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
 size_t jn_column_sums_workspace_bytes(int64_t rows, int64_t dim) {
   return rows < 1 || dim < 1 ? 0 : (size_t)(sum_slabs(rows) * dim) * sizeof(float);
 }
@@ -758,19 +1227,8 @@ int jn_column_sums(const void* x, int64_t rows, int64_t dim, int32_t type, void*
   JN_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, kWorkspaceTooSmall,
              "column_sums: needs %zu workspace bytes on a 16-byte address, got %zu", need, workspace_bytes);
   const auto s = static_cast<hipStream_t>(stream);
-  const int64_t slabs = sum_slabs(rows), each = (rows + slabs - 1) / slabs;
-  const unsigned columns = (unsigned)((dim + 255) / 256);
-  MixedArgs g{};
-  g.bias_partial = static_cast<float*>(workspace), g.bias_grad = sums, g.m = dim;
   return with_type(type, [&](auto* t) -> int {
-    using T = std::remove_pointer_t<decltype(t)>;
-    JN_PROFILE("column_sums_kernel", s);
-    hipLaunchKernelGGL(column_sums_kernel<T>, dim3(columns, (unsigned)slabs), dim3(256), 0, s,
-                       static_cast<const T*>(x), rows, dim, each, g.bias_partial);
-    JN_LAUNCH_CHECK();
-    hipLaunchKernelGGL(mx_sum_kernel<T>, dim3(columns), dim3(256), 0, s, g, (int)slabs);
-    JN_LAUNCH_CHECK();
-    return kOk;
+    return launch_column_sums<std::remove_pointer_t<decltype(t)>>(x, rows, dim, static_cast<float*>(workspace), sums, s);
   });
 }
 

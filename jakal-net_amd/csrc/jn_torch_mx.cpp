@@ -172,7 +172,7 @@ Tensor mx_product_meta(const Tensor& x, const Tensor& codes, const Tensor&, cons
 Tensor mx_product(const Tensor& x_in, const Tensor& codes_in, const Tensor& scales_in,
                   const std::optional<Tensor>& bias_in, int64_t acts) {
   check_mx_linear(x_in, codes_in, scales_in, given(bias_in), acts);
-  const Tensor x = plain(x_in), codes = aligned(codes_in), scales = aligned(scales_in), bias = plain(given(bias_in));
+  const Tensor x = aligned(x_in), codes = aligned(codes_in), scales = aligned(scales_in), bias = plain(given(bias_in));
   const c10::DeviceGuard guard(x.device());
   const Tensor y = mx_product_meta(x, codes, scales, bias_in, acts);
   const int64_t dim = x.size(-1), rows = x.numel() / dim;
@@ -194,7 +194,7 @@ Tensor mx_input_grad(const Tensor& grad_in, const Tensor& codes_in, const Tensor
   TORCH_CHECK(codes_in.dim() == 2 && codes_in.size(0) == grad_in.size(-1),
               "mx_linear backward: gradients of another number of outputs than the weight has.");
   check_gpu(codes_in, grad_in);
-  const Tensor grad = plain(grad_in), codes = aligned(codes_in), scales = plain(scales_in);
+  const Tensor grad = aligned(grad_in), codes = aligned(codes_in), scales = plain(scales_in);
   const c10::DeviceGuard guard(grad.device());
   const Tensor out = mx_input_grad_meta(grad, codes, scales, size);
   const int64_t dim = out.size(-1), rows = out.numel() / dim, outs = grad.size(-1);
@@ -279,7 +279,7 @@ std::tuple<Tensor, Tensor> mx_weight_grad(const Tensor& grad_in, const Tensor& c
   const int64_t out = grad_in.size(-1), rows = grad_in.numel() / out;
   TORCH_CHECK(scales_in.numel() == rows * scales_in.size(-1),
               "linear backward: gradients of another number of rows than were kept.");
-  const Tensor grad = plain(grad_in), codes = aligned(codes_in), scales = plain(scales_in);
+  const Tensor grad = aligned(grad_in), codes = aligned(codes_in), scales = plain(scales_in);
   const c10::DeviceGuard guard(grad.device());
   auto [gw, gb] = mx_weight_grad_meta(grad, codes, scales, size, bias);
   if (rows == 0) {
@@ -296,9 +296,38 @@ std::tuple<Tensor, Tensor> mx_weight_grad(const Tensor& grad_in, const Tensor& c
   return {gw, gb};
 }
 
+Tensor linear_input_grad_meta(const Tensor& grad, const Tensor& weight) {
+  return at::empty_symint(with_last(grad.sym_sizes(), weight.sym_size(1)), grad.options());
+}
+
+// grad . weight: here where the output has few tiles and the sum is long, else the
+// library product that a plain linear layer's backward is.
+Tensor linear_input_grad(const Tensor& grad_in, const Tensor& weight_in) {
+  check_rows("linear backward", grad_in);
+  TORCH_CHECK(weight_in.dim() == 2 && weight_in.size(0) == grad_in.size(-1) &&
+                  weight_in.scalar_type() == grad_in.scalar_type(),
+              "linear backward: a weight that does not pair with the gradients.");
+  check_gpu(weight_in, grad_in);
+  const int64_t out = grad_in.size(-1), rows = grad_in.numel() / out, dim = weight_in.size(1);
+  const int32_t type = type_code("linear backward", grad_in);
+  const c10::DeviceGuard guard(grad_in.device());
+  if (rows == 0 || !jn_linear_input_grad_fits(rows, dim, out, type)) {
+    const Tensor product = at::mm(grad_in.reshape({rows, out}), weight_in);
+    std::vector<int64_t> sizes(grad_in.sizes().begin(), grad_in.sizes().end());
+    sizes.back() = dim;
+    return product.view(sizes);
+  }
+  const Tensor grad = aligned(grad_in), weight = aligned(weight_in);
+  const Tensor gx = linear_input_grad_meta(grad, weight);
+  const size_t bytes = jn_linear_input_grad_workspace_bytes(rows, dim, out, type);
+  const Tensor ws = bytes_like(grad, (int64_t)bytes);
+  check(jn_linear_input_grad(ptr(grad), ptr(weight), rows, dim, out, type, ptr(gx), ptr(ws), bytes, stream_of(grad)));
+  return gx;
+}
+
 struct JakalLinearSavedBackward : torch::autograd::Node {
   Kept codes_, scales_, weight_;
-  std::vector<c10::SymInt> sizes;  // of x
+  c10::SymInt dim = 0;
   at::ScalarType type = at::kFloat;
 
   std::string name() const override { return "JakalLinearSavedBackward"; }
@@ -321,13 +350,12 @@ struct JakalLinearSavedBackward : torch::autograd::Node {
     Tensor gx, gw, gb;
     const at::AutoDispatchBelowADInplaceOrView below;
     if (need_x) {
-      const Tensor weight = weight_.get();
-      // the plain product of a plain linear layer's backward
-      gx = at::mm(g.reshape_symint({-1, g.sym_size(-1)}), weight).reshape_symint(sizes);
+      static const auto op = inner<Tensor(const Tensor&, const Tensor&)>("jakal_net_hip::linear_input_grad");
+      gx = op.call(g, weight_.get());
     }
     if (need_w) {
       static const auto op = inner<WeightGrad>("jakal_net_hip::mx_weight_grad");
-      std::tie(gw, gb) = op.call(g, codes_.get(), scales_.get(), sizes.back(), need_b);
+      std::tie(gw, gb) = op.call(g, codes_.get(), scales_.get(), dim, need_b);
     } else if (need_b) {
       gb = call_column_sums(g);
     }
@@ -360,7 +388,7 @@ Tensor linear_saved(const Tensor& x, const Tensor& weight, const std::optional<T
       node->scales_.set(scales);
     }
     if (torch::autograd::compute_requires_grad(x)) node->weight_.set(weight);
-    node->sizes = x.sym_sizes().vec();
+    node->dim = x.sym_size(-1);
     node->type = x.scalar_type();
     torch::autograd::set_history(y, node);
   }
@@ -676,6 +704,7 @@ TORCH_LIBRARY_FRAGMENT(jakal_net_hip, m) {
   m.def("mx_product(Tensor x, Tensor codes, Tensor scales, Tensor? bias, int activations) -> Tensor");
   m.def("mx_input_grad(Tensor grad, Tensor codes, Tensor scales, SymInt size) -> Tensor");
   m.def("mx_weight_grad(Tensor grad, Tensor codes, Tensor scales, SymInt size, bool bias) -> (Tensor, Tensor)");
+  m.def("linear_input_grad(Tensor grad, Tensor weight) -> Tensor");
   m.def("gelu_forward(Tensor x, bool keep) -> (Tensor, Tensor, Tensor)");
   m.def("gelu_backward(Tensor grad, Tensor codes, Tensor scales) -> Tensor");
   m.def("kept_norm_forward(Tensor? state, Tensor x, Tensor? weight, Tensor? bias, float eps, float scale)"
@@ -692,6 +721,7 @@ TORCH_LIBRARY_IMPL(jakal_net_hip, CUDA, m) {
   m.impl("mx_product", &mx_product);
   m.impl("mx_input_grad", &mx_input_grad);
   m.impl("mx_weight_grad", &mx_weight_grad);
+  m.impl("linear_input_grad", &linear_input_grad);
   m.impl("gelu_forward", &gelu_forward);
   m.impl("gelu_backward", &gelu_backward);
   m.impl("kept_norm_forward", &kept_norm_forward);
@@ -705,6 +735,7 @@ TORCH_LIBRARY_IMPL(jakal_net_hip, Meta, m) {
   m.impl("mx_product", &mx_product_meta);
   m.impl("mx_input_grad", &mx_input_grad_meta);
   m.impl("mx_weight_grad", &mx_weight_grad_meta);
+  m.impl("linear_input_grad", &linear_input_grad_meta);
   m.impl("gelu_forward", &gelu_forward_meta);
   m.impl("gelu_backward", &gelu_backward_meta);
   m.impl("kept_norm_forward", &kept_norm_forward_meta);

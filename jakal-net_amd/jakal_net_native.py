@@ -235,6 +235,9 @@ _declare("jn_mx_linear_backward_workspace_bytes", [_I64] * 3 + [_I32], _SZ)
 _declare("jn_mx_linear_backward", [_P] * 3 + [_I64] * 3 + [_I32] + [_P] * 2 + [_SZ, _P])
 _declare("jn_mx_weight_grad_workspace_bytes", [_I64] * 3 + [_I32] * 2, _SZ)
 _declare("jn_mx_weight_grad", [_P] * 3 + [_I64] * 3 + [_I32] + [_P] * 3 + [_SZ, _P])
+_declare("jn_linear_input_grad_fits", [_I64] * 3 + [_I32], _I32)
+_declare("jn_linear_input_grad_workspace_bytes", [_I64] * 3 + [_I32], _SZ)
+_declare("jn_linear_input_grad", [_P] * 2 + [_I64] * 3 + [_I32] + [_P] * 2 + [_SZ, _P])
 _declare("jn_column_sums_workspace_bytes", [_I64] * 2, _SZ)
 _declare("jn_column_sums", [_P] + [_I64] * 2 + [_I32] + [_P] * 2 + [_SZ, _P])
 _declare("jn_layer_norm_forward_kept", [_P] * 4 + [_I64] * 2 + [_F] * 2 + [_I32] * 3 + [_P] * 6)

@@ -163,12 +163,45 @@ def test_linear_saved(dev, rows, dim, out, bias, dtype):
     plain = torch.nn.functional.linear(*leaves)
     assert torch.equal(y, plain)  # the forward is the plain layer's
     grads = torch.autograd.grad(y, leaves, g.to(dev))
-    want = torch.autograd.grad(plain, leaves[0], g.to(dev))[0]
     what = f"linear {dtype} {rows}x{dim}x{out}"
-    assert torch.equal(grads[0], want)
+    _rounded(what + " grad_x", grads[0], M.product(g, w), kind)
     _rounded(what + " grad_weight", grads[1], M.product(g.t(), M.quantize(x, "e4m3")[0]), kind)
     if bias:
         _rounded(what + " grad_bias", grads[2], M.sums(g), kind)
+
+
+@pytest.mark.parametrize("rows,dim,out", [(256, 256, 16384), (300, 520, 16392), (1024, 256, 4104), (8, 2048, 131072)])
+def test_linear_saved_wide_tiles(dev, rows, dim, out):
+    """bf16 sums over many outputs, split over workgroups: the input gradient's wide tiles, whole and ragged."""
+    import jakal_net as J
+
+    x, w = _rand(1, rows, dim).bfloat16(), _rand(2, out, dim, scale=dim ** -0.5, spread=0.0).bfloat16()
+    g = _rand(4, rows, out, spread=0.0).bfloat16()
+    xd = x.to(dev).requires_grad_()
+    gx, = torch.autograd.grad(J.linear(xd, w.to(dev).requires_grad_(), saved="e4m3"), xd, g.to(dev))
+    _rounded(f"linear {rows}x{dim}x{out} grad_x", gx, M.product(g, w), torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows,dim,out", [(512, 4096, 4096), (520, 4104, 4360), (2048, 1000, 16384)])
+def test_products_of_wide_tiles(dev, rows, dim, out):
+    """bf16 outputs of many wide tiles, whole and ragged: forward, input gradient and weight gradient."""
+    import jakal_net as J
+
+    weight, w = _weight(dev, out, dim, 3)
+    x, g = _rand(1, rows, dim).bfloat16(), _rand(2, rows, out, spread=0.0).bfloat16()
+    b = _rand(3, out, spread=0.0).bfloat16()
+    xd, gd = x.to(dev).requires_grad_(), g.to(dev)
+    w, gs, xs = w.to(dev), gd.double(), x.to(dev).double()
+    for acts in (None, "e2m1"):
+        y = J.mx_linear(xd, weight, b.to(dev), activations=acts)
+        a = xs if acts is None else M.quantize(x, acts)[0].to(dev)
+        _rounded(f"{acts} y", y, M.product(a, w.t(), b.to(dev)), torch.bfloat16)
+    gx, = torch.autograd.grad(y, xd, gd)
+    _rounded("grad_x", gx, M.product(gs, w), torch.bfloat16)
+    codes, scales = torch.ops.jakal_net_hip.mx_codes(x.to(dev), 0)
+    gw, gb = torch.ops.jakal_net_hip.mx_weight_grad(gd, codes, scales, dim, True)
+    _rounded("grad_weight", gw, M.product(gs.t(), M.quantize(x, "e4m3")[0].to(dev)), torch.bfloat16)
+    _rounded("grad_bias", gb, M.sums(gs), torch.bfloat16)
 
 
 @pytest.mark.parametrize("rows", [4096, 10007])

@@ -97,6 +97,14 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[kTerm
   }
 }
 
+// A uniform stride that the compiler takes for new wherever it is asked for: it would keep
+// the multiples of it that a loop needs in registers that the loop's operands need.
+__device__ __forceinline__ uint32_t fresh(int64_t v) {
+  uint32_t x = (uint32_t)v;
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
 // Places in LDS, in bf16 elements, so that the lanes of one read fall on all banks.
 // [row][SLICE] with the slice along the row: 16-byte chunks permuted by the row.
 template <int SLICE>
@@ -147,6 +155,66 @@ template <typename T>
 __device__ __forceinline__ void load_bias(const T* bias, int64_t c, int64_t n, float (&b)[4]) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) b[q] = bias && c + q < n ? (float)bias[c + q] : 0.f;
+}
+
+// A wave's MT x NT tiles of outputs, the first at (m0, n0), plus the bias where there is
+// one.  Rows of whole 16-byte packs go through the wave's part of LDS, GROUP tiles of rows
+// by a line of 128 bytes (or all there is) at a time; others straight from the registers.
+template <typename T, int NT>
+constexpr int kLineTiles = NT * 16 * sizeof(T) > 128 ? 128 / (16 * (int)sizeof(T)) : NT;
+template <typename T, int NT>
+constexpr int kLineBytes = kLineTiles<T, NT> * 16 * (int)sizeof(T) + 16;  // sixteen more, so that rows begin on other banks
+
+template <typename T, int MT, int NT, int GROUP>
+__device__ __forceinline__ void store_tile(const floatx4 (&acc)[NT][MT], uint8_t* lds, const T* bias, T* out, int64_t m0,
+                                           int64_t n0, int64_t rows, int64_t cols, int lane) {
+  const int grp = lane >> 4, col = lane & 15;
+  float b[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) load_bias(bias, n0 + i * 16 + grp * 4, cols, b[i]);
+  if (cols * sizeof(T) % 16 != 0) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int64_t n = n0 + i * 16 + grp * 4;
+      if (n >= cols) continue;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const int64_t m = m0 + j * 16 + col;
+        if (m >= rows) continue;
+        const float v[4] = {acc[i][j][0] + b[i][0], acc[i][j][1] + b[i][1], acc[i][j][2] + b[i][2],
+                            acc[i][j][3] + b[i][3]};
+        store_quad(out + m * cols + n, n, cols, v);
+      }
+    }
+    return;
+  }
+  constexpr int LT = kLineTiles<T, NT>, kRow = kLineBytes<T, NT>;
+  constexpr int kChunks = LT * 16 * (int)sizeof(T) / 16, kLaneRows = kWave / kChunks;
+  const int chunk = lane % kChunks, first = lane / kChunks;
+#pragma unroll
+  for (int j0 = 0; j0 < MT; j0 += GROUP) {
+#pragma unroll
+    for (int i0 = 0; i0 < NT; i0 += LT) {
+#pragma unroll
+      for (int j = j0; j < j0 + GROUP; ++j) {
+#pragma unroll
+        for (int i = i0; i < i0 + LT; ++i) {
+          const float v[4] = {acc[i][j][0] + b[i][0], acc[i][j][1] + b[i][1], acc[i][j][2] + b[i][2],
+                              acc[i][j][3] + b[i][3]};
+          store_raw<T, 4>(reinterpret_cast<T*>(lds + ((j - j0) * 16 + col) * kRow) + (i - i0) * 16 + grp * 4, v);
+        }
+      }
+      wave_lds_sync();
+      const int64_t n = n0 + i0 * 16 + chunk * (16 / (int)sizeof(T));
+#pragma unroll
+      for (int r = 0; r < GROUP * 16; r += kLaneRows) {
+        const int64_t m = m0 + j0 * 16 + r + first;
+        const uint4 v = *reinterpret_cast<const uint4*>(lds + (r + first) * kRow + chunk * 16);
+        if (m < rows && n < cols) *reinterpret_cast<uint4*>(out + m * cols + n) = v;
+      }
+      wave_lds_sync();
+    }
+  }
 }
 
 // Two elements of e4m3 or e2m1 as bf16, times the run's scale: one instruction.
@@ -386,13 +454,6 @@ __global__ __launch_bounds__(512, 2) void mx_wide_kernel(MixedArgs g) {
     return make_rsrc(static_cast<const char*>(base) + skip, (uint32_t)max((int64_t)0, min(end - skip, (int64_t)0x7FFFFFFF)));
   };
   auto load = [&](int s) {
-    // (strides that the compiler takes for new in every slice: it would keep the offsets
-    // of all units in registers that the operands need)
-    const auto fresh = [](int64_t v) {
-      uint32_t x = (uint32_t)v;
-      asm volatile("" : "+s"(x));
-      return x;
-    };
     const int64_t r0 = rbeg + (int64_t)s * SLICE;
     const int left = (int)max((int64_t)0, min((int64_t)SLICE, rend - r0));  // of r in the slice
     const uint32_t skip = uunit * 8 < left ? 0u : kOobOffset;               // of a unit along r
@@ -506,25 +567,16 @@ __global__ __launch_bounds__(512, 2) void mx_wide_kernel(MixedArgs g) {
     half(next, 0, [](int) {});
   }
 
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int64_t n = n0 + wn * 64 + i * 16 + grp * 4;
-    if (n >= g.n) continue;
-    float bias[4] = {0.f, 0.f, 0.f, 0.f};
-    if (P == kForward && g.out) load_bias(static_cast<const bf16_t*>(g.bias), n, g.n, bias);
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const int64_t m = m0 + wm * 128 + j * 16 + col;
-      if (m >= g.m) continue;
-      if (g.out) {
-        const float v[4] = {acc[i][j][0] + bias[0], acc[i][j][1] + bias[1], acc[i][j][2] + bias[2],
-                            acc[i][j][3] + bias[3]};
-        store_quad(static_cast<bf16_t*>(g.out) + m * g.n + n, n, g.n, v);
-      } else {
-        *reinterpret_cast<floatx4*>(g.partial + ((int64_t)at.split * g.m + m) * g.ldp + n) = acc[i][j];
-      }
-    }
-  }
+  constexpr int kWaveBytes = 2 * kStage * (int)sizeof(bf16_t) / 8;
+  static_assert(64 * kLineBytes<float, NT> <= kWaveBytes && 64 * kLineBytes<bf16_t, NT> <= kWaveBytes, "a wave's part of LDS");
+  uint8_t* const lds = reinterpret_cast<uint8_t*>(smem) + wave * kWaveBytes;
+  __syncthreads();  // LDS is used anew
+  if (g.out)
+    store_tile<bf16_t, MT, NT, 4>(acc, lds, P == kForward ? static_cast<const bf16_t*>(g.bias) : nullptr,
+                                  static_cast<bf16_t*>(g.out), m0 + wm * 128, n0 + wn * 64, g.m, g.n, lane);
+  else
+    store_tile<float, MT, NT, 4>(acc, lds, nullptr, g.partial + (int64_t)at.split * g.m * g.ldp, m0 + wm * 128,
+                                 n0 + wn * 64, g.m, g.ldp, lane);
 }
 
 // The splits' sums in order, rounded once.  One thread four elements of a row.
@@ -887,20 +939,12 @@ __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_linear_kernel(LinearArgs 
     });
   }
 
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int64_t n = n0 + wn * (TN / WN) + i * 16 + grp * 4;
-    if (n >= g.n) continue;
-    float b[4];
-    load_bias(static_cast<const T*>(g.bias), n, g.n, b);
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const int64_t m = m0 + wm * (TM / WM) + j * 16 + col;
-      if (m >= g.m) continue;
-      const float v[4] = {acc[i][j][0] + b[0], acc[i][j][1] + b[1], acc[i][j][2] + b[2], acc[i][j][3] + b[3]};
-      store_quad(static_cast<T*>(g.y) + m * g.n + n, n, g.n, v);
-    }
-  }
+  constexpr int kWaveBytes = 2 * kStage / WAVES, GROUP = MT < 4 ? MT : 4;
+  static_assert(GROUP * 16 * kLineBytes<T, NT> <= kWaveBytes, "a wave's part of LDS");
+  wait_loads();     // those past the last step too:
+  __syncthreads();  // LDS is used anew
+  store_tile<T, MT, NT, GROUP>(acc, smem + wave * kWaveBytes, static_cast<const T*>(g.bias), static_cast<T*>(g.y),
+                               m0 + wm * (TM / WM), n0 + wn * (TN / WN), g.m, g.n, lane);
 }
 
 // W's scales with rows of whole steps, 2^0 past their ends: for weights whose rows are not.

@@ -37,9 +37,39 @@ struct UnitPlace {
 
 constexpr float kRsqrt2 = 0.70710678118654752f, kRsqrt2Pi = 0.39894228040143268f;
 
-__device__ __forceinline__ float gelu_f(float x) { return 0.5f * x * (1.0f + erff(x * kRsqrt2)); }
+// Phi(x), and phi(x) sqrt(2 pi) where the slope needs it.  fp32 takes the library's error
+// function.  Half precision has less time for it (one element's error function and
+// exponential cost as much as its bytes: 8,192 x 2,048 bf16 forward 19.0 and backward 24.8
+// us), and takes the tail of the distribution, which keeps its digits on both sides:
+//   Phi(-|x|) = exp(-x^2 / 2) t Q(t) / 2,  t = 1 / (1 + |x| / sqrt 8)
+// with Q the polynomial of degree 8 whose t Q(t) is nearest to exp(z^2) erfc(z), z =
+// |x| / sqrt 2, in relative terms for z up to 10 (off by 5e-8, and 3e-7 as computed).
+template <typename T>
+__device__ __forceinline__ float normal_cdf(float x, float& dense) {
+  if constexpr (sizeof(T) == 4) {
+    dense = expf(-0.5f * x * x);
+    return 0.5f * (1.0f + erff(x * kRsqrt2));
+  } else {
+    dense = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
+    const float t = __builtin_amdgcn_rcpf(1.0f + fabsf(x) * (0.5f * kRsqrt2));
+    constexpr float q[9] = {0.282086432f, 0.282375246f, 0.243104205f, 0.202685177f, -0.0266217813f, 0.278061688f, -0.487195253f, 0.28457278f, -0.0590685233f};
+    float p = q[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) p = p * t + q[i];
+    const float tail = 0.5f * dense * t * p;
+    return x < 0.f ? tail : 1.0f - tail;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float gelu_f(float x) {
+  float dense;
+  return x * normal_cdf<T>(x, dense);
+}
+template <typename T>
 __device__ __forceinline__ float gelu_slope(float x) {
-  return 0.5f * (1.0f + erff(x * kRsqrt2)) + x * (kRsqrt2Pi * expf(-0.5f * x * x));
+  float dense;
+  const float cdf = normal_cdf<T>(x, dense);
+  return cdf + x * (kRsqrt2Pi * dense);
 }
 
 template <typename T, int FORM, bool PACKED>
@@ -75,7 +105,7 @@ __global__ __launch_bounds__(256) void gelu_forward_kernel(UnitArgs a) {
     mx_store<kE4m3>(a.codes, a.scales, at.unit, code, s);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = gelu_f(v[i]);
+  for (int i = 0; i < 8; ++i) v[i] = gelu_f<T>(v[i]);
   store_unit<T, PACKED>(static_cast<T*>(a.y) + at.row * a.dim, at.e, a.dim, v);
 }
 
@@ -88,7 +118,7 @@ __global__ __launch_bounds__(256) void gelu_backward_kernel(UnitArgs a) {
   load_unit<T, PACKED>(static_cast<const T*>(a.x) + at.row * a.dim, at.e, a.dim, g);
   mx_load<kE4m3>(a.codes, a.scales, at.unit, v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) g[i] *= gelu_slope(v[i]);
+  for (int i = 0; i < 8; ++i) g[i] *= gelu_slope<T>(v[i]);
   store_unit<T, PACKED>(static_cast<T*>(a.y) + at.row * a.dim, at.e, a.dim, g);
 }
 

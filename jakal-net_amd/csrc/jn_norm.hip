@@ -178,11 +178,24 @@ __device__ __forceinline__ void load_row(const NormArgs& a, int64_t row, Raw<T, 
   load_row<T, W, NP, G>(a.x, row, a, raw);
 }
 
+// A value from another lane, both its words moved alike.
+template <typename F>
+__device__ __forceinline__ double moved(double v, F move) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint64_t lo = (uint32_t)move((int)(uint32_t)u), hi = (uint32_t)move((int)(uint32_t)(u >> 32));
+  return __builtin_bit_cast(double, lo | hi << 32);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_64(double v) {
+  return moved(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, true); });
+}
+
 // The sum of a value over each group of TH threads in 64 bits, in all of them.
 template <int TH, int BLOCK>
 __device__ __forceinline__ double group_sum_64(double v, double* lds) {
-#pragma unroll
-  for (int i = 1; i < (TH < kWave ? TH : kWave); i *= 2) v += __shfl_xor(v, i);
+  v += dpp_64<0xB1>(v), v += dpp_64<0x4E>(v), v += dpp_64<0x141>(v), v += dpp_64<0x140>(v);  // sixteen lanes
+  if constexpr (TH >= 32) v += moved(v, [](int x) { return xor16_i(x); });
+  if constexpr (TH >= 64) v += moved(v, [](int x) { return xor32_i(x); });
   if constexpr (TH > kWave) {
     constexpr int kWaves = TH / kWave;
     __syncthreads();  // the readers before are done

@@ -123,11 +123,18 @@ __device__ __forceinline__ shortx4 read_tr(const bf16_t* p) {
       (__attribute__((address_space(3))) shortx4*)(const_cast<bf16_t*>(p)));
 }
 
-// The wide kernel's [r][256]: rows of 32 bytes more, and 128 more every eight rows, so
+// The bf16 kernel's [r][WIDTH]: rows of 32 bytes more, and 128 more every eight rows, so
 // that four rows and those eight further on fall on different banks.  Sums of what a row
 // and a column add, where a permutation would take an address for every tile.
-constexpr int kPadRow = 256 + 16, kPadEight = 64, kPadPlane = 64 * kPadRow + 8 * kPadEight;
-__device__ __forceinline__ int lds_pad(int r, int c) { return r * kPadRow + (r >> 3) * kPadEight + c; }
+constexpr int kPadEight = 64;
+template <int WIDTH>
+constexpr int kPadRow = WIDTH + 16;
+template <int WIDTH>
+constexpr int kPadPlane = 64 * kPadRow<WIDTH> + 8 * kPadEight;
+template <int WIDTH>
+__device__ __forceinline__ int lds_pad(int r, int c) {
+  return r * kPadRow<WIDTH> + (r >> 3) * kPadEight + c;
+}
 
 // Eight consecutive r from r0 on of column c16 * 16 + (lane & 15), for lane group g: r0 = 8 g.
 template <int WIDTH>
@@ -413,27 +420,29 @@ __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_mixed_kernel(MixedArgs g)
   }
 }
 
-// The same for bf16 A with rows of whole, aligned 16-byte packs, where the output has
-// wide tiles enough: 256 x 256 over 2 x 4 waves.  A slice is two half steps of 32 r.  Its
-// operands are read from LDS while the half step before is multiplied, each as soon as
-// its register is free; the slice after lies in registers by then and goes to the other
-// stage meanwhile, and the one after that is on its way from memory.  B may be plain bf16
-// too (kPlainGrad: a linear layer's input gradient).
-template <Product P>
-__global__ __launch_bounds__(512, 2) void mx_wide_kernel(MixedArgs g) {
+// The same for bf16 A with rows of whole, aligned 16-byte packs: tiles of TM x TN over
+// WM x WN waves.  A slice is two half steps of 32 r.  Its operands are read from LDS while
+// the half step before is multiplied, each as soon as its register is free; the slice
+// after lies in registers by then and goes to the other stage meanwhile, and AHEAD slices
+// after that are on their way from memory.  B may be plain bf16 too (kPlainGrad: a linear
+// layer's input gradient).
+template <Product P, int TM, int TN, int WM, int WN, int AHEAD>
+__global__ __launch_bounds__(WM* WN* kWave, 2) void mx_bf16_kernel(MixedArgs g) {
   constexpr int FORM = P == kWeightGrad ? kE4m3 : kE2m1;
   constexpr bool A_R = P != kWeightGrad, B_R = P == kForward, B_PLAIN = P == kPlainGrad;
-  constexpr int TILE = 256, SLICE = 64, U = TILE * SLICE / 8 / 512;  // units of eight elements a thread
-  constexpr int kA = A_R ? TILE * SLICE : kPadPlane, kB = B_R ? TILE * SLICE : kPadPlane, kStage = kA + kB;
-  constexpr int MT = 8, NT = 4;
-  static_assert(U == NT, "a unit is stored after each row of products");
+  // sums of A over r, where there are registers for them
+  constexpr bool SUMS = P == kWeightGrad && TM < 256;
+  constexpr int SLICE = 64, THREADS = WM * WN * kWave;
+  constexpr int UA = TM * SLICE / 8 / THREADS, UB = TN * SLICE / 8 / THREADS;  // units of eight elements a thread
+  constexpr int kA = A_R ? TM * SLICE : kPadPlane<TM>, kB = B_R ? TN * SLICE : kPadPlane<TN>, kStage = kA + kB;
+  constexpr int MT = TM / WM / 16, NT = TN / WN / 16;
   __shared__ __align__(16) bf16_t smem[2 * kStage];
 
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
   const int grp = lane >> 4, col = lane & 15;
-  const int wm = wave >> 2, wn = wave & 3;
+  const int wm = wave / WN, wn = wave % WN;
   const TilePlace at(g.tiles_m, g.tiles_n);
-  const int64_t m0 = (int64_t)at.mi * TILE, n0 = (int64_t)at.ni * TILE;
+  const int64_t m0 = (int64_t)at.mi * TM, n0 = (int64_t)at.ni * TN;
   const int64_t rbeg = at.split * g.chunk, rend = min(g.r, rbeg + g.chunk);
   const int slices = rend > rbeg ? (int)((rend - rbeg + SLICE - 1) / SLICE) : 0;
 
@@ -441,34 +450,37 @@ __global__ __launch_bounds__(512, 2) void mx_wide_kernel(MixedArgs g) {
   // What lies past the last row, or past r's end, is out of range and reads as zeros; m
   // and n past the end within rows of r are the next row's numbers (their outputs are
   // not written).
-  constexpr int UR = SLICE / 8, UT = TILE / 8;  // units of a row along r, and across
-  const int urow = tid / UR, uunit = tid % UR, trow = tid / UT, tunit = tid % UT;
-  constexpr int kStepR = 512 / UR, kStepT = 512 / UT;
-  uint4 ra[U];
-  u32x4_nt rb[U];
-  uint32_t rs[U];
+  constexpr int UR = SLICE / 8, UTA = TM / 8, UTB = TN / 8;  // units of a row along r, and across
+  const int urow = tid / UR, uunit = tid % UR;
+  const int arow = tid / UTA, aunit = tid % UTA, brow = tid / UTB, bunit = tid % UTB;
+  constexpr int kStepR = THREADS / UR, kStepA = THREADS / UTA, kStepB = THREADS / UTB;
+  struct Slice {
+    uint4 a[UA];
+    u32x4_nt b[UB];
+    uint32_t s[UB];
+  } held[AHEAD];
   // `first`: the operand's first row and first unit here, `bytes` a row's, `unit` a unit's
   const auto place = [&](bool rows_r, const void* base, int64_t rows, int64_t first, int64_t c, int64_t bytes, int left) {
     const int64_t skip = first * bytes + c;
     const int64_t end = rows_r ? rows * bytes : min(rows, first + left) * bytes;
     return make_rsrc(static_cast<const char*>(base) + skip, (uint32_t)max((int64_t)0, min(end - skip, (int64_t)0x7FFFFFFF)));
   };
-  auto load = [&](int s) {
+  auto load = [&](int s, Slice& to) {
     const int64_t r0 = rbeg + (int64_t)s * SLICE;
     const int left = (int)max((int64_t)0, min((int64_t)SLICE, rend - r0));  // of r in the slice
     const uint32_t skip = uunit * 8 < left ? 0u : kOobOffset;               // of a unit along r
     const auto rsa = A_R ? place(true, g.a, g.m, m0, r0 * 2, g.lda * 2, left) : place(false, g.a, g.r, r0, m0 * 2, g.lda * 2, left);
     const uint32_t lda = fresh(g.lda * 2);
-    const uint32_t oa = A_R ? (uint32_t)urow * lda + uunit * 16 + skip : (uint32_t)trow * lda + tunit * 16;
+    const uint32_t oa = A_R ? (uint32_t)urow * lda + uunit * 16 + skip : (uint32_t)arow * lda + aunit * 16;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      ra[u] = __builtin_bit_cast(
-          uint4, __builtin_amdgcn_raw_buffer_load_b128(rsa, oa + u * (A_R ? kStepR : kStepT) * lda, 0, 0));
+    for (int u = 0; u < UA; ++u)
+      to.a[u] = __builtin_bit_cast(
+          uint4, __builtin_amdgcn_raw_buffer_load_b128(rsa, oa + u * (A_R ? kStepR : kStepA) * lda, 0, 0));
     if constexpr (B_PLAIN) {
-      const uint32_t ldb = fresh(g.n * 2), ob = (uint32_t)trow * ldb + tunit * 16;
+      const uint32_t ldb = fresh(g.n * 2), ob = (uint32_t)brow * ldb + bunit * 16;
       const auto rsb = place(false, g.codes, g.r, r0, n0 * 2, g.n * 2, left);
 #pragma unroll
-      for (int u = 0; u < U; ++u) rb[u] = __builtin_amdgcn_raw_buffer_load_b128(rsb, ob + u * kStepT * ldb, 0, 0);
+      for (int u = 0; u < UB; ++u) to.b[u] = __builtin_amdgcn_raw_buffer_load_b128(rsb, ob + u * kStepB * ldb, 0, 0);
     } else {
       constexpr int UNIT = FORM == kE4m3 ? 8 : 4;  // bytes of a unit's codes
       const uint32_t pitch = fresh(g.pitch), runs = fresh(g.runs);
@@ -476,56 +488,68 @@ __global__ __launch_bounds__(512, 2) void mx_wide_kernel(MixedArgs g) {
                            : place(false, g.codes, g.r, r0, n0 / 8 * UNIT, g.pitch, left);
       const auto rss = B_R ? place(true, g.scales, g.n, n0, r0 / kMxRun, g.runs, left)
                            : place(false, g.scales, g.r, r0, n0 / kMxRun, g.runs, left);
-      const uint32_t ob = B_R ? (uint32_t)urow * pitch + uunit * UNIT + skip : (uint32_t)trow * pitch + tunit * UNIT;
-      const uint32_t os = B_R ? (uint32_t)urow * runs + uunit / 4 + skip : (uint32_t)trow * runs + tunit / 4;
+      const uint32_t ob = B_R ? (uint32_t)urow * pitch + uunit * UNIT + skip : (uint32_t)brow * pitch + bunit * UNIT;
+      const uint32_t os = B_R ? (uint32_t)urow * runs + uunit / 4 + skip : (uint32_t)brow * runs + bunit / 4;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t step = u * (B_R ? kStepR : kStepT);
+      for (int u = 0; u < UB; ++u) {
+        const uint32_t step = u * (B_R ? kStepR : kStepB);
         if constexpr (FORM == kE4m3) {
           const auto v = __builtin_amdgcn_raw_buffer_load_b64(rsb, ob + step * pitch, 0, 0);
-          rb[u][0] = v[0], rb[u][1] = v[1];
+          to.b[u][0] = v[0], to.b[u][1] = v[1];
         } else {
-          rb[u][0] = __builtin_amdgcn_raw_buffer_load_b32(rsb, ob + step * pitch, 0, 0);
+          to.b[u][0] = __builtin_amdgcn_raw_buffer_load_b32(rsb, ob + step * pitch, 0, 0);
         }
-        rs[u] = __builtin_amdgcn_raw_buffer_load_b8(rss, os + step * runs, 0, 0);
+        to.s[u] = __builtin_amdgcn_raw_buffer_load_b8(rss, os + step * runs, 0, 0);
       }
     }
   };
   // (a unit's row is a whole number of eight rows and of the chunks' permutation further on)
-  const int along = lds_kc<SLICE>(urow, uunit), across = lds_pad(trow, tunit * 8);
-  constexpr int kAlong = kStepR * SLICE, kAcross = kStepT * kPadRow + kStepT / 8 * kPadEight;
-  static_assert(kStepR % 16 == 0 && kStepT % 8 == 0, "a unit's place is the first one's and a constant");
-  auto store = [&](int stage, int u) {
-    *reinterpret_cast<uint4*>(smem + stage + (A_R ? along + u * kAlong : across + u * kAcross)) = ra[u];
+  const int along = lds_kc<SLICE>(urow, uunit);
+  const int aplace = A_R ? along : lds_pad<TM>(arow, aunit * 8), bplace = B_R ? along : lds_pad<TN>(brow, bunit * 8);
+  constexpr int kNextA = A_R ? kStepR * SLICE : kStepA * kPadRow<TM> + kStepA / 8 * kPadEight;
+  constexpr int kNextB = B_R ? kStepR * SLICE : kStepB * kPadRow<TN> + kStepB / 8 * kPadEight;
+  static_assert(kStepR % 16 == 0 && kStepA % 8 == 0 && kStepB % 8 == 0, "a unit's place is the first one's and a constant");
+  float total[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto store_a = [&](int stage, int u, const Slice& from) {
+    *reinterpret_cast<uint4*>(smem + stage + aplace + u * kNextA) = from.a[u];
+    if constexpr (SUMS) {
+      const auto v = __builtin_bit_cast(bf16x8v, from.a[u]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) total[j] += (float)v[j];
+    }
+  };
+  auto store_b = [&](int stage, int u, const Slice& from) {
+    const u32x4_nt b = from.b[u];
     uint4 d;
     if constexpr (B_PLAIN) {
-      d = make_uint4(rb[u][0], rb[u][1], rb[u][2], rb[u][3]);
+      d = make_uint4(b[0], b[1], b[2], b[3]);
     } else {
-      const float scale = mx_scale((int)rs[u]);
+      const float scale = mx_scale((int)from.s[u]);
       if constexpr (FORM == kE4m3)
-        d = make_uint4(decode_pair<FORM, 0>(rb[u][0], scale), decode_pair<FORM, 1>(rb[u][0], scale),
-                       decode_pair<FORM, 0>(rb[u][1], scale), decode_pair<FORM, 1>(rb[u][1], scale));
+        d = make_uint4(decode_pair<FORM, 0>(b[0], scale), decode_pair<FORM, 1>(b[0], scale),
+                       decode_pair<FORM, 0>(b[1], scale), decode_pair<FORM, 1>(b[1], scale));
       else
-        d = make_uint4(decode_pair<FORM, 0>(rb[u][0], scale), decode_pair<FORM, 1>(rb[u][0], scale),
-                       decode_pair<FORM, 2>(rb[u][0], scale), decode_pair<FORM, 3>(rb[u][0], scale));
+        d = make_uint4(decode_pair<FORM, 0>(b[0], scale), decode_pair<FORM, 1>(b[0], scale),
+                       decode_pair<FORM, 2>(b[0], scale), decode_pair<FORM, 3>(b[0], scale));
     }
-    *reinterpret_cast<uint4*>(smem + stage + kA + (B_R ? along + u * kAlong : across + u * kAcross)) = d;
+    *reinterpret_cast<uint4*>(smem + stage + kA + bplace + u * kNextB) = d;
   };
 
   bf16x8v a[MT], b[NT];  // one half step's operands
   // one address an operand and constants: sixteen rows further on the chunks are permuted
   // alike, and the other half step's are four chunks further on
-  const auto read = [&](bool rows_r, int origin, int base, int k, int t) -> bf16x8v {
+  const auto read = [&](bool rows_r, int row, int origin, int base, int k, int t) -> bf16x8v {
     if (rows_r) return *reinterpret_cast<const bf16x8v*>(smem + origin + (base ^ (32 * k)) + t * 16 * SLICE);
-    const bf16_t* p = smem + origin + base + k * (32 * kPadRow + 4 * kPadEight) + t * 16;
-    const shortx4 lo = read_tr(p), hi = read_tr(p + 4 * kPadRow);
+    const bf16_t* p = smem + origin + base + k * (32 * row + 4 * kPadEight) + t * 16;
+    const shortx4 lo = read_tr(p), hi = read_tr(p + 4 * row);
     typedef short shortx8 __attribute__((ext_vector_type(8)));
     return __builtin_bit_cast(bf16x8v, (shortx8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  const int abase = A_R ? lds_kc<SLICE>(wm * 128 + col, grp) : lds_pad(grp * 8 + (col >> 2), wm * 128 + (col & 3) * 4);
-  const int bbase = B_R ? lds_kc<SLICE>(wn * 64 + col, grp) : lds_pad(grp * 8 + (col >> 2), wn * 64 + (col & 3) * 4);
-  auto read_a = [&](int stage, int k, int j) { a[j] = read(A_R, stage, abase, k, j); };
-  auto read_b = [&](int stage, int k, int i) { b[i] = read(B_R, stage + kA, bbase, k, i); };
+  const int am = wm * (TM / WM), bn = wn * (TN / WN);  // the wave's part of the tile
+  const int abase = A_R ? lds_kc<SLICE>(am + col, grp) : lds_pad<TM>(grp * 8 + (col >> 2), am + (col & 3) * 4);
+  const int bbase = B_R ? lds_kc<SLICE>(bn + col, grp) : lds_pad<TN>(grp * 8 + (col >> 2), bn + (col & 3) * 4);
+  auto read_a = [&](int stage, int k, int j) { a[j] = read(A_R, kPadRow<TM>, stage, abase, k, j); };
+  auto read_b = [&](int stage, int k, int i) { b[i] = read(B_R, kPadRow<TN>, stage + kA, bbase, k, i); };
   floatx4 acc[NT][MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -545,38 +569,73 @@ __global__ __launch_bounds__(512, 2) void mx_wide_kernel(MixedArgs g) {
     }
   };
 
-  if (slices > 0) {
-    load(0);
+  // Slice s, whose first operands are in registers; the slice after it, on hand in `after`.
+  auto step = [&](int s, int cur, int next, Slice& after) {
+    half(cur, 1, [&](int i) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) store(0, u);
-    load(1);
+      for (int u = i * UA / NT; u < (i + 1) * UA / NT; ++u) store_a(next, u, after);
+#pragma unroll
+      for (int u = i * UB / NT; u < (i + 1) * UB / NT; ++u) store_b(next, u, after);
+    });
+    load(s + 1 + AHEAD, after);  // (nothing past the last)
+    // every wave has this slice's operands in registers, and has stored its part of the next
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    half(next, 0, [](int) {});
+  };
+  if (slices > 0) {
+    load(0, held[0]);
+#pragma unroll
+    for (int u = 0; u < UA; ++u) store_a(0, u, held[0]);
+#pragma unroll
+    for (int u = 0; u < UB; ++u) store_b(0, u, held[0]);
+#pragma unroll
+    for (int i = 1; i <= AHEAD; ++i) load(i, held[i % AHEAD]);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < MT; ++j) read_a(0, 0, j);
 #pragma unroll
     for (int i = 0; i < NT; ++i) read_b(0, 0, i);
   }
-  for (int s = 0; s < slices; ++s) {
-    const int cur = (s & 1) * kStage, next = kStage - cur;
-    half(cur, 1, [&](int i) { store(next, i); });
-    load(s + 2);  // (nothing past the last)
-    // every wave has this slice's operands in registers, and has stored its part of the next
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    half(next, 0, [](int) {});
+  if constexpr (AHEAD == 1) {
+    for (int s = 0; s < slices; ++s) step(s, (s & 1) * kStage, kStage - (s & 1) * kStage, held[0]);
+  } else {
+    static_assert(AHEAD % 2 == 0, "a slice's stage is its number's parity");
+    for (int s = 0; s < slices; s += AHEAD) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        if (s + i < slices) step(s + i, (i & 1) * kStage, kStage - (i & 1) * kStage, held[(i + 1) % AHEAD]);
+      }
+    }
   }
 
-  constexpr int kWaveBytes = 2 * kStage * (int)sizeof(bf16_t) / 8;
-  static_assert(64 * kLineBytes<float, NT> <= kWaveBytes && 64 * kLineBytes<bf16_t, NT> <= kWaveBytes, "a wave's part of LDS");
+  constexpr int kWaveBytes = 2 * kStage * (int)sizeof(bf16_t) / (WM * WN);
+  constexpr int GROUP = MT < 4 ? MT : 4;
+  static_assert(GROUP * 16 * kLineBytes<float, NT> <= kWaveBytes && GROUP * 16 * kLineBytes<bf16_t, NT> <= kWaveBytes,
+                "a wave's part of LDS");
   uint8_t* const lds = reinterpret_cast<uint8_t*>(smem) + wave * kWaveBytes;
   __syncthreads();  // LDS is used anew
   if (g.out)
-    store_tile<bf16_t, MT, NT, 4>(acc, lds, P == kForward ? static_cast<const bf16_t*>(g.bias) : nullptr,
-                                  static_cast<bf16_t*>(g.out), m0 + wm * 128, n0 + wn * 64, g.m, g.n, lane);
+    store_tile<bf16_t, MT, NT, GROUP>(acc, lds, P == kForward ? static_cast<const bf16_t*>(g.bias) : nullptr,
+                                  static_cast<bf16_t*>(g.out), m0 + am, n0 + bn, g.m, g.n, lane);
   else
-    store_tile<float, MT, NT, 4>(acc, lds, nullptr, g.partial + (int64_t)at.split * g.m * g.ldp, m0 + wm * 128,
-                                 n0 + wn * 64, g.m, g.ldp, lane);
+    store_tile<float, MT, NT, GROUP>(acc, lds, nullptr, g.partial + (int64_t)at.split * g.m * g.ldp, m0 + am, n0 + bn,
+                                 g.m, g.ldp, lane);
+  if constexpr (SUMS) {  // the threads that had the same eight columns, in order
+    if (!g.bias_partial || at.ni != 0) return;
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sums[arow * TM + aunit * 8 + j] = total[j];
+    __syncthreads();
+    if (tid < TM && m0 + tid < g.m) {
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < kStepA; ++i) t += sums[i * TM + tid];
+      g.bias_partial[(int64_t)at.split * g.m + m0 + tid] = t;
+    }
+  }
 }
 
 // The splits' sums in order, rounded once.  One thread four elements of a row.
@@ -665,48 +724,61 @@ int launch_column_sums(const void* x, int64_t rows, int64_t dim, float* partial,
   return kOk;
 }
 
-// Splits of the narrow tiles' sum by what they were measured to cost: a slice's time with
-// one workgroup on a CU and with two, and for more than one split a second launch and the
-// partial sums' way to memory and back (in us).
-int64_t narrow_splits(int32_t type, int64_t outputs, int64_t tiles, int64_t slices) {
-  const double one = type == kTypeBf16 ? 1.2 : 1.3, two = type == kTypeF32 ? 2.2 : type == kTypeF16 ? 1.9 : 1.5;
-  int64_t best = 1;
-  double least = 0.0;
-  for (int64_t s = 1; s <= std::min<int64_t>(64, slices); ++s) {
-    const int64_t groups = tiles * s, each = (slices + s - 1) / s;
-    const double time = (groups <= 256 ? one : two * (double)((groups + 511) / 512)) * (double)each +
-                        (s > 1 ? 4.0 + (double)s * (double)outputs * 8.0 / 6e6 : 0.0);
-    if (s == 1 || time < least) best = s, least = time;
-  }
-  return best;
+// Tiles of a product's output and splits of its sum by what they were measured to cost (in
+// us): a slice's time by how many workgroups a CU has, and for more than one split a second
+// launch and the partial sums' way to memory and back.
+struct TileCost {
+  int m, n;
+  double least, first, each;  // of a slice: max(least, first + each * workgroups a CU)
+};
+// bf16 rows of whole packs (mx_bf16_kernel).  Wide tiles feed the matrix units, narrow ones
+// keep more CUs busy and cost less each: 128 x 2,048 x 16,384 forward with tiles of 256 x
+// 256, 128 x 128, 128 x 64 and 64 x 64 55, 29, 23 and 23 us, 512 x 2,048 x 16,384 56, 44, 56
+// and 65 us; the weight gradient of 1,024 x 512 x 2,048 32, 22, 18 and 14 us.
+constexpr TileCost kPackedTiles[] = {
+    {256, 256, 0, 0, 1.6}, {128, 128, 0.85, 0.41, 0.44}, {128, 64, 0.62, 0.1, 0.385}, {64, 64, 0.53, 0.13, 0.235}};
+// others (mx_mixed_kernel)
+constexpr TileCost mixed_tile(int32_t type) {
+  return type == kTypeF32 ? TileCost{128, 128, 1.3, 0.4, 0.9}
+                          : TileCost{128, 128, 1.3, 0.7, type == kTypeF16 ? 0.6 : 0.4};
 }
 
 // Which tiles, and how many splits of the sum.
 struct MixedPlan {
-  int tile, tiles_m, tiles_n, splits;
+  TileCost tile;
+  bool packed;  // mx_bf16_kernel's
+  int tiles_m, tiles_n, splits;
   int64_t chunk, ldp;
   size_t partial_bytes, bias_bytes;
+
+  bool wide() const { return tile.m == 256; }
 
   MixedPlan(Product p, int64_t m, int64_t n, int64_t r, int32_t type, bool bias) {
     // A's rows of whole packs of 16 bytes, and offsets of a tile's rows below 2^31
     const int64_t lda = p == kWeightGrad ? m : r;
-    const bool packed = lda % 8 == 0 && lda < (1 << 21) && n < (1 << 21) && (p != kPlainGrad || n % 8 == 0);
+    packed = type == kTypeBf16 && lda % 8 == 0 && lda < (1 << 21) && n < (1 << 21) && (p != kPlainGrad || n % 8 == 0);
     const int slice = type == kTypeBf16 ? kSlice<bf16_t> : kSlice<float>;
-    const auto tiles = [&](int64_t t) { return (m + t - 1) / t * ((n + t - 1) / t); };
     const int64_t slices = std::max<int64_t>(1, (r + slice - 1) / slice);
-    // wide tiles where they, split at most eight slices deep, keep three quarters of the CUs
-    // busy (one workgroup each)
-    const int64_t deep = std::max<int64_t>(1, std::min<int64_t>({256 / tiles(256), slices / 8, 64}));
-    const bool wide = type == kTypeBf16 && packed && tiles(256) * deep >= 192;
-    tile = wide ? 256 : 128;
-    tiles_m = (int)((m + tile - 1) / tile), tiles_n = (int)((n + tile - 1) / tile);
-    const int64_t want = wide ? deep : narrow_splits(type, m * n, tiles(128), slices);
-    const int64_t each = (slices + want - 1) / want;
-    splits = (int)std::max<int64_t>(1, (slices + each - 1) / each);
-    chunk = each * slice;
+    double least = 1e300;
+    const auto consider = [&](const TileCost& c) {
+      const int64_t tm = (m + c.m - 1) / c.m, tn = (n + c.n - 1) / c.n;
+      for (int64_t want = 1; want <= std::min<int64_t>(64, slices); ++want) {
+        const int64_t each = (slices + want - 1) / want, groups = tm * tn * ((slices + each - 1) / each);
+        const double busy = (double)((groups + 255) / 256);
+        double time = std::max(c.least, c.first + c.each * busy) * (double)each;
+        if (want > 1) time += 4.0 + (double)want * (double)m * (double)n * 8.0 / 6e6;
+        if (bias && c.m == 256) time += 10.0;  // (the wide tiles leave them to launches of their own)
+        if (time >= least) continue;
+        least = time, tile = c, tiles_m = (int)tm, tiles_n = (int)tn, chunk = each * slice;
+        splits = (int)((slices + each - 1) / each);
+      }
+    };
+    if (p == kPlainGrad) consider(kPackedTiles[0]);
+    else if (packed) for (const auto& c : kPackedTiles) consider(c);
+    else consider(mixed_tile(type));
     ldp = (n + 3) / 4 * 4;
     partial_bytes = splits > 1 ? (size_t)splits * m * ldp * sizeof(float) : 0;
-    bias_bytes = bias ? (size_t)(wide ? sum_slabs(r) : splits) * m * sizeof(float) : 0;
+    bias_bytes = bias ? (size_t)(wide() ? sum_slabs(r) : (int64_t)splits) * m * sizeof(float) : 0;
   }
   size_t bytes() const { return (partial_bytes + 255) / 256 * 256 + bias_bytes; }
 };
@@ -715,7 +787,7 @@ template <Product P>
 int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size_t workspace_bytes,
               hipStream_t s) {
   const MixedPlan plan(P, g.m, g.n, g.r, type, g.bias_grad != nullptr);
-  JN_REQUIRE(plan.tile != 256 || aligned16(g.a), kInvalidArgument, "%s: the operand must start on 16 bytes", what);
+  JN_REQUIRE(!plan.packed || aligned16(g.a), kInvalidArgument, "%s: the operand must start on 16 bytes", what);
   JN_REQUIRE(plan.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes()),
              kWorkspaceTooSmall, "%s: needs %zu workspace bytes on a 16-byte address, got %zu", what, plan.bytes(),
              workspace_bytes);
@@ -731,7 +803,7 @@ int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size
   const dim3 grid((unsigned)((int64_t)plan.tiles_m * plan.tiles_n * plan.splits));
   return with_type(type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (plan.tile == 256 && g.bias_grad) {  // (the wide tiles have no registers for them)
+    if (plan.wide() && g.bias_grad) {  // (the wide tiles have no registers for them)
       if (const int rc = launch_column_sums<T>(g.a, g.r, g.m, g.bias_partial, g.bias_grad, s)) return rc;
       g.bias_grad = nullptr, g.bias_partial = nullptr;
     }
@@ -741,10 +813,13 @@ int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size
                  : P == kWeightGrad ? "mx_weight_grad_kernel"
                                     : "linear_input_grad_kernel",
                  s);
-      if (plan.tile == 256) {
-        hipLaunchKernelGGL(mx_wide_kernel<P>, grid, dim3(512), 0, s, g);
+      if (plan.wide()) {
+        hipLaunchKernelGGL((mx_bf16_kernel<P, 256, 256, 2, 4, 1>), grid, dim3(512), 0, s, g);
       } else if constexpr (P != kPlainGrad) {
-        hipLaunchKernelGGL((mx_mixed_kernel<T, P, 128, 128, 2, 2>), grid, dim3(256), 0, s, g);
+        if (!plan.packed) hipLaunchKernelGGL((mx_mixed_kernel<T, P, 128, 128, 2, 2>), grid, dim3(256), 0, s, g);
+        else if (plan.tile.n == 128) hipLaunchKernelGGL((mx_bf16_kernel<P, 128, 128, 2, 2, 2>), grid, dim3(256), 0, s, g);
+        else if (plan.tile.m == 128) hipLaunchKernelGGL((mx_bf16_kernel<P, 128, 64, 2, 2, 2>), grid, dim3(256), 0, s, g);
+        else hipLaunchKernelGGL((mx_bf16_kernel<P, 64, 64, 2, 2, 2>), grid, dim3(256), 0, s, g);
       }
       JN_LAUNCH_CHECK();
     }
@@ -1233,11 +1308,12 @@ int jn_mx_weight_grad(const void* grad_y, const void* codes, const void* scales,
 
 int32_t jn_linear_input_grad_fits(int64_t rows, int64_t dim, int64_t out, int32_t type) {
   if (check_product("linear backward", rows, dim, out, type)) return 0;
-  // Measured with the library's product (us): 1,024 x 2,048 outputs over 16,384 83 and 112,
-  // 32,768 138 and 284, 8,192 60 and 68, 4,096 42 and 35; 512 x 1,024 over 16,384 42 and 65,
-  // 2,048 x 2,048 139 and 146; 4,096 x 2,048 266 and 245, 8,192 x 4,096 over 4,096 250 and 210.
+  // Measured with the library's product (us): 1,024 x 2,048 outputs over 16,384 80 and 112,
+  // 32,768 138 and 284, 8,192 60 and 68, 4,096 42 and 35; 512 x 1,024 over 16,384 39 and 64;
+  // 2,048 x 2,048 over 16,384 139 and 146, 8,192 84 and 77; 4,096 x 2,048 266 and 245.
   const MixedPlan plan(kPlainGrad, rows, dim, out, type, false);
-  return plan.tile == 256 && out >= 8192 && (int64_t)plan.tiles_m * plan.tiles_n <= 64;
+  const int64_t tiles = (int64_t)plan.tiles_m * plan.tiles_n;
+  return plan.packed && out >= std::max<int64_t>(8192, 256 * tiles) && tiles <= 64 && tiles * std::min<int64_t>(64, out / 512) >= 192;
 }
 
 size_t jn_linear_input_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type) {

@@ -204,6 +204,26 @@ def test_products_of_wide_tiles(dev, rows, dim, out):
     _rounded("grad_bias", gb, M.sums(gs), torch.bfloat16)
 
 
+# (tiles of 64 x 64, 128 x 64, 128 x 128 and 256 x 256, each with a whole sum and with a split one)
+@pytest.mark.parametrize("m,n,r", [(72, 72, 72), (72, 72, 520), (200, 16392, 72), (72, 520, 16392), (1544, 2056, 72),
+                                   (72, 1000, 8200), (1000, 8200, 72), (152, 4104, 8200)])
+def test_products_of_every_tile(dev, m, n, r):
+    """bf16 outputs [m, n] of sums over r: forward, input gradient and weight gradient with its bias."""
+    import jakal_net as J
+
+    ops = torch.ops.jakal_net_hip
+    x, g, a = _rand(1, m, r).bfloat16().to(dev), _rand(2, m, r, spread=0.0).bfloat16().to(dev), _rand(4, r, m).bfloat16().to(dev)
+    weight, w = _weight(dev, n, r, 3)
+    b = _rand(3, n, spread=0.0).bfloat16().to(dev)
+    _rounded("y", J.mx_linear(x, weight, b), M.product(x, w.to(dev).t(), b), torch.bfloat16)
+    weight, w = _weight(dev, r, n, 5)
+    _rounded("grad_x", ops.mx_input_grad(g, weight.codes, weight.scales, n), M.product(g, w.to(dev)), torch.bfloat16)
+    kept = _rand(6, r, n).bfloat16()
+    gw, gb = ops.mx_weight_grad(a, *ops.mx_codes(kept.to(dev), 0), n, True)
+    _rounded("grad_weight", gw, M.product(a.t(), M.quantize(kept, "e4m3")[0].to(dev)), torch.bfloat16)
+    _rounded("grad_bias", gb, M.sums(a), torch.bfloat16)
+
+
 @pytest.mark.parametrize("rows", [4096, 10007])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_saved_many_rows(dev, rows, dtype):

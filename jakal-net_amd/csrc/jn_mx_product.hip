@@ -254,6 +254,37 @@ struct Eight {
   }
 };
 
+// Loads straight into LDS, 16 or 4 bytes a lane, at `base` + lane * BYTES.  In assembly,
+// since the compiler would wait for all of them before any later read of LDS: whoever
+// reads waits itself (wait_loads, then the barrier).  They have no result registers.
+typedef __attribute__((address_space(3))) const uint8_t lds_byte;
+typedef int intx4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t lds_offset(const uint8_t* p) { return (uint32_t)(uintptr_t)(lds_byte*)p; }
+
+// The resource over [base, base + bytes), or its first 2^32 - 1 bytes: a tile's rows
+// reach no further.  Empty where bytes is negative.
+__device__ __forceinline__ intx4 rows_rsrc(const uint8_t* base, int64_t bytes) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  return intx4{__builtin_amdgcn_readfirstlane((int)(uint32_t)p),
+               __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xFFFFu)),
+               __builtin_amdgcn_readfirstlane((int)(uint32_t)max((int64_t)0, min(bytes, (int64_t)0xFFFFFFFF))), 0x00020000};
+}
+
+// `base` and the resource are uniform over the wave.
+template <int BYTES>
+__device__ __forceinline__ void load_lds(intx4 rs, uint32_t base, uint32_t offset) {
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(base), "v"(offset), "s"(rs)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(base), "v"(offset), "s"(rs)
+                 : "memory", "m0");
+}
+
+// Until the wave's loads have landed and its reads of LDS are done.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
 // Tiles of TM x TN over WM x WN waves, LDS double buffered with the next slice in registers.
 template <typename T, Product P, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_mixed_kernel(MixedArgs g) {
@@ -638,6 +669,136 @@ __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_bf16_kernel(MixedArgs g) 
   }
 }
 
+// The forward of bf16 x whose rows are whole steps of 128 k, where there are few: tiles of
+// TM x TN over 2 x 2 waves, a column of them half the outputs, a row of them half of each
+// run of 32 k (their sums join at the end).  x, W's codes and scales go straight into LDS,
+// STAGES - 1 steps ahead, and W's are decoded as they are read, so that neither a register
+// nor a wait lies between memory and LDS, and two workgroups fit a CU.  The four bf16
+// operands of a step take k as a run has them: lane group g eight k of run g each.  What
+// bounds it are those loads, at sixteen bytes a clock and CU (33 KB a us).
+template <int TM, int TN, int STAGES>
+__global__ __launch_bounds__(256, 2) void mx_direct_kernel(MixedArgs g) {
+  constexpr int STEP = 128, MT = TM / 16, NT = TN / 32;
+  constexpr int XU = TM / 16, WU = TN / 64;  // 16-byte loads a lane and step, four and sixteen rows each
+  constexpr int kX = TM * STEP * 2, kW = TN * STEP / 2, kS = TN * 4, kStage = kX + kW + kS;
+  constexpr int kLoads = XU + WU + 1;
+  __shared__ __align__(16) uint8_t smem[STAGES * kStage];
+
+  const int lane = lane_id(), wave = wave_id();
+  const int grp = lane >> 4, col = lane & 15;
+  const int wn = wave & 1, half = wave >> 1;
+  const TilePlace at(g.tiles_m, g.tiles_n);
+  const int64_t m0 = (int64_t)at.mi * TM, n0 = (int64_t)at.ni * TN;
+  const int mrows = (int)min((int64_t)TM, g.m - m0), nrows = (int)min((int64_t)TN, g.n - n0);
+  const int64_t rbeg = at.split * g.chunk, rend = min(g.r, rbeg + g.chunk);
+  const int steps = (int)((rend - rbeg) / STEP);
+
+  // A row's sixteen chunks of 16 bytes permuted so that lanes that are read together
+  // (rows 0-3 and 12-15 of one group, 4-11 of the next) fall on all banks.
+  const auto turn = [](int row) { return (row & 11) | (row >> 1 & 4); };
+  const int xrow = wave * 4 + lane / 16, xchunk = (lane % 16) ^ turn(xrow & 15);
+  uint32_t ox[XU];
+#pragma unroll
+  for (int u = 0; u < XU; ++u) ox[u] = (uint32_t)min(u * 16 + xrow, mrows - 1) * (uint32_t)(g.lda * 2) + xchunk * 16;
+  uint32_t ow[WU];
+#pragma unroll
+  for (int u = 0; u < WU; ++u)
+    ow[u] = (uint32_t)min(u * 64 + wave * 16 + lane / 4, nrows - 1) * (uint32_t)g.pitch + lane % 4 * 16;
+  const int srows = wave % WU * 64;
+  const uint32_t os = (uint32_t)min(srows + lane, nrows - 1) * (uint32_t)g.runs;
+  const uint32_t lds = lds_offset(smem);
+  auto load = [&](int step, uint32_t stage) {
+    const int64_t k = rbeg + (int64_t)step * STEP;
+    const bool any = step < steps;  // (nothing past the last)
+    const auto rows = [&](const uint8_t* base, int64_t skip, int64_t end) {
+      return rows_rsrc(base + skip, any ? end - skip : 0);
+    };
+    const auto rx = rows(static_cast<const uint8_t*>(g.a), m0 * g.lda * 2 + k * 2, g.m * g.lda * 2);
+    const auto rw = rows(g.codes, n0 * g.pitch + k / 2, g.n * g.pitch);
+    const auto rs = rows(g.scales, n0 * g.runs + k / kMxRun, g.n * g.runs);
+#pragma unroll
+    for (int u = 0; u < XU; ++u) load_lds<16>(rx, lds + stage + (u * 4 + wave) * 1024, ox[u]);
+#pragma unroll
+    for (int u = 0; u < WU; ++u) load_lds<16>(rw, lds + stage + kX + (u * 4 + wave) * 1024, ow[u]);
+    load_lds<4>(rs, lds + stage + kX + kW + srows * 4, os);  // (every wave, so that each has as many loads)
+  };
+
+  floatx4 acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const int wat = kX + (wn * (TN / 2) + col) * 64 + grp * 16 + half * 8;
+  const int sat = kX + kW + (wn * (TN / 2) + col) * 4 + grp;
+  const int xat[2] = {col * 256 + ((grp * 4 + half * 2) ^ turn(col)) * 16, col * 256 + ((grp * 4 + half * 2 + 1) ^ turn(col)) * 16};
+
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) load(i, i * kStage);
+  uint32_t cur = 0, behind = (STAGES - 1) * kStage;  // the stage of this step, and of the one before
+  for (int s = 0; s < steps; ++s) {
+    // this step's loads have landed and the reads of the one before are done, for all waves
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads * (STAGES - 2)) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    load(s + STAGES - 1, behind);
+    const uint8_t* const stage = smem + cur;
+    uint2 w[NT];
+    float scale[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      w[i] = *reinterpret_cast<const uint2*>(stage + wat + i * 16 * 64);
+      scale[i] = mx_scale(stage[sat + i * 16 * 4]);
+    }
+    bf16x8v x[2][MT];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) x[q][j] = *reinterpret_cast<const bf16x8v*>(stage + xat[q] + j * 16 * 256);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      bf16x8v b[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const uint32_t code = q ? w[i].y : w[i].x;
+        b[i] = __builtin_bit_cast(bf16x8v, make_uint4(decode_pair<kE2m1, 0>(code, scale[i]), decode_pair<kE2m1, 1>(code, scale[i]),
+                                                      decode_pair<kE2m1, 2>(code, scale[i]), decode_pair<kE2m1, 3>(code, scale[i])));
+      }
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[i], x[q][j], acc[i][j], 0, 0, 0);
+      }
+    }
+    behind = cur;
+    cur = cur == (STAGES - 1) * kStage ? 0 : cur + kStage;
+  }
+
+  constexpr int kWaveBytes = NT * MT * kWave * 16, GROUP = 2;
+  static_assert(2 * kWaveBytes <= STAGES * kStage && GROUP * 16 * kLineBytes<float, NT> <= kWaveBytes, "LDS to join in");
+  wait_loads();     // those past the last step too:
+  __syncthreads();  // LDS is used anew
+  uint8_t* const mine = smem + wn * kWaveBytes;
+  if (half == 1) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) *reinterpret_cast<floatx4*>(mine + ((i * MT + j) * kWave + lane) * 16) = acc[i][j];
+  }
+  __syncthreads();
+  if (half == 1) return;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] += *reinterpret_cast<const floatx4*>(mine + ((i * MT + j) * kWave + lane) * 16);
+  wave_lds_sync();
+  if (g.out)
+    store_tile<bf16_t, MT, NT, GROUP>(acc, mine, static_cast<const bf16_t*>(g.bias), static_cast<bf16_t*>(g.out), m0,
+                                      n0 + wn * (TN / 2), g.m, g.n, lane);
+  else
+    store_tile<float, MT, NT, GROUP>(acc, mine, nullptr, g.partial + (int64_t)at.split * g.m * g.ldp, m0, n0 + wn * (TN / 2),
+                                     g.m, g.ldp, lane);
+}
+
 // The splits' sums in order, rounded once.  One thread four elements of a row.
 template <typename T>
 __global__ __launch_bounds__(256) void mx_sum_kernel(MixedArgs g, int splits) {
@@ -730,6 +891,8 @@ int launch_column_sums(const void* x, int64_t rows, int64_t dim, float* partial,
 struct TileCost {
   int m, n;
   double least, first, each;  // of a slice: max(least, first + each * workgroups a CU)
+  int slice = 64;             // of r, for bf16
+  bool direct = false;        // mx_direct_kernel
 };
 // bf16 rows of whole packs (mx_bf16_kernel).  Wide tiles feed the matrix units, narrow ones
 // keep more CUs busy and cost less each: 128 x 2,048 x 16,384 forward with tiles of 256 x
@@ -737,6 +900,10 @@ struct TileCost {
 // and 65 us; the weight gradient of 1,024 x 512 x 2,048 32, 22, 18 and 14 us.
 constexpr TileCost kPackedTiles[] = {
     {256, 256, 0, 0, 1.6}, {128, 128, 0.85, 0.41, 0.44}, {128, 64, 0.62, 0.1, 0.385}, {64, 64, 0.53, 0.13, 0.235}};
+// Forward rows of whole steps of 128 (mx_direct_kernel; the others' least beside it): 128 x
+// 2,048 x 16,384 19 and 23 us, 256 x 2,048 x 16,384 26 and 31, 1,024 x 2,048 x 2,048 18 and
+// 23, 512 x 2,048 x 16,384 48 and 44.
+constexpr TileCost kDirectTiles[] = {{128, 64, 1.0, 0.1, 0.67, 128, true}, {64, 64, 0.62, 0.15, 0.43, 128, true}};
 // others (mx_mixed_kernel)
 constexpr TileCost mixed_tile(int32_t type) {
   return type == kTypeF32 ? TileCost{128, 128, 1.3, 0.4, 0.9}
@@ -757,10 +924,10 @@ struct MixedPlan {
     // A's rows of whole packs of 16 bytes, and offsets of a tile's rows below 2^31
     const int64_t lda = p == kWeightGrad ? m : r;
     packed = type == kTypeBf16 && lda % 8 == 0 && lda < (1 << 21) && n < (1 << 21) && (p != kPlainGrad || n % 8 == 0);
-    const int slice = type == kTypeBf16 ? kSlice<bf16_t> : kSlice<float>;
-    const int64_t slices = std::max<int64_t>(1, (r + slice - 1) / slice);
     double least = 1e300;
     const auto consider = [&](const TileCost& c) {
+      const int slice = type == kTypeBf16 ? c.slice : kSlice<float>;
+      const int64_t slices = std::max<int64_t>(1, (r + slice - 1) / slice);
       const int64_t tm = (m + c.m - 1) / c.m, tn = (n + c.n - 1) / c.n;
       for (int64_t want = 1; want <= std::min<int64_t>(64, slices); ++want) {
         const int64_t each = (slices + want - 1) / want, groups = tm * tn * ((slices + each - 1) / each);
@@ -773,9 +940,12 @@ struct MixedPlan {
         splits = (int)((slices + each - 1) / each);
       }
     };
-    if (p == kPlainGrad) consider(kPackedTiles[0]);
-    else if (packed) for (const auto& c : kPackedTiles) consider(c);
-    else consider(mixed_tile(type));
+    if (!packed) consider(mixed_tile(type));
+    else if (p == kPlainGrad) consider(kPackedTiles[0]);
+    else
+      for (const auto& c : kPackedTiles) consider(c);
+    if (p == kForward && packed && r % 128 == 0)
+      for (const auto& c : kDirectTiles) consider(c);
     ldp = (n + 3) / 4 * 4;
     partial_bytes = splits > 1 ? (size_t)splits * m * ldp * sizeof(float) : 0;
     bias_bytes = bias ? (size_t)(wide() ? sum_slabs(r) : (int64_t)splits) * m * sizeof(float) : 0;
@@ -787,6 +957,8 @@ template <Product P>
 int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size_t workspace_bytes,
               hipStream_t s) {
   const MixedPlan plan(P, g.m, g.n, g.r, type, g.bias_grad != nullptr);
+  JN_REQUIRE(!plan.tile.direct || (reinterpret_cast<uintptr_t>(g.scales) & 3) == 0, kInvalidArgument,
+             "%s: weight scales must start on 4 bytes", what);
   JN_REQUIRE(!plan.packed || aligned16(g.a), kInvalidArgument, "%s: the operand must start on 16 bytes", what);
   JN_REQUIRE(plan.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes()),
              kWorkspaceTooSmall, "%s: needs %zu workspace bytes on a 16-byte address, got %zu", what, plan.bytes(),
@@ -817,7 +989,12 @@ int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size
         hipLaunchKernelGGL((mx_bf16_kernel<P, 256, 256, 2, 4, 1>), grid, dim3(512), 0, s, g);
       } else if constexpr (P != kPlainGrad) {
         if (!plan.packed) hipLaunchKernelGGL((mx_mixed_kernel<T, P, 128, 128, 2, 2>), grid, dim3(256), 0, s, g);
-        else if (plan.tile.n == 128) hipLaunchKernelGGL((mx_bf16_kernel<P, 128, 128, 2, 2, 2>), grid, dim3(256), 0, s, g);
+        else if (plan.tile.direct) {
+          if constexpr (P == kForward) {
+            if (plan.tile.m == 128) hipLaunchKernelGGL((mx_direct_kernel<128, 64, 2>), grid, dim3(256), 0, s, g);
+            else hipLaunchKernelGGL((mx_direct_kernel<64, 64, 3>), grid, dim3(256), 0, s, g);
+          }
+        } else if (plan.tile.n == 128) hipLaunchKernelGGL((mx_bf16_kernel<P, 128, 128, 2, 2, 2>), grid, dim3(256), 0, s, g);
         else if (plan.tile.m == 128) hipLaunchKernelGGL((mx_bf16_kernel<P, 128, 64, 2, 2, 2>), grid, dim3(256), 0, s, g);
         else hipLaunchKernelGGL((mx_bf16_kernel<P, 64, 64, 2, 2, 2>), grid, dim3(256), 0, s, g);
       }
@@ -858,37 +1035,6 @@ __device__ __forceinline__ int lds_row(int row, int chunk) { return row * 128 + 
 
 // An e2m1 operand: four of the instruction's eight words.
 __device__ __forceinline__ intx8 wide(u32x4_nt v) { return intx8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; }
-
-// Loads straight into LDS, 16 or 4 bytes a lane, at `base` + lane * BYTES.  In assembly,
-// since the compiler would wait for all of them before any later read of LDS: whoever
-// reads waits itself (wait_loads, then the barrier).  They have no result registers.
-typedef __attribute__((address_space(3))) const uint8_t lds_byte;
-typedef int intx4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ uint32_t lds_offset(const uint8_t* p) { return (uint32_t)(uintptr_t)(lds_byte*)p; }
-
-// The resource over [base, base + bytes), or its first 2^32 - 1 bytes: a tile's rows
-// reach no further.  Empty where bytes is negative.
-__device__ __forceinline__ intx4 rows_rsrc(const uint8_t* base, int64_t bytes) {
-  const uint64_t p = reinterpret_cast<uint64_t>(base);
-  return intx4{__builtin_amdgcn_readfirstlane((int)(uint32_t)p),
-               __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xFFFFu)),
-               __builtin_amdgcn_readfirstlane((int)(uint32_t)max((int64_t)0, min(bytes, (int64_t)0xFFFFFFFF))), 0x00020000};
-}
-
-// `base` and the resource are uniform over the wave.
-template <int BYTES>
-__device__ __forceinline__ void load_lds(intx4 rs, uint32_t base, uint32_t offset) {
-  if constexpr (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(base), "v"(offset), "s"(rs)
-                 : "memory", "m0");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(base), "v"(offset), "s"(rs)
-                 : "memory", "m0");
-}
-
-// Until the wave's loads have landed and its reads of LDS are done.
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 // Tiles of TM x TN over WM x WN waves in steps of 256 k, LDS double buffered: a step's
 // loads go there directly while the step before is multiplied.  Rows past the operands'
@@ -1261,8 +1407,11 @@ int jn_mx_linear_forward(const void* x, const void* weight_codes, const void* we
   return with_type(type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
     const auto tiles = [&](int64_t tm, int64_t tn) { return (rows + tm - 1) / tm * ((out + tn - 1) / tn); };
-    if (tiles(256, 256) >= 256) return launch_linear<T, 256, 256, 2, 4>(g, s);
-    if (tiles(128, 128) >= 256) return launch_linear<T, 128, 128, 2, 2>(g, s);
+    // The widest tiles that keep three quarters of the CUs busy (bf16, us with tiles of 256,
+    // 128 and 64: 768 x 2,048 x 16,384 28.3, 29.3 and 45.9; 768 x 4,096 x 4,096 38.5, 23.6 and
+    // 28.9; 512 x 4,096 x 4,096 37.9, 22.1 and 20.1; 4,096 x 2,048 x 2,048 30.5, 24.8, 36.7).
+    if (tiles(256, 256) >= 192) return launch_linear<T, 256, 256, 2, 4>(g, s);
+    if (tiles(128, 128) >= 192) return launch_linear<T, 128, 128, 2, 2>(g, s);
     return launch_linear<T, 64, 64, 2, 2>(g, s);
   });
 }

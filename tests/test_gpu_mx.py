@@ -204,9 +204,17 @@ def test_products_of_wide_tiles(dev, rows, dim, out):
     _rounded("grad_bias", gb, M.sums(gs), torch.bfloat16)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,out", [(100, 300, 700), (300, 100, 9000), (600, 72, 20000)])
+def test_mx_linear_every_tile(dev, rows, dim, out, dtype):
+    """Both operands e2m1: tiles of 64, 128 and 256."""
+    _mx_case(dev, rows, dim, out, dtype, "e2m1")
+
+
 # (tiles of 64 x 64, 128 x 64, 128 x 128 and 256 x 256, each with a whole sum and with a split one)
 @pytest.mark.parametrize("m,n,r", [(72, 72, 72), (72, 72, 520), (200, 16392, 72), (72, 520, 16392), (1544, 2056, 72),
-                                   (72, 1000, 8200), (1000, 8200, 72), (152, 4104, 8200)])
+                                   (72, 1000, 8200), (1000, 8200, 72), (152, 4104, 8200), (72, 72, 128), (136, 520, 8192),
+                                   (200, 16390, 256), (1536, 2056, 384)])
 def test_products_of_every_tile(dev, m, n, r):
     """bf16 outputs [m, n] of sums over r: forward, input gradient and weight gradient with its bias."""
     import jakal_net as J

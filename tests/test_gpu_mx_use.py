@@ -450,3 +450,137 @@ def test_head_of_4_bits(dev, activations, monkeypatch):
     again.load_state_dict(state)
     with torch.no_grad():
         assert torch.equal(again.query_logits(again.encode_prefix(prefix), target), logits)
+
+
+@pytest.mark.parametrize("kind", ["cpu", "order", "checkpoint", "reentrant checkpoint"])
+def test_saved_tensors_that_come_back(dev, kind):
+    from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
+    from torch.utils.checkpoint import checkpoint
+
+    leaves, q = _leaves(dev, 40, 96, 64, torch.bfloat16), _frozen(dev, 48, 64)
+    run = lambda *t: sum(o.float().sum() for o in _block(*t, q))
+    want = torch.autograd.grad(run(*leaves), leaves)
+    if kind == "cpu":
+        with save_on_cpu():
+            loss = run(*leaves)
+    elif kind == "order":
+        other = lambda t: t.transpose(0, -1).contiguous().transpose(0, -1) if t.dim() > 1 else t.clone()
+        with saved_tensors_hooks(lambda t: t, other):
+            loss = run(*leaves)
+    else:
+        loss = checkpoint(run, *leaves, use_reentrant=kind.startswith("reentrant"))
+    loss.backward()
+    assert all(torch.equal(p.grad, g) for p, g in zip(leaves, want))
+
+
+def test_captured_training_steps_that_keep_8_bits(dev):
+    """Whole steps (loss, clipping, AdamW under autocast) of two models in two graphs, replayed in turn."""
+    from jakal_net.progressive import train_step
+
+    steps = []
+    for seed in (11, 12):
+        model, batch = _model("e4m3", seed)
+        model = model.to(dev)
+        opt = torch.optim.AdamW(model.parameters(), lr=1e-3, capturable=True)
+        prefix, target = (t.to(dev) for t in batch)
+        cast = dict(device_type="cuda", dtype=torch.bfloat16, cache_enabled=False)
+        steps.append((model, opt, lambda m=model, o=opt, p=prefix, t=target: train_step(m, o, p, t, max_norm=0.1, autocast=cast)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _, _, step in steps:
+            for _ in range(2):
+                step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    tensors = lambda m, o: [p.data for p in m.parameters()] + [v for s in o.state.values() for v in s.values() if torch.is_tensor(v)]
+    kept = [[t.clone() for t in tensors(m, o)] for m, o, _ in steps]
+
+    def restore():
+        for (m, o, _), saved in zip(steps, kept):
+            for t, v in zip(tensors(m, o), saved):
+                t.copy_(v)
+        torch.cuda.synchronize()
+
+    want = []
+    for m, _, step in steps:
+        loss, norm = step()
+        want.append([loss.clone(), norm.clone()] + [p.data.clone() for p in m.parameters()])
+        del loss, norm
+    restore()
+    graphs, outs = [], []
+    for _, _, step in steps:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step())
+    for rep in range(3):
+        restore()
+        for graph in graphs:
+            graph.replay()
+        torch.randn(1 << 20, device=dev).sum()
+        torch.cuda.synchronize()
+        for (m, _, _), (loss, norm), w in zip(steps, outs, want):
+            got = [loss, norm] + [p.data for p in m.parameters()]
+            assert all(torch.equal(a, b) for a, b in zip(got, w)), f"replay {rep}"
+
+
+def test_compiled_training_step(dev):
+    torch._dynamo.reset()
+    model, (prefix, target) = _model("e4m3")
+    model, prefix, target = model.to(dev), prefix.to(dev), target.to(dev)
+    used = list(model.parameters())
+    loss = model(prefix, target)
+    want = torch.autograd.grad(loss, used, allow_unused=True)
+    again = torch.compile(model, backend="aot_eager")(prefix, target)
+    got = torch.autograd.grad(again, used, allow_unused=True)
+    torch._dynamo.reset()
+    # the same kernels between decomposed torch operators: fp32 roundings apart
+    assert float(again.detach()) == pytest.approx(float(loss.detach()), rel=1e-5)
+    # which may move a kept value by a step of its code (2^-3 of itself), in few places
+    for p, a, b in zip(used, want, got):
+        a, b = (torch.zeros_like(p) if t is None else t for t in (a, b))
+        assert float((a - b).norm()) <= 2.0 ** -3 * float(a.norm()) + 1e-7
+
+
+def test_products_past_32_bits(dev):
+    """Outputs and gradients of more than 2^31 elements: the last rows against float64, and sums over all of them."""
+    import jakal_net as J
+
+    rows, dim, out = 140_003, 64, 16_384  # 2.29e9
+    x = torch.empty(rows, dim, device=dev, dtype=torch.bfloat16).normal_().requires_grad_()
+    q = _frozen(dev, out, dim)
+    w = J.mx_dequantize(q).double()
+    for acts in (None, "e2m1"):
+        y = J.mx_linear(x, q, activations=acts)
+        a = x.detach()[-3:].double() if acts is None else M.quantize(x.detach()[-3:], acts)[0].to(dev)
+        value, bound = M.product(a, w.t())
+        O.close(f"{acts} y", y[-3:], value, bound + O.half(torch.bfloat16) * value.abs() + O.floor(torch.bfloat16))
+        del y
+    g = torch.empty(rows, out, device=dev, dtype=torch.bfloat16)
+    for at in range(0, rows, 20_000):
+        g[at:at + 20_000].normal_()
+    gx = torch.ops.jakal_net_hip.mx_input_grad(g, q.codes, q.scales, dim)
+    value, bound = M.product(g[-3:], w)
+    O.close("grad_x", gx[-3:], value, bound + O.half(torch.bfloat16) * value.abs() + O.floor(torch.bfloat16))
+    codes, scales = torch.ops.jakal_net_hip.mx_codes(x.detach(), 0)
+    gw, gb = torch.ops.jakal_net_hip.mx_weight_grad(g, codes, scales, dim, True)
+    some = [0, 5, out - 1]
+    value, bound = M.product(g[:, some].t(), M.quantize(x.detach(), "e4m3")[0].to(dev))
+    O.close("grad_w", gw[some], value, bound + O.half(torch.bfloat16) * value.abs())
+    value, bound = M.sums(g[:, some])
+    O.close("grad_b", gb[some], value, bound + O.half(torch.bfloat16) * value.abs())
+
+
+def test_calls_on_two_streams_at_once(dev):
+    leaves, q = [_leaves(dev, 900, 128, 520, torch.bfloat16, seed=i) for i in range(2)], _frozen(dev, 1000, 520)
+    want = [_step(m, q) for m in leaves]
+    streams = [torch.cuda.Stream() for _ in leaves]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(4):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i] = _step(leaves[i], q)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(s, t) for s, t in zip(a, b))

@@ -1005,8 +1005,9 @@ int jn_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_
  * y [rows, out] = x . W^T + bias with W [out, dim] in JN_E2M1 and x [rows, dim] as
  * it is (activations JN_PLAIN) or microscaled on the way in (JN_E2M1); products are
  * exact, sums fp32, one rounding to `type` (of x, bias and y; bias [out] may be
- * null).  y starts on 16 bytes.
- * grad_x [rows, dim] = grad_y . W: the rounding of x passes the gradient through.
+ * null).  x, the codes and y start on 16 bytes, the scales on 4.
+ * grad_x [rows, dim] = grad_y . W: the rounding of x passes the gradient through;
+ * grad_y, the codes and grad_x start on 16 bytes.
  */
 size_t jn_mx_linear_forward_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t activations);
 int jn_mx_linear_forward(const void* x, const void* weight_codes, const void* weight_scales, const void* bias,
@@ -1021,7 +1022,8 @@ int jn_mx_linear_backward(const void* grad_y, const void* weight_codes, const vo
  * Weight gradient of a linear layer from its input kept in JN_E4M3:
  *   grad_weight [out, dim] = grad_y^T . x,  grad_bias [out] = sum over rows of grad_y
  * grad_y [rows, out], grad_weight and grad_bias (may be null) are of `type`;
- * grad_weight starts on 16 bytes.  Exact products, fp32 sums in a fixed order.
+ * grad_y, the codes and grad_weight start on 16 bytes.  Exact products, fp32 sums in a
+ * fixed order.
  */
 size_t jn_mx_weight_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type, int32_t bias);
 int jn_mx_weight_grad(const void* grad_y, const void* codes, const void* scales, int64_t rows, int64_t dim,

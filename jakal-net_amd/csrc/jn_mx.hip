@@ -72,6 +72,11 @@ __device__ __forceinline__ float gelu_slope(float x) {
   return cdf + x * (kRsqrt2Pi * dense);
 }
 
+// The four below move bytes: a thread has a unit of eight elements, four threads a run,
+// whose largest magnitude meets in the quad's lanes; no LDS, no loop.  16,384 x 2,048 bf16
+// to e2m1 15 us (85 MB, 5.7 TB/s) and back 18.6 (4.6); GELU of 8,192 x 2,048 bf16 19 us
+// forward (84 MB, 4.4 TB/s) and 18.5 backward (4.6), where the polynomial is as long as the
+// bytes; a device copy reaches 4.8 TB/s.  64 x 512 fp32 2.4 us, one launch's latency.
 template <typename T, int FORM, bool PACKED>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(UnitArgs a) {
   const UnitPlace at(a);

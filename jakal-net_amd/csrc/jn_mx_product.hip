@@ -286,6 +286,9 @@ __device__ __forceinline__ void load_lds(intx4 rs, uint32_t base, uint32_t offse
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 // Tiles of TM x TN over WM x WN waves, LDS double buffered with the next slice in registers.
+// For fp32, fp16 and rows that are no whole packs.  Splitting x into its terms and their way
+// through LDS bound it: 1,531 x 383 x 4,099 fp32 forward 42 us (114 TFLOP/s; the library's
+// fp32 product by dequantised weights 88 us), 128 x 2,048 x 16,384 fp32 53 us (77), fp16 43 (19).
 template <typename T, Product P, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_mixed_kernel(MixedArgs g) {
   constexpr int FORM = P == kWeightGrad ? kE4m3 : kE2m1;
@@ -457,6 +460,12 @@ __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_mixed_kernel(MixedArgs g)
 // after lies in registers by then and goes to the other stage meanwhile, and AHEAD slices
 // after that are on their way from memory.  B may be plain bf16 too (kPlainGrad: a linear
 // layer's input gradient).
+// The widest tiles are bound by LDS: 192 KB of reads and 64 KB of writes a slice take 2,048
+// clocks at 128 bytes each, as long as their products (8,192 x 2,048 x 16,384 forward 470 us,
+// 1,170 TFLOP/s; the library by dequantised weights 375 us; a long sum's input gradient, 1,024
+// x 2,048 over 16,384, 83 against 115).  The narrow ones wait for each other once a slice:
+// 0.53 to 0.85 us whatever they multiply, and loads further ahead (four slices) or twice the
+// waves changed nothing.
 template <Product P, int TM, int TN, int WM, int WN, int AHEAD>
 __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_bf16_kernel(MixedArgs g) {
   constexpr int FORM = P == kWeightGrad ? kE4m3 : kE2m1;
@@ -1040,6 +1049,10 @@ __device__ __forceinline__ intx8 wide(u32x4_nt v) { return intx8{(int)v[0], (int
 // loads go there directly while the step before is multiplied.  Rows past the operands'
 // ends are their last rows (their outputs are not written); past a row's end x is zeros,
 // so that W may be anything finite there.
+// 8,192 cubed takes 321 us (3,425 TFLOP/s, near what the card sustains on random data),
+// 8,192 x 2,048 x 16,384 bf16 205 (2,680): eight steps a tile, and its outputs' way out, 256
+// KB of fp32 sums rounded through LDS, has no products of another tile beside it (a loop over
+// tiles in one workgroup left no registers for that, and was slower).
 template <typename T, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_linear_kernel(LinearArgs g) {
   constexpr int WAVES = WM * WN;
@@ -1185,7 +1198,9 @@ __global__ __launch_bounds__(256) void mx_pad_scales_kernel(const uint8_t* scale
 // waves every WAVES-th step of 128 k, straight from memory into registers (a lane has a
 // run of 32 k of its row of W, and the same run of its rows of x); their sums join in
 // LDS in order.  FORM e2m1: a lane microscales its run of x itself.  Plain x: W's run is
-// four bf16 operands of eight, x's as many of each of its terms.
+// four bf16 operands of eight, x's as many of each of its terms.  One row by 2,048 x 16,384
+// 9 us (17.8 MB of weights, 2 TB/s: a launch, two steps' latency and the join), 64 fp32 rows
+// by 512 x 2,048 7 us.
 struct RowsArgs {
   const void* x;      // [m][dim]
   const uint8_t* w;   // [n][pitch]

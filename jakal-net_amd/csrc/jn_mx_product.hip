@@ -938,15 +938,16 @@ struct MixedPlan {
       const int slice = type == kTypeBf16 ? c.slice : kSlice<float>;
       const int64_t slices = std::max<int64_t>(1, (r + slice - 1) / slice);
       const int64_t tm = (m + c.m - 1) / c.m, tn = (n + c.n - 1) / c.n;
-      for (int64_t want = 1; want <= std::min<int64_t>(64, slices); ++want) {
-        const int64_t each = (slices + want - 1) / want, groups = tm * tn * ((slices + each - 1) / each);
-        const double busy = (double)((groups + 255) / 256);
-        double time = std::max(c.least, c.first + c.each * busy) * (double)each;
-        if (want > 1) time += 4.0 + (double)want * (double)m * (double)n * 8.0 / 6e6;
-        if (bias && c.m == 256) time += 10.0;  // (the wide tiles leave them to launches of their own)
+      for (const int64_t want : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64}) {
+        // the splits' join, and the bias's gradient, which the wide tiles leave to launches of its own
+        const double join = (want > 1 ? 4.0 + (double)want * (double)m * (double)n * 8.0 / 6e6 : 0.0) +
+                            (bias && c.m == 256 ? 10.0 : 0.0);
+        if (want > slices || join >= least) break;
+        const int64_t each = (slices + want - 1) / want, parts = (slices + each - 1) / each;
+        const double busy = (double)((tm * tn * parts + 255) / 256);
+        const double time = join + std::max(c.least, c.first + c.each * busy) * (double)each;
         if (time >= least) continue;
-        least = time, tile = c, tiles_m = (int)tm, tiles_n = (int)tn, chunk = each * slice;
-        splits = (int)((slices + each - 1) / each);
+        least = time, tile = c, tiles_m = (int)tm, tiles_n = (int)tn, chunk = each * slice, splits = (int)parts;
       }
     };
     if (!packed) consider(mixed_tile(type));

@@ -460,10 +460,11 @@ __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_mixed_kernel(MixedArgs g)
 // after lies in registers by then and goes to the other stage meanwhile, and AHEAD slices
 // after that are on their way from memory.  B may be plain bf16 too (kPlainGrad: a linear
 // layer's input gradient).
-// The widest tiles are bound by LDS: 192 KB of reads and 64 KB of writes a slice take 2,048
-// clocks at 128 bytes each, as long as their products (8,192 x 2,048 x 16,384 forward 470 us,
-// 1,170 TFLOP/s; the library by dequantised weights 375 us; a long sum's input gradient, 1,024
-// x 2,048 over 16,384, 83 against 115).  The narrow ones wait for each other once a slice:
+// The widest tiles keep the matrix units at 1,220 TFLOP/s over long sums (8,192 x 2,048 over
+// 8,192 225 us, the library by dequantised weights 202); what is left is a tile's start and
+// its outputs' way out, with no other workgroup on the CU (8,192 x 2,048 x 16,384 forward 490
+// us, 1,110 TFLOP/s, the library 404).  A quarter less LDS traffic (B there as its codes) and
+// the barrier under the first row of products gained 2 %.  The narrow ones wait for each other once a slice:
 // 0.53 to 0.85 us whatever they multiply, and loads further ahead (four slices) or twice the
 // waves changed nothing.
 template <Product P, int TM, int TN, int WM, int WN, int AHEAD>

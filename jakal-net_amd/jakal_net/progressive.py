@@ -245,7 +245,9 @@ class ProgressiveBStep(nn.Module):
     def quantize_head(self, activations: str | None = None) -> ProgressiveBStep:
         """Gives the head frozen 4-bit weights, to answer with; ``activations="e2m1"``:
         its two products microscale their inputs too.  Gradients still reach what
-        comes before the head."""
+        comes before the head.  A head that has such weights stays as it is."""
+        if activations is not None and any(isinstance(m, MXLinear) and m.activations != activations for m in self.head):
+            raise RuntimeError(f"the head's products are quantized already, with other activations than {activations!r}.")
         self.head = nn.Sequential(*(
             MXLinear.from_linear(m, activations=activations, implementation=self.implementation)
             if isinstance(m, nn.Linear) else m for m in self.head))

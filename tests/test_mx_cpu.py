@@ -172,6 +172,9 @@ def test_modules_and_the_model():
     model = models[0][0].quantize_head(activations="e2m1").quantize_head()
     assert [type(m).__name__ for m in model.head] == ["MXLinear", "GELU", "MXLinear"]
     assert model.head[0].activations == "e2m1"
+    plain = models[1][0].quantize_head()
+    with pytest.raises(RuntimeError, match="quantized already"):
+        plain.quantize_head(activations="e2m1")
     s = model.encode_prefix(prefix)
     assert model.query_logits(s, target).shape == (2, 8, 97)
     with pytest.raises(ValueError):

@@ -1032,8 +1032,8 @@ int jn_mx_weight_grad(const void* grad_y, const void* codes, const void* scales,
 
 /*
  * grad_x [rows, dim] = grad_y [rows, out] . weight [out, dim] of a plain linear layer,
- * JN_BF16, for the sizes that jn_linear_input_grad_fits answers 1 to (few output tiles
- * over a long sum); exact products, fp32 sums in a fixed order.  All start on 16 bytes.
+ * JN_BF16, for the sizes that jn_linear_input_grad_fits answers 1 to (short sums, and few
+ * outputs over long ones); exact products, fp32 sums in a fixed order.  All start on 16 bytes.
  */
 int32_t jn_linear_input_grad_fits(int64_t rows, int64_t dim, int64_t out, int32_t type);
 size_t jn_linear_input_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type);

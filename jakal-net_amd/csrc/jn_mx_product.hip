@@ -954,7 +954,6 @@ struct MixedPlan {
       }
     };
     if (!packed) consider(mixed_tile(type));
-    else if (p == kPlainGrad) consider(kPackedTiles[0]);
     else
       for (const auto& c : kPackedTiles) consider(c);
     if (p == kForward && packed && r % 128 == 0)
@@ -1000,16 +999,20 @@ int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size
                  s);
       if (plan.wide()) {
         hipLaunchKernelGGL((mx_bf16_kernel<P, 256, 256, 2, 4, 1>), grid, dim3(512), 0, s, g);
-      } else if constexpr (P != kPlainGrad) {
-        if (!plan.packed) hipLaunchKernelGGL((mx_mixed_kernel<T, P, 128, 128, 2, 2>), grid, dim3(256), 0, s, g);
-        else if (plan.tile.direct) {
-          if constexpr (P == kForward) {
-            if (plan.tile.m == 128) hipLaunchKernelGGL((mx_direct_kernel<128, 64, 2>), grid, dim3(256), 0, s, g);
-            else hipLaunchKernelGGL((mx_direct_kernel<64, 64, 3>), grid, dim3(256), 0, s, g);
-          }
-        } else if (plan.tile.n == 128) hipLaunchKernelGGL((mx_bf16_kernel<P, 128, 128, 2, 2, 2>), grid, dim3(256), 0, s, g);
-        else if (plan.tile.m == 128) hipLaunchKernelGGL((mx_bf16_kernel<P, 128, 64, 2, 2, 2>), grid, dim3(256), 0, s, g);
-        else hipLaunchKernelGGL((mx_bf16_kernel<P, 64, 64, 2, 2, 2>), grid, dim3(256), 0, s, g);
+      } else if (!plan.packed) {
+        if constexpr (P != kPlainGrad)  // (whose callers ask whether it fits)
+          hipLaunchKernelGGL((mx_mixed_kernel<T, P, 128, 128, 2, 2>), grid, dim3(256), 0, s, g);
+      } else if (plan.tile.direct) {
+        if constexpr (P == kForward) {
+          if (plan.tile.m == 128) hipLaunchKernelGGL((mx_direct_kernel<128, 64, 2>), grid, dim3(256), 0, s, g);
+          else hipLaunchKernelGGL((mx_direct_kernel<64, 64, 3>), grid, dim3(256), 0, s, g);
+        }
+      } else if (plan.tile.n == 128) {
+        hipLaunchKernelGGL((mx_bf16_kernel<P, 128, 128, 2, 2, 2>), grid, dim3(256), 0, s, g);
+      } else if (plan.tile.m == 128) {
+        hipLaunchKernelGGL((mx_bf16_kernel<P, 128, 64, 2, 2, 2>), grid, dim3(256), 0, s, g);
+      } else {
+        hipLaunchKernelGGL((mx_bf16_kernel<P, 64, 64, 2, 2, 2>), grid, dim3(256), 0, s, g);
       }
       JN_LAUNCH_CHECK();
     }
@@ -1476,12 +1479,19 @@ int jn_mx_weight_grad(const void* grad_y, const void* codes, const void* scales,
 
 int32_t jn_linear_input_grad_fits(int64_t rows, int64_t dim, int64_t out, int32_t type) {
   if (check_product("linear backward", rows, dim, out, type)) return 0;
-  // Measured with the library's product (us): 1,024 x 2,048 outputs over 16,384 80 and 112,
-  // 32,768 138 and 284, 8,192 60 and 68, 4,096 42 and 35; 512 x 1,024 over 16,384 39 and 64;
-  // 2,048 x 2,048 over 16,384 139 and 146, 8,192 84 and 77; 4,096 x 2,048 266 and 245.
+  // Measured with the library's product (us).  Long sums leave most CUs to the splits that the
+  // library does not make: 16,384 by 64 x 512 17 and 69, 1 x 1,024 17 and 29, 1,024 x 2,048 82
+  // and 117, 2,048 x 4,096 265 and 245; 8,192 by 16 x 2,048 14 and 21, 1,024 x 2,048 55 and 61,
+  // 1 x 1,024 14 and 13, 2,048 squared 86 and 81.  Short ones are a launch, and the library's
+  // takes the host 12 us more: 256 by 512 x 1,024 6.1 and 6.2, 4,096 squared 18.7 and 18.7; 512
+  // by 1,024 x 2,048 9.6 and 9.9, 16 x 512 7.1 and 5.4.  Between them the library's is as fast
+  // or faster (1,536 by 1,024 x 2,048 18.7 and 16.2).
   const MixedPlan plan(kPlainGrad, rows, dim, out, type, false);
-  const int64_t tiles = (int64_t)plan.tiles_m * plan.tiles_n;
-  return plan.packed && out >= std::max<int64_t>(8192, 256 * tiles) && tiles <= 64 && tiles * std::min<int64_t>(64, out / 512) >= 192;
+  const int64_t outputs = rows * dim;
+  if (!plan.packed) return 0;
+  if (out >= 16384) return outputs <= (1 << 22);
+  if (out >= 8192) return rows >= 16 && outputs <= (1 << 21);
+  return out <= 512 && rows >= (out <= 256 ? 16 : 64) && outputs <= (1 << 24);
 }
 
 size_t jn_linear_input_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t out, int32_t type) {

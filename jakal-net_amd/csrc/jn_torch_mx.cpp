@@ -300,8 +300,8 @@ Tensor linear_input_grad_meta(const Tensor& grad, const Tensor& weight) {
   return at::empty_symint(with_last(grad.sym_sizes(), weight.sym_size(1)), grad.options());
 }
 
-// grad . weight: here where the output has few tiles and the sum is long, else the
-// library product that a plain linear layer's backward is.
+// grad . weight: here where the sum is short, or long over few outputs, else the library
+// product that a plain linear layer's backward is.
 Tensor linear_input_grad(const Tensor& grad_in, const Tensor& weight_in) {
   check_rows("linear backward", grad_in);
   TORCH_CHECK(weight_in.dim() == 2 && weight_in.size(0) == grad_in.size(-1) &&

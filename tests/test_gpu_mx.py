@@ -3,6 +3,8 @@ in 8 bits on the HIP library, against tests/mx_oracle.py in float64: every forma
 and type, lengths from one element, runs and tiles that end inside, rows off 16
 bytes, infinities and NaN, each gradient alone."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -230,6 +232,22 @@ def test_products_of_every_tile(dev, m, n, r):
     gw, gb = ops.mx_weight_grad(a, *ops.mx_codes(kept.to(dev), 0), n, True)
     _rounded("grad_weight", gw, M.product(a.t(), M.quantize(kept, "e4m3")[0].to(dev)), torch.bfloat16)
     _rounded("grad_bias", gb, M.sums(a), torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows,dim,out", [(16, 8, 8), (33, 1000, 256), (72, 72, 512), (72, 520, 16392), (200, 16392, 72),
+                                          (1544, 2056, 72), (64, 1000, 8200), (1, 520, 16384), (2000, 4104, 136)])
+def test_linear_saved_input_grads(dev, rows, dim, out):
+    """The input gradient's own products of bf16: short sums and long ones, every tile, whole and split."""
+    import jakal_net_native as jn
+
+    i64 = ctypes.c_int64
+    assert ctypes.CDLL(str(jn.library_path())).jn_linear_input_grad_fits(i64(rows), i64(dim), i64(out), 1) == 1
+    g, w = _rand(1, rows, out, spread=0.0).bfloat16().to(dev), _rand(2, out, dim, spread=0.0).bfloat16().to(dev)
+    got = torch.ops.jakal_net_hip.linear_input_grad(g, w)
+    _rounded(f"{rows}x{dim}x{out}", got, M.product(g, w), torch.bfloat16)
+    loose = torch.empty(out, dim + 1, dtype=torch.bfloat16, device=dev)[:, 1:]
+    loose.copy_(w)
+    assert torch.equal(torch.ops.jakal_net_hip.linear_input_grad(g, loose), got)
 
 
 @pytest.mark.parametrize("rows", [4096, 10007])

@@ -168,7 +168,7 @@ class _MXLinear(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             gx = (g @ _dequantize(*ctx.saved_tensors, "e2m1", ctx.size, torch.float32)).to(ctx.dtype)
         if ctx.needs_input_grad[3]:
-            gb = g.flatten(0, -2).sum(0).to(ctx.dtype)
+            gb = g.reshape(-1, g.shape[-1]).sum(0).to(ctx.dtype)
         return gx, None, None, gb, None
 
 

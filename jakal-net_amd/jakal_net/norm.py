@@ -50,7 +50,7 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
             if implementation == "native":
                 raise
     if saved is not None:
-        return layer_norm_saved(_autocast_rows(x), weight, bias, eps, 1.0)
+        return layer_norm_saved(x, weight, bias, eps, 1.0)
     return F.layer_norm(x, x.shape[-1:], weight, bias, eps)
 
 
@@ -69,7 +69,7 @@ def stabilize(state: Tensor, val: Tensor, weight: Tensor | None = None, bias: Te
                 raise
     if saved is not None:
         return (torch.tanh(state if scale == 1.0 else state * scale),
-                layer_norm_saved(_autocast_rows(val), weight, bias, eps, scale))
+                layer_norm_saved(val, weight, bias, eps, scale))
     if scale != 1.0:
         state, val = state * scale, val * scale
     return torch.tanh(state), F.layer_norm(val, val.shape[-1:], weight, bias, eps)

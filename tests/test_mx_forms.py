@@ -1,4 +1,4 @@
-"""The PyTorch forms of the operators on microscaled numbers: values of one axis."""
+"""The PyTorch forms of the operators on microscaled numbers: values of one axis, autocast."""
 
 import pytest
 import torch
@@ -27,3 +27,38 @@ def test_values_of_one_axis(mode, acts):
     assert torch.equal(gb, g)
     value, bound = M.product(g[None], w)
     O.close("grad_x", gx[None], value, bound + O.U * value.abs())
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("cast", [False, True])
+@pytest.mark.parametrize("dtype", list(O.DTYPES))
+def test_norms_under_autocast_give_what_they_give_without_saved(dtype, cast, mode):
+    """CPU autocast leaves a norm's values in their type, as it leaves torch's layer norm."""
+    _norms_with_and_without_saved(torch.device("cpu"), dtype, cast, mode)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["reference", "native"])
+@pytest.mark.parametrize("cast", [False, True])
+@pytest.mark.parametrize("dtype", list(O.DTYPES))
+def test_norms_under_autocast_on_the_gpu(dtype, cast, mode):
+    """GPU autocast takes torch's layer norm in fp32."""
+    _norms_with_and_without_saved(torch.device("cuda:0"), dtype, cast, mode)
+
+
+def _norms_with_and_without_saved(dev, dtype, cast, mode):
+    import jakal_net as J
+
+    kind = O.DTYPES[dtype]
+    state, x = (_rand(i, *s).to(dev, kind).requires_grad_() for i, s in ((1, (3, 7)), (2, (3, 7, 40))))
+    # (torch's own layer norm on the GPU takes parameters of the values' type)
+    weight = (1 + 0.1 * _rand(3, 40)).to(dev, torch.float32 if cast or dev.type == "cpu" else kind).requires_grad_()
+    with torch.autocast(dev.type, dtype=torch.bfloat16, enabled=cast):
+        y, want = (J.layer_norm(x, weight, saved=s, implementation=mode) for s in ("e4m3", None))
+        t, z = J.stabilize(state, x, weight, scale=0.4, saved="e4m3", implementation=mode)
+        plain = J.stabilize(state, x, weight, scale=0.4, implementation=mode)
+    for got, expected in ((y, want), (t, plain[0]), (z, plain[1])):
+        assert got.dtype is expected.dtype and torch.equal(got, expected)
+    for out in (y, z):
+        gx, gw = torch.autograd.grad(out.float().sum(), (x, weight), retain_graph=True)
+        assert gx.dtype is kind and gw.dtype is weight.dtype

@@ -251,7 +251,8 @@ def layer_norm_saved(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps:
 def _autocast(*tensors: Tensor | None) -> tuple[Tensor | None, ...]:
     """The operands of a product as autocast has them where it is on."""
     kind = tensors[0].device.type
-    if not torch.is_autocast_enabled(kind) or tensors[0].dtype == torch.float64:
+    # (asking for meta tensors raises: they have no autocast)
+    if kind == "meta" or not torch.is_autocast_enabled(kind) or tensors[0].dtype == torch.float64:
         return tensors
     dtype = torch.get_autocast_dtype(kind)
     return tuple(t if t is None else t.to(dtype) for t in tensors)

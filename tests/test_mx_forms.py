@@ -1,4 +1,5 @@
-"""The PyTorch forms of the operators on microscaled numbers: values of one axis, autocast."""
+"""The PyTorch forms of the operators on microscaled numbers: values of one axis, autocast, meta
+tensors."""
 
 import pytest
 import torch
@@ -62,3 +63,20 @@ def _norms_with_and_without_saved(dev, dtype, cast, mode):
     for out in (y, z):
         gx, gw = torch.autograd.grad(out.float().sum(), (x, weight), retain_graph=True)
         assert gx.dtype is kind and gw.dtype is weight.dtype
+
+
+@pytest.mark.parametrize("mode", ["reference", "streaming"])
+def test_meta_tensors(mode):
+    """Shapes and types without memory, for which there is no autocast."""
+    import jakal_net as J
+
+    x, w, b = (torch.empty(*s, device="meta", requires_grad=True) for s in ((4, 7, 50), (9, 50), (9,)))
+    weight = J.mx_quantize(torch.empty(9, 50, device="meta"), "e2m1", implementation=mode)
+    assert weight.codes.shape == (9, 32) and weight.device.type == "meta"
+    for y in (J.linear(x, w, b, saved="e4m3", implementation=mode), J.mx_linear(x, weight, b, implementation=mode),
+              J.mx_linear(x, weight, b, activations="e2m1", implementation=mode)):
+        assert y.shape == (4, 7, 9) and [g.shape for g in torch.autograd.grad(y.sum(), (x, b))] == [x.shape, b.shape]
+    for kind in (torch.float32, torch.bfloat16):
+        v = x.detach().to(kind).requires_grad_()
+        for y in (J.gelu(v, saved="e4m3", implementation=mode), J.layer_norm(v, saved="e4m3", implementation=mode)):
+            assert y.shape == x.shape and y.dtype is kind and torch.autograd.grad(y.sum(), v)[0].shape == x.shape

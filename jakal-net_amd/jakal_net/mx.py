@@ -107,7 +107,7 @@ def _two_to(exponents: Tensor) -> Tensor:
 
 def _quantize(x: Tensor, format: str) -> tuple[Tensor, Tensor]:
     top, significand, bits, least = _SHAPES[format]
-    if x.shape[-1] < 1:
+    if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"mx_quantize needs a last axis of at least one element, got shape {tuple(x.shape)}.")
     v = F.pad(x.detach().float(), (0, -x.shape[-1] % RUN)).unflatten(-1, (-1, RUN))
     most = v.abs().amax(-1)

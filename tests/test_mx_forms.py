@@ -80,3 +80,17 @@ def test_meta_tensors(mode):
         v = x.detach().to(kind).requires_grad_()
         for y in (J.gelu(v, saved="e4m3", implementation=mode), J.layer_norm(v, saved="e4m3", implementation=mode)):
             assert y.shape == x.shape and y.dtype is kind and torch.autograd.grad(y.sum(), v)[0].shape == x.shape
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_a_tensor_without_axes_is_refused(mode):
+    """As the library refuses it: with a RuntimeError that names the shape."""
+    import jakal_net as J
+
+    x = torch.tensor(1.0, requires_grad=True)
+    for call in (lambda: J.mx_quantize(x, implementation=mode), lambda: J.gelu(x, saved="e4m3", implementation=mode),
+                 lambda: J.layer_norm(x, saved="e4m3", implementation=mode),
+                 lambda: J.linear(x, torch.ones(3, 1), saved="e4m3", implementation=mode),
+                 lambda: J.mx_linear(x, J.mx_quantize(torch.ones(3, 1), "e2m1"), implementation=mode)):
+        with pytest.raises(RuntimeError, match=r"shape \(\)"):
+            call()

@@ -105,7 +105,13 @@ def _two_to(exponents: Tensor) -> Tensor:
     return ((exponents.to(torch.int32) + 127) << 23).view(torch.float32)
 
 
+def _check_real(what: str, x: Tensor) -> None:
+    if x.is_complex():
+        raise NotImplementedError(f"{what} takes real values, got {x.dtype}.")
+
+
 def _quantize(x: Tensor, format: str) -> tuple[Tensor, Tensor]:
+    _check_real("mx_quantize", x)
     top, significand, bits, least = _SHAPES[format]
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"mx_quantize needs a last axis of at least one element, got shape {tuple(x.shape)}.")
@@ -152,6 +158,7 @@ def _wide(t: Tensor) -> Tensor:
 class _MXLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, codes, scales, bias, activations):
+        _check_real("mx_linear", x)
         ctx.save_for_backward(codes, scales)
         ctx.size, ctx.dtype = x.shape[-1], x.dtype
         v = x.float()

@@ -1,5 +1,5 @@
-"""The PyTorch forms of the operators on microscaled numbers: values of one axis, autocast, meta
-tensors."""
+"""The PyTorch forms of the operators on microscaled numbers: values of one axis and of none,
+autocast, meta tensors, complex ones."""
 
 import pytest
 import torch
@@ -93,4 +93,20 @@ def test_a_tensor_without_axes_is_refused(mode):
                  lambda: J.linear(x, torch.ones(3, 1), saved="e4m3", implementation=mode),
                  lambda: J.mx_linear(x, J.mx_quantize(torch.ones(3, 1), "e2m1"), implementation=mode)):
         with pytest.raises(RuntimeError, match=r"shape \(\)"):
+            call()
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_complex_values_are_refused(mode):
+    """Microscaled numbers are real: the imaginary parts would be lost."""
+    import jakal_net as J
+
+    x = torch.complex(_rand(1, 3, 32), _rand(2, 3, 32))
+    weight = J.mx_quantize(_rand(4, 9, 32), "e2m1")
+    for call in (lambda: J.mx_quantize(x, implementation=mode), lambda: J.gelu(x, saved="e4m3", implementation=mode),
+                 lambda: J.linear(x, x, saved="e4m3", implementation=mode),
+                 lambda: J.layer_norm(x, saved="e4m3", implementation=mode),
+                 lambda: J.mx_linear(x, weight, implementation=mode),
+                 lambda: J.mx_linear(x, weight, activations="e2m1", implementation=mode)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
             call()

@@ -18,13 +18,14 @@ struct UnitArgs {
   int64_t rows, dim;
   int64_t units;      // of all rows
   int64_t row_units;  // of one
+  int64_t first;      // of this launch
 };
 
 // A workgroup takes 256 units in a row; where rows are whole runs they are one long row.
 struct UnitPlace {
   int64_t unit, row, e;
   __device__ explicit UnitPlace(const UnitArgs& a) {
-    unit = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    unit = a.first + (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (a.rows == 1) row = 0, e = unit * 8;
     else if (a.units < (int64_t(1) << 32)) {
       const uint32_t r = (uint32_t)unit / (uint32_t)a.row_units;
@@ -159,7 +160,17 @@ int with_form(int32_t form, F f) {
   return form == kE4m3 ? f(std::integral_constant<int, kE4m3>{}) : f(std::integral_constant<int, kE2m1>{});
 }
 
-dim3 unit_grid(const UnitArgs& a) { return dim3((unsigned)((a.units + 255) / 256)); }
+// A grid has fewer than 2^32 threads along an axis (what is asked beyond them is dropped
+// without an error), so that more units go in several launches.
+constexpr int64_t kLaunchUnits = int64_t(1) << 31;
+template <typename F>
+int launch_units(UnitArgs a, F launch) {
+  for (; a.first < a.units; a.first += kLaunchUnits) {
+    launch(dim3((unsigned)((std::min(kLaunchUnits, a.units - a.first) + 255) / 256)), a);
+    JN_LAUNCH_CHECK();
+  }
+  return kOk;
+}
 
 }  // namespace
 
@@ -172,9 +183,9 @@ int launch_mx_quantize(const void* x, int64_t rows, int64_t dim, int32_t type, i
       return with_packs(packed_rows(a, type), [&](auto p) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
         JN_PROFILE("mx_quantize_kernel", s);
-        hipLaunchKernelGGL((mx_quantize_kernel<T, f(), p()>), unit_grid(a), dim3(256), 0, s, a);
-        JN_LAUNCH_CHECK();
-        return kOk;
+        return launch_units(a, [&](dim3 grid, const UnitArgs& part) {
+          hipLaunchKernelGGL((mx_quantize_kernel<T, f(), p()>), grid, dim3(256), 0, s, part);
+        });
       });
     });
   });
@@ -205,9 +216,9 @@ int jn_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_
       return with_packs(packed_rows(a, type), [&](auto p) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
         JN_PROFILE("mx_dequantize_kernel", s);
-        hipLaunchKernelGGL((mx_dequantize_kernel<T, f(), p()>), unit_grid(a), dim3(256), 0, s, a);
-        JN_LAUNCH_CHECK();
-        return kOk;
+        return launch_units(a, [&](dim3 grid, const UnitArgs& part) {
+          hipLaunchKernelGGL((mx_dequantize_kernel<T, f(), p()>), grid, dim3(256), 0, s, part);
+        });
       });
     });
   });
@@ -223,9 +234,9 @@ int jn_gelu_forward(const void* x, int64_t rows, int64_t dim, int32_t type, void
     return with_packs(packed_rows(a, type), [&](auto p) -> int {
       using T = std::remove_pointer_t<decltype(t)>;
       JN_PROFILE("gelu_forward_kernel", s);
-      hipLaunchKernelGGL((gelu_forward_kernel<T, p()>), unit_grid(a), dim3(256), 0, s, a);
-      JN_LAUNCH_CHECK();
-      return kOk;
+      return launch_units(a, [&](dim3 grid, const UnitArgs& part) {
+        hipLaunchKernelGGL((gelu_forward_kernel<T, p()>), grid, dim3(256), 0, s, part);
+      });
     });
   });
 }
@@ -240,9 +251,9 @@ int jn_gelu_backward(const void* codes, const void* scales, const void* grad_y, 
     return with_packs(packed_rows(a, type), [&](auto p) -> int {
       using T = std::remove_pointer_t<decltype(t)>;
       JN_PROFILE("gelu_backward_kernel", s);
-      hipLaunchKernelGGL((gelu_backward_kernel<T, p()>), unit_grid(a), dim3(256), 0, s, a);
-      JN_LAUNCH_CHECK();
-      return kOk;
+      return launch_units(a, [&](dim3 grid, const UnitArgs& part) {
+        hipLaunchKernelGGL((gelu_backward_kernel<T, p()>), grid, dim3(256), 0, s, part);
+      });
     });
   });
 }

@@ -59,6 +59,10 @@ const char* last_error();
     }                                                                           \
   } while (0)
 
+// Whether a grid of `blocks` workgroups along an axis has fewer than 2^32 threads there:
+// those that a launch asks for beyond them are dropped without an error.
+inline bool fits_grid(int64_t blocks, int64_t threads) { return blocks <= ((int64_t(1) << 32) - 1) / threads; }
+
 // Optional per-kernel timing with HIP events, off unless jn_profile_enable(1)
 // was called.  A scope records an event on `stream` before and after the
 // launch it encloses; jn_profile_collect() reads the elapsed times back.

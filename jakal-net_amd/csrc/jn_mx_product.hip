@@ -975,8 +975,11 @@ int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size
   JN_REQUIRE(plan.bytes() == 0 || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes()),
              kWorkspaceTooSmall, "%s: needs %zu workspace bytes on a 16-byte address, got %zu", what, plan.bytes(),
              workspace_bytes);
-  JN_REQUIRE((int64_t)plan.tiles_m * plan.tiles_n * plan.splits < (int64_t(1) << 31), kUnsupported,
-             "%s: too many output tiles", what);
+  const int64_t threads =  // of the launch that joins the sums
+      (plan.partial_bytes ? g.m * (plan.ldp / 4) : 0) + (g.bias_grad && !plan.wide() ? g.m : 0);
+  JN_REQUIRE(fits_grid((int64_t)plan.tiles_m * plan.tiles_n * plan.splits, plan.wide() ? 512 : 256) &&
+                 fits_grid((threads + 255) / 256, 256),
+             kUnsupported, "%s: too many outputs for a launch (%lld x %lld)", what, (long long)g.m, (long long)g.n);
   void* const out = g.out;
   g.tiles_m = plan.tiles_m, g.tiles_n = plan.tiles_n, g.chunk = plan.chunk, g.ldp = plan.ldp;
   const int64_t along = P == kForward ? g.r : g.n;
@@ -1019,7 +1022,6 @@ int run_mixed(const char* what, MixedArgs g, int32_t type, void* workspace, size
     if (g.partial || g.bias_partial) {
       JN_PROFILE("mx_sum_kernel", s);
       g.out = out;
-      const int64_t threads = (g.partial ? g.m * (g.ldp / 4) : 0) + (g.bias_partial ? g.m : 0);
       hipLaunchKernelGGL(mx_sum_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, g, plan.splits);
       JN_LAUNCH_CHECK();
     }
@@ -1349,10 +1351,9 @@ size_t linear_codes_bytes(int64_t rows, int64_t dim) { return (size_t)(rows * st
 template <typename T, int TM, int TN, int WM, int WN>
 int launch_linear(LinearArgs g, hipStream_t s) {
   g.tiles_m = (int)((g.m + TM - 1) / TM), g.tiles_n = (int)((g.n + TN - 1) / TN);
-  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
-  JN_REQUIRE(tiles < (int64_t(1) << 31), kUnsupported, "mx_linear: too many output tiles");
   JN_PROFILE("mx_linear_kernel", s);
-  hipLaunchKernelGGL((mx_linear_kernel<T, TM, TN, WM, WN>), dim3((unsigned)tiles), dim3(WM * WN * kWave), 0, s, g);
+  hipLaunchKernelGGL((mx_linear_kernel<T, TM, TN, WM, WN>), dim3((unsigned)((int64_t)g.tiles_m * g.tiles_n)),
+                     dim3(WM * WN * kWave), 0, s, g);
   JN_LAUNCH_CHECK();
   return kOk;
 }
@@ -1416,9 +1417,16 @@ int jn_mx_linear_forward(const void* x, const void* weight_codes, const void* we
   g.w = static_cast<const uint8_t*>(weight_codes), g.ws = static_cast<const uint8_t*>(weight_scales);
   g.bias = bias, g.y = y, g.m = rows, g.n = out, g.pitch = mx_pitch(dim, kE2m1);
   g.x_runs = step_runs(dim), g.x_pitch = g.x_runs * 16;
-  if (mx_runs(dim) % kStepRuns) {
+  // The widest tiles that keep three quarters of the CUs busy (bf16, us with tiles of 256,
+  // 128 and 64: 768 x 2,048 x 16,384 28.3, 29.3 and 45.9; 768 x 4,096 x 4,096 38.5, 23.6 and
+  // 28.9; 512 x 4,096 x 4,096 37.9, 22.1 and 20.1; 4,096 x 2,048 x 2,048 30.5, 24.8, 36.7).
+  const auto tiles = [&](int64_t edge) { return (rows + edge - 1) / edge * ((out + edge - 1) / edge); };
+  const int64_t tile = tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
+  const int64_t words = mx_runs(dim) % kStepRuns ? out * g.x_runs / 4 : 0;  // of W's scales in rows of whole steps
+  JN_REQUIRE(fits_grid(tiles(tile), tile == 256 ? 512 : 256) && fits_grid((words + 255) / 256, 256), kUnsupported,
+             "mx_linear: too many outputs for a launch (%lld x %lld)", (long long)rows, (long long)out);
+  if (words) {
     uint8_t* const padded = scales + rows * g.x_runs;
-    const int64_t words = out * g.x_runs / 4;
     JN_PROFILE("mx_pad_scales_kernel", s);
     hipLaunchKernelGGL(mx_pad_scales_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, g.ws, out,
                        mx_runs(dim), g.x_runs, padded);
@@ -1428,12 +1436,8 @@ int jn_mx_linear_forward(const void* x, const void* weight_codes, const void* we
   if (const int rc = launch_mx_quantize(x, rows, dim, type, kE2m1, codes, scales, s, g.x_runs)) return rc;
   return with_type(type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
-    const auto tiles = [&](int64_t tm, int64_t tn) { return (rows + tm - 1) / tm * ((out + tn - 1) / tn); };
-    // The widest tiles that keep three quarters of the CUs busy (bf16, us with tiles of 256,
-    // 128 and 64: 768 x 2,048 x 16,384 28.3, 29.3 and 45.9; 768 x 4,096 x 4,096 38.5, 23.6 and
-    // 28.9; 512 x 4,096 x 4,096 37.9, 22.1 and 20.1; 4,096 x 2,048 x 2,048 30.5, 24.8, 36.7).
-    if (tiles(256, 256) >= 192) return launch_linear<T, 256, 256, 2, 4>(g, s);
-    if (tiles(128, 128) >= 192) return launch_linear<T, 128, 128, 2, 2>(g, s);
+    if (tile == 256) return launch_linear<T, 256, 256, 2, 4>(g, s);
+    if (tile == 128) return launch_linear<T, 128, 128, 2, 2>(g, s);
     return launch_linear<T, 64, 64, 2, 2>(g, s);
   });
 }

@@ -32,7 +32,11 @@ using at::Tensor;
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
-void check(int rc) { TORCH_CHECK(rc == 0, "jakal_net HIP library error ", rc, ": ", jn_last_error()); }
+// What the library declines (2) is a NotImplementedError, for which callers have another form.
+void check(int rc) {
+  TORCH_CHECK_NOT_IMPLEMENTED(rc != 2, "jakal_net HIP library error ", rc, ": ", jn_last_error());
+  TORCH_CHECK(rc == 0, "jakal_net HIP library error ", rc, ": ", jn_last_error());
+}
 
 int32_t type_code(const char* what, const Tensor& t) {
   switch (t.scalar_type()) {

@@ -87,3 +87,15 @@ def test_quantize_whole_runs_of_more_than_2_32_threads(dev):
     # the other rows are zeros, whose scale is the least (the last two places share a row)
     written = sorted({at + i for at in places for i in (0, 1)})
     assert len(written) == 7 and int((q.scales != 1).sum()) == int((q.scales[written] != 1).sum()) == 7 * dim // 32
+
+
+def test_products_beyond_a_grid_are_declined(dev):
+    """2^24 tiles of 256 threads: a NotImplementedError, as for every call that the library has no kernel for."""
+    import jakal_net as J
+
+    _need(40)
+    x, weight = torch.zeros((1 << 31) - 1, 1, device=dev), J.mx_quantize(torch.ones(1, 1, device=dev), "e2m1")
+    with pytest.raises(NotImplementedError, match="too many outputs"):
+        J.mx_linear(x, weight)
+    with pytest.raises(NotImplementedError, match="too many outputs"):
+        torch.ops.jakal_net_hip.mx_input_grad(x, weight.codes, weight.scales, 1)

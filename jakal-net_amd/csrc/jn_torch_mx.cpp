@@ -23,10 +23,15 @@ Tensor aligned(const Tensor& t) {
   return p.numel() && reinterpret_cast<uintptr_t>(p.data_ptr()) % 16 ? p.clone() : p;
 }
 
+void check_width(const char* what, const c10::SymInt& size) {
+  TORCH_CHECK_NOT_IMPLEMENTED(size < (int64_t(1) << 31), what, " takes rows of up to 2^31 - 1 elements, got ", size, ".");
+}
+
 void check_rows(const char* what, const Tensor& x) {
   type_code(what, x);
   TORCH_CHECK(x.dim() >= 1 && x.sym_size(-1) >= 1, what, " needs a last axis of at least one element, got shape ",
               x.sym_sizes(), ".");
+  check_width(what, x.sym_size(-1));
   check_gpu(x, x);
 }
 void check_form(const char* what, int64_t form) {
@@ -115,6 +120,7 @@ Packed mx_quantize(const Tensor& x, int64_t form) {
 
 Tensor mx_dequantize(const Tensor& codes, const Tensor& scales, int64_t form, c10::SymInt size, at::ScalarType type) {
   check_packed("mx_dequantize", codes, scales, form, size);
+  check_width("mx_dequantize", size);
   static const auto op = inner<Values>("jakal_net_hip::mx_values");
   const at::AutoDispatchBelowADInplaceOrView below;
   return op.call(codes, scales, form, std::move(size), type);
@@ -141,6 +147,14 @@ Tensor call_column_sums(const Tensor& x) {
   return op.call(x);
 }
 
+// What the library's products of x [..., inputs] and their gradients take.
+void check_product(const char* what, const Tensor& x, const c10::SymInt& out) {
+  constexpr int64_t kRows = int64_t(1) << 31, kWidth = int64_t(1) << 24;
+  TORCH_CHECK_NOT_IMPLEMENTED(x.sym_size(-1) < kWidth && out < kWidth && x.sym_numel() < x.sym_size(-1) * kRows, what,
+                              " takes up to 2^31 - 1 rows and 2^24 - 1 inputs and outputs, got shape ", x.sym_sizes(),
+                              " and ", out, " outputs.");
+}
+
 // ---- products by 4-bit weights ------------------------------------------------
 void check_linear(const char* what, const Tensor& x, const Tensor& weight, const Tensor& bias, const c10::SymInt& out) {
   check_rows(what, x);
@@ -160,6 +174,7 @@ void check_mx_linear(const Tensor& x, const Tensor& codes, const Tensor& scales,
   check_linear("mx_linear", x, codes, bias, codes.sym_size(0));
   check_packed("mx_linear", codes, scales, JN_E2M1, x.sym_size(-1));
   TORCH_CHECK(codes.sym_size(0) >= 1, "mx_linear: a weight without outputs.");
+  check_product("mx_linear", x, codes.sym_size(0));
 }
 
 using Product = Tensor(const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&, int64_t);
@@ -373,6 +388,8 @@ Tensor linear_saved(const Tensor& x, const Tensor& weight, const std::optional<T
   TORCH_CHECK(weight.sym_size(0) >= 1, "linear: a weight without outputs.");
   std::shared_ptr<JakalLinearSavedBackward> node;
   if (records(x, weight, bias)) {
+    // (the input's gradient may be the library product's)
+    if (torch::autograd::compute_requires_grad(weight, bias)) check_product("linear", x, weight.sym_size(0));
     node = make_node<JakalLinearSavedBackward>();
     node->set_next_edges(torch::autograd::collect_next_edges(x, weight, bias));
   }

@@ -38,8 +38,8 @@ void check(int rc) {
   TORCH_CHECK(rc == 0, "jakal_net HIP library error ", rc, ": ", jn_last_error());
 }
 
-int32_t type_code(const char* what, const Tensor& t) {
-  switch (t.scalar_type()) {
+int32_t type_code(const char* what, at::ScalarType type) {
+  switch (type) {
     case at::kFloat:
       return JN_F32;
     case at::kBFloat16:
@@ -49,8 +49,9 @@ int32_t type_code(const char* what, const Tensor& t) {
     default:
       break;
   }
-  TORCH_CHECK_NOT_IMPLEMENTED(false, what, " takes fp32, bf16 and fp16 tensors, got ", t.scalar_type(), ".");
+  TORCH_CHECK_NOT_IMPLEMENTED(false, what, " takes fp32, bf16 and fp16 tensors, got ", type, ".");
 }
+int32_t type_code(const char* what, const Tensor& t) { return type_code(what, t.scalar_type()); }
 
 void check_gpu(const Tensor& t, const Tensor& first) {
   if (!t.defined()) return;

@@ -121,6 +121,7 @@ Packed mx_quantize(const Tensor& x, int64_t form) {
 Tensor mx_dequantize(const Tensor& codes, const Tensor& scales, int64_t form, c10::SymInt size, at::ScalarType type) {
   check_packed("mx_dequantize", codes, scales, form, size);
   check_width("mx_dequantize", size);
+  type_code("mx_dequantize", type);
   static const auto op = inner<Values>("jakal_net_hip::mx_values");
   const at::AutoDispatchBelowADInplaceOrView below;
   return op.call(codes, scales, form, std::move(size), type);

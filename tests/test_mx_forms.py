@@ -110,3 +110,17 @@ def test_complex_values_are_refused(mode):
                  lambda: J.mx_linear(x, weight, activations="e2m1", implementation=mode)):
         with pytest.raises((RuntimeError, NotImplementedError)):
             call()
+
+
+def test_dequantising_to_other_types_is_declined_for_tensors_without_memory_too():
+    """A traced call takes the form that the call itself takes."""
+    import jakal_net as J
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        q = J.mx_quantize(torch.empty(3, 64, device="cuda"), "e2m1")
+        for kind in (torch.float64, torch.int32):
+            with pytest.raises(NotImplementedError):
+                J.mx_dequantize(q, kind)
+            assert J.mx_dequantize(q, kind, implementation="kernel").dtype is kind
+        assert J.mx_dequantize(q, torch.float16).dtype is torch.float16

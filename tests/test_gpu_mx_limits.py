@@ -3,6 +3,9 @@
 import pytest
 import torch
 
+import mx_exact as X
+import step_oracle as O
+
 pytestmark = pytest.mark.gpu
 
 
@@ -99,3 +102,38 @@ def test_products_beyond_a_grid_are_declined(dev):
         J.mx_linear(x, weight)
     with pytest.raises(NotImplementedError, match="too many outputs"):
         torch.ops.jakal_net_hip.mx_input_grad(x, weight.codes, weight.scales, 1)
+
+
+@pytest.mark.parametrize("dtype", list(O.DTYPES))
+def test_every_element_of_products_past_32_bits(dev, dtype):
+    """2.29e9 outputs, and gradients of as many: whole numbers, each result against float64."""
+    import jakal_net as J
+
+    _need(60)
+    kind, ops = O.DTYPES[dtype], torch.ops.jakal_net_hip
+    rows, dim, out = 140_003, 64, 16_384
+    chunks = [slice(at, min(rows, at + 10_000)) for at in range(0, rows, 10_000)]
+    w, x = X.kept(1, out, dim, "e2m1", dev), X.kept(2, rows, dim, "e2m1", dev)
+    weight = J.mx_quantize(w, "e2m1")
+    for acts in (None, "e2m1"):
+        y = J.mx_linear(x.to(kind), weight, activations=acts)
+        for at in chunks:
+            X.same(f"y of {acts}, rows from {at.start}", y[at], X.product(x[at], w.t()))
+        del y
+    g = torch.empty(rows, out, device=dev, dtype=kind)
+    for i, at in enumerate(chunks):
+        g[at] = X.whole(3 + i, at.stop - at.start, out, dev=dev, top=1).to(kind)
+    gx = ops.mx_input_grad(g, weight.codes, weight.scales, dim)
+    k = X.kept(4, rows, dim, "e4m3", dev)
+    gw, gb = ops.mx_weight_grad(g, *ops.mx_codes(k, 0), dim, True)
+    sums = ops.column_sums(g)
+    want, size, bias = 0.0, 0.0, 0.0
+    for at in chunks:
+        part, kept = g[at].double(), k[at].double()
+        X.same(f"grad_x, rows from {at.start}", gx[at], X.product(part, w))
+        want, size, bias = want + part.t() @ kept, size + part.abs().t() @ kept.abs(), bias + part.sum(0)
+        del part
+    assert float(size.max()) < 2.0 ** 24  # sums that fp32 holds whatever their order
+    X.same("grad_w", gw, want)
+    X.same("grad_b", gb, bias)
+    X.same("sums", sums, bias)

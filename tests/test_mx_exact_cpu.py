@@ -41,3 +41,23 @@ def test_lost_bits_are_seen(dtype):
             X.same("lost", X.product(short, w).to(kind), want)
     at = (x != 0).nonzero()[:, 1]
     assert {0, 399, 398, 392, 391, 32, 31, 64, 63, 128, 127, 256, 255} <= set(at.tolist())
+
+
+@pytest.mark.parametrize("dtype", list(O.DTYPES))
+def test_lost_rows_of_a_long_sum_are_seen(dtype):
+    """A gradient over 140,003 rows: half of them gone, those past 2^31 elements of 16,384 columns, rows read twice."""
+    kind, rows = O.DTYPES[dtype], 140_003
+    g, k = X.whole(3, rows, 4, top=1), X.kept(4, rows, 64, "e4m3")
+    want, sums = X.product(g.t(), k), g.double().sum(0)
+    past = 2 ** 31 // 16_384
+    for lost in (slice(0, rows // 2), slice(past, rows), slice(rows - 64, rows)):
+        part = g.clone()
+        part[lost] = 0
+        with pytest.raises(AssertionError, match="differ"):
+            X.same("lost", X.product(part.t(), k).to(kind), want)
+        with pytest.raises(AssertionError, match="differ"):
+            X.same("lost", part.double().sum(0).to(kind), sums)
+    part = g.clone()
+    part[past:] = g[:rows - past]
+    with pytest.raises(AssertionError, match="differ"):
+        X.same("wrapped", X.product(part.t(), k).to(kind), want)

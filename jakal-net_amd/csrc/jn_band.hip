@@ -420,7 +420,7 @@ int launch_band_aggregate(const BandAggArgs& a, hipStream_t stream) {
   const bool narrow = (int64_t)a.B * tiles * ((a.D + kBandColsWide - 1) / kBandColsWide) < kBandNarrowBelow;
   const int cols = narrow ? kBandColsNarrow : kBandColsWide;
   const int64_t blocks = (int64_t)a.B * tiles * ((a.D + cols - 1) / cols);
-  JN_REQUIRE(blocks < (1LL << 31) && (int64_t)a.B * a.N * a.k < (1LL << 31), kInvalidArgument, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256) && (int64_t)a.B * a.N * a.k < (1LL << 31), kInvalidArgument, "too many rows");
   const size_t lds = band_aggregate_lds_bytes(a.k, cols);
   const dim3 grid((unsigned)blocks);
   JN_PROFILE(a.trans ? "band_columns_kernel" : "band_forward_kernel", stream);
@@ -447,7 +447,7 @@ int launch_band_dots(const BandDotsArgs& a, hipStream_t stream) {
              "null tensor pointer or bf16 scores");
   const int64_t tiles = (a.N + kBandRows - 1) / kBandRows;
   const int64_t blocks = (int64_t)a.B * tiles * (scores ? 1 : 2);
-  JN_REQUIRE(blocks < (1LL << 31) && (int64_t)a.B * a.N * a.k < (1LL << 31), kInvalidArgument, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256) && (int64_t)a.B * a.N * a.k < (1LL << 31), kInvalidArgument, "too many rows");
   const dim3 grid((unsigned)blocks);
   JN_PROFILE(scores ? "band_scores_kernel" : "band_dots_kernel", stream);
   if (scores) launch_band_dots_nt<float, true>(a, grid, stream);

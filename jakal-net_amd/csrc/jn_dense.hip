@@ -301,7 +301,7 @@ int launch_colsum_rows(const float* M, const float* a, const float* c, int B, in
   const bool narrow = al && (int64_t)B * ((Nc + 63) / 64) < 256;
   const int ct = vec ? 256 : narrow ? 16 : 64;
   const int64_t blocks = (int64_t)B * ((Nc + ct - 1) / ct);
-  JN_REQUIRE(blocks < (1LL << 31), kUnsupported, "too many columns");
+  JN_REQUIRE(fits_grid(blocks, 1024), kUnsupported, "too many columns");
   JN_PROFILE(name, stream);
   const dim3 grid((unsigned)blocks), block(1024);
   if (vec) hipLaunchKernelGGL(colsum_rows_kernel<true>, grid, block, 0, stream, M, a, c, B, Nr, Nc, out);
@@ -328,7 +328,7 @@ int launch_dense_compress(float* S, const float* bias, const float* ps, int B, i
                           float* delta_state, hipStream_t stream) {
   const int64_t rows = (int64_t)B * N;
   const int64_t blocks = (rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kUnsupported, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kUnsupported, "too many rows");
   const bool vec = (N % 4 == 0) && ((reinterpret_cast<uintptr_t>(S) & 15) == 0) &&
                    ((reinterpret_cast<uintptr_t>(ps) & 15) == 0);
   JN_PROFILE("dense_compress_kernel", stream);
@@ -344,7 +344,7 @@ int launch_dense_compress_backward(float* G, const float* E, const float* gds, c
                                    int compress, int causal, float* rowsum, hipStream_t stream) {
   const int64_t rows = (int64_t)B * N;
   const int64_t blocks = (rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kUnsupported, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kUnsupported, "too many rows");
   const bool vec = (N % 4 == 0) && ((reinterpret_cast<uintptr_t>(G) & 15) == 0) &&
                    ((reinterpret_cast<uintptr_t>(E) & 15) == 0) && ((reinterpret_cast<uintptr_t>(ps) & 15) == 0);
   JN_PROFILE("dense_compress_backward_kernel", stream);
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(256) void dense_part_rowsum_kernel(const float* par
 
 int launch_dense_part_rowsum(const float* part, int P, int64_t rows, float* out, hipStream_t stream) {
   const int64_t blocks = (rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kUnsupported, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kUnsupported, "too many rows");
   JN_PROFILE("dense_part_rowsum_kernel", stream);
   hipLaunchKernelGGL(dense_part_rowsum_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, part, P, rows, out);
   JN_LAUNCH_CHECK();
@@ -419,7 +419,7 @@ int launch_head_rowsum(const float* G, const uint8_t* head, int N, int64_t ld, i
                        hipStream_t stream) {
   JN_REQUIRE(H >= 1 && H <= kMaxHeads, kUnsupported, "1 to %d heads", kMaxHeads);
   const int64_t blocks = (rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kUnsupported, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kUnsupported, "too many rows");
   if (rows == 0) return kOk;
   const bool vec = (N % 4 == 0) && (ld % 4 == 0) && ((reinterpret_cast<uintptr_t>(G) & 15) == 0) &&
                    ((reinterpret_cast<uintptr_t>(head) & 3) == 0);
@@ -440,7 +440,7 @@ int launch_scale_grad_partials(float* dps, int64_t ld_dps, const float* src, int
                                int r, int64_t rows, float* part, hipStream_t stream) {
   const int64_t n = rows * r;
   if (n == 0) return kOk;
-  JN_REQUIRE((n + 255) / 256 < (1LL << 31), kUnsupported, "too many rows");
+  JN_REQUIRE(fits_grid((n + 255) / 256, 256), kUnsupported, "too many rows");
   JN_PROFILE("scale_grad_partials_kernel", stream);
   hipLaunchKernelGGL(scale_grad_partials_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, dps,
                      ld_dps, src, ld_src, w_hat, r, rows, part);

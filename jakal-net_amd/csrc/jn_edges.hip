@@ -117,7 +117,7 @@ int launch_rows_forward(const RowsFwdArgs& args, hipStream_t stream) {
     while (a.slab > 64 * pw && a.slab % (128 * pw) == 0 && (int64_t)a.Nk * a.slab * eb > (2LL << 20)) a.slab /= 2;
   const int64_t slabs = (a.D + a.slab - 1) / a.slab;
   const int64_t blocks = (a.rows + 3) / 4 * slabs;
-  JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kInvalidArgument, "too many rows");
   JN_PROFILE("rows_forward_kernel", stream);
   const dim3 grid((unsigned)blocks);
   if (a.bf16) {
@@ -528,7 +528,7 @@ int launch_rows_backward(const RowsBwdArgs& a, hipStream_t stream) {
   }
   JN_REQUIRE(a.r >= 0 && a.r <= kRegRank, kUnsupported, "rank must be in [1, %d]", kRegRank);
   const int64_t blocks = (a.rows + 3) / 4;
-  JN_REQUIRE(2 * blocks < (1LL << 31), kInvalidArgument, "too many rows");
+  JN_REQUIRE(fits_grid(2 * blocks, 256), kInvalidArgument, "too many rows");
   JN_REQUIRE((int64_t)a.Nk * a.ld_pv * 4 < (1LL << 31) && (int64_t)a.Nk * a.ldk * 4 < (1LL << 31) &&
                  (int64_t)a.D * 4 < (1LL << 31),
              kUnsupported, "one batch element of the value or key rows must stay below 2 GiB");
@@ -645,7 +645,7 @@ int launch_rank_rows_grad(const RankRowsArgs& a, hipStream_t stream) {
   JN_REQUIRE((int64_t)a.Nk * a.ldk * 4 < (1LL << 31), kUnsupported,
              "one batch element of the key rows must stay below 2 GiB");
   const int64_t blocks = (a.rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kInvalidArgument, "too many rows");
   const bool vec = (a.r % 4 == 0) && (a.ldk % 4 == 0) && (a.lddq % 4 == 0) &&
                    ((reinterpret_cast<uintptr_t>(a.key) & 15) == 0) &&
                    ((reinterpret_cast<uintptr_t>(a.qscale) & 15) == 0);
@@ -1392,7 +1392,7 @@ int launch_cols_gather_dots(const ColsBwdArgs& a, hipStream_t stream) {
   JN_REQUIRE(slabs > 0, kInvalidArgument, "fused column pass needs CSR records with edge ids and aligned rows");
   JN_REQUIRE((int64_t)a.B * a.Nq * a.k < (1LL << 31), kUnsupported, "edge count exceeds int32 ids");
   const int64_t blocks = (total_cols + 3) / 4 * slabs;
-  JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "too many columns");
+  JN_REQUIRE(fits_grid(blocks, 256), kInvalidArgument, "too many columns");
   JN_PROFILE("cols_gather_dots_kernel", stream);
   const dim3 grid((unsigned)blocks);
   const bool buf = (int64_t)a.Nq * a.D * (a.bf16 ? 2 : 4) < (int64_t)kOobOffset;
@@ -1426,7 +1426,7 @@ int launch_edge_coefficients(const int32_t* idx, const float* score, int64_t row
                              hipStream_t stream) {
   if (rows == 0) return kOk;
   const int64_t blocks = (rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kInvalidArgument, "too many rows");
   JN_PROFILE("edge_coefficients_kernel", stream);
   hipLaunchKernelGGL(edge_coefficients_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, idx, score, rows, k,
                      compress, coef);
@@ -1562,8 +1562,8 @@ __global__ __launch_bounds__(64) void unit_scale_kernel(const float* w, const fl
 int launch_unit_scale(const float* w, const float* grad, int64_t rows, int64_t r, float eps, float* out,
                       hipStream_t stream) {
   JN_REQUIRE(w && out, kInvalidArgument, "null tensor pointer");
-  JN_REQUIRE(rows >= 1 && r >= 1 && rows < (1LL << 31) && r < (1LL << 30), kInvalidArgument,
-             "unit scale needs 1 <= rows < 2^31 and 1 <= r < 2^30 (rows=%lld, r=%lld)", (long long)rows,
+  JN_REQUIRE(rows >= 1 && r >= 1 && fits_grid(rows, kWave) && r < (1LL << 30), kInvalidArgument,
+             "unit scale needs 1 <= rows < 2^26 and 1 <= r < 2^30 (rows=%lld, r=%lld)", (long long)rows,
              (long long)r);
   JN_REQUIRE(eps > 0.0f, kInvalidArgument, "eps must be positive");
   JN_PROFILE(grad ? "unit_scale_backward_kernel" : "unit_scale_kernel", stream);
@@ -1662,7 +1662,7 @@ int launch_cols_backward(const ColsBwdArgs& a, hipStream_t stream) {
       while (slab > 64 * pw && slab % (128 * pw) == 0 && (int64_t)a.Nq * slab * eb > (2LL << 20)) slab /= 2;
     const int64_t slabs = a.grad_pv ? (a.D + slab - 1) / slab : 1;
     const int64_t blocks = (total_cols + 3) / 4 * slabs;
-    JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "too many columns");
+    JN_REQUIRE(fits_grid(blocks, 256), kInvalidArgument, "too many columns");
     JN_PROFILE(a.profile_name ? a.profile_name : "cols_gather_kernel", stream);
     const dim3 grid((unsigned)blocks);
     if (a.band) {
@@ -1685,7 +1685,7 @@ int launch_cols_backward(const ColsBwdArgs& a, hipStream_t stream) {
   if (a.q && a.r > kRegRank) {  // ranks beyond the column kernel's rank slots
     const bool vec = (a.r % 4 == 0) && (a.ldq % 4 == 0) && ((reinterpret_cast<uintptr_t>(a.q) & 15) == 0);
     const int64_t blocks = cols_backward_parts(total_cols);
-    JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "too many columns");
+    JN_REQUIRE(fits_grid(blocks, 256), kInvalidArgument, "too many columns");
     JN_PROFILE("rank_cols_grad_kernel", stream);
     const dim3 grid((unsigned)blocks);
     if (a.band) {
@@ -1703,7 +1703,7 @@ int launch_cols_backward(const ColsBwdArgs& a, hipStream_t stream) {
     const bool vec = (a.r % 4 == 0) && (a.ldq % 4 == 0) && ((reinterpret_cast<uintptr_t>(a.q) & 15) == 0) &&
                      (!mh || a.head_rank % 4 == 0);
     const int64_t blocks = cols_backward_parts(total_cols);
-    JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "too many columns");
+    JN_REQUIRE(fits_grid(blocks, 256), kInvalidArgument, "too many columns");
     JN_PROFILE("cols_keygrad_kernel", stream);
     const dim3 grid((unsigned)blocks);
     if (a.band) {

@@ -1643,7 +1643,7 @@ static bool fast_choice(const GemmArgs& g, GemmUse use, int64_t zdim, int forced
   const GemmUseInfo& info = kGemmUses[use];
   const int64_t tiles128 = (int64_t)((g.M + kFT - 1) / kFT) * ((g.N + kFT - 1) / kFT) * zdim;
   const bool big = forced ? forced == kFT : (g.M >= kFT && g.N >= kFT && tiles128 >= 256);
-  return big && tiles128 < (1LL << 31) && fast_path_ok(g, info.a_kc, info.b_kc) &&
+  return big && fits_grid(tiles128, 256) && fast_path_ok(g, info.a_kc, info.b_kc) &&
          (!info.a_kscale || g.a_kscale != nullptr);
 }
 
@@ -1696,7 +1696,7 @@ int launch_gemm(const GemmArgs& g, GemmUse use, int splits, hipStream_t stream, 
   if (gemm_use_dense_bf16(use)) {
     JN_REQUIRE(bf16_path_ok(g, use, splits), kUnsupported,
                "%s needs M, N >= 128, N and the strides multiples of 8 and 16-byte aligned operands", info.name);
-    JN_REQUIRE(tiles < (1LL << 31), kUnsupported, "GEMM grid too large");
+    JN_REQUIRE(fits_grid(tiles, 256), kUnsupported, "GEMM grid too large");
     JN_PROFILE(info.name, stream);
     at_tile([&](auto tc) {
       constexpr int T = decltype(tc)::value;
@@ -1731,7 +1731,7 @@ int launch_gemm(const GemmArgs& g, GemmUse use, int splits, hipStream_t stream, 
     return kOk;
   }
   if (gemm_use_bf16(use) && forced != 32 && forced != 64 && bf16_path_ok(g, use, splits)) {
-    JN_REQUIRE(tiles < (1LL << 31), kUnsupported, "GEMM grid too large");
+    JN_REQUIRE(fits_grid(tiles, 256), kUnsupported, "GEMM grid too large");
     JN_PROFILE(use == kGemmProjectBf16 ? "gemm_bf16_kernel<project_bf16>"
                : use == kGemmGradInputBf16 ? "gemm_bf16_kernel<grad_input_bf16>"
                                            : "gemm_bf16_kernel<grad_weight_bf16>",
@@ -1759,7 +1759,7 @@ int launch_gemm(const GemmArgs& g, GemmUse use, int splits, hipStream_t stream, 
   if ((use == kGemmProject || use == kGemmGradInput || use == kGemmGradWeight || use == kGemmDenseAggregate ||
        use == kGemmDenseValueGrad) &&
       forced == 0 && x3_path_ok(g, use, splits)) {
-    JN_REQUIRE(tiles < (1LL << 31), kUnsupported, "GEMM grid too large");
+    JN_REQUIRE(fits_grid(tiles, 256), kUnsupported, "GEMM grid too large");
     JN_PROFILE(use == kGemmProject          ? "gemm_x3_kernel<project>"
                : use == kGemmGradInput      ? "gemm_x3_kernel<grad_input>"
                : use == kGemmGradWeight     ? "gemm_x3_kernel<grad_weight>"
@@ -1945,7 +1945,7 @@ int gemm_grad_weight(const float* dP, int64_t ldp, const float* X, int64_t ldx, 
                        beside && !x_bf16 && K > kBesideRows ? kTile64Beside : kTile64Below);
   if (rc != kOk) return rc;
   const int64_t total = (int64_t)M * N;
-  JN_REQUIRE((total + 63) / 64 < (1LL << 31), kUnsupported, "weight gradient too large");
+  JN_REQUIRE(fits_grid((total + 63) / 64, 256), kUnsupported, "weight gradient too large");
   const int blocks = (int)((total + 63) / 64);
   JN_PROFILE("splitk_reduce_kernel", stream);
   hipLaunchKernelGGL(splitk_reduce_kernel, dim3(blocks), dim3(256), 0, stream, partial, splits, M, N,

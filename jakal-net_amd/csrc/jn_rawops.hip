@@ -129,7 +129,7 @@ int check_raw_edges(int64_t B, int64_t Nq, int64_t Nk, int64_t k, int64_t D) {
 
 int grid_rows(int64_t rows) {
   const int64_t blocks = (rows + 3) / 4;
-  return blocks < (1LL << 31) ? (int)blocks : -1;
+  return fits_grid(blocks, 256) ? (int)blocks : -1;
 }
 
 }  // namespace
@@ -183,7 +183,7 @@ int jn_softsign_backward(const float* scores, const float* grad_edges, int64_t c
   JN_REQUIRE(count >= 0 && (count == 0 || (scores && grad_edges && grad_scores)), kInvalidArgument,
              "null tensor pointer");
   if (count == 0) return kOk;
-  JN_REQUIRE((count + 255) / 256 < (1LL << 31), kUnsupported, "too many elements");
+  JN_REQUIRE(fits_grid((count + 255) / 256, 256), kUnsupported, "too many elements");
   hipStream_t st = static_cast<hipStream_t>(stream);
   JN_PROFILE("softsign_backward_kernel", st);
   hipLaunchKernelGGL(softsign_backward_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, st, scores,

@@ -118,7 +118,7 @@ int launch_route_coef(const int32_t* idx, const float* logit, const float* rho, 
              kSelectLargeMaxK, k);
   if (rows == 0) return kOk;
   const int64_t blocks = (rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kInvalidArgument, "too many rows");
   JN_PROFILE(k > kWave ? "route_coef_large_kernel" : "route_coef_kernel", stream);
   if (k > kWave)
     hipLaunchKernelGGL(route_coef_large_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, idx, logit, rho, k,
@@ -519,7 +519,7 @@ int launch_route_rows_backward(const RouteRowsBwdArgs& a, hipStream_t stream) {
              kSelectLargeMaxK, a.k);
   JN_REQUIRE(a.compress >= 0 && a.compress <= 2, kUnsupported, "route compress kind must be 0, 1 or 2");
   const int64_t blocks = (a.rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kInvalidArgument, "too many rows");
   JN_REQUIRE((int64_t)a.Nd * a.D * 4 < (1LL << 31) && (int64_t)a.Nd * a.ldk * 4 < (1LL << 31), kUnsupported,
              "one batch element of the destination rows must stay below 2 GiB");
   const int pw = a.bf16 ? 8 : 4;  // one 16-byte pack: 4 fp32 or 8 bf16 elements

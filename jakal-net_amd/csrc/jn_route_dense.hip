@@ -205,7 +205,7 @@ int launch_route_dense_compress(float* L, const float* bias, float inv_temp, int
                                 hipStream_t stream) {
   const int64_t rows = (int64_t)B * Ns;
   const int64_t blocks = (rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kUnsupported, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kUnsupported, "too many rows");
   JN_PROFILE("route_dense_compress_kernel", stream);
   if (rows_vec(Nd, L))
     hipLaunchKernelGGL(route_dense_compress_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, stream, L, bias,
@@ -227,7 +227,7 @@ int launch_route_dense_compress_backward(float* H, const float* R, const float* 
                                          float* grad_rho, float* grad_ps, float* rowsum, hipStream_t stream) {
   const int64_t rows = (int64_t)B * Ns;
   const int64_t blocks = (rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kUnsupported, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kUnsupported, "too many rows");
   JN_PROFILE("route_dense_compress_backward_kernel", stream);
   if (rows_vec(Nd, H, R, gds))
     hipLaunchKernelGGL(route_dense_compress_backward_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, stream, H,

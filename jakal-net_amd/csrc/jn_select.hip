@@ -1383,7 +1383,7 @@ int launch_topk_select(const SelectArgs& a_in, hipStream_t stream) {
              (long long)a.ldk);
   const int tiles = (a.Nq + kSelRows - 1) / kSelRows;
   const int64_t blocks = (int64_t)tiles * a.B;
-  JN_REQUIRE(blocks > 0 && blocks < (1LL << 31), kInvalidArgument, "bad grid size");
+  JN_REQUIRE(blocks > 0 && fits_grid(blocks, 256), kInvalidArgument, "bad grid size");
   dim3 grid((unsigned)blocks);
   const bool mh = a.heads > 1;
   JN_REQUIRE(!(mh && a.bf16), kUnsupported, "bf16 score operands take one head");
@@ -1438,7 +1438,7 @@ int launch_topk_select(const SelectArgs& a_in, hipStream_t stream) {
                      (mode == kSelectSplitF16KeySplit ||
                       (mode == kSelectSplitF16 && blocks < ksp_max && a.Nk >= ksp_keys));
     const int64_t kblocks = (int64_t)((a.Nq + kSelRowsPerWave - 1) / kSelRowsPerWave) * a.B;
-    JN_REQUIRE(!ksp || kblocks < (1LL << 31), kInvalidArgument, "bad grid size");
+    JN_REQUIRE(!ksp || fits_grid(kblocks, 256), kInvalidArgument, "bad grid size");
     const dim3 kgrid((unsigned)kblocks);
     JN_PROFILE("lowrank_topk_select_kernel", stream);
     if (mh) {

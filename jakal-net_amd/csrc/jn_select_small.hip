@@ -282,7 +282,7 @@ int launch_topk_select_small(const SelectArgs& a, hipStream_t stream) {
              kSelectSmallMaxKeys, kSelectMaxK, kRegRank, a.k, a.Nk, a.r);
   JN_REQUIRE(a.q && a.key && a.out_idx && a.out_score, kInvalidArgument, "null tensor pointer");
   const int64_t blocks = (int64_t)a.B * ((a.Nq + kSmRows - 1) / kSmRows);
-  JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "bad grid size");
+  JN_REQUIRE(fits_grid(blocks, 1024), kInvalidArgument, "bad grid size");
   auto a16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const bool vec = a.r % 4 == 0 && a.ldq % 4 == 0 && a.ldk % 4 == 0 && a.q_batch_stride % 4 == 0 &&
                    a.k_batch_stride % 4 == 0 && a16(a.q) && a16(a.key) && (!a.scale || a16(a.scale));

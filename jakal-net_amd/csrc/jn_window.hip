@@ -105,7 +105,7 @@ int launch_window_scores(const WindowScoreArgs& a, hipStream_t stream) {
   const int64_t rows = (int64_t)a.B * a.Nq;
   if (rows == 0) return kOk;
   const int64_t blocks = (rows + 3) / 4;
-  JN_REQUIRE(blocks < (1LL << 31), kInvalidArgument, "too many rows");
+  JN_REQUIRE(fits_grid(blocks, 256), kInvalidArgument, "too many rows");
   const bool vec = (a.r % 4 == 0) && (!mh || a.head_rank % 4 == 0) && (a.ldk % 4 == 0) &&
                    ((reinterpret_cast<uintptr_t>(a.key) & 15) == 0);
   JN_PROFILE(mh ? "window_scores_heads_kernel" : "window_scores_kernel", stream);

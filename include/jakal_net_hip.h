@@ -39,7 +39,7 @@ typedef void* jn_stream_t;
 /* Message of the last failing call on this host thread ("" if none). */
 const char* jn_last_error(void);
 
-/* ABI revision of this header (bumped on any signature or accepted-range change); this is 20. */
+/* ABI revision of this header (bumped on any signature or accepted-range change); this is 21. */
 int jn_abi_version(void);
 
 /*

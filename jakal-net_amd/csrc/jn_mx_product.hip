@@ -1328,14 +1328,24 @@ int launch_rows(const RowsArgs& g, hipStream_t s) {
   return kOk;
 }
 
-// Tiles of outputs a workgroup, and tiles of rows: as many as leave a workgroup for every
-// CU (x's way into registers is the most of the work of many rows; 64 x 2,048 x 16,384
-// bf16 with one, two and four tiles of outputs 27.9, 22.8 and 17.3 us, one row 8.2 to 8.7).
+// Tiles of outputs a workgroup, and tiles of rows.  x's way into registers is the most of
+// the work of many rows, so four tiles of outputs share it from 640 on, when that leaves 160
+// workgroups.  us with one tile and with four, over 2,048 (bf16 unless said):
+//   rows              8,192 outputs  12,000         16,000         16,384
+//   1                 4.9 and 6.9    6.6 and 7.0    7.8 and 7.5    7.8 and 7.4
+//   16                7.4 and 7.8    10.0 and 7.9   12.6 and 8.2   12.6 and 8.2
+//   32                10.9 and 9.9   15.4 and 10.1  19.8 and 10.3  19.8 and 10.4
+//   32, e2m1 by e2m1  12.4 and 10.3  16.2 and 10.5  20.5 and 10.9  20.6 and 10.9
+//   64                18.2 and 14.9  26.1 and 15.2  33.8 and 15.4  33.9 and 15.4
+//   64 fp32           39.1 and 25.8  53.9 and 26.2  68.5 and 27.7  68.5 and 27.5
+// (4,096 outputs: 64 rows 10.3 and 14.9, fp32 20.1 and 25.5, 1 row 4.1 and 6.9.)
+constexpr int64_t kShareOuts = 640;
 template <typename T, bool SCALED>
 int run_rows(const RowsArgs& g, hipStream_t s) {
   const int64_t rows = (g.m + 15) / 16, outs = (g.n + 15) / 16;
-  if (rows == 1) return outs >= 1024 ? launch_rows<T, SCALED, 1, 4>(g, s) : launch_rows<T, SCALED, 1, 1>(g, s);
-  if (outs >= 1024) return rows == 2 ? launch_rows<T, SCALED, 2, 4>(g, s) : launch_rows<T, SCALED, 4, 4>(g, s);
+  const bool share = outs >= kShareOuts;
+  if (rows == 1) return share ? launch_rows<T, SCALED, 1, 4>(g, s) : launch_rows<T, SCALED, 1, 1>(g, s);
+  if (share) return rows == 2 ? launch_rows<T, SCALED, 2, 4>(g, s) : launch_rows<T, SCALED, 4, 4>(g, s);
   if (outs >= 256) return rows == 2 ? launch_rows<T, SCALED, 2, 1>(g, s) : launch_rows<T, SCALED, 4, 1>(g, s);
   return rows > 2 && outs >= 128 ? launch_rows<T, SCALED, 2, 1>(g, s) : launch_rows<T, SCALED, 1, 1>(g, s);
 }

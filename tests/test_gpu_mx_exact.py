@@ -85,3 +85,19 @@ def test_linear_input_grad(dev, m, n, r):
     w = X.whole(1, r, n, dev=dev)
     for what, g in (("grad_x", X.whole(3, m, r, dev=dev)), ("single elements", X.lonely(5, m, r, torch.bfloat16, 8, dev))):
         X.same(what, torch.ops.jakal_net_hip.linear_input_grad(g.bfloat16(), w.bfloat16()), X.product(g, w))
+
+
+@pytest.mark.parametrize("acts", [None, "e2m1"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 17, 32, 33, 64])
+def test_few_rows_give_an_output_the_same_bits_however_many_there_are(dev, rows, dtype, acts):
+    """Tiles of outputs are shared out by how many there are; a sum's order is not."""
+    import jakal_net as J
+
+    kind = O.DTYPES[dtype]
+    g = torch.Generator(device=dev).manual_seed(rows)
+    w, x = torch.randn(17000, 2048, generator=g, device=dev), torch.randn(rows, 2048, generator=g, device=dev).to(kind)
+    most = J.mx_linear(x, J.mx_quantize(w, "e2m1"), activations=acts)
+    for outs in (16000, 10256, 10225, 8192, 4097, 300, 16):
+        some = J.mx_linear(x, J.mx_quantize(w[:outs], "e2m1"), activations=acts)
+        assert torch.equal(some, most[:, :outs]), outs

@@ -358,7 +358,9 @@ def gelu(x: Tensor, *, saved: str | None = None, implementation: ImplementationM
 # modules
 # ---------------------------------------------------------------------------
 class Linear(nn.Linear):
-    """``nn.Linear`` (its parameters, names and initialisation) on ``linear``."""
+    """``nn.Linear`` (its parameters, names and initialisation) on ``linear``.  Unlike the
+    function and ``LayerNorm`` it keeps its input in e4m3 unless told not to: its weight's
+    gradient is that at the kept input.  ``saved=None`` gives the plain layer."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, *, saved: str | None = "e4m3",
                  implementation: ImplementationMode = "native", device=None, dtype=None) -> None:
@@ -373,7 +375,8 @@ class Linear(nn.Linear):
 
 
 class GELU(nn.Module):
-    """``gelu`` as a module."""
+    """``gelu`` as a module.  Unlike the function it keeps its input in e4m3 unless told not
+    to: its gradient is that at the kept input.  ``saved=None`` gives the plain activation."""
 
     def __init__(self, *, saved: str | None = "e4m3", implementation: ImplementationMode = "native") -> None:
         check_implementation(implementation)

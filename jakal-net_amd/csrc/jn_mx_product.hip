@@ -40,8 +40,8 @@ struct TilePlace {
 };
 
 // ---- ordinary numbers by microscaled ones ---------------------------------------
-// v_mfma_f32_16x16x32_bf16 over tiles of 128 x 128: microscaled values are bf16
-// values (at most four significant bits), and A is one, two or three bf16 terms
+// v_mfma_f32_16x16x32_bf16 over tiles of 64 x 64 to 256 x 256: microscaled values are
+// bf16 values (at most four significant bits), and A is one, two or three bf16 terms
 // that add up to it exactly (bf16, fp16, fp32), so every product is exact and the
 // sums are fp32.  Both operands pass through registers on their way into LDS.  An
 // operand whose rows run along r lies there as it does in memory ([row][r]); one
@@ -287,8 +287,10 @@ __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) 
 
 // Tiles of TM x TN over WM x WN waves, LDS double buffered with the next slice in registers.
 // For fp32, fp16 and rows that are no whole packs.  Splitting x into its terms and their way
-// through LDS bound it: 1,531 x 383 x 4,099 fp32 forward 42 us (114 TFLOP/s; the library's
-// fp32 product by dequantised weights 88 us), 128 x 2,048 x 16,384 fp32 53 us (77), fp16 43 (19).
+// through LDS bound it: 1,531 x 383 x 4,099 fp32 forward 41 us (117 TFLOP/s; the library's
+// fp32 product by dequantised weights 88 us), 128 x 2,048 x 16,384 fp32 53 us (the library
+// 77).  fp16 is slower than the library's fp16 product by dequantised weights: 128 rows 40 us
+// and 17, 1,024 rows 177 and 55.
 template <typename T, Product P, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_mixed_kernel(MixedArgs g) {
   constexpr int FORM = P == kWeightGrad ? kE4m3 : kE2m1;
@@ -466,7 +468,8 @@ __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_mixed_kernel(MixedArgs g)
 // us, 1,110 TFLOP/s, the library 404).  A quarter less LDS traffic (B there as its codes) and
 // the barrier under the first row of products gained 2 %.  The narrow ones wait for each other once a slice:
 // 0.53 to 0.85 us whatever they multiply, and loads further ahead (four slices) or twice the
-// waves changed nothing.
+// waves changed nothing.  256 x 256 takes all 256 registers: the forward keeps one more in
+// scratch and the input gradient two.
 template <Product P, int TM, int TN, int WM, int WN, int AHEAD>
 __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_bf16_kernel(MixedArgs g) {
   constexpr int FORM = P == kWeightGrad ? kE4m3 : kE2m1;
@@ -899,7 +902,13 @@ int launch_column_sums(const void* x, int64_t rows, int64_t dim, float* partial,
 
 // Tiles of a product's output and splits of its sum by what they were measured to cost (in
 // us): a slice's time by how many workgroups a CU has, and for more than one split a second
-// launch and the partial sums' way to memory and back.
+// launch and the partial sums' way to memory and back.  A launch, a tile's start and its
+// outputs' way out are not in it, so that it is near over long sums (input gradient of 1,024
+// x 2,048 over 16,384 77.6 for 76 us, weight gradient of 8,192 x 512 x 2,048 35.8 for 38.4)
+// and short over few slices and many outputs (forward of 1,024 x 512 x 2,048 4.0 for 8.6, of
+// 1,024 x 2,048 x 16,384 51 for 63, of 8,192 rows 410 for 486; the head's weight gradient 51
+// for 74), where the tiles' order by it is not always the measured one (192 x 2,048 x 16,384
+// takes 27 us in tiles of 64 x 64, 256 rows 24 in tiles of 128 x 64).
 struct TileCost {
   int m, n;
   double least, first, each;  // of a slice: max(least, first + each * workgroups a CU)
@@ -1060,8 +1069,9 @@ __device__ __forceinline__ intx8 wide(u32x4_nt v) { return intx8{(int)v[0], (int
 // so that W may be anything finite there.
 // 8,192 cubed takes 321 us (3,425 TFLOP/s, near what the card sustains on random data),
 // 8,192 x 2,048 x 16,384 bf16 205 (2,680): eight steps a tile, and its outputs' way out, 256
-// KB of fp32 sums rounded through LDS, has no products of another tile beside it (a loop over
-// tiles in one workgroup left no registers for that, and was slower).
+// KB of fp32 sums rounded through LDS, has no products of another tile beside it (256 x 256
+// takes all 256 registers and keeps two more in scratch; a loop over tiles in one workgroup
+// had many more there, and was slower).
 template <typename T, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN* kWave, 2) void mx_linear_kernel(LinearArgs g) {
   constexpr int WAVES = WM * WN;
@@ -1351,7 +1361,8 @@ int run_rows(const RowsArgs& g, hipStream_t s) {
 }
 
 // Few rows: microscaling x apart costs more than it does here until it is shared by
-// more workgroups (bf16, 2,048 x 16,384: 64 rows 17.6 us, 65 in two launches 13.3).
+// more workgroups (bf16, 2,048 x 16,384, both e2m1: 32 rows 11.0 us here, 64 in two launches
+// 11.0).  x as it is: 64 rows 15.4 us here, 65 in tiles 18.4.
 bool few_rows(int64_t rows, int32_t activations) { return rows <= (activations == kPlain ? 64 : 32); }
 
 // x microscaled for this product: rows of whole steps.
@@ -1493,13 +1504,22 @@ int jn_mx_weight_grad(const void* grad_y, const void* codes, const void* scales,
 
 int32_t jn_linear_input_grad_fits(int64_t rows, int64_t dim, int64_t out, int32_t type) {
   if (check_product("linear backward", rows, dim, out, type)) return 0;
-  // Measured with the library's product (us).  Long sums leave most CUs to the splits that the
-  // library does not make: 16,384 by 64 x 512 17 and 69, 1 x 1,024 17 and 29, 1,024 x 2,048 82
-  // and 117, 2,048 x 4,096 265 and 245; 8,192 by 16 x 2,048 14 and 21, 1,024 x 2,048 55 and 61,
-  // 1 x 1,024 14 and 13, 2,048 squared 86 and 81.  Short ones are a launch, and the library's
-  // takes the host 12 us more: 256 by 512 x 1,024 6.1 and 6.2, 4,096 squared 18.7 and 18.7; 512
-  // by 1,024 x 2,048 9.6 and 9.9, 16 x 512 7.1 and 5.4.  Between them the library's is as fast
-  // or faster (1,536 by 1,024 x 2,048 18.7 and 16.2).
+  // Measured with the library's product (us, here and there, in captured calls; eager, the
+  // library's takes the host 12 us more).  Long sums leave most CUs to the splits that the
+  // library does not make:
+  //   outputs  1 x 2,048      64 x 512      256 x 2,048   1,024 x 2,048  2,048 x 2,048
+  //   16,384   23.1 and 36.4  16.1 and 68   33.8 and 65   78 and 112     133 and 144
+  //   12,000   21.5 and 26.7  14.6 and 59   30.0 and 56   66 and 90      106 and 117
+  //   8,192    18.1 and 14.6  10.6 and 36   23.9 and 35   52 and 58      79 and 76
+  //   6,144    14.3 and 10.0  10.3 and 28   20.8 and 27   46 and 44      66 and 59
+  //   4,096    16.4 and 7.8   9.7 and 21    21.4 and 20   34 and 32      53 and 42
+  //   2,048    10.1 and 6.2   7.8 and 12    15.1 and 12   22 and 19      29 and 24
+  //   768      6.9 and 4.5    7.0 and 7.4   7.8 and 7.0   11.0 and 9.7   14.1 and 12.1
+  //   512      5.9 and 4.2    6.1 and 6.2   6.3 and 6.9   8.6 and 8.6    11.2 and 11.0
+  //   256      4.5 and 3.9    4.6 and 4.9   4.7 and 5.2   6.3 and 6.6    8.1 and 8.3
+  // (16,384: 2,048 x 4,096 265 and 245.)  Between 512 and 8,192 outputs the library's is as
+  // fast or faster but for tens of rows (from 4,096 on, hundreds), which are left to it too;
+  // up to 16,384 the limits are those of 8,192, though 12,000 would bear 16,384's.
   const MixedPlan plan(kPlainGrad, rows, dim, out, type, false);
   const int64_t outputs = rows * dim;
   if (!plan.packed) return 0;

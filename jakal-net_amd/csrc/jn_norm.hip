@@ -10,10 +10,13 @@
 //
 // Or keeping c = x - p in e4m3 for the backward (jn_layer_norm_*_kept), p being the
 // mean of x in 64 bits rounded to fp32: the forward is the same, h in the gradients
-// is scale r times the kept c.  16 x 512 x 512 fp32 12.2 us forward (38 MB) and 12.0
-// backward (38 MB, where reading x would be 50).  What is kept is centred so that its rounding is
-// relative to h whatever the mean is; the mean in 64 bits is the same number in any
-// order of summing, and with it the codes are.
+// is scale r times the kept c.  16 x 512 x 512 fp32 11.8 us forward (38 MB) and 12.0
+// backward (38 MB, where reading x would be 50).  What is kept is centred so that its
+// rounding is relative to h whatever the mean is.  A sum in 64 bits has 29 bits more than
+// the numbers it adds: p, and with it the codes, is the same in any order of summing (the
+// kernels' orders differ) unless the row cancels to within those bits (1e30, 1, -1e30, 3)
+// or p falls on a border between two fp32 numbers; the codes are then those of a mean
+// that differs in its last bits.
 #include "../../include/jakal_net_hip.h"
 #include "jn_internal.hpp"
 #include "jn_mx.hpp"

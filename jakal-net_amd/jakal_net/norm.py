@@ -10,8 +10,9 @@ HIP library for GPU tensors of fp32, bf16 or fp16 and raises where it cannot,
 CPU tensors (and a native module without these operators) take the PyTorch form;
 ``"kernel"`` takes the PyTorch form where the library declines; ``"reference"``
 and ``"streaming"`` are the PyTorch form.
-The library computes in fp32 and rounds once; under autocast half-precision
-values come back in fp32, as torch's layer norm returns them.
+The library computes in fp32 and rounds once; under GPU autocast half-precision
+values come back in fp32, as torch's layer norm returns them there (on the CPU it
+returns them in their own type, and so does the PyTorch form).
 
 ``saved="e4m3"`` keeps for the backward the centred values in 8 bits
 (``jakal_net.mx``): the outputs are the same, and the gradients are the norm's
